@@ -1,0 +1,494 @@
+"""Cases, plain forms and 64-bit definitions of the operators around the 8-bit paged KV cache:
+
+  map      block tables, slots and positions of one serving step, built on the GPU from the requests' lengths
+  append   new K and V rows (K rotated) into a paged cache of int8 values with one scale per page and KV head
+  attend   attention of the step's query rows over that cache: one-token decode and ragged prompts, with optional
+           tanh score cap, distance bias, document mask and prefix mask
+
+With `own` False, `run` computes them from elementary torch operations in 32 bits; with `own` True it makes the
+framework's calls. Layouts: pools int8 [n_pages, kv_heads, page, dim], scales fp32 [n_pages, kv_heads], block table
+int32 [batch, max_pages]; row t of sequence b is row t % page of page block_table[b, t // page].
+"""
+import math
+import random
+
+import numpy as np
+import torch
+
+own = False
+
+THETA = 500000.0  # rotary base of the batched-decode and long-prompt configurations
+
+
+# --------------------------------------------------------------------------------------------- the cases
+
+def _case(name, op, **kw):
+    c = dict(op=op, batch=1, q_heads=32, kv_heads=8, dim=128, page=64, cached_lo=0, cached_hi=0, new_lo=1, new_hi=1,
+             mix=1, io="f16", rope=0, cap=0.0, bias=False, prefix=False, docs=False)
+    c.update(kw)
+    if name:
+        c["name"] = name
+    return c
+
+
+def listed():
+    return [
+        # a decode step of a full batch: every request gets one row, a few cross into a new page
+        _case("map decode", "map", batch=64, cached_lo=256, cached_hi=8192, mix=3),
+        # a scheduler's step with many requests, some idle, some with whole prompts
+        _case("map prompts", "map", batch=512, page=16, cached_lo=0, cached_hi=4096, new_lo=0, new_hi=300, mix=5),
+        # the rows of one decode step, rotated and stored
+        _case("append decode", "append", batch=64, cached_lo=256, cached_hi=8192, rope=1, mix=3),
+        # four prompt chunks of uneven length, half-split rotation
+        _case("append prompts", "append", batch=4, cached_lo=0, cached_hi=3000, new_lo=900, new_hi=3100, rope=2, mix=7),
+        # a small model in 32 bits on small pages, odd lengths, no rotation
+        _case("append f32", "append", batch=5, q_heads=32, kv_heads=4, dim=64, page=16, cached_lo=3, cached_hi=700,
+              new_lo=1, new_hi=77, io="f32", mix=2),
+        # one user's next token on a small model: latency
+        _case("decode one", "attend", q_heads=14, kv_heads=2, dim=64, page=16, cached_lo=513, cached_hi=513, rope=1),
+        # the batched-decode configuration's lengths
+        _case("decode batch", "attend", batch=64, cached_lo=256, cached_hi=8192, mix=3),
+        # the largest decode: 64 query heads, long caches, capped scores
+        _case("decode long", "attend", batch=32, q_heads=64, page=128, cached_lo=16384, cached_hi=16384, cap=30.0),
+        # 32-bit tensors of a small model, distance bias
+        _case("decode f32", "attend", batch=7, q_heads=32, kv_heads=4, dim=64, page=32, cached_lo=37, cached_hi=3001,
+              io="f32", bias=True, mix=4),
+        # short continuations of running chats, prompt prefixes visible both ways, capped scores
+        _case("prompt ragged", "attend", batch=6, q_heads=14, kv_heads=2, dim=64, page=16, cached_lo=0, cached_hi=2111,
+              new_lo=3, new_hi=611, rope=2, prefix=True, cap=50.0, mix=6),
+        # several documents packed in one prompt, attending within their own document
+        _case("prompt docs", "attend", batch=2, page=64, new_lo=3900, new_hi=4096, rope=1, docs=True, mix=8),
+        # a long prompt's later chunk
+        _case("prompt long", "attend", page=128, cached_lo=14336, cached_hi=14336, new_lo=2048, new_hi=2048, rope=1),
+    ]
+
+
+def _spread(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["map", "append", "append", "attend", "attend", "attend", "attend", "attend"])
+    page = rng.choice([16, 32, 64, 128])
+    heads, kv, dim = rng.choice([(32, 8, 128), (64, 8, 128), (14, 2, 64), (32, 4, 64), (12, 4, 128), (8, 8, 64)])
+    base = dict(q_heads=heads, kv_heads=kv, dim=dim, page=page, mix=rng.randrange(1, 1 << 20))
+    io = rng.choice(["f16", "f16", "f32"])
+    if op == "map":
+        batch = _spread(rng, 1, 1024)
+        hi = _spread(rng, 16, 8192)
+        if rng.random() < 0.5:
+            return _case(None, op, batch=batch, cached_lo=rng.randrange(0, hi), cached_hi=hi, **base)
+        return _case(None, op, batch=batch, cached_hi=hi, new_lo=0, new_hi=_spread(rng, 2, max(3, 65536 // batch)),
+                     **base)
+    rope = rng.choice([0, 1, 2])
+    if op == "append":
+        if rng.random() < 0.5:
+            hi = _spread(rng, 1, 8192)
+            return _case(None, op, batch=_spread(rng, 1, 128), cached_lo=rng.randrange(0, hi + 1), cached_hi=hi,
+                         rope=rope, io=io if rope == 0 else "f16", **base)
+        batch = _spread(rng, 1, 16)
+        new = _spread(rng, 2, 12000 // batch)
+        return _case(None, op, batch=batch, cached_hi=_spread(rng, 1, 3000), new_lo=rng.randrange(1, new + 1),
+                     new_hi=new, rope=rope, io=io if rope == 0 else "f16", **base)
+    if rng.random() < 0.55:  # one token per sequence
+        batch = _spread(rng, 1, 64)
+        hi = _spread(rng, 1, min(32768, 300000 // batch))
+        return _case(None, op, batch=batch, cached_lo=rng.randrange(0, hi + 1), cached_hi=hi, io=io,
+                     rope=rope if io == "f16" else 0, cap=rng.choice([0.0, 0.0, 30.0]), bias=rng.random() < 0.25, **base)
+    batch = _spread(rng, 1, 8)
+    new = _spread(rng, 2, 2048 // batch)
+    hi = _spread(rng, 1, 6144 // batch)
+    docs = rng.random() < 0.3
+    return _case(None, op, batch=batch, cached_lo=rng.randrange(0, hi + 1), cached_hi=hi, new_lo=rng.randrange(1, new + 1),
+                 new_hi=new, rope=rope, cap=rng.choice([0.0, 0.0, 50.0]), bias=rng.random() < 0.25, docs=docs,
+                 prefix=not docs and rng.random() < 0.4, **base)
+
+
+def _lengths(case):
+    """Cached and new rows of every sequence: part of the case, not of the data's seed."""
+    r = random.Random(case["mix"])
+    n = case["batch"]
+    cached = [r.randint(case["cached_lo"], case["cached_hi"]) for _ in range(n)]
+    new = [r.randint(case["new_lo"], case["new_hi"]) for _ in range(n)]
+    if sum(new) == 0:
+        new[0] = 1
+    return cached, new
+
+
+def _prefix(case, b, cached, new):
+    """A prompt's two-way prefix: it may end among the cached rows, the new ones, or be absent."""
+    return random.Random(case["mix"] * 1000 + b).choice([0, cached // 2, cached + new // 2, cached + new])
+
+
+def _first_rows(case, cached, new):
+    """First visible cache row of every new row: the start of its document (documents of 100 to 900 rows)."""
+    first = []
+    for b, (c, n) in enumerate(zip(cached, new)):
+        r, start, row = random.Random(case["mix"] * 1000 + b), 0, []
+        end = r.randint(100, 900)
+        for p in range(c + n):
+            if p == end:
+                start, end = p, p + r.randint(100, 900)
+            if p >= c:
+                row.append(start)
+        first += row
+    return first
+
+
+def _pairs(case):
+    """(query row, visible cache row) pairs of one query head."""
+    cached, new = _lengths(case)
+    if case["docs"]:
+        first, at, total = _first_rows(case, cached, new), 0, 0
+        for c, n in zip(cached, new):
+            total += sum(c + i + 1 - first[at + i] for i in range(n))
+            at += n
+        return total
+    total = 0
+    for b, (c, n) in enumerate(zip(cached, new)):
+        pre = _prefix(case, b, c, n) if case["prefix"] else 0
+        total += sum(max(c + i + 1, pre) for i in range(n))
+    return total
+
+
+def work(case):
+    cached, new = _lengths(case)
+    T, H, D, P, B = sum(new), case["kv_heads"], case["dim"], case["page"], case["batch"]
+    io = 2 if case["io"] == "f16" else 4
+    if case["op"] == "map":
+        # lengths in; slots, positions, starts, new lengths, the pages taken and their table entries out
+        taken = sum((c + n + P - 1) // P - (c + P - 1) // P for c, n in zip(cached, new))
+        return {"bytes": 12 * T + 16 * B + 8 * taken, "flops": 0}
+    if case["op"] == "append":
+        old = sum(c % P for c, n in zip(cached, new) if n)
+        pages = sum((c + n + P - 1) // P - c // P for c, n in zip(cached, new) if n)
+        # rows in, int8 out; then the touched pages' rows out as the values they stand for
+        return {"bytes": 2 * H * D * (T * (io + 1) + (T + old) * io) + 12 * T + 8 * (T + old) + 16 * H * pages,
+                "flops": 2 * H * D * T * 4}
+    rows = 0  # cache rows that some query row sees
+    first, at = (_first_rows(case, cached, new) if case["docs"] else None), 0
+    for c, n in zip(cached, new):
+        rows += (c + n - (first[at] if first and n else 0)) if n else 0
+        at += n
+    return {"bytes": 2 * rows * H * D + 8 * H * (rows // P + B) + 2 * T * case["q_heads"] * D * io,
+            "flops": 4 * case["q_heads"] * D * _pairs(case)}
+
+
+# --------------------------------------------------------------------------------------------- inputs
+
+def _dtype(case):
+    return torch.float16 if case["io"] == "f16" else torch.float32
+
+
+def _fill(g, n_pages, H, P, D, dev):
+    """Pages as a running server holds them: normal rows, quantised by their page's largest value."""
+    pool = torch.empty(n_pages, H, P, D, dtype=torch.int8, device=dev)
+    scale = torch.empty(n_pages, H, device=dev)
+    step = max(1, (1 << 27) // (H * P * D))
+    for a in range(0, n_pages, step):
+        x = torch.randn(min(step, n_pages - a), H, P, D, generator=g, device=dev)
+        s = x.abs().amax(dim=(2, 3)) * (1.0 / 127.0)
+        pool[a:a + step] = torch.round(x / s[:, :, None, None]).to(torch.int8)
+        scale[a:a + step] = s
+    return pool, scale
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed)
+    cached, new = _lengths(case)
+    B, P, H, D, Hq = case["batch"], case["page"], case["kv_heads"], case["dim"], case["q_heads"]
+    T = sum(new)
+    i32 = dict(dtype=torch.int32, device=dev)
+    s = dict(case=case, tokens=T, max_new=max(new), max_kv=max(c + n for c, n in zip(cached, new)))
+    s["max_pages"] = -(-s["max_kv"] // P) + 2
+    have = [-(-c // P) for c in cached]
+    after = [-(-(c + n) // P) for c, n in zip(cached, new)]
+    s["n_pages"] = n_pages = sum(after) + 5  # the last one in no request's hands
+    order = torch.randperm(n_pages - 1, generator=g, device=dev).to(torch.int32)
+    s["seq_len"] = torch.tensor(cached, **i32)
+    s["n_new"] = torch.tensor(new, **i32)
+    # the pages before (map) or after (append, attend) this step, scattered over the pool
+    held = have if case["op"] == "map" else after
+    table = np.full((B, s["max_pages"]), -1, dtype=np.int64)
+    at = 0
+    for b, n in enumerate(held):
+        table[b, :n] = np.arange(at, at + n)
+        at += n
+    t = torch.from_numpy(table).to(dev)
+    s["block_table"] = torch.where(t >= 0, order[t.clamp(min=0)], -1).to(torch.int32)
+    if case["op"] == "map":
+        s["free_pages"] = torch.cat([order[at:], order[:at]])
+        s["free_count"] = torch.tensor([n_pages - 1 - at], **i32)
+        return s
+    starts = np.concatenate([[0], np.cumsum(new)])
+    s["row_start"] = torch.tensor(starts, **i32)
+    s["kv_len"] = s["seq_len"] + s["n_new"]
+    pos = np.concatenate([np.arange(c, c + n) for c, n in zip(cached, new)])
+    seq = np.repeat(np.arange(B), new)
+    s["positions"] = torch.tensor(pos, **i32)
+    tab = s["block_table"].to(torch.int64)
+
+    def slots_of(q, p):
+        q, p = torch.from_numpy(q).to(dev), torch.from_numpy(p).to(dev)
+        return tab[q, p // P] * P + p % P
+
+    s["slots"] = slots_of(seq, pos)
+    for n in ("k", "v"):
+        s[n + "_pool"], s[n + "_scale"] = _fill(g, n_pages, H, P, D, dev)
+    dt = _dtype(case)
+    if case["op"] == "append":
+        # the rows that the touched pages hold after the step: the older ones, then the new ones
+        keep = [(b, c - c % P, c) for b, (c, n) in enumerate(zip(cached, new)) if n]
+        oq = np.concatenate([np.full(hi - lo, b) for b, lo, hi in keep] + [seq]).astype(np.int64)
+        op = np.concatenate([np.arange(lo, hi) for _, lo, hi in keep] + [pos]).astype(np.int64)
+        s["held_slots"] = slots_of(oq, op)
+        # rows of a fused projection's output: K and V beside each other
+        kv = torch.randn(T, 2, H, D, generator=g, device=dev).to(dt)
+        s["k_new"], s["v_new"] = kv[:, 0], kv[:, 1]
+        return s
+    s["q"] = (torch.randn(T, Hq, D, generator=g, device=dev) * (2.0 if case["cap"] else 1.0)).to(dt)
+    s["prefix"] = s["first"] = s["slopes"] = None
+    if case["prefix"]:
+        s["prefix"] = torch.tensor([_prefix(case, b, c, n) for b, (c, n) in enumerate(zip(cached, new))], **i32)
+    if case["docs"]:
+        s["first"] = torch.tensor(_first_rows(case, cached, new), **i32)
+    if case["bias"]:  # the usual geometric slopes
+        s["slopes"] = torch.tensor([2.0 ** (-8.0 * (h + 1) / Hq) for h in range(Hq)], device=dev)
+    return s
+
+
+# --------------------------------------------------------------------------------------------- plain forms
+
+def _freqs(D):
+    """Rotary frequencies 1 / theta^(2i/D), every step rounded to 32 bits."""
+    f = np.float32
+    return [float(f(1) / f(THETA ** float(f(2 * i) / f(D)))) for i in range(D // 2)]
+
+
+def _rotate(x, pos, mode, f64=False):
+    """x [n, heads, D] rotated at pos [n] (mode 1: pairs (2i, 2i+1); 2: pairs (i, i + D/2)). The angle is the 32-bit
+    product of position and frequency, as everywhere in the framework."""
+    if mode == 0:
+        return x
+    D = x.shape[-1]
+    ang = pos.to(torch.float32)[:, None] * torch.tensor(_freqs(D), dtype=torch.float32, device=x.device)
+    ang = (ang.double() if f64 else ang)[:, None, :]
+    c, s = torch.cos(ang), torch.sin(ang)
+    if mode == 1:
+        a, b = x[..., 0::2], x[..., 1::2]
+        return torch.stack([a * c - b * s, a * s + b * c], dim=-1).flatten(-2)
+    a, b = x[..., :D // 2], x[..., D // 2:]
+    return torch.cat([a * c - b * s, a * s + b * c], dim=-1)
+
+
+def _plain_map(s):
+    P, B, T = s["case"]["page"], s["case"]["batch"], s["tokens"]
+    n, c, table = s["n_new"], s["seq_len"], s["block_table"]
+    kv_len = c + n
+    have, need = (c + P - 1) // P, (kv_len + P - 1) // P
+    start = torch.zeros(B + 1, dtype=torch.int32, device=n.device)
+    start[1:] = torch.cumsum(n, 0)
+    before = torch.cumsum(need - have, 0) - (need - have)
+    # new pages from the top of the free stack, sequence by sequence
+    p = torch.arange(s["max_pages"], device=n.device)[None, :]
+    k = s["free_count"] - 1 - before[:, None] - (p - have[:, None])
+    takes = (p >= have[:, None]) & (p < need[:, None])
+    table.copy_(torch.where(takes, s["free_pages"][k.clamp(0, s["n_pages"] - 2)], table))
+    t = torch.arange(T, dtype=torch.int32, device=n.device)
+    b = torch.searchsorted(start, t, right=True) - 1
+    pos = c[b] + t - start[b]
+    slots = table[b, pos // P].to(torch.int64) * P + pos % P
+    return [table, kv_len, start, slots, pos, s["free_count"] - (need - have).sum(dtype=torch.int32)]
+
+
+def _plain_store(s, x, pool, scale):
+    """One of K and V [T, H, D] (32 bits) into its pages."""
+    P, c, n = s["case"]["page"], s["seq_len"].to(torch.int64), s["n_new"]
+    page, row = s["slots"] // P, s["slots"] % P
+    count = torch.zeros(2, s["n_pages"], dtype=torch.int32, device=x.device)
+    count[0].index_add_(0, page, torch.ones_like(page, dtype=torch.int32))
+    count[1].index_add_(0, page, (row == 0).to(torch.int32))
+    touched, anew = (count > 0)[:, :, None]
+    # every page's new scale: what it had (0 for a page begun anew) or what its new rows need
+    top = torch.zeros_like(scale).scatter_reduce_(0, page[:, None].expand(-1, scale.shape[1]), x.abs().amax(-1), "amax")
+    had = torch.where(anew, 0.0, scale)
+    now = torch.where(touched, torch.maximum(had, top * (1.0 / 127.0)), scale)
+    # the older rows of each sequence's first touched page, in the new scale
+    first = s["block_table"].to(torch.int64).gather(1, (c // P)[:, None]).squeeze(1).clamp(min=0)
+    ratio = torch.where(now[first] > 0, had[first] / now[first], 0.0)
+    old = pool[first]
+    moved = torch.round(old.to(torch.float32) * ratio[:, :, None, None]).to(torch.int8)
+    on = (c % P > 0) & (n > 0)
+    keep = on[:, None] & (torch.arange(P, device=c.device)[None, :] < (c % P)[:, None])
+    # a sequence without new rows may point at any page: it writes none
+    pool[torch.where(on, first, s["n_pages"] - 1)] = torch.where(
+        on[:, None, None, None], torch.where(keep[:, None, :, None], moved, old), pool[s["n_pages"] - 1])
+    scale.copy_(now)
+    inv = torch.where(now > 0, 1.0 / now, 0.0)
+    pool[page, :, row] = torch.round(x * inv[page][:, :, None]).clamp(-127, 127).to(torch.int8)
+
+
+def _plain_held(s, pool, scale, dt):
+    P, at = s["case"]["page"], s["held_slots"]
+    return (pool[at // P, :, at % P].to(torch.float32) * scale[at // P][:, :, None]).to(dt)
+
+
+def _plain_append(s):
+    k = _rotate(s["k_new"].to(torch.float32), s["positions"], s["case"]["rope"])
+    v = s["v_new"].to(torch.float32)
+    dt = _dtype(s["case"])
+    _plain_store(s, k, s["k_pool"], s["k_scale"])
+    _plain_store(s, v, s["v_pool"], s["v_scale"])
+    return [_plain_held(s, s["k_pool"], s["k_scale"], dt), _plain_held(s, s["v_pool"], s["v_scale"], dt), s["k_scale"],
+            s["v_scale"]]
+
+
+def _plain_attend(s):
+    case, T, S, L = s["case"], s["tokens"], s["max_new"], s["max_kv"]
+    B, P, H, D, Hq = case["batch"], case["page"], case["kv_heads"], case["dim"], case["q_heads"]
+    dev = s["q"].device
+    start, kv_len = s["row_start"].to(torch.int64), s["kv_len"].to(torch.int64)
+    t = torch.arange(T, device=dev)
+    tb = torch.searchsorted(start, t, right=True) - 1
+    c = kv_len - (start[1:] - start[:-1])
+    q = _rotate(s["q"].to(torch.float32), c[tb] + t - start[tb], case["rope"])
+    # sequences side by side, padded to the longest
+    i, j = torch.arange(S, device=dev), torch.arange(L, device=dev)
+    tok = (start[:-1, None] + i).clamp(max=T - 1)
+    q = q[tok].reshape(B, S, H, Hq // H, D).permute(0, 2, 3, 1, 4).reshape(B, H, Hq // H * S, D)
+    page = s["block_table"].to(torch.int64).clamp(min=0)[:, j // P]
+    k = s["k_pool"][page, :, j % P].to(torch.float32) * s["k_scale"][page][..., None]
+    x = torch.matmul(q, k.permute(0, 2, 3, 1)) * (1.0 / math.sqrt(D))
+    del k
+    x = x.reshape(B, H, Hq // H, S, L)
+    if case["cap"]:
+        x = torch.tanh(x / case["cap"]) * case["cap"]
+    pos = c[:, None] + i
+    if s["slopes"] is not None:
+        far = (pos[:, :, None] - j).abs().to(torch.float32)
+        x = x - s["slopes"].reshape(1, H, Hq // H, 1, 1) * far[:, None, None]
+    end = pos + 1 if s["prefix"] is None else torch.maximum(pos + 1, torch.minimum(s["prefix"], kv_len)[:, None])
+    seen = j < torch.minimum(end, kv_len[:, None])[..., None]
+    if s["first"] is not None:
+        seen = seen & (j >= s["first"][tok][..., None])
+    x = x.masked_fill(~seen[:, None, None], -math.inf)
+    top = x.amax(-1, keepdim=True)
+    x = torch.exp(x - torch.where(top > -math.inf, top, 0.0))
+    total = x.sum(-1, keepdim=True)
+    x = x / torch.where(total > 0, total, 1.0)
+    v = s["v_pool"][page, :, j % P].to(torch.float32) * s["v_scale"][page][..., None]
+    o = torch.matmul(x.reshape(B, H, Hq // H * S, L), v.permute(0, 2, 1, 3))
+    o = o.reshape(B, H, Hq // H, S, D).permute(0, 3, 1, 2, 4).reshape(B, S, Hq, D)
+    return o[tb, t - start[tb]].to(s["q"].dtype)
+
+
+# --------------------------------------------------------------------------------------------- one pass
+
+_context = []
+
+
+def _ops(s):
+    """The handle that a user's program keeps: one context, one description of the layer."""
+    from aihost_b200 import F16, F32, ROPE_INTERLEAVED, ROPE_NEOX, ROPE_NONE
+    from aihost_b200.kv8 import Kv8Ops, Kv8Spec
+    from aihost_b200.ops import Context
+
+    if not _context:
+        _context.append(Context(0))
+    case = s["case"]
+    code = F16 if case["io"] == "f16" else F32
+    spec = Kv8Spec(case["q_heads"], case["kv_heads"], case["dim"], page_rows=case["page"], n_pages=s["n_pages"],
+                   max_pages=s["max_pages"], io_dtype=code, out_dtype=code, score_cap=case["cap"], rope_theta=THETA,
+                   rope_mode=(ROPE_NONE, ROPE_INTERLEAVED, ROPE_NEOX)[case["rope"]])
+    s["ops"] = Kv8Ops(_context[0], spec)
+    return s["ops"]
+
+
+def run(state):
+    s = state
+    op = s["case"]["op"]
+    if not own:
+        return (_plain_map if op == "map" else _plain_append if op == "append" else _plain_attend)(s)
+    ops = s.get("ops") or _ops(s)
+    if op == "map":
+        m = ops.map_pages(s["seq_len"], s["n_new"], s["free_pages"], s["free_count"], s["block_table"], s["tokens"])
+        return [s["block_table"], m.kv_len, m.row_start, m.slots, m.positions, m.free_count]
+    if op == "append":
+        ops.append(s["k_new"], s["v_new"], s["slots"], s["positions"], s["k_pool"], s["v_pool"], s["k_scale"], s["v_scale"])
+        dt = s["k_new"].dtype
+        return [ops.read(s["k_pool"], s["k_scale"], s["held_slots"], dt),
+                ops.read(s["v_pool"], s["v_scale"], s["held_slots"], dt), s["k_scale"], s["v_scale"]]
+    return ops.attend(s["q"], s["row_start"], s["kv_len"], s["block_table"], s["k_pool"], s["v_pool"], s["k_scale"],
+                      s["v_scale"], max_new=s["max_new"], max_kv=s["max_kv"], prefix_len=s["prefix"],
+                      row_first=s["first"], alibi_slopes=s["slopes"])
+
+
+# --------------------------------------------------------------------------------------------- the definitions, in 64 bits
+
+def _exact_append(s):
+    """Page by page: the scale that a page's rows need, the older rows brought to it, the new ones rounded to it."""
+    case, P, out = s["case"], s["case"]["page"], []
+    cached, new = _lengths(case)
+    k = _rotate(s["k_new"].double(), s["positions"], case["rope"], f64=True)
+    scales = []
+    for x, name in ((k, "k"), (s["v_new"].double(), "v")):
+        pool, scale = s[name + "_pool"].double(), s[name + "_scale"].double()
+        at = 0
+        for b, (c, n) in enumerate(zip(cached, new)):
+            done = 0
+            while done < n:
+                page, row = int(s["block_table"][b, (c + done) // P]), (c + done) % P
+                m = min(P - row, n - done)
+                rows = x[at + done:at + done + m].permute(1, 0, 2)
+                old = scale[page] if row else torch.zeros_like(scale[page])
+                now = torch.maximum(old, rows.abs().amax(dim=(1, 2)) / 127.0)
+                safe = torch.where(now > 0, now, 1.0)[:, None, None]
+                pool[page, :, :row] = torch.round(pool[page, :, :row] * (old[:, None, None] / safe))
+                pool[page, :, row:row + m] = torch.round(rows / safe)
+                scale[page] = now
+                done += m
+            at += n
+        held = s["held_slots"]
+        out.append(pool[held // P, :, held % P] * scale[held // P][:, :, None])
+        scales.append(scale)
+    return out + scales
+
+
+def _exact_attend(s):
+    case, P, D = s["case"], s["case"]["page"], s["case"]["dim"]
+    H, G = case["kv_heads"], case["q_heads"] // case["kv_heads"]
+    cached, new = _lengths(case)
+    out = torch.zeros(s["q"].shape, dtype=torch.float64, device=s["q"].device)
+    at = 0
+    for b, (c, n) in enumerate(zip(cached, new)):
+        if not n:
+            continue
+        j = torch.arange(c + n, device=out.device)
+        pages = s["block_table"][b, :-(-(c + n) // P)].long()
+        i = torch.arange(c, c + n, device=out.device)
+        q = _rotate(s["q"][at:at + n].double(), i, case["rope"], f64=True)
+        end = (i + 1).clamp(min=_prefix(case, b, c, n) if case["prefix"] else 0)
+        hidden = j[None, :] >= end[:, None]
+        if case["docs"]:
+            hidden |= j[None, :] < s["first"][at:at + n, None]
+        for h in range(H):
+            k = (s["k_pool"][pages, h].double() * s["k_scale"][pages, h].double()[:, None, None]).reshape(-1, D)[:c + n]
+            v = (s["v_pool"][pages, h].double() * s["v_scale"][pages, h].double()[:, None, None]).reshape(-1, D)[:c + n]
+            for g in range(h * G, h * G + G):
+                x = (q[:, g] @ k.T) / math.sqrt(D)
+                if case["cap"]:
+                    x = case["cap"] * torch.tanh(x / case["cap"])
+                if case["bias"]:
+                    x -= 2.0 ** (-8.0 * (g + 1) / case["q_heads"]) * (i[:, None] - j[None, :]).abs()
+                out[at:at + n, g] = torch.softmax(x.masked_fill(hidden, -math.inf), dim=-1) @ v
+        at += n
+    return out
+
+
+def exact(case, seed):
+    if case["op"] == "map":
+        return None  # whole numbers only
+    s = prepare(case, seed)
+    return _exact_append(s) if case["op"] == "append" else _exact_attend(s)
