@@ -219,7 +219,7 @@ def prepare(case, seed):
     t = torch.from_numpy(table).to(dev)
     s["block_table"] = torch.where(t >= 0, order[t.clamp(min=0)], -1).to(torch.int32)
     if case["op"] == "map":
-        s["free_pages"] = torch.cat([order[at:], order[:at]])
+        s["free_pages"] = torch.cat([order[at:], order[:at], torch.tensor([n_pages - 1], **i32)])
         s["free_count"] = torch.tensor([n_pages - 1 - at], **i32)
         return s
     starts = np.concatenate([[0], np.cumsum(new)])
@@ -295,7 +295,7 @@ def _plain_map(s):
     p = torch.arange(s["max_pages"], device=n.device)[None, :]
     k = s["free_count"] - 1 - before[:, None] - (p - have[:, None])
     takes = (p >= have[:, None]) & (p < need[:, None])
-    table.copy_(torch.where(takes, s["free_pages"][k.clamp(0, s["n_pages"] - 2)], table))
+    table.copy_(torch.where(takes, s["free_pages"][k.clamp(0, s["n_pages"] - 1)], table))
     t = torch.arange(T, dtype=torch.int32, device=n.device)
     b = torch.searchsorted(start, t, right=True) - 1
     pos = c[b] + t - start[b]
