@@ -9,12 +9,14 @@ import argparse
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libaihost_attn.so"
+OBJ = PKG / "_build"  # one object file per source (ignored by git)
 SOURCES = ["api.cu", "rope_append.cu", "decode.cu", "prefill_sm100.cu", "noalloc.cu", "decode_mma.cu", "dist.cu",
            "matmul_sm100.cu"]
 HEADERS = ["common.cuh", "kernels.h", "rows.cuh"]
@@ -27,29 +29,46 @@ def nvcc_path() -> str:
     return "nvcc"
 
 
+def _deps(src: str) -> list[Path]:
+    return [CSRC / h for h in [src] + HEADERS] + [ROOT / "include" / "aihost_attn.h", Path(__file__)]
+
+
+def _stale(out: Path, deps: list[Path]) -> bool:
+    return not out.exists() or any(p.stat().st_mtime >= out.stat().st_mtime for p in deps)
+
+
 def needs_build() -> bool:
-    if not LIB.exists():
-        return True
-    mtime = LIB.stat().st_mtime
-    deps = [CSRC / s for s in SOURCES + HEADERS] + [ROOT / "include" / "aihost_attn.h", Path(__file__)]
-    return any(p.stat().st_mtime > mtime for p in deps)
+    return any(_stale(LIB, _deps(s)) for s in SOURCES)
 
 
-def build(force: bool = False, verbose: bool = False) -> Path:
-    if not force and not needs_build():
-        return LIB
-    cmd = [
-        nvcc_path(), "-O3", "-std=c++17", "-lineinfo",
-        "-gencode", "arch=compute_100a,code=sm_100a",
-        "-Xcompiler", "-fPIC", "-shared",
-        "-Xptxas", "-v" if verbose else "-O3",
-        "-o", str(LIB) + ".tmp",
-    ] + [str(CSRC / s) for s in SOURCES] + ["-ldl"]
+def _run(cmd: list[str], what: str, verbose: bool) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
     if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}) building {LIB.name}")
+        raise RuntimeError(f"nvcc failed ({res.returncode}) building {what}")
+
+
+def build(force: bool = False, verbose: bool = False) -> Path:
+    """Compile what changed, one object per source and all of them at once, then link."""
+    if not force and not needs_build():
+        return LIB
+    OBJ.mkdir(exist_ok=True)
+    common = [nvcc_path(), "-O3", "-std=c++17", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
+              "-Xcompiler", "-fPIC", "-Xptxas", "-v" if verbose else "-O3"]
+
+    def compile_one(src: str) -> None:
+        obj = OBJ / (src + ".o")
+        if not force and not _stale(obj, _deps(src)):
+            return
+        tmp = f"{obj}.{os.getpid()}.tmp.o"
+        _run(common + ["-c", "-o", tmp, str(CSRC / src)], src, verbose)
+        os.replace(tmp, obj)
+
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        list(pool.map(compile_one, SOURCES))
+    _run(common + ["-shared", "-o", str(LIB) + ".tmp"] + [str(OBJ / (s + ".o")) for s in SOURCES] + ["-ldl"], LIB.name,
+         verbose)
     os.replace(str(LIB) + ".tmp", LIB)
     return LIB
 
