@@ -30,9 +30,12 @@ EXPORTS = (
     "aihost_attn_decode_partial", "aihost_attn_merge_partials", "aihost_qk_norm_rope", "aihost_attn_forward_paged",
     "aihost_attn_noalloc_sync_status", "aihost_attn_dist_init_bounded", "aihost_attn_dist_sync",
     "aihost_matmul_workspace_size", "aihost_matmul_weights", "aihost_dequantize",
+    "aihost_page_map", "aihost_page_release", "aihost_kv8_append", "aihost_kv8_read", "aihost_kv8_workspace_size",
+    "aihost_kv8_attention",
 )
 # aihost_kernel ids of the device-time profiler
 KERNEL_APPEND, KERNEL_DECODE, KERNEL_COMBINE, KERNEL_PREFILL, KERNEL_CONVERT, KERNEL_MATMUL = range(6)
+KERNEL_PAGES, KERNEL_KV8_APPEND, KERNEL_KV8_ATTN = range(6, 9)
 
 
 class AttnDesc(ctypes.Structure):
@@ -44,6 +47,18 @@ class AttnDesc(ctypes.Structure):
         ("q_dtype", ctypes.c_int32), ("kv_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32),
         ("kv_capacity", ctypes.c_int32),
         ("kv_seq_stride", ctypes.c_int64), ("kv_token_stride", ctypes.c_int64), ("kv_head_stride", ctypes.c_int64),
+    ]
+
+
+class Kv8Desc(ctypes.Structure):
+    """aihost_kv8_desc."""
+
+    _fields_ = [
+        ("n_q_heads", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("page_rows", ctypes.c_int32), ("n_pages", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+        ("io_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("scale", ctypes.c_float),
+        ("score_cap", ctypes.c_float), ("rope_theta", ctypes.c_float), ("rope_mode", ctypes.c_int32),
+        ("q_token_stride", ctypes.c_int64), ("kv_token_stride", ctypes.c_int64),
     ]
 
 
@@ -95,6 +110,13 @@ def lib() -> ctypes.CDLL:
     L.aihost_attn_merge_partials.argtypes = [vp, i32, i32, i32, i32, vp, vp, vp, vp, vp]
     L.aihost_attn_forward_paged.argtypes = [vp, dp, i32, i32, vp, vp, vp, vp, vp, i32, i32, vp, i32, vp, vp, vp, vp]
     L.aihost_qk_norm_rope.argtypes = [vp, i32, i32, i32, i32, vp, ctypes.c_float, i32, ctypes.c_float, i32, vp]
+    k8 = ctypes.POINTER(Kv8Desc)
+    L.aihost_page_map.argtypes = [vp, i32, i32, i32, i32, i32] + [vp] * 11
+    L.aihost_page_release.argtypes = [vp, i32, i32, i32, i32] + [vp] * 6
+    L.aihost_kv8_append.argtypes = [vp, k8, i32] + [vp] * 9
+    L.aihost_kv8_read.argtypes = [vp, k8, i32, vp, vp, vp, vp, i32, vp]
+    L.aihost_kv8_workspace_size.argtypes = [k8, i32, i32, i32, i32, ctypes.POINTER(sz)]
+    L.aihost_kv8_attention.argtypes = [vp, k8, i32, i32, i32, i32] + [vp] * 13
     for name in EXPORTS:
         fn = getattr(L, name)
         if name not in ("aihost_attn_abi_version", "aihost_attn_last_error"):
@@ -110,5 +132,5 @@ def check(status: int) -> None:
         raise AttnError(status, msg.decode() if msg else "")
 
 
-__all__ = ["lib", "check", "AttnDesc", "AttnError", "F32", "F16", "Q8_0", "Q2_K", "Q3_K", "Q4_K", "Q5_K", "Q6_K", "ROPE_INTERLEAVED", "ROPE_NEOX",
+__all__ = ["lib", "check", "AttnDesc", "Kv8Desc", "AttnError", "F32", "F16", "Q8_0", "Q2_K", "Q3_K", "Q4_K", "Q5_K", "Q6_K", "ROPE_INTERLEAVED", "ROPE_NEOX",
            "ROPE_NONE", "EXPORTS", "LIB_PATH"]

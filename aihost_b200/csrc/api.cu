@@ -16,30 +16,10 @@
 
 #include "../../include/aihost_attn.h"
 #include "common.cuh"
+#include "ctx.h"
 #include "kernels.h"
 
 using namespace aihost;
-
-// Per-kernel-kind device-time accumulator (events recorded around each launch while enabled).
-struct ProfSlot {
-  std::vector<std::pair<cudaEvent_t, cudaEvent_t>> pending;
-  int64_t launches = 0;
-  double total_ms = 0.0;
-};
-
-struct aihost_attn_ctx {
-  int32_t device = 0;
-  int32_t num_sms = 148;
-  int32_t* d_status = nullptr;
-  void* scratch = nullptr;
-  size_t scratch_bytes = 0;
-  unsigned long long* counters = nullptr;  // fused split merge: epoch-tagged arrival counts
-  uint32_t epoch = 0;
-  bool profiling = false;
-  std::mutex prof_mu;
-  ProfSlot prof[AIHOST_KERNEL_COUNT];
-  std::vector<cudaEvent_t> event_pool;
-};
 
 namespace {
 thread_local char g_err[512] = "";
@@ -58,37 +38,11 @@ aihost_status api_fail(aihost_status st, const char* fmt, ...) {
 
 namespace {
 
-#define fail api_fail
-
-aihost_status cuda_fail(cudaError_t e, const char* what) {
-  return fail(AIHOST_ECUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
-}
-
-// Runs `f` with the context's device current and restores the caller's device afterwards.
-class DeviceGuard {
- public:
-  explicit DeviceGuard(int32_t dev) {
-    ok_ = cudaGetDevice(&prev_) == cudaSuccess;
-    if (ok_ && prev_ != dev) ok_ = cudaSetDevice(dev) == cudaSuccess;
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    if (cudaGetDevice(&cur) == cudaSuccess && cur != prev_) cudaSetDevice(prev_);
-  }
-  bool ok() const { return ok_; }
-
- private:
-  int prev_ = 0;
-  bool ok_ = false;
-};
-
 int64_t row_bytes(int32_t dtype, int32_t head_dim) {
   if (dtype == AIHOST_F32) return 4LL * head_dim;
   if (dtype == AIHOST_F16) return 2LL * head_dim;
   return 34LL * (head_dim / 32);
 }
-
-bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // Validates the static description; fills the resolved cache layout and scale.
 aihost_status check_desc(const aihost_attn_desc* d, KvLayout* kv, float* scale) {
@@ -125,14 +79,6 @@ aihost_status check_desc(const aihost_attn_desc* d, KvLayout* kv, float* scale) 
     return fail(AIHOST_EINVAL, "kv strides must be multiples of %lld bytes", static_cast<long long>(need_align));
   *scale = d->scale != 0.0f ? d->scale : 1.0f / sqrtf(static_cast<float>(d->head_dim));
   return AIHOST_OK;
-}
-
-RopeFreqs make_freqs(float theta, int32_t head_dim) {
-  RopeFreqs f;
-  memset(&f, 0, sizeof(f));
-  for (int i = 0; i < head_dim / 2 && i < kMaxHeadDim / 2; ++i)
-    f.f[i] = 1.0f / powf(theta, static_cast<float>(2 * i) / static_cast<float>(head_dim));
-  return f;
 }
 
 // Decode split plan: rows per split chosen from the capacity (so the scratch size is a
@@ -256,34 +202,6 @@ aihost_status encode_q8_map(CUtensorMap* map, const void* base, const KvLayout& 
 aihost_status check_ctx(aihost_attn_ctx* ctx) {
   if (!ctx) return fail(AIHOST_EINVAL, "ctx is NULL");
   return AIHOST_OK;
-}
-
-cudaEvent_t take_event(aihost_attn_ctx* ctx) {
-  if (!ctx->event_pool.empty()) {
-    cudaEvent_t e = ctx->event_pool.back();
-    ctx->event_pool.pop_back();
-    return e;
-  }
-  cudaEvent_t e = nullptr;
-  if (cudaEventCreate(&e) != cudaSuccess) return nullptr;
-  return e;
-}
-
-// Launch through `fn`, bracketed by timing events on `st` when the profiler is on.
-template <class F>
-cudaError_t timed_launch(aihost_attn_ctx* ctx, int kind, cudaStream_t st, F&& fn) {
-  if (!ctx->profiling) return fn();
-  std::lock_guard<std::mutex> lk(ctx->prof_mu);
-  cudaEvent_t a = take_event(ctx), b = take_event(ctx);
-  if (!a || !b) return cudaErrorMemoryAllocation;
-  cudaError_t e = cudaEventRecord(a, st);
-  if (e != cudaSuccess) return e;
-  e = fn();
-  if (e != cudaSuccess) return e;
-  e = cudaEventRecord(b, st);
-  if (e != cudaSuccess) return e;
-  ctx->prof[kind].pending.emplace_back(a, b);
-  return cudaSuccess;
 }
 
 // One-token attention over rows [0, start + len_offset). With k_new / v_new (forward decode) the
@@ -547,6 +465,8 @@ aihost_status aihost_attn_create(int32_t device, aihost_attn_ctx** out_ctx) {
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDeviceProperties");
   if (prop.major != 10) return fail(AIHOST_EUNSUPPORTED, "device %d is sm_%d%d; this build targets sm_100a", device,
                                     prop.major, prop.minor);
+  // the split-merge counters, and one more for the page map's blocks
+  constexpr size_t kCounterBytes = (kMaxSplitCounters + 1) * sizeof(unsigned long long);
   auto* ctx = new aihost_attn_ctx();
   ctx->device = device;
   ctx->num_sms = prop.multiProcessorCount;
@@ -556,8 +476,8 @@ aihost_status aihost_attn_create(int32_t device, aihost_attn_ctx** out_ctx) {
     return cuda_fail(e, "cudaMalloc(status)");
   }
   e = cudaMemset(ctx->d_status, 0, sizeof(int32_t));
-  if (e == cudaSuccess) e = cudaMalloc(&ctx->counters, kMaxSplitCounters * sizeof(unsigned long long));
-  if (e == cudaSuccess) e = cudaMemset(ctx->counters, 0, kMaxSplitCounters * sizeof(unsigned long long));
+  if (e == cudaSuccess) e = cudaMalloc(&ctx->counters, kCounterBytes);
+  if (e == cudaSuccess) e = cudaMemset(ctx->counters, 0, kCounterBytes);
   if (e != cudaSuccess) {
     cudaFree(ctx->counters);
     cudaFree(ctx->d_status);
@@ -1126,6 +1046,9 @@ aihost_status aihost_attn_sync_status(aihost_attn_ctx* ctx, int32_t* out_bits) {
   if (out_bits) *out_bits = bits;
   if (bits & kStatusWaitTimeout) return fail(AIHOST_ETIMEOUT, "a kernel's bounded wait expired (status 0x%x)", bits);
   if (bits & kStatusBadLength) return fail(AIHOST_EINVAL, "a device-side sequence length exceeded kv_capacity");
+  if (bits & kStatusBadIndex)
+    return fail(AIHOST_EINVAL, "a device-side page, slot, token count or length of the 8-bit cache was out of bounds");
+  if (bits & kStatusNoPages) return fail(AIHOST_ENOMEM, "a page map needed more pages than were free");
   return AIHOST_OK;
 }
 

@@ -18,6 +18,8 @@ namespace aihost {
 enum : int32_t {
   kStatusWaitTimeout = 1,   // a bounded mbarrier wait gave up
   kStatusBadLength = 2,     // a device-side length exceeded kv_capacity
+  kStatusNoPages = 4,       // a page map needed more pages than are free
+  kStatusBadIndex = 8,      // a device-side page, slot, token count or length of the 8-bit cache was out of bounds
 };
 
 // Iteration bound of every spin on an mbarrier. try_wait suspends the thread for a

@@ -1,0 +1,548 @@
+// kv8_attn.cu — attention of few query rows over the 8-bit paged cache (decode, short prompts).
+//
+// One block takes R = 8 or 16 query rows (tokens x heads of one KV head, so the cache is read once
+// for the whole head group), one KV head and a chunk of the cache rows; its four warps walk 16-row
+// steps of the chunk. Per step, with the transposed products that make cache rows the M = 16 of
+// mma.sync m16n8k16 and query rows its N = 8:
+//   S^T = K Q^T     K's int8 go to fp16 exactly in registers, one fp32 factor per page afterwards
+//   online softmax  running maximum per query row, moved only when it grows by more than 2^8
+//   O^T += V^T P^T  V likewise exact; P carries the page's scale relative to the chunk's largest
+// The k order of either product is free, so it is chosen such that every lane reads 16 bytes of a
+// cache row at a time straight from global memory: 8 lanes (V) or 4 lanes of two loads (K) cover a
+// 128-byte row, and no shared memory or transpose is needed. The next step's rows are in flight in
+// registers while a step is computed. Warps merge through shared memory, chunks through partials
+// that the last block to arrive merges (no block waits for another).
+#include "common.cuh"
+#include "kv8.h"
+#include "rows.cuh"
+
+namespace aihost {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kStep = 16;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -1e30f;
+
+// What the products take: fp16 operands, q as a pair of fp16 (rotated in fp32), or q and P as pairs
+// (fp32 tensors).
+enum { kPlain = 0, kPairQ = 1, kPairQP = 2 };
+
+// The maximum may lag by 2^kSlack before O is rescaled, and P enters times v scale / (the chunk's
+// largest v scale) * kVUnit, at most 2^15: inside fp16's range with as much as possible above its
+// smallest step. A pair's rest has that same smallest step, so pairs keep the maximum up to date and
+// use the whole range.
+template <int PREC>
+constexpr float kSlack = PREC == kPairQP ? 0.0f : 8.0f;
+template <int PREC>
+constexpr float kVUnit = PREC == kPairQP ? 32768.0f : 128.0f;
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t movmatrix_t(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Bytes 0,1 (sel 0x4140) or 2,3 (0x4342) of `u` as exact fp16 integers: u holds value + 128, the
+// byte becomes the mantissa of 1024 + u, and 1152 comes off again.
+__device__ __forceinline__ uint32_t half2_of(uint32_t u, uint32_t sel) {
+  const uint32_t h = __byte_perm(u, 0x64646464u, sel);
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// The rest of (lo, hi) after the fp16 pair `h`, in fp16.
+__device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t h) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return pack2(lo - f.x, hi - f.y);
+}
+
+// tanh x = 1 - 2 / (1 + e^2x): absolute error ~1e-7, which is what the capped score keeps.
+__device__ __forceinline__ float tanh_of(float x) {
+  const float e = ex2_approx(x * (2.0f * kLog2e));
+  return 1.0f - __fdividef(2.0f, 1.0f + e);
+}
+
+// Where a tile of query rows lies. Tiles of sequence b start at floor(row_start[b] * G / R) + b:
+// room for every tile whatever the lengths, so the grid needs only host-known bounds and each
+// block finds its sequence by itself. (One tile per sequence where max_new * G <= R.)
+struct Tile {
+  int32_t b, n_new, start, row0, kv_len, pos0;  // pos0: cache row of the sequence's first new token
+  bool ok;
+};
+
+__device__ __forceinline__ Tile find_tile(const Kv8AttnArgs& a, int64_t tile, int32_t G, int32_t R, int lane) {
+  Tile t;
+  t.ok = false;
+  t.row0 = 0;
+  if (static_cast<int64_t>(a.max_new) * G <= R) {
+    t.b = static_cast<int32_t>(tile);
+  } else {
+    int32_t lo = 0, n = a.batch;
+    while (n > 1) {  // 32 candidates at a time
+      const int32_t step = (n + 31) / 32, i = lo + lane * step;
+      const bool at = i < lo + n && static_cast<int64_t>(a.row_start[i]) * G / R + i <= tile;
+      const int32_t c = __popc(__ballot_sync(0xffffffffu, at));
+      const int32_t skip = (c > 0 ? c - 1 : 0) * step;
+      lo += skip;
+      n = min(step, n - skip);
+    }
+    t.b = lo;
+  }
+  t.start = a.row_start[t.b];
+  t.n_new = a.row_start[t.b + 1] - t.start;
+  t.kv_len = a.kv_len[t.b];
+  if (static_cast<int64_t>(a.max_new) * G > R) {
+    const int64_t k = tile - (static_cast<int64_t>(t.start) * G / R + t.b);
+    if (k < 0 || k * R >= static_cast<int64_t>(t.n_new) * G) {
+      if (t.n_new > 0 || t.start < 0 || t.n_new < 0) t.ok = false;
+      return t;
+    }
+    t.row0 = static_cast<int32_t>(k * R);
+  }
+  t.pos0 = t.kv_len - t.n_new;
+  t.ok = t.n_new > 0;
+  if (t.n_new < 0 || t.start < 0 || static_cast<int64_t>(t.start) + t.n_new > a.n_tokens || t.n_new > a.max_new ||
+      t.pos0 < 0 || t.kv_len > a.max_kv || t.kv_len > static_cast<int64_t>(a.g.max_pages) << a.g.page_shift) {
+    t.ok = false;
+    atomicOr(a.status, kStatusBadIndex);
+  }
+  return t;
+}
+
+template <int D, int NT, int PREC, bool MOD>
+__global__ void __launch_bounds__(kWarps * 32) kv8_mma_kernel(const __grid_constant__ Kv8AttnArgs a) {
+  constexpr int R = NT * 8;
+  constexpr int KS = D / 16;       // k steps of S^T = K Q^T
+  constexpr int KC = D / 64;       // 16-byte chunks of a K row per lane
+  constexpr int MT = D / 16;       // 16-row tiles of O^T
+  constexpr int VW = D / 32;       // 32-bit words of a V row per lane
+  constexpr int NQ = PREC == kPlain ? 1 : 2;
+  __shared__ float o_sh[kWarps][R][D + 4];
+  __shared__ float ml_sh[kWarps][R][2];
+  __shared__ float vmax_sh[kWarps];
+  __shared__ int32_t last_sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+  const int32_t H = a.g.n_kv_heads, G = a.g.n_q_heads / H, ps = a.g.page_shift;
+  const int32_t h = static_cast<int32_t>(blockIdx.x % H);
+  const int64_t tile = blockIdx.x / H;
+  const int32_t split = static_cast<int32_t>(blockIdx.y);
+  const Tile tl = find_tile(a, tile, G, R, lane);
+  if (!tl.ok) return;
+  const int32_t n_rows = min(R, tl.n_new * G - tl.row0);
+
+  // ---- which cache rows each query row sees; this lane's two columns per N tile, and the tile's range
+  auto range_of = [&](int r, int32_t& first, int32_t& end, int32_t& pos) {
+    const int32_t row = tl.row0 + min(r, n_rows - 1), i = row / G;
+    pos = tl.pos0 + i;
+    end = pos + 1;
+    if (a.prefix_len) end = max(end, min(a.prefix_len[tl.b], tl.kv_len));
+    first = a.row_first ? max(a.row_first[tl.start + i], 0) : 0;
+  };
+  int32_t c_first[NT][2], c_end[NT][2];
+  float c_pos[NT][2], c_slope[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int r = nt * 8 + 2 * t4 + c;
+      int32_t pos;
+      range_of(r, c_first[nt][c], c_end[nt][c], pos);
+      c_pos[nt][c] = static_cast<float>(pos);
+      c_slope[nt][c] =
+          MOD && a.alibi_slopes ? a.alibi_slopes[h * G + (tl.row0 + min(r, n_rows - 1)) % G] * kLog2e : 0.0f;
+    }
+  int32_t lo, hi, lo_max, hi_min;
+  {
+    int32_t first, end, pos;
+    range_of(lane & (R - 1), first, end, pos);
+    lo = __reduce_min_sync(0xffffffffu, first);
+    lo_max = __reduce_max_sync(0xffffffffu, first);
+    hi = __reduce_max_sync(0xffffffffu, end);
+    hi_min = __reduce_min_sync(0xffffffffu, end);
+  }
+  const int32_t base = min(lo, hi) & ~(kStep - 1);
+  const int32_t n_splits = max(1, (hi - base + a.chunk - 1) / a.chunk);
+  if (split >= n_splits) return;
+  const int32_t k_begin = base + split * a.chunk, k_end = min(hi, k_begin + a.chunk);
+  const int32_t* const table = a.block_table + static_cast<int64_t>(tl.b) * a.g.max_pages;
+  // a page id outside the pool reads page 0 and sets the status
+  bool stray = false;
+  auto page_at = [&](int32_t row) -> int64_t {
+    const int32_t p = table[row >> ps];
+    if (p < 0 || p >= a.g.n_pages) {
+      stray = true;
+      return 0;
+    }
+    return p;
+  };
+
+  // ---- the step's rows, one step ahead
+  uint4 kb[2][KC];
+  uint32_t vb[4][VW];
+  float ks_next = 0.0f, vs_next = 0.0f;
+  auto fetch = [&](int32_t k, int64_t page) {
+    const int64_t ph = page * H + h;
+    const int64_t at = ((ph << ps) + (k & (a.g.page_rows - 1))) * D;
+    const int8_t* kp = a.k_pool + at + (g * D + t4 * (KC * 16));
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) kb[r][c] = __ldg(reinterpret_cast<const uint4*>(kp + r * 8 * D + c * 16));
+    const int8_t* vp = a.v_pool + at + (2 * t4 * D + g * (VW * 4));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int8_t* p = vp + ((r & 1) + (r >> 1) * 8) * D;
+      if constexpr (VW == 4) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+        vb[r][0] = v.x, vb[r][1] = v.y, vb[r][2] = v.z, vb[r][3] = v.w;
+      } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        vb[r][0] = v.x, vb[r][1] = v.y;
+      }
+    }
+    ks_next = __ldg(a.k_scale + ph);
+    vs_next = __ldg(a.v_scale + ph);
+  };
+  const int32_t k0 = k_begin + warp * kStep;
+  int64_t page = 0;
+  if (k0 < k_end) fetch(k0, page_at(k0));
+  if (k0 + kWarps * kStep < k_end) page = page_at(k0 + kWarps * kStep);
+
+  // ---- the chunk's largest V scale: P is scaled relative to it (a NaN scale is passed over here and
+  // reaches the result through its own page's factor)
+  float vmax = 0.0f;
+  for (int32_t k = (k_begin >> ps) + static_cast<int32_t>(threadIdx.x); k < (k_end + a.g.page_rows - 1) >> ps;
+       k += kWarps * 32)
+    vmax = fmaxf(vmax, __ldg(a.v_scale + page_at(k << ps) * H + h));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+  if (lane == 0) vmax_sh[warp] = vmax;
+  __syncthreads();
+  vmax = fmaxf(fmaxf(vmax_sh[0], vmax_sh[1]), fmaxf(vmax_sh[2], vmax_sh[3]));
+  const float v_unit = vmax > 0.0f ? kVUnit<PREC> / vmax : 0.0f;
+
+  // ---- query rows as B fragments: lane (g, t4) holds row g's elements [t4 * D/4, (t4 + 1) * D/4)
+  uint32_t qf[NQ][NT][KS][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    constexpr int E = D / 4;
+    float x[E];
+    const int r = nt * 8 + g;
+    const int32_t row = tl.row0 + min(r, n_rows - 1), i = row / G;
+    const uint8_t* src = static_cast<const uint8_t*>(a.q) + (tl.start + static_cast<int64_t>(i)) * a.q_token_stride;
+    const int64_t el = static_cast<int64_t>(h * G + row % G) * D + t4 * E;
+    if (a.q_dtype == AIHOST_F16) {
+      const uint4* p = reinterpret_cast<const uint4*>(src + el * 2);
+#pragma unroll
+      for (int k = 0; k < E / 8; ++k) {
+        const uint4 v = p[k];
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[m]));
+          x[8 * k + 2 * m] = f.x, x[8 * k + 2 * m + 1] = f.y;
+        }
+      }
+    } else {
+      const float4* p = reinterpret_cast<const float4*>(src + el * 4);
+#pragma unroll
+      for (int k = 0; k < E / 4; ++k) {
+        const float4 v = p[k];
+        x[4 * k] = v.x, x[4 * k + 1] = v.y, x[4 * k + 2] = v.z, x[4 * k + 3] = v.w;
+      }
+    }
+    if (PREC != kPlain && a.rope_mode != AIHOST_ROPE_NONE) {
+      const float pos = static_cast<float>(tl.pos0 + i);
+      if (a.rope_mode == AIHOST_ROPE_INTERLEAVED) {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          float sn, cs;
+          sincosf(__fmul_rn(pos, a.freqs.f[(t4 * E + e) >> 1]), &sn, &cs);
+          rotate_pair(x[e], x[e + 1], cs, sn);
+        }
+      } else {  // pairs D/2 apart: lanes t4 and t4 ^ 2
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float other = __shfl_xor_sync(0xffffffffu, x[e], 2);
+          float sn, cs;
+          sincosf(__fmul_rn(pos, a.freqs.f[(t4 & 1) * E + e]), &sn, &cs);
+          float x1 = t4 < 2 ? x[e] : other, x2 = t4 < 2 ? other : x[e];
+          rotate_pair(x1, x2, cs, sn);
+          x[e] = t4 < 2 ? x1 : x2;
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      qf[0][nt][k][0] = pack2(x[4 * k], x[4 * k + 1]);
+      qf[0][nt][k][1] = pack2(x[4 * k + 2], x[4 * k + 3]);
+      if constexpr (NQ == 2) {
+        qf[1][nt][k][0] = pack2_rest(x[4 * k], x[4 * k + 1], qf[0][nt][k][0]);
+        qf[1][nt][k][1] = pack2_rest(x[4 * k + 2], x[4 * k + 3], qf[0][nt][k][1]);
+      }
+    }
+  }
+
+  float o[MT][NT][4];
+  float m[NT][2], l[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt][0] = m[nt][1] = kNoMax;
+    l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
+  }
+  const bool capped = MOD && a.score_cap > 0.0f;
+  const float s_unit = capped ? a.scale / a.score_cap : a.scale * kLog2e;
+  const float cap2 = a.score_cap * kLog2e;
+
+  for (int32_t k = k0; k < k_end; k += kWarps * kStep) {
+    // ---- S^T = K Q^T (this step's K leaves its registers here)
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const uint32_t w0[4] = {kb[0][c].x, kb[0][c].y, kb[0][c].z, kb[0][c].w};
+      const uint32_t w1[4] = {kb[1][c].x, kb[1][c].y, kb[1][c].z, kb[1][c].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t u0 = w0[j] ^ 0x80808080u, u1 = w1[j] ^ 0x80808080u;
+        const uint32_t a0 = half2_of(u0, 0x4140), a1 = half2_of(u1, 0x4140);
+        const uint32_t a2 = half2_of(u0, 0x4342), a3 = half2_of(u1, 0x4342);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) mma16816(s[nt], a0, a1, a2, a3, qf[n][nt][4 * c + j][0], qf[n][nt][4 * c + j][1]);
+      }
+    }
+    const float kf = ks_next * s_unit, vf = vs_next * v_unit;
+    uint32_t vw[4][VW];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int w = 0; w < VW; ++w) vw[r][w] = vb[r][w] ^ 0x80808080u;
+    // ---- the next step's rows
+    const int32_t k_next = k + kWarps * kStep;
+    if (k_next < k_end) {
+      fetch(k_next, page);
+      if (k_next + kWarps * kStep < k_end) page = page_at(k_next + kWarps * kStep);
+    }
+    // ---- scores (log2 units), masks, running maximum
+    const bool edge = k < lo_max || k + kStep > hi_min;
+    bool grow = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int32_t row = k + g + (e >> 1) * 8;
+        float v = s[nt][e] * kf;
+        if constexpr (MOD) {
+          if (capped) v = cap2 * tanh_of(v);
+          if (a.alibi_slopes) v -= c_slope[nt][e & 1] * fabsf(c_pos[nt][e & 1] - static_cast<float>(row));
+        }
+        if (edge && (row < c_first[nt][e & 1] || row >= c_end[nt][e & 1])) v = -INFINITY;
+        s[nt][e] = v;
+        grow |= v > m[nt][e & 1] + kSlack<PREC>;
+      }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float mx = fmaxf(s[nt][c], s[nt][c + 2]);
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          const float m_new = fmaxf(m[nt][c], mx), f = ex2_approx(m[nt][c] - m_new);
+          m[nt][c] = m_new;
+          l[nt][c] *= f;
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            o[i][nt][c] *= f;
+            o[i][nt][c + 2] *= f;
+          }
+        }
+    }
+    // ---- P and its fragments
+    uint32_t pf[PREC == kPairQP ? 2 : 1][NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        p[e] = ex2_approx(s[nt][e] - m[nt][e & 1]);
+        l[nt][e & 1] += p[e];
+        // a hidden row adds nothing even where its page's scale is NaN
+        p[e] = edge && s[nt][e] == -INFINITY ? 0.0f : p[e] * vf;
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t hi2 = pack2(p[2 * c], p[2 * c + 1]);
+        pf[0][nt][c] = movmatrix_t(hi2);
+        if constexpr (PREC == kPairQP) pf[1][nt][c] = movmatrix_t(pack2_rest(p[2 * c], p[2 * c + 1], hi2));
+      }
+    }
+    // ---- O^T += V^T P^T
+#pragma unroll
+    for (int w = 0; w < VW; ++w) {
+      const uint32_t x0 = __byte_perm(vw[0][w], vw[1][w], 0x5140), x1 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
+      const uint32_t y0 = __byte_perm(vw[2][w], vw[3][w], 0x5140), y1 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t x = i ? x1 : x0, y = i ? y1 : y0;
+        const uint32_t a0 = half2_of(x, 0x4140), a1 = half2_of(x, 0x4342);
+        const uint32_t a2 = half2_of(y, 0x4140), a3 = half2_of(y, 0x4342);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816(o[2 * w + i][nt], a0, a1, a2, a3, pf[0][nt][0], pf[0][nt][1]);
+          if constexpr (PREC == kPairQP) mma16816(o[2 * w + i][nt], a0, a1, a2, a3, pf[1][nt][0], pf[1][nt][1]);
+        }
+      }
+    }
+  }
+  if (stray) atomicOr(a.status, kStatusBadIndex);
+
+  // ---- merge the four warps: lane (g, t4) holds elements [g * D/8, (g + 1) * D/8) of rows 2 t4 and 2 t4 + 1
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], d);
+      const int r = nt * 8 + 2 * t4 + c;
+      if (g == 0) ml_sh[warp][r][0] = m[nt][c], ml_sh[warp][r][1] = l[nt][c];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        o_sh[warp][r][g * (D / 8) + 2 * i] = o[i][nt][c];
+        o_sh[warp][r][g * (D / 8) + 2 * i + 1] = o[i][nt][c + 2];
+      }
+    }
+  __syncthreads();
+  const float o_unit = vmax * (1.0f / kVUnit<PREC>);
+  auto store = [&](int r, int d, float v0, float v1) {
+    const int32_t row = tl.row0 + r;
+    const int64_t at = ((tl.start + static_cast<int64_t>(row / G)) * a.g.n_q_heads + h * G + row % G) * D + d;
+    if (a.out_dtype == AIHOST_F16)
+      *reinterpret_cast<__half2*>(static_cast<__half*>(a.out) + at) = __floats2half2_rn(v0, v1);
+    else
+      *reinterpret_cast<float2*>(static_cast<float*>(a.out) + at) = make_float2(v0, v1);
+  };
+  const int64_t unit = static_cast<int64_t>(blockIdx.x);
+  for (int i = threadIdx.x; i < n_rows * (D / 2); i += kWarps * 32) {
+    const int r = i / (D / 2), d = i % (D / 2) * 2;
+    float mm = kNoMax;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, ml_sh[w][r][0]);
+    float ll = 0.0f, v0 = 0.0f, v1 = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = ex2_approx(ml_sh[w][r][0] - mm);
+      ll += ml_sh[w][r][1] * f;
+      v0 += o_sh[w][r][d] * f;
+      v1 += o_sh[w][r][d + 1] * f;
+    }
+    if (n_splits == 1) {
+      const float inv = ll != 0.0f ? o_unit / ll : 0.0f;  // NaN stays NaN
+      store(r, d, v0 * inv, v1 * inv);
+    } else {
+      const int64_t at = (unit * a.max_splits + split) * R + r;
+      *reinterpret_cast<float2*>(a.part_o + at * D + d) = make_float2(v0 * o_unit, v1 * o_unit);
+      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(mm, ll);
+    }
+  }
+  if (n_splits == 1) return;
+
+  // ---- merge the chunks: the last block of this tile and head to arrive
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last_sh = split_arrive(a.counters + unit, a.epoch, n_splits, a.status);
+  __syncthreads();
+  if (!last_sh) return;
+  __threadfence();
+  if (threadIdx.x == 0) a.counters[unit] = 0;  // a replayed launch counts from zero again
+  for (int i = threadIdx.x; i < n_rows * (D / 2); i += kWarps * 32) {
+    const int r = i / (D / 2), d = i % (D / 2) * 2;
+    const int64_t at = unit * a.max_splits * R + r;
+    float mm = kNoMax;
+    for (int sp = 0; sp < n_splits; ++sp) mm = fmaxf(mm, __ldcg(a.part_ml + (at + static_cast<int64_t>(sp) * R) * 2));
+    float ll = 0.0f, v0 = 0.0f, v1 = 0.0f;
+    for (int sp = 0; sp < n_splits; ++sp) {
+      const int64_t p = at + static_cast<int64_t>(sp) * R;
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml + p * 2));
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(a.part_o + p * D + d));
+      const float f = ex2_approx(ml.x - mm);
+      ll += ml.y * f;
+      v0 += v.x * f;
+      v1 += v.y * f;
+    }
+    const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+    store(r, d, v0 * inv, v1 * inv);
+  }
+}
+
+template <int D, int NT, int PREC>
+cudaError_t launch_mod(const Kv8AttnArgs& a, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(a.tiles) * a.g.n_kv_heads, a.max_splits);
+  if (a.score_cap > 0.0f || a.alibi_slopes) kv8_mma_kernel<D, NT, PREC, true><<<grid, kWarps * 32, 0, st>>>(a);
+  else kv8_mma_kernel<D, NT, PREC, false><<<grid, kWarps * 32, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <int D, int NT>
+cudaError_t launch_prec(const Kv8AttnArgs& a, cudaStream_t st) {
+  if (a.q_dtype == AIHOST_F32) return launch_mod<D, NT, kPairQP>(a, st);
+  if (a.rope_mode != AIHOST_ROPE_NONE) return launch_mod<D, NT, kPairQ>(a, st);
+  return launch_mod<D, NT, kPlain>(a, st);
+}
+
+}  // namespace
+
+int32_t kv8_mma_rows(const Kv8Geom& g, int32_t max_new) {
+  return static_cast<int64_t>(max_new) * (g.n_q_heads / g.n_kv_heads) <= 8 ? 8 : 16;
+}
+
+void kv8_mma_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max_new, int32_t max_kv, int32_t num_sms,
+                  int32_t* tiles, int32_t* chunk, int32_t* splits) {
+  const int32_t R = kv8_mma_rows(g, max_new), G = g.n_q_heads / g.n_kv_heads;
+  const int64_t n = static_cast<int64_t>(max_new) * G <= R ? batch : static_cast<int64_t>(n_tokens) * G / R + batch;
+  const int64_t units = n * g.n_kv_heads;
+  // enough blocks for four on every SM, chunks of 256 to 2048 rows
+  int64_t want = (4LL * num_sms + units - 1) / units;
+  int64_t c = (max_kv + want - 1) / want;
+  c = (c + 63) / 64 * 64;
+  if (c < 256) c = 256;
+  if (c > 2048) c = 2048;
+  int64_t s = (max_kv + kStep + c - 1) / c;  // a tile's range may start up to 15 rows before its first row
+  if (units > kMaxSplitCounters || s > 65535) {
+    c = (static_cast<int64_t>(max_kv) + kStep + 63) / 64 * 64;
+    s = 1;
+  }
+  *tiles = static_cast<int32_t>(n);
+  *chunk = static_cast<int32_t>(c);
+  *splits = static_cast<int32_t>(s);
+}
+
+size_t kv8_mma_scratch_bytes(const Kv8Geom& g, int32_t tiles, int32_t rows, int32_t splits) {
+  return splits <= 1 ? 0 : static_cast<size_t>(tiles) * g.n_kv_heads * splits * rows * (g.head_dim + 2) * sizeof(float);
+}
+
+cudaError_t launch_kv8_mma(const Kv8AttnArgs& a, cudaStream_t st) {
+  const bool eight = kv8_mma_rows(a.g, a.max_new) == 8;
+  if (a.g.head_dim == 64) return eight ? launch_prec<64, 1>(a, st) : launch_prec<64, 2>(a, st);
+  return eight ? launch_prec<128, 1>(a, st) : launch_prec<128, 2>(a, st);
+}
+
+}  // namespace aihost

@@ -179,7 +179,10 @@ typedef enum {
   AIHOST_KERNEL_PREFILL = 3,  /* tcgen05 prefill */
   AIHOST_KERNEL_CONVERT = 4,  /* fp16 staging of fp32 / Q8_0 prefill operands, weight dequantisation */
   AIHOST_KERNEL_MATMUL = 5,   /* tcgen05 weight product (aihost_matmul_weights) */
-  AIHOST_KERNEL_COUNT = 6
+  AIHOST_KERNEL_PAGES = 6,    /* page maps and releases */
+  AIHOST_KERNEL_KV8_APPEND = 7, /* append to and read from the 8-bit cache */
+  AIHOST_KERNEL_KV8_ATTN = 8, /* attention over the 8-bit cache */
+  AIHOST_KERNEL_COUNT = 9
 } aihost_kernel;
 aihost_status aihost_attn_profiler_enable(aihost_attn_ctx* ctx, int32_t enable);
 aihost_status aihost_attn_profiler_read(aihost_attn_ctx* ctx, int32_t kernel, int64_t* launches, double* total_ms);
@@ -304,9 +307,97 @@ aihost_status aihost_matmul_weights(aihost_attn_ctx* ctx, const aihost_matmul_de
 aihost_status aihost_dequantize(const void* w, int32_t w_dtype, int64_t n_elems, void* out, int32_t out_dtype,
                                 void* stream);
 
+/* ---- The 8-bit paged cache: int8 values with one fp32 scale for each page and KV head, the page
+ * bookkeeping of a serving step done on the GPU, and attention that reads the cache as stored.
+ * It replaces the unwired QuantizedKVCache (Inference/QuantizedKVCache.cs:46-133) and, like
+ * aihost_attn_forward_paged, KVCache.Add's per-token Concat (InferenceEngine.cs:598-622).
+ *
+ *   k_pool, v_pool    int8 [n_pages][n_kv_heads][page_rows][head_dim]  (a page's rows of one head lie together)
+ *   k_scale, v_scale  fp32 [n_pages][n_kv_heads]; a stored value stands for int8 * scale
+ *   block_table       int32 [batch][max_pages]: row t of sequence b is row t % page_rows of page
+ *                     block_table[b][t / page_rows]
+ * A step's new rows of all sequences lie one after another ("tokens"): rows row_start[b] ..
+ * row_start[b + 1] of q, k_new, v_new and out belong to sequence b, any number of them, none
+ * included. All arrays below are device memory. Lengths stay on the device; the host passes upper
+ * bounds. A page id, slot or length outside its bounds is not followed: the row is skipped and a
+ * status bit set (aihost_attn_sync_status then returns AIHOST_EINVAL). */
+typedef struct {
+  int32_t n_q_heads, n_kv_heads; /* Hq % Hkv == 0 */
+  int32_t head_dim;              /* 64 or 128 */
+  int32_t page_rows;             /* 16, 32, 64 or 128 */
+  int32_t n_pages;               /* pages in the pools */
+  int32_t max_pages;             /* row length of block_table */
+  int32_t io_dtype;              /* q, k_new, v_new: F32 or F16 */
+  int32_t out_dtype;             /* F32 or F16 */
+  float scale;                   /* 0 -> 1/sqrtf(head_dim) */
+  float score_cap;               /* > 0: scores become cap * tanh(score / cap); 0: as they are */
+  float rope_theta;              /* as in aihost_attn_desc; K is rotated when it is appended, q when it is read */
+  int32_t rope_mode;
+  int64_t q_token_stride;        /* bytes between tokens of q;            0 -> n_q_heads rows, packed */
+  int64_t kv_token_stride;       /* bytes between tokens of k_new, v_new; 0 -> n_kv_heads rows, packed */
+} aihost_kv8_desc;
+
+/* One step's page bookkeeping in one launch: sequence b has seq_len[b] cached rows and gets
+ * n_new[b] >= 0 more. Pages that the new rows need are taken from the top of the stack free_pages
+ * (int32 [n_pages], its first *free_count entries are free), sequence by sequence, and entered in
+ * block_table. Written besides: kv_len[b] = seq_len[b] + n_new[b]; row_start [batch + 1], the
+ * running sum of n_new; for every token (row_start order) slots = page * page_rows + row (int64)
+ * and positions = its row in its sequence; *free_count_out. Entries of slots and positions past the
+ * last token, up to max_tokens, become -1 and 0, so a captured step can have spare tokens.
+ * kv_len may be seq_len itself, and free_count_out free_count. A step that cannot be taken whole
+ * is refused whole: too few free pages (AIHOST_ENOMEM from aihost_attn_sync_status), or a negative
+ * count, more than max_tokens tokens, or a sequence beyond max_pages pages (AIHOST_EINVAL): then
+ * nothing is taken, kv_len = seq_len, row_start is 0 and every slot -1. batch <= 8192. */
+aihost_status aihost_page_map(aihost_attn_ctx* ctx, int32_t batch, int32_t page_rows, int32_t n_pages, int32_t max_pages,
+                              int32_t max_tokens, const int32_t* seq_len, const int32_t* n_new,
+                              const int32_t* free_pages, const int32_t* free_count, int32_t* block_table,
+                              int32_t* kv_len, int32_t* row_start, int64_t* slots, int32_t* positions,
+                              int32_t* free_count_out, void* stream);
+/* Ends the sequences with done[b] != 0: their pages go back on the stack (sequence by sequence, in
+ * table order), their table rows become -1 and seq_len[b] 0. free_count is updated in place. */
+aihost_status aihost_page_release(aihost_attn_ctx* ctx, int32_t batch, int32_t page_rows, int32_t n_pages,
+                                  int32_t max_pages, const int32_t* done, int32_t* seq_len, int32_t* block_table,
+                                  int32_t* free_pages, int32_t* free_count, void* stream);
+
+/* Stores n_tokens rows k_new, v_new [n_tokens][Hkv][d] at slots (-1: skipped), K rotated at
+ * positions first. Tokens of one page have to be consecutive and in row order, as aihost_page_map
+ * gives them. For each page and head (K and V apart): had = the stored scale, or 0 if the page's
+ * row 0 is among the new rows; scale = max(had, amax(new rows) * fl32(1/127)); the page's older
+ * rows become rint(value * (had / scale)) where the scale grew, the new ones
+ * rint(x * (1 / scale)). A NaN or infinity among a page's new rows makes its scale NaN, until the
+ * page is begun anew. */
+aihost_status aihost_kv8_append(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t n_tokens, const void* k_new,
+                                const void* v_new, const int64_t* slots, const int32_t* positions, int8_t* k_pool,
+                                int8_t* v_pool, float* k_scale, float* v_scale, void* stream);
+/* out [n_rows][Hkv][d] (out_dtype: F32 or F16) = the values that the rows at slots of one pool stand
+ * for; zeros for slot -1. */
+aihost_status aihost_kv8_read(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t n_rows, const int64_t* slots,
+                              const int8_t* pool, const float* scale, void* out, int32_t out_dtype, void* stream);
+
+/* Scratch bytes of an aihost_kv8_attention call with these arguments (0 if none). */
+aihost_status aihost_kv8_workspace_size(const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens, int32_t max_new,
+                                        int32_t max_kv, size_t* out_bytes);
+/* Attention of q [n_tokens][Hq][d] over the cache, into out [n_tokens][Hq][d] (packed). Sequence b has
+ * kv_len[b] cached rows, its new ones (already appended) included; its query row i sits at position
+ * p = kv_len[b] - (row_start[b + 1] - row_start[b]) + i and sees the cache rows j with
+ *   row_first[token] <= j < max(p + 1, min(prefix_len[b], kv_len[b])):
+ * causal, but for a prefix that all rows of the sequence see (prefix_len, int32 [batch], or NULL),
+ * and from the start of its own document on (row_first, int32 [n_tokens], or NULL: 0). A row that
+ * sees nothing gets zeros. score = scale * q.k, capped if score_cap > 0, then minus
+ * alibi_slopes[head] * |p - j| (fp32 [Hq], or NULL). No sequence may have more than max_new new
+ * rows or max_kv cached ones. Softmax state and sums are fp32. Precision of the products: with F16 q,
+ * q (after its rotation) and the softmax weights enter as fp16; with F32 q as pairs of fp16, whose
+ * sum holds 22 bits. int8 values enter exactly. */
+aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens,
+                                   int32_t max_new, int32_t max_kv, const void* q, const int32_t* row_start,
+                                   const int32_t* kv_len, const int32_t* block_table, const int8_t* k_pool,
+                                   const int8_t* v_pool, const float* k_scale, const float* v_scale,
+                                   const int32_t* prefix_len, const int32_t* row_first, const float* alibi_slopes,
+                                   void* out, void* stream);
+
 /* Synchronise the context's device and read-and-clear the device status word that kernels
- * set when a bounded wait expired (AIHOST_ETIMEOUT) or a device-side length exceeded
- * kv_capacity (AIHOST_EINVAL). *out_bits receives the raw bits (may be NULL). */
+ * set when a bounded wait expired (AIHOST_ETIMEOUT), a device-side length exceeded kv_capacity or
+ * another bound (AIHOST_EINVAL), or aihost_page_map ran out of free pages (AIHOST_ENOMEM). *out_bits receives the raw bits (may be NULL). */
 aihost_status aihost_attn_sync_status(aihost_attn_ctx* ctx, int32_t* out_bits);
 
 #ifdef __cplusplus
