@@ -18,7 +18,8 @@ CSRC = PKG / "csrc"
 LIB = PKG / "libaihost_attn.so"
 OBJ = PKG / "_build"  # one object file per source (ignored by git)
 SOURCES = ["api.cu", "rope_append.cu", "decode.cu", "prefill_sm100.cu", "noalloc.cu", "decode_mma.cu", "dist.cu",
-           "matmul_sm100.cu", "kv8_api.cu", "kv8_pages.cu", "kv8_append.cu", "kv8_attn.cu"]
+           "matmul_sm100.cu", "kv8_api.cu", "kv8_pages.cu", "kv8_append.cu", "kv8_attn.cu",
+           "kv8_prefill_sm100.cu"]
 HEADERS = ["common.cuh", "ctx.h", "kernels.h", "rows.cuh"]
 
 
@@ -30,7 +31,7 @@ def nvcc_path() -> str:
 
 
 def _deps(src: str) -> list[Path]:
-    own = ["kv8.h"] if src.startswith("kv8_") else []
+    own = ["kv8.h", "kv8_tile.cuh"] if src.startswith("kv8_") else []
     return [CSRC / h for h in [src] + HEADERS + own] + [ROOT / "include" / "aihost_attn.h", Path(__file__)]
 
 

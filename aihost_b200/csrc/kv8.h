@@ -103,11 +103,18 @@ cudaError_t launch_page_release(const PageReleaseArgs& a, cudaStream_t st);
 cudaError_t launch_kv8_append(const Kv8AppendArgs& a, cudaStream_t st);
 cudaError_t launch_kv8_read(const Kv8ReadArgs& a, cudaStream_t st);
 
-// The split-cache kernel's query rows per tile (8 or 16) and its plan over the cache rows.
+// The split-cache kernel (mma.sync, query rows per tile 8 or 16) and its plan over the cache rows:
+// tiles of query rows, cache rows per chunk, chunks of the longest range.
 int32_t kv8_mma_rows(const Kv8Geom& g, int32_t max_new);
 void kv8_mma_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max_new, int32_t max_kv, int32_t num_sms,
                   int32_t* tiles, int32_t* chunk, int32_t* splits);
-size_t kv8_mma_scratch_bytes(const Kv8Geom& g, int32_t tiles, int32_t rows, int32_t splits);
 cudaError_t launch_kv8_mma(const Kv8AttnArgs& a, cudaStream_t st);
+
+// The tcgen05 kernel (query rows per block 256), for this many query rows of a sequence's KV head on.
+constexpr int32_t kKv8TensorMinRows = 64;
+int32_t kv8_prefill_rows();
+void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max_new, int32_t max_kv, int32_t num_sms,
+                      int32_t* tiles, int32_t* chunk, int32_t* splits);
+cudaError_t launch_kv8_prefill(const Kv8AttnArgs& a, cudaStream_t st);
 
 }  // namespace aihost

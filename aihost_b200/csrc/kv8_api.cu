@@ -73,6 +73,30 @@ aihost_status check_pages(const aihost_attn_ctx* ctx, int32_t batch, int32_t pag
   return AIHOST_OK;
 }
 
+// Which kernel an attention call runs, and its plan over the cache rows.
+struct Plan {
+  bool tensor;  // the tcgen05 kernel (many query rows a sequence, fp16), else the split-cache one
+  int32_t rows, tiles, chunk, splits;
+  size_t scratch(const Kv8Geom& g) const {
+    return splits <= 1 ? 0 : static_cast<size_t>(tiles) * g.n_kv_heads * splits * rows * (g.head_dim + 2) * sizeof(float);
+  }
+};
+
+Plan make_plan(const aihost_kv8_desc* d, const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max_new,
+               int32_t max_kv, int32_t num_sms) {
+  Plan p;
+  p.tensor = d->io_dtype == AIHOST_F16 &&
+             static_cast<int64_t>(max_new) * (g.n_q_heads / g.n_kv_heads) >= kKv8TensorMinRows;
+  if (p.tensor) {
+    p.rows = kv8_prefill_rows();
+    kv8_prefill_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.chunk, &p.splits);
+  } else {
+    p.rows = kv8_mma_rows(g, max_new);
+    kv8_mma_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.chunk, &p.splits);
+  }
+  return p;
+}
+
 // Sizes of an attention call, from host-known bounds.
 aihost_status check_sizes(int32_t batch, int32_t n_tokens, int32_t max_new, int32_t max_kv) {
   if (batch < 1) return fail(AIHOST_EINVAL, "batch (%d) must be >= 1", batch);
@@ -220,9 +244,7 @@ aihost_status aihost_kv8_workspace_size(const aihost_kv8_desc* desc, int32_t bat
   if (s != AIHOST_OK) return s;
   int sms = 148, dev = 0;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  int32_t tiles, chunk, splits;
-  kv8_mma_plan(r.g, batch, n_tokens, max_new, max_kv, sms, &tiles, &chunk, &splits);
-  *out_bytes = kv8_mma_scratch_bytes(r.g, tiles, kv8_mma_rows(r.g, max_new), splits);
+  *out_bytes = make_plan(desc, r.g, batch, n_tokens, max_new, max_kv, sms).scratch(r.g);
   return AIHOST_OK;
 }
 
@@ -271,24 +293,28 @@ aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* 
   a.score_cap = desc->score_cap;
   a.status = ctx->d_status;
   if (desc->rope_mode != AIHOST_ROPE_NONE) a.freqs = make_freqs(desc->rope_theta, desc->head_dim);
-  kv8_mma_plan(r.g, batch, n_tokens, max_new, max_kv, ctx->num_sms, &a.tiles, &a.chunk, &a.max_splits);
-  const int32_t rows = kv8_mma_rows(r.g, max_new);
+  const Plan plan = make_plan(desc, r.g, batch, n_tokens, max_new, max_kv, ctx->num_sms);
+  a.tiles = plan.tiles;
+  a.chunk = plan.chunk;
+  a.max_splits = plan.splits;
   if (static_cast<int64_t>(a.tiles) * r.g.n_kv_heads > INT32_MAX)
     return fail(AIHOST_EUNSUPPORTED, "n_tokens %d needs too many blocks", n_tokens);
-  const size_t need = kv8_mma_scratch_bytes(r.g, a.tiles, rows, a.max_splits);
+  const size_t need = plan.scratch(r.g);
   if (need > ctx->scratch_bytes)
     return fail(AIHOST_ENOMEM, "attention needs %zu bytes of scratch, context has %zu (call aihost_attn_reserve)", need,
                 ctx->scratch_bytes);
   if (need) {
     a.part_o = static_cast<float*>(ctx->scratch);
-    a.part_ml = a.part_o + static_cast<size_t>(a.tiles) * r.g.n_kv_heads * a.max_splits * rows * r.g.head_dim;
+    a.part_ml = a.part_o + static_cast<size_t>(a.tiles) * r.g.n_kv_heads * a.max_splits * plan.rows * r.g.head_dim;
     a.counters = ctx->counters;
     a.epoch = ctx->epoch++;
   }
   DeviceGuard g(ctx->device);
   if (!g.ok()) return fail(AIHOST_ECUDA, "cudaSetDevice(%d) failed", ctx->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = timed_launch(ctx, AIHOST_KERNEL_KV8_ATTN, st, [&] { return launch_kv8_mma(a, st); });
+  cudaError_t e = timed_launch(ctx, AIHOST_KERNEL_KV8_ATTN, st, [&] {
+    return plan.tensor ? launch_kv8_prefill(a, st) : launch_kv8_mma(a, st);
+  });
   return e == cudaSuccess ? AIHOST_OK : cuda_fail(e, "8-bit attention launch");
 }
 

@@ -14,6 +14,7 @@
 // that the last block to arrive merges (no block waits for another).
 #include "common.cuh"
 #include "kv8.h"
+#include "kv8_tile.cuh"
 #include "rows.cuh"
 
 namespace aihost {
@@ -21,8 +22,6 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kStep = 16;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNoMax = -1e30f;
 
 // What the products take: fp16 operands, q as a pair of fp16 (rotated in fp32), or q and P as pairs
 // (fp32 tensors).
@@ -51,75 +50,10 @@ __device__ __forceinline__ uint32_t movmatrix_t(uint32_t x) {
   return y;
 }
 
-// Bytes 0,1 (sel 0x4140) or 2,3 (0x4342) of `u` as exact fp16 integers: u holds value + 128, the
-// byte becomes the mantissa of 1024 + u, and 1152 comes off again.
-__device__ __forceinline__ uint32_t half2_of(uint32_t u, uint32_t sel) {
-  const uint32_t h = __byte_perm(u, 0x64646464u, sel);
-  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 // The rest of (lo, hi) after the fp16 pair `h`, in fp16.
 __device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t h) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
   return pack2(lo - f.x, hi - f.y);
-}
-
-// tanh x = 1 - 2 / (1 + e^2x): absolute error ~1e-7, which is what the capped score keeps.
-__device__ __forceinline__ float tanh_of(float x) {
-  const float e = ex2_approx(x * (2.0f * kLog2e));
-  return 1.0f - __fdividef(2.0f, 1.0f + e);
-}
-
-// Where a tile of query rows lies. Tiles of sequence b start at floor(row_start[b] * G / R) + b:
-// room for every tile whatever the lengths, so the grid needs only host-known bounds and each
-// block finds its sequence by itself. (One tile per sequence where max_new * G <= R.)
-struct Tile {
-  int32_t b, n_new, start, row0, kv_len, pos0;  // pos0: cache row of the sequence's first new token
-  bool ok;
-};
-
-__device__ __forceinline__ Tile find_tile(const Kv8AttnArgs& a, int64_t tile, int32_t G, int32_t R, int lane) {
-  Tile t;
-  t.ok = false;
-  t.row0 = 0;
-  if (static_cast<int64_t>(a.max_new) * G <= R) {
-    t.b = static_cast<int32_t>(tile);
-  } else {
-    int32_t lo = 0, n = a.batch;
-    while (n > 1) {  // 32 candidates at a time
-      const int32_t step = (n + 31) / 32, i = lo + lane * step;
-      const bool at = i < lo + n && static_cast<int64_t>(a.row_start[i]) * G / R + i <= tile;
-      const int32_t c = __popc(__ballot_sync(0xffffffffu, at));
-      const int32_t skip = (c > 0 ? c - 1 : 0) * step;
-      lo += skip;
-      n = min(step, n - skip);
-    }
-    t.b = lo;
-  }
-  t.start = a.row_start[t.b];
-  t.n_new = a.row_start[t.b + 1] - t.start;
-  t.kv_len = a.kv_len[t.b];
-  if (static_cast<int64_t>(a.max_new) * G > R) {
-    const int64_t k = tile - (static_cast<int64_t>(t.start) * G / R + t.b);
-    if (k < 0 || k * R >= static_cast<int64_t>(t.n_new) * G) {
-      if (t.n_new > 0 || t.start < 0 || t.n_new < 0) t.ok = false;
-      return t;
-    }
-    t.row0 = static_cast<int32_t>(k * R);
-  }
-  t.pos0 = t.kv_len - t.n_new;
-  t.ok = t.n_new > 0;
-  if (t.n_new < 0 || t.start < 0 || static_cast<int64_t>(t.start) + t.n_new > a.n_tokens || t.n_new > a.max_new ||
-      t.pos0 < 0 || t.kv_len > a.max_kv || t.kv_len > static_cast<int64_t>(a.g.max_pages) << a.g.page_shift) {
-    t.ok = false;
-    atomicOr(a.status, kStatusBadIndex);
-  }
-  return t;
 }
 
 template <int D, int NT, int PREC, bool MOD>
@@ -144,13 +78,6 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mma_kernel(const __grid_const
   const int32_t n_rows = min(R, tl.n_new * G - tl.row0);
 
   // ---- which cache rows each query row sees; this lane's two columns per N tile, and the tile's range
-  auto range_of = [&](int r, int32_t& first, int32_t& end, int32_t& pos) {
-    const int32_t row = tl.row0 + min(r, n_rows - 1), i = row / G;
-    pos = tl.pos0 + i;
-    end = pos + 1;
-    if (a.prefix_len) end = max(end, min(a.prefix_len[tl.b], tl.kv_len));
-    first = a.row_first ? max(a.row_first[tl.start + i], 0) : 0;
-  };
   int32_t c_first[NT][2], c_end[NT][2];
   float c_pos[NT][2], c_slope[NT][2];
 #pragma unroll
@@ -159,7 +86,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mma_kernel(const __grid_const
     for (int c = 0; c < 2; ++c) {
       const int r = nt * 8 + 2 * t4 + c;
       int32_t pos;
-      range_of(r, c_first[nt][c], c_end[nt][c], pos);
+      row_range(a, tl, G, n_rows, r, c_first[nt][c], c_end[nt][c], pos);
       c_pos[nt][c] = static_cast<float>(pos);
       c_slope[nt][c] =
           MOD && a.alibi_slopes ? a.alibi_slopes[h * G + (tl.row0 + min(r, n_rows - 1)) % G] * kLog2e : 0.0f;
@@ -167,7 +94,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mma_kernel(const __grid_const
   int32_t lo, hi, lo_max, hi_min;
   {
     int32_t first, end, pos;
-    range_of(lane & (R - 1), first, end, pos);
+    row_range(a, tl, G, n_rows, lane & (R - 1), first, end, pos);
     lo = __reduce_min_sync(0xffffffffu, first);
     lo_max = __reduce_max_sync(0xffffffffu, first);
     hi = __reduce_max_sync(0xffffffffu, end);
@@ -180,14 +107,7 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mma_kernel(const __grid_const
   const int32_t* const table = a.block_table + static_cast<int64_t>(tl.b) * a.g.max_pages;
   // a page id outside the pool reads page 0 and sets the status
   bool stray = false;
-  auto page_at = [&](int32_t row) -> int64_t {
-    const int32_t p = table[row >> ps];
-    if (p < 0 || p >= a.g.n_pages) {
-      stray = true;
-      return 0;
-    }
-    return p;
-  };
+  auto page_at = [&](int32_t row) -> int64_t { return page_or_first(table[row >> ps], a.g.n_pages, stray); };
 
   // ---- the step's rows, one step ahead
   uint4 kb[2][KC];
@@ -533,10 +453,6 @@ void kv8_mma_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max
   *tiles = static_cast<int32_t>(n);
   *chunk = static_cast<int32_t>(c);
   *splits = static_cast<int32_t>(s);
-}
-
-size_t kv8_mma_scratch_bytes(const Kv8Geom& g, int32_t tiles, int32_t rows, int32_t splits) {
-  return splits <= 1 ? 0 : static_cast<size_t>(tiles) * g.n_kv_heads * splits * rows * (g.head_dim + 2) * sizeof(float);
 }
 
 cudaError_t launch_kv8_mma(const Kv8AttnArgs& a, cudaStream_t st) {

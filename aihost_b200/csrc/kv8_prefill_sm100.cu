@@ -1,0 +1,615 @@
+// kv8_prefill_sm100.cu — attention of many query rows over the 8-bit paged cache on the
+// 5th-generation tensor cores (prompts and long continuations, fp16 tensors).
+//
+// One block takes 256 query rows of one KV head (tokens x the heads of its group, so a cache row is
+// converted once for the whole group), as two tiles of 128, and walks a range of the cache in
+// 128-row tiles (flash attention, online softmax):
+//   warpgroup 3  reads int8 rows straight from their pages (16 bytes a lane, the next tile's already
+//                in flight in registers), makes them fp16 exactly and stores them in the 128-byte
+//                swizzled layout the MMAs read; K and V rings of their own. Row scales stay out of
+//                the products: one factor per 16 rows of K (times scale and log2 e) and of V (over
+//                the range's largest) goes to a small ring in shared memory.
+//   warp 0       issues tcgen05.mma: S = Q K^T into tensor memory, O += P V with P read from there;
+//                the two tiles take turns, so one's softmax runs under the other's products.
+//   warpgroups 1, 2  one thread per query row: S from tensor memory, K's factors, cap and bias, masks
+//                on tiles that cross the row's range, running maximum (O is rescaled only when it
+//                grows by more than 2^8), exp2, row sum, P times V's factors as fp16.
+// Ranges are cut into chunks where there are few tiles; the last block of a tile to arrive merges.
+#include "common.cuh"
+#include "kv8.h"
+#include "kv8_tile.cuh"
+
+namespace aihost {
+namespace {
+
+constexpr int kTileRows = 128;
+constexpr int kRows = 2 * kTileRows;  // query rows of a block
+constexpr int kKeys = 128;            // cache rows of a tile
+constexpr int kThreads = 512;
+// setmaxnreg split of the 128 x 512 registers at launch: MMA warpgroup, softmax warpgroups, converters
+constexpr uint32_t kRegsMma = 40, kRegsSoftmax = 184, kRegsConvert = 104;
+static_assert(128 * (kRegsMma + 2 * kRegsSoftmax + kRegsConvert) <= 128 * kThreads, "setmaxnreg split exceeds the launch");
+constexpr float kSlack = 8.0f;    // the maximum may lag by 2^8 before O is rescaled
+constexpr float kVUnit = 128.0f;  // P * (v scale / largest) * 128 <= 2^15 stays in fp16's range
+constexpr int kFactors = kKeys / 16;
+constexpr int kFactorRing = 4;
+
+template <int D>
+struct Cfg {
+  static constexpr int KB = D / 64;                   // 64-element (128-byte) column blocks
+  static constexpr int TILE = KB * kKeys * 128;       // one [128 x D] fp16 tile
+  static constexpr int NS = D == 64 ? 3 : 2;          // K and V ring depth
+  static constexpr int K_OFF = 2 * TILE;              // after the two Q tiles
+  static constexpr int V_OFF = K_OFF + NS * TILE;
+  static constexpr int BAR_OFF = V_OFF + NS * TILE;
+  static constexpr int SMEM = BAR_OFF + 1024 + 1024;  // barriers and factors, alignment slack
+  static __device__ __forceinline__ uint32_t s_col(int t) { return t ? 128u : 0u; }
+  static __device__ __forceinline__ uint32_t o_col(int t) { return 256u + static_cast<uint32_t>(t * D); }
+};
+
+struct Shared {
+  uint64_t q_ready[2], s_full[2], p_full[2], o_full[2];
+  uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
+  float k_factor[kFactorRing][kFactors];
+  float v_factor[kFactorRing][kFactors];
+  float v_max[4];
+  uint32_t tmem_base;
+  int32_t last;
+};
+static_assert(sizeof(Shared) <= 1024, "the layout reserves 1024 bytes");
+
+// Byte offset of 16-byte chunk c of row `row` in a [128 x D] fp16 tile: 128-byte swizzled rows of
+// 64 elements, blocks of 64 columns one after another.
+__device__ __forceinline__ uint32_t chunk_off(int row, int c) {
+  return static_cast<uint32_t>((c >> 3) * (kKeys * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+}
+
+// Packed fp32 pairs: one instruction for two.
+__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 ra, rb, rc, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n mov.b64 rc, {%6, %7};\n"
+      " fma.rn.f32x2 rd, ra, rb, rc;\n mov.b64 {%0, %1}, rd;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 ra, rb, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n add.rn.f32x2 rd, ra, rb;\n"
+      " mov.b64 {%0, %1}, rd;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 ra, rb, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n mul.rn.f32x2 rd, ra, rb;\n"
+      " mov.b64 {%0, %1}, rd;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 16 int8 as two 16-byte chunks of fp16, exactly.
+__device__ __forceinline__ void convert16(const uint4& v, uint4& lo, uint4& hi) {
+  const uint32_t w0 = v.x ^ 0x80808080u, w1 = v.y ^ 0x80808080u, w2 = v.z ^ 0x80808080u, w3 = v.w ^ 0x80808080u;
+  lo = make_uint4(half2_of(w0, 0x4140), half2_of(w0, 0x4342), half2_of(w1, 0x4140), half2_of(w1, 0x4342));
+  hi = make_uint4(half2_of(w2, 0x4140), half2_of(w2, 0x4342), half2_of(w3, 0x4140), half2_of(w3, 0x4342));
+}
+
+template <int D, bool MOD>
+__global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_constant__ Kv8AttnArgs a) {
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Shared& sh = *reinterpret_cast<Shared*>(smem + C::BAR_OFF);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int32_t H = a.g.n_kv_heads, G = a.g.n_q_heads / H, ps = a.g.page_shift;
+  // longest ranges first: a sequence's last tiles see the most
+  const int32_t h = static_cast<int32_t>(blockIdx.x % H);
+  const int32_t tile = a.tiles - 1 - static_cast<int32_t>(blockIdx.x / H);
+  const int32_t split = static_cast<int32_t>(blockIdx.y);
+  const Tile tl = find_tile(a, tile, G, kRows, lane);
+  if (!tl.ok) return;
+  const int32_t n_rows = min(static_cast<int64_t>(kRows), static_cast<int64_t>(tl.n_new) * G - tl.row0);
+
+  // ---- cache tiles [j0, j1) of either query tile, and this block's chunk of them
+  int32_t j0[2], j1[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    int32_t lo = INT32_MAX, hi = 0;
+#pragma unroll
+    for (int k = 0; k < kTileRows / 32; ++k) {
+      const int r = t * kTileRows + k * 32 + lane;
+      int32_t first, end, pos;
+      row_range(a, tl, G, n_rows, r, first, end, pos);
+      if (r < n_rows && first < end) {
+        lo = min(lo, first);
+        hi = max(hi, end);
+      }
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    j0[t] = hi > 0 ? lo / kKeys : 0;
+    j1[t] = hi > 0 ? (hi + kKeys - 1) / kKeys : 0;
+  }
+  const bool any0 = j1[0] > 0, any1 = j1[1] > 0;
+  const int32_t all0 = any0 ? (any1 ? min(j0[0], j0[1]) : j0[0]) : j0[1], all1 = max(j1[0], j1[1]);
+  const int32_t chunk = a.chunk / kKeys;
+  const int32_t n_splits = max(1, (all1 - all0 + chunk - 1) / chunk);
+  if (split >= n_splits) return;
+  const int32_t jb = all0 + split * chunk, je = min(all1, jb + chunk);
+  const int32_t n_load = max(je - jb, 0);  // 0: no row of the block sees anything
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    j0[t] = max(j0[t], jb);
+    j1[t] = min(j1[t], je);
+  }
+  int32_t* const status = a.status;
+
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&sh.q_ready[t], kTileRows);
+      mbar_init(&sh.s_full[t], 2);  // the products' commit, and the issuing thread's own arrival
+      mbar_init(&sh.p_full[t], kTileRows);
+      mbar_init(&sh.o_full[t], 1);
+    }
+    for (int i = 0; i < C::NS; ++i) {
+      mbar_init(&sh.k_full[i], 128);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_full[i], 128);
+      mbar_init(&sh.v_empty[i], 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(&sh.tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem_base;
+
+  if (warp < 4) {
+    // ------------------------------------------------------------------ MMA issuer (one thread)
+    regs_dealloc<kRegsMma>();
+    if (threadIdx.x == 0 && n_load > 0) {
+      constexpr uint32_t idesc_qk = make_idesc_f16(kTileRows, kKeys, 0, 0);
+      constexpr uint32_t idesc_pv = make_idesc_f16(kTileRows, D, 0, 1);
+      const uint32_t q_addr = smem_u32(smem), k_addr = smem_u32(smem + C::K_OFF), v_addr = smem_u32(smem + C::V_OFF);
+      auto issue_qk = [&](int t, int s) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * (kKeys * 128) + (kk & 3) * 32;
+          umma_f16_ss(tmem + C::s_col(t), make_sw128_desc(q_addr + t * C::TILE + off, 16, 1024),
+                      make_sw128_desc(k_addr + s * C::TILE + off, 16, 1024), idesc_qk, kk > 0);
+        }
+        umma_commit(&sh.s_full[t]);
+        mbar_arrive(&sh.s_full[t]);  // passes on what the converters wrote besides (the factors)
+      };
+      auto issue_pv = [&](int t, int s, bool first) {
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          umma_f16_ts(tmem + C::o_col(t), tmem + C::s_col(t) + kk * 8,
+                      make_sw128_desc(v_addr + s * C::TILE + kk * 2048, kKeys * 128, 1024), idesc_pv, !first || kk > 0);
+      };
+      const int32_t t_lo[2] = {j0[0] - jb, j0[1] - jb}, t_hi[2] = {j1[0] - jb, j1[1] - jb};
+      bool ok = mbar_wait(&sh.q_ready[0], 0, status) && mbar_wait(&sh.q_ready[1], 0, status) &&
+                mbar_wait(&sh.k_full[0], 0, status);
+      tc_fence_after();
+      if (ok) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (t_lo[t] <= 0 && t_hi[t] > 0) issue_qk(t, 0);
+        umma_commit(&sh.k_empty[0]);
+      }
+      for (int32_t i = 0; ok && i < n_load; ++i) {
+        const int s = i % C::NS, s1 = (i + 1) % C::NS;
+        if (!mbar_wait(&sh.v_full[s], (i / C::NS) & 1, status)) break;
+        if (i + 1 < n_load && !mbar_wait(&sh.k_full[s1], ((i + 1) / C::NS) & 1, status)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (i >= t_lo[t] && i < t_hi[t]) {
+            if (!mbar_wait(&sh.p_full[t], (i - t_lo[t]) & 1, status)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            issue_pv(t, s, i == t_lo[t]);
+            if (i + 1 == t_hi[t]) umma_commit(&sh.o_full[t]);
+          }
+          if (i + 1 >= t_lo[t] && i + 1 < t_hi[t]) issue_qk(t, s1);
+        }
+        if (!ok) break;
+        umma_commit(&sh.v_empty[s]);
+        if (i + 1 < n_load) umma_commit(&sh.k_empty[s1]);
+      }
+    }
+  } else if (warp >= 12) {
+    // ------------------------------------------------------------------ converters
+    regs_dealloc<kRegsConvert>();
+    const int w = warp - 12;
+    const int32_t* const table = a.block_table + static_cast<int64_t>(tl.b) * a.g.max_pages;
+    const int32_t row_end = min(je * kKeys, tl.kv_len);  // rows from here on are not read
+    bool stray = false;
+    // the chunk's largest V scale
+    float vmax = 0.0f;
+    for (int32_t k = ((jb * kKeys) >> ps) + w * 32 + lane; k < (row_end + a.g.page_rows - 1) >> ps; k += 128)
+      vmax = fmaxf(vmax, __ldg(a.v_scale + page_or_first(table[k], a.g.n_pages, stray) * H + h));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+    if (lane == 0) sh.v_max[w] = vmax;
+    asm volatile("bar.sync 2, 128;" ::: "memory");
+    vmax = fmaxf(fmaxf(sh.v_max[0], sh.v_max[1]), fmaxf(sh.v_max[2], sh.v_max[3]));
+    const float v_unit = vmax > 0.0f ? kVUnit / vmax : 0.0f;
+    const bool capped = MOD && a.score_cap > 0.0f;
+    const float k_unit = capped ? a.scale / a.score_cap : a.scale * kLog2e;
+
+    // A warp and load step covers 512 consecutive bytes of a page: 4 rows of 128 (or 8 of 64), so that
+    // 8 lanes storing together fall into different banks.
+    constexpr int RPL = 512 / D;          // rows per load
+    constexpr int NL = kKeys / (4 * RPL);  // loads per tile and lane
+    const int c = D == 128 ? (lane & 3) + ((lane >> 3) & 1) * 4 : lane & 3;                  // 16-byte chunk of the row
+    const int r_in = D == 128 ? ((lane >> 2) & 1) + ((lane >> 4) << 1) : lane >> 2;          // row of the load
+    uint4 kr[NL], vr[NL];
+    int32_t page = 0;  // lane f < 8: page of the tile's rows [16 f, 16 f + 16), -1 past the end
+    float ksf = 0.0f, vsf = 0.0f;
+    auto pages_of = [&](int32_t i) {
+      const int32_t row = (jb + i) * kKeys + (lane & 7) * 16;
+      page = row < row_end ? static_cast<int32_t>(page_or_first(table[row >> ps], a.g.n_pages, stray)) : -1;
+    };
+    auto scales_of = [&] {
+      if (w == 0 && lane < kFactors && page >= 0) {
+        ksf = __ldg(a.k_scale + static_cast<int64_t>(page) * H + h);
+        vsf = __ldg(a.v_scale + static_cast<int64_t>(page) * H + h);
+      }
+    };
+    auto load = [&](const int8_t* pool, int32_t i, uint4 (&v)[NL]) {
+#pragma unroll
+      for (int k = 0; k < NL; ++k) {
+        const int unit = k * 4 + w;  // rows [unit * RPL, (unit + 1) * RPL) of the tile: within one page
+        const int32_t p = __shfl_sync(0xffffffffu, page, unit * RPL / 16);
+        const int32_t row = (jb + i) * kKeys + unit * RPL + r_in;
+        v[k] = make_uint4(0, 0, 0, 0);
+        if (p >= 0)
+          v[k] = __ldg(reinterpret_cast<const uint4*>(
+              pool + (((static_cast<int64_t>(p) * H + h) << ps) + (row & (a.g.page_rows - 1))) * D + c * 16));
+      }
+    };
+    auto store = [&](uint8_t* dst, const uint4 (&v)[NL]) {
+#pragma unroll
+      for (int k = 0; k < NL; ++k) {
+        const int row = (k * 4 + w) * RPL + r_in;
+        uint4 lo, hi;
+        convert16(v[k], lo, hi);
+        *reinterpret_cast<uint4*>(dst + chunk_off(row, 2 * c)) = lo;
+        *reinterpret_cast<uint4*>(dst + chunk_off(row, 2 * c + 1)) = hi;
+      }
+      fence_proxy_async_smem();
+    };
+    if (n_load > 0) {
+      pages_of(0);
+      load(a.k_pool, 0, kr);
+    }
+    for (int32_t i = 0; i < n_load; ++i) {
+      const int s = i % C::NS;
+      const uint32_t par = ((i / C::NS) & 1) ^ 1;
+      load(a.v_pool, i, vr);
+      scales_of();
+      const int32_t now = page;
+      if (i + 1 < n_load) pages_of(i + 1);
+      if (!mbar_wait(&sh.k_empty[s], par, status)) break;
+      if (w == 0 && lane < kFactors) {
+        // A scale that is no number marks the page through K's factor: a hidden row's weight is then 0
+        // and its V factor must not turn it into NaN again.
+        const bool fine = vsf < INFINITY;
+        sh.k_factor[i % kFactorRing][lane] = now < 0 ? 0.0f : fine ? ksf * k_unit : __uint_as_float(0x7fffffffu);
+        sh.v_factor[i % kFactorRing][lane] = now < 0 || !fine ? 0.0f : vsf * v_unit;
+      }
+      store(smem + C::K_OFF + s * C::TILE, kr);
+      mbar_arrive(&sh.k_full[s]);
+      if (i + 1 < n_load) load(a.k_pool, i + 1, kr);
+      if (!mbar_wait(&sh.v_empty[s], par, status)) break;
+      store(smem + C::V_OFF + s * C::TILE, vr);
+      mbar_arrive(&sh.v_full[s]);
+    }
+    if (stray) atomicOr(status, kStatusBadIndex);
+  } else {
+    // ------------------------------------------------------------------ softmax: a thread per query row
+    regs_alloc<kRegsSoftmax>();
+    const int t = warp >= 8 ? 1 : 0;
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;  // row within the tile == tensor memory lane
+    const int rr = t * kTileRows + r;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const bool valid = rr < n_rows;
+    int32_t first, end, pos;
+    row_range(a, tl, G, n_rows, rr, first, end, pos);
+    if (!valid) end = first = 0;
+    const int32_t row = tl.row0 + min(rr, n_rows - 1), tok = row / G, head = h * G + row % G;
+    // ---- the row of Q, rotated in fp32 and rounded once
+    {
+      uint8_t* const q_tile = smem + t * C::TILE;
+      const uint8_t* const src = static_cast<const uint8_t*>(a.q) +
+                                 (tl.start + static_cast<int64_t>(tok)) * a.q_token_stride + static_cast<int64_t>(head) * D * 2;
+      auto rot = [&](uint32_t& w1, uint32_t& w2, float angle) {
+        float sn, cs;
+        sincos_reduced(angle, &sn, &cs);
+        const float x1 = __half2float(__ushort_as_half(static_cast<unsigned short>(w1)));
+        const float x2 = __half2float(__ushort_as_half(static_cast<unsigned short>(w2)));
+        w1 = __half_as_ushort(__float2half_rn(x1 * cs - x2 * sn));
+        w2 = __half_as_ushort(__float2half_rn(x1 * sn + x2 * cs));
+      };
+      const float fpos = static_cast<float>(pos);
+      constexpr int NC = D / 8;
+#pragma unroll 2
+      for (int c = 0; c < NC / 2; ++c) {
+        uint4 v[2] = {__ldg(reinterpret_cast<const uint4*>(src) + c), __ldg(reinterpret_cast<const uint4*>(src) + c + NC / 2)};
+        uint32_t* const u0 = reinterpret_cast<uint32_t*>(&v[0]);
+        uint32_t* const u1 = reinterpret_cast<uint32_t*>(&v[1]);
+        if (a.rope_mode == AIHOST_ROPE_NEOX) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t a0 = u0[k] & 0xffffu, a1 = u0[k] >> 16, b0 = u1[k] & 0xffffu, b1 = u1[k] >> 16;
+            rot(a0, b0, fpos * a.freqs.f[8 * c + 2 * k]);
+            rot(a1, b1, fpos * a.freqs.f[8 * c + 2 * k + 1]);
+            u0[k] = a0 | (a1 << 16);
+            u1[k] = b0 | (b1 << 16);
+          }
+        } else if (a.rope_mode == AIHOST_ROPE_INTERLEAVED) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t lo = u0[k] & 0xffffu, hi = u0[k] >> 16;
+            rot(lo, hi, fpos * a.freqs.f[4 * c + k]);
+            u0[k] = lo | (hi << 16);
+            lo = u1[k] & 0xffffu, hi = u1[k] >> 16;
+            rot(lo, hi, fpos * a.freqs.f[4 * (c + NC / 2) + k]);
+            u1[k] = lo | (hi << 16);
+          }
+        }
+        *reinterpret_cast<uint4*>(q_tile + chunk_off(r, c)) = v[0];
+        *reinterpret_cast<uint4*>(q_tile + chunk_off(r, c + NC / 2)) = v[1];
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&sh.q_ready[t]);
+    }
+
+    const float slope = MOD && a.alibi_slopes ? a.alibi_slopes[head] * kLog2e : 0.0f;
+    const bool capped = MOD && a.score_cap > 0.0f;
+    const float cap2 = a.score_cap * kLog2e, fpos = static_cast<float>(pos);
+    float m = kNoMax, l = 0.0f;
+    const uint32_t s_tmem = tmem + lane_base + C::s_col(t), o_tmem = tmem + lane_base + C::o_col(t);
+    const int32_t lo_j = t ? j0[1] : j0[0], hi_j = t ? j1[1] : j1[0], n_own = hi_j - lo_j;
+    bool ok = true;
+    for (int32_t i = 0; i < n_own; ++i) {
+      if (!mbar_wait(&sh.s_full[t], i & 1, status)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t sr[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + c * 32, sr[c]);
+      const int slot = (lo_j + i - jb) % kFactorRing;
+      const int32_t kv0 = (lo_j + i) * kKeys;
+      const bool need_mask = __any_sync(0xffffffffu, valid && (kv0 < first || kv0 + kKeys > end));
+      float kf[kFactors];
+#pragma unroll
+      for (int f = 0; f < kFactors; ++f) kf[f] = sh.k_factor[slot][f];
+      tmem_wait_ld();
+      if (MOD || need_mask) {  // scores in log2 units, hidden ones -inf; the factors are then spent
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int32_t j = kv0 + c * 32 + e;
+            float x = __uint_as_float(sr[c][e]) * kf[c * 2 + e / 16];
+            if constexpr (MOD) {
+              if (capped) x = cap2 * tanh_of(x);
+              x = fmaf(-slope, fabsf(fpos - static_cast<float>(j)), x);
+            }
+            if (j < first || j >= end) x = -INFINITY;
+            sr[c][e] = __float_as_uint(x);
+          }
+#pragma unroll
+        for (int f = 0; f < kFactors; ++f) kf[f] = 1.0f;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int f = 0; f < kFactors; ++f) {
+        const uint32_t* const g = &sr[f / 2][(f & 1) * 16];
+        float p0 = fmax3(__uint_as_float(g[0]), __uint_as_float(g[1]), __uint_as_float(g[2]));
+        float p1 = fmax3(__uint_as_float(g[3]), __uint_as_float(g[4]), __uint_as_float(g[5]));
+        float p2 = fmax3(__uint_as_float(g[6]), __uint_as_float(g[7]), __uint_as_float(g[8]));
+        float p3 = fmax3(__uint_as_float(g[9]), __uint_as_float(g[10]), __uint_as_float(g[11]));
+        p0 = fmax3(p0, __uint_as_float(g[12]), __uint_as_float(g[13]));
+        p1 = fmax3(p1, __uint_as_float(g[14]), __uint_as_float(g[15]));
+        mx = fmaxf(mx, fmax3(fmaxf(p0, p1), p2, p3) * kf[f]);
+      }
+      const bool grow = mx > m + kSlack;
+      float f_o = 1.0f;
+      if (grow) {
+        f_o = ex2_approx(m - mx);
+        l *= f_o;
+        m = mx;
+      }
+      const float2 neg_m = make_float2(-m, -m);
+      float2 sum[4] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+      uint32_t pk[4][16];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int f = c * 2 + e / 8;
+          const float2 x = ffma2(make_float2(__uint_as_float(sr[c][2 * e]), __uint_as_float(sr[c][2 * e + 1])),
+                                 make_float2(kf[f], kf[f]), neg_m);
+          const float2 p = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+          sum[e & 3] = fadd2(sum[e & 3], p);
+          const float vf = sh.v_factor[slot][f];
+          const float2 pv = fmul2(p, make_float2(vf, vf));
+          pk[c][e] = pack2(pv.x, pv.y);
+        }
+      l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
+      // the P V before was committed ahead of this S: O is at rest
+      if (i > 0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(o_tmem + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f_o);
+          tmem_st32(o_tmem + c * 32, o);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_st16(s_tmem + c * 16, pk[c]);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&sh.p_full[t]);
+    }
+    // ---- O / l, or this chunk's share of it
+    if (ok && n_own > 0) ok = mbar_wait(&sh.o_full[t], 0, status);
+    tc_fence_after();
+    // written by the converters before the first S; with no tile there is nothing to scale
+    const float vmax =
+        n_own > 0 ? fmaxf(fmaxf(sh.v_max[0], sh.v_max[1]), fmaxf(sh.v_max[2], sh.v_max[3])) : 0.0f;
+    const float o_unit = vmax * (1.0f / kVUnit);
+    const int64_t out_row = ((tl.start + static_cast<int64_t>(tok)) * a.g.n_q_heads + head) * D;
+    auto store32 = [&](int c, const float (&o)[32]) {
+      if (!valid) return;
+      if (a.out_dtype == AIHOST_F16) {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(a.out) + out_row + c * 32);
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          dst[v] = make_uint4(pack2(o[8 * v], o[8 * v + 1]), pack2(o[8 * v + 2], o[8 * v + 3]),
+                              pack2(o[8 * v + 4], o[8 * v + 5]), pack2(o[8 * v + 6], o[8 * v + 7]));
+      } else {
+        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(a.out) + out_row + c * 32);
+#pragma unroll
+        for (int v = 0; v < 8; ++v) dst[v] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+      }
+    };
+    const bool whole = __all_sync(0xffffffffu, ok);
+    const int64_t unit = static_cast<int64_t>(tile) * H + h;
+    // partials: [unit][split][D / 4][256 rows] of 4 floats, so that a warp's rows lie together
+    float4* const part = reinterpret_cast<float4*>(a.part_o) + (unit * a.max_splits) * (D / 4) * kRows + rr;
+    float2* const part_ml = reinterpret_cast<float2*>(a.part_ml) + unit * a.max_splits * kRows + rr;
+    if (whole) {
+      const float unit_o = n_splits > 1 ? o_unit : l != 0.0f ? o_unit / l : 0.0f;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        float o[32];
+        if (n_own > 0) {
+          uint32_t u[32];
+          tmem_ld32(o_tmem + c * 32, u);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(u[e]) * unit_o;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+        }
+        if (n_splits == 1) {
+          store32(c, o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            part[(static_cast<int64_t>(split) * (D / 4) + c * 8 + e) * kRows] =
+                make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        }
+      }
+      if (n_splits > 1) part_ml[static_cast<int64_t>(split) * kRows] = make_float2(m, l);
+    }
+    if (n_splits > 1) {  // the last block of this tile and head to arrive merges the chunks
+      __threadfence();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (threadIdx.x == 128) {
+        sh.last = split_arrive(a.counters + unit, a.epoch, n_splits, status);
+        if (sh.last) a.counters[unit] = 0;  // a replayed launch counts from zero again
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (sh.last) {
+        __threadfence();
+        float mm = kNoMax;
+        for (int sp = 0; sp < n_splits; ++sp) mm = fmaxf(mm, __ldcg(part_ml + static_cast<int64_t>(sp) * kRows).x);
+        float ll = 0.0f;
+        for (int sp = 0; sp < n_splits; ++sp) {
+          const float2 v = __ldcg(part_ml + static_cast<int64_t>(sp) * kRows);
+          ll += v.y * ex2_approx(v.x - mm);
+        }
+        const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+          for (int sp = 0; sp < n_splits; ++sp) {
+            const float f = ex2_approx(__ldcg(part_ml + static_cast<int64_t>(sp) * kRows).x - mm) * inv;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float4 v = __ldcg(part + (static_cast<int64_t>(sp) * (D / 4) + c * 8 + e) * kRows);
+              o[4 * e] += v.x * f, o[4 * e + 1] += v.y * f, o[4 * e + 2] += v.z * f, o[4 * e + 3] += v.w * f;
+            }
+          }
+          store32(c, o);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int D, bool MOD>
+cudaError_t launch_d(const Kv8AttnArgs& a, cudaStream_t st) {
+  auto kern = kv8_prefill_kernel<D, MOD>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+  if (e != cudaSuccess) return e;
+  kern<<<dim3(static_cast<unsigned>(a.tiles) * a.g.n_kv_heads, a.max_splits), kThreads, Cfg<D>::SMEM, st>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max_new, int32_t max_kv, int32_t num_sms,
+                      int32_t* tiles, int32_t* chunk, int32_t* splits) {
+  const int32_t G = g.n_q_heads / g.n_kv_heads;
+  const int64_t n = static_cast<int64_t>(max_new) * G <= kRows ? batch : static_cast<int64_t>(n_tokens) * G / kRows + batch;
+  const int64_t units = n * g.n_kv_heads, tiles_kv = (max_kv + kKeys - 1) / kKeys;
+  // one block per SM at a time: cut the ranges where that evens out the waves, into chunks of 8 tiles at least
+  int64_t best = 1;
+  double best_cost = 1e30;
+  for (int64_t s = 1; s <= 16 && (s == 1 || tiles_kv / s >= 8); ++s) {
+    const int64_t waves = (units * s + num_sms - 1) / num_sms;
+    const double cost = static_cast<double>(waves) * (static_cast<double>((tiles_kv + s - 1) / s) + 3.0);
+    if (cost < best_cost * 0.97) {
+      best_cost = cost;
+      best = s;
+    }
+  }
+  if (units > kMaxSplitCounters) best = 1;
+  const int64_t c = (tiles_kv + best - 1) / best;
+  *tiles = static_cast<int32_t>(n);
+  *chunk = static_cast<int32_t>(c * kKeys);
+  *splits = static_cast<int32_t>((tiles_kv + c - 1) / c);
+}
+
+int32_t kv8_prefill_rows() { return kRows; }
+
+cudaError_t launch_kv8_prefill(const Kv8AttnArgs& a, cudaStream_t st) {
+  const bool mod = a.score_cap > 0.0f || a.alibi_slopes;
+  if (a.g.head_dim == 64) return mod ? launch_d<64, true>(a, st) : launch_d<64, false>(a, st);
+  return mod ? launch_d<128, true>(a, st) : launch_d<128, false>(a, st);
+}
+
+}  // namespace aihost

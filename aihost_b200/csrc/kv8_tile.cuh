@@ -1,0 +1,98 @@
+// kv8_tile.cuh — where a tile of query rows of the ragged batch lies, and small pieces that the
+// kernels over the 8-bit cache share.
+#pragma once
+
+#include "common.cuh"
+#include "kv8.h"
+
+namespace aihost {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -1e30f;
+
+// A KV head's query rows of sequence b are its tokens' heads, token by token: row = token * G + head
+// in the group. Tiles of R rows of sequence b start at floor(row_start[b] * G / R) + b: room for every
+// tile whatever the lengths, so the grid needs only host-known bounds and each block finds its
+// sequence by itself. (One tile per sequence where max_new * G <= R.)
+struct Tile {
+  int32_t b, n_new, start, row0, kv_len, pos0;  // pos0: cache row of the sequence's first new token
+  bool ok;
+};
+
+// The tile's place; ok is false for a tile without rows and for one whose lengths are out of bounds
+// (which sets the status). Called by whole warps.
+__device__ __forceinline__ Tile find_tile(const Kv8AttnArgs& a, int64_t tile, int32_t G, int32_t R, int lane) {
+  Tile t;
+  t.ok = false;
+  t.row0 = 0;
+  const bool one = static_cast<int64_t>(a.max_new) * G <= R;
+  if (one) {
+    t.b = static_cast<int32_t>(tile);
+  } else {
+    int32_t lo = 0, n = a.batch;
+    while (n > 1) {  // 32 candidates at a time
+      const int32_t step = (n + 31) / 32, i = lo + lane * step;
+      const bool at = i < lo + n && static_cast<int64_t>(a.row_start[i]) * G / R + i <= tile;
+      const int32_t c = __popc(__ballot_sync(0xffffffffu, at));
+      const int32_t skip = (c > 0 ? c - 1 : 0) * step;
+      lo += skip;
+      n = min(step, n - skip);
+    }
+    t.b = lo;
+  }
+  t.start = a.row_start[t.b];
+  t.n_new = a.row_start[t.b + 1] - t.start;
+  t.kv_len = a.kv_len[t.b];
+  t.pos0 = t.kv_len - t.n_new;
+  if (t.n_new == 0) return t;
+  if (t.n_new < 0 || t.start < 0 || static_cast<int64_t>(t.start) + t.n_new > a.n_tokens || t.n_new > a.max_new ||
+      t.pos0 < 0 || t.kv_len > a.max_kv || t.kv_len > static_cast<int64_t>(a.g.max_pages) << a.g.page_shift) {
+    if (lane == 0) atomicOr(a.status, kStatusBadIndex);
+    return t;
+  }
+  if (!one) {
+    const int64_t k = tile - (static_cast<int64_t>(t.start) * G / R + t.b);
+    if (k < 0 || k * R >= static_cast<int64_t>(t.n_new) * G) return t;
+    t.row0 = static_cast<int32_t>(k * R);
+  }
+  t.ok = true;
+  return t;
+}
+
+// The cache rows [first, end) that the tile's row r sees, and its position. r is clamped to n_rows - 1.
+__device__ __forceinline__ void row_range(const Kv8AttnArgs& a, const Tile& t, int32_t G, int32_t n_rows, int r,
+                                          int32_t& first, int32_t& end, int32_t& pos) {
+  const int32_t i = (t.row0 + min(r, n_rows - 1)) / G;
+  pos = t.pos0 + i;
+  end = pos + 1;
+  if (a.prefix_len) end = max(end, min(a.prefix_len[t.b], t.kv_len));
+  first = a.row_first ? max(a.row_first[t.start + i], 0) : 0;
+}
+
+// Bytes 0,1 (sel 0x4140) or 2,3 (0x4342) of `u` as exact fp16 integers: u holds value + 128, the
+// byte becomes the mantissa of 1024 + u, and 1152 comes off again.
+__device__ __forceinline__ uint32_t half2_of(uint32_t u, uint32_t sel) {
+  const uint32_t h = __byte_perm(u, 0x64646464u, sel);
+  const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// tanh x = 1 - 2 / (1 + e^2x): absolute error ~1e-7, which is what the capped score keeps.
+__device__ __forceinline__ float tanh_of(float x) {
+  const float e = ex2_approx(x * (2.0f * kLog2e));
+  return 1.0f - __fdividef(2.0f, 1.0f + e);
+}
+
+// Page id of a table entry; one outside the pool becomes page 0 and sets `stray`.
+__device__ __forceinline__ int64_t page_or_first(int32_t p, int32_t n_pages, bool& stray) {
+  if (p >= 0 && p < n_pages) return p;
+  stray = true;
+  return 0;
+}
+
+}  // namespace aihost
