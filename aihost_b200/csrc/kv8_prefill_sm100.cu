@@ -4,13 +4,15 @@
 // One block takes 256 query rows of one KV head (tokens x the heads of its group, so a cache row is
 // converted once for the whole group), as two tiles of 128, and walks a range of the cache in
 // 128-row tiles (flash attention, online softmax):
-//   warpgroup 3  reads int8 rows straight from their pages (16 bytes a lane, the next tile's already
-//                in flight in registers), makes them fp16 exactly and stores them in the 128-byte
-//                swizzled layout the MMAs read; K and V rings of their own. Row scales stay out of
-//                the products: one factor per 16 rows of K (times scale and log2 e) and of V (over
-//                the range's largest) goes to a small ring in shared memory.
+//   warp 1       copies the int8 rows of each tile, page by page, into a ring (bulk copies).
+//   warpgroup 3  makes them fp16 exactly and stores them in the 128-byte swizzled layout the MMAs
+//                read; K and V rings of their own.
+//   warp 2       the pages' scales, which stay out of the products: one factor per 16 rows of K
+//                (times scale and log2 e) and of V (over the range's largest), in a small ring.
 //   warp 0       issues tcgen05.mma: S = Q K^T into tensor memory, O += P V with P read from there;
-//                the two tiles take turns, so one's softmax runs under the other's products.
+//                the two tiles take turns, so one's softmax runs under the other's products. The
+//                whole warp runs this code on warp-uniform values and one elected lane issues:
+//                descriptors then stay in uniform registers.
 //   warpgroups 1, 2  one thread per query row: S from tensor memory, K's factors, cap and bias, masks
 //                on tiles that cross the row's range, running maximum (O is rescaled only when it
 //                grows by more than 2^8), exp2, row sum, P times V's factors as fp16.
@@ -26,8 +28,8 @@ constexpr int kTileRows = 128;
 constexpr int kRows = 2 * kTileRows;  // query rows of a block
 constexpr int kKeys = 128;            // cache rows of a tile
 constexpr int kThreads = 512;
-// setmaxnreg split of the 128 x 512 registers at launch: MMA warpgroup, softmax warpgroups, converters
-constexpr uint32_t kRegsMma = 40, kRegsSoftmax = 184, kRegsConvert = 104;
+// setmaxnreg split of the 128 x 512 registers at launch: warps 0-3, softmax warpgroups, converters
+constexpr uint32_t kRegsMma = 64, kRegsSoftmax = 184, kRegsConvert = 80;
 static_assert(128 * (kRegsMma + 2 * kRegsSoftmax + kRegsConvert) <= 128 * kThreads, "setmaxnreg split exceeds the launch");
 constexpr float kSlack = 8.0f;    // the maximum may lag by 2^8 before O is rescaled
 constexpr float kVUnit = 128.0f;  // P * (v scale / largest) * 128 <= 2^15 stays in fp16's range
@@ -41,7 +43,10 @@ struct Cfg {
   static constexpr int NS = D == 64 ? 3 : 2;          // K and V ring depth
   static constexpr int K_OFF = 2 * TILE;              // after the two Q tiles
   static constexpr int V_OFF = K_OFF + NS * TILE;
-  static constexpr int BAR_OFF = V_OFF + NS * TILE;
+  static constexpr int RAW = kKeys * D;               // one tile's int8 rows
+  static constexpr int NR = D == 64 ? 4 : 2;          // ring of them, K and V in turn
+  static constexpr int RAW_OFF = V_OFF + NS * TILE;
+  static constexpr int BAR_OFF = RAW_OFF + NR * RAW;
   static constexpr int SMEM = BAR_OFF + 1024 + 1024;  // barriers and factors, alignment slack
   static __device__ __forceinline__ uint32_t s_col(int t) { return t ? 128u : 0u; }
   static __device__ __forceinline__ uint32_t o_col(int t) { return 256u + static_cast<uint32_t>(t * D); }
@@ -50,6 +55,7 @@ struct Cfg {
 struct Shared {
   uint64_t q_ready[2], s_full[2], p_full[2], o_full[2];
   uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
+  uint64_t raw_full[4], raw_empty[4];
   float k_factor[kFactorRing][kFactors];
   float v_factor[kFactorRing][kFactors];
   float v_max[4];
@@ -102,13 +108,54 @@ __device__ __forceinline__ void convert16(const uint4& v, uint4& lo, uint4& hi) 
   hi = make_uint4(half2_of(w2, 0x4140), half2_of(w2, 0x4342), half2_of(w3, 0x4140), half2_of(w3, 0x4342));
 }
 
+// D[tmem] (+)= A * B with A's descriptor or tensor memory address, issued by one lane of the warp, which
+// runs this together on warp-uniform operands.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(ad), "l"(bd), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t at, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(at), "l"(bd), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void commit_elected(uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void arrive_elected(uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n @e mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];\n}\n" ::"r"(
+          smem_u32(bar))
+      : "memory");
+}
+// `bytes` (a multiple of 16) from global to shared memory, both 16-byte aligned, counted on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// A wait that the whole warp leaves together, with one answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_t* status) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
+}
+
 template <int D, bool MOD>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_constant__ Kv8AttnArgs a) {
   using C = Cfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Shared& sh = *reinterpret_cast<Shared*>(smem + C::BAR_OFF);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int32_t H = a.g.n_kv_heads, G = a.g.n_q_heads / H, ps = a.g.page_shift;
   // longest ranges first: a sequence's last tiles see the most
   const int32_t h = static_cast<int32_t>(blockIdx.x % H);
@@ -160,10 +207,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       mbar_init(&sh.o_full[t], 1);
     }
     for (int i = 0; i < C::NS; ++i) {
-      mbar_init(&sh.k_full[i], 128);
+      mbar_init(&sh.k_full[i], 128 + 1);  // the converters, and warp 2 with the tile's factors
       mbar_init(&sh.k_empty[i], 1);
       mbar_init(&sh.v_full[i], 128);
       mbar_init(&sh.v_empty[i], 1);
+    }
+    for (int i = 0; i < C::NR; ++i) {
+      mbar_init(&sh.raw_full[i], 1);
+      mbar_init(&sh.raw_empty[i], 4);
     }
     fence_mbar_init();
   }
@@ -173,114 +224,177 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
   tc_fence_after();
   const uint32_t tmem = sh.tmem_base;
 
+  const int32_t row_end = min(je * kKeys, tl.kv_len);  // rows from here on are not read
+  const int32_t* const table = a.block_table + static_cast<int64_t>(tl.b) * a.g.max_pages;
+  bool stray = false;
   if (warp < 4) {
-    // ------------------------------------------------------------------ MMA issuer (one thread)
     regs_dealloc<kRegsMma>();
-    if (threadIdx.x == 0 && n_load > 0) {
+    if (warp == 0) {
+      // ---------------------------------------------------------------- MMA issuer
       constexpr uint32_t idesc_qk = make_idesc_f16(kTileRows, kKeys, 0, 0);
       constexpr uint32_t idesc_pv = make_idesc_f16(kTileRows, D, 0, 1);
-      const uint32_t q_addr = smem_u32(smem), k_addr = smem_u32(smem + C::K_OFF), v_addr = smem_u32(smem + C::V_OFF);
+      auto uni = [](int32_t v) { return __shfl_sync(0xffffffffu, v, 0); };
+      const int32_t n = uni(n_load);
+      const int32_t lo0 = uni(j0[0] - jb), hi0 = uni(j1[0] - jb), lo1 = uni(j0[1] - jb), hi1 = uni(j1[1] - jb);
+      const uint32_t tm = static_cast<uint32_t>(uni(static_cast<int32_t>(tmem)));
+      const uint32_t base = static_cast<uint32_t>(uni(static_cast<int32_t>(smem_u32(smem))));
+      // descriptors count in 16-byte units: an operand `off` bytes on is + off / 16
+      const uint64_t q_desc = make_sw128_desc(base, 16, 1024), k_desc = make_sw128_desc(base + C::K_OFF, 16, 1024);
+      const uint64_t v_desc = make_sw128_desc(base + C::V_OFF, kKeys * 128, 1024);
       auto issue_qk = [&](int t, int s) {
+        const uint64_t qd = q_desc + t * (C::TILE / 16), kd = k_desc + s * (C::TILE / 16);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * (kKeys * 128) + (kk & 3) * 32;
-          umma_f16_ss(tmem + C::s_col(t), make_sw128_desc(q_addr + t * C::TILE + off, 16, 1024),
-                      make_sw128_desc(k_addr + s * C::TILE + off, 16, 1024), idesc_qk, kk > 0);
+          constexpr int kBlock = kKeys * 128;
+          const uint32_t off = ((kk >> 2) * kBlock + (kk & 3) * 32) / 16;
+          mma_ss(tm + C::s_col(t), qd + off, kd + off, idesc_qk, kk > 0);
         }
-        umma_commit(&sh.s_full[t]);
-        mbar_arrive(&sh.s_full[t]);  // passes on what the converters wrote besides (the factors)
+        commit_elected(&sh.s_full[t]);
+        arrive_elected(&sh.s_full[t]);  // passes on what was written besides (the factors)
       };
       auto issue_pv = [&](int t, int s, bool first) {
+        const uint64_t vd = v_desc + s * (C::TILE / 16);
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
-          umma_f16_ts(tmem + C::o_col(t), tmem + C::s_col(t) + kk * 8,
-                      make_sw128_desc(v_addr + s * C::TILE + kk * 2048, kKeys * 128, 1024), idesc_pv, !first || kk > 0);
+          mma_ts(tm + C::o_col(t), tm + C::s_col(t) + kk * 8, vd + kk * (2048 / 16), idesc_pv, !first || kk > 0);
       };
-      const int32_t t_lo[2] = {j0[0] - jb, j0[1] - jb}, t_hi[2] = {j1[0] - jb, j1[1] - jb};
-      bool ok = mbar_wait(&sh.q_ready[0], 0, status) && mbar_wait(&sh.q_ready[1], 0, status) &&
-                mbar_wait(&sh.k_full[0], 0, status);
+      bool ok = n > 0 && warp_wait(&sh.q_ready[0], 0, status) && warp_wait(&sh.q_ready[1], 0, status) &&
+                warp_wait(&sh.k_full[0], 0, status);
       tc_fence_after();
       if (ok) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (t_lo[t] <= 0 && t_hi[t] > 0) issue_qk(t, 0);
-        umma_commit(&sh.k_empty[0]);
+        if (lo0 <= 0 && hi0 > 0) issue_qk(0, 0);
+        if (lo1 <= 0 && hi1 > 0) issue_qk(1, 0);
+        commit_elected(&sh.k_empty[0]);
       }
-      for (int32_t i = 0; ok && i < n_load; ++i) {
-        const int s = i % C::NS, s1 = (i + 1) % C::NS;
-        if (!mbar_wait(&sh.v_full[s], (i / C::NS) & 1, status)) break;
-        if (i + 1 < n_load && !mbar_wait(&sh.k_full[s1], ((i + 1) / C::NS) & 1, status)) break;
+      int s = 0;
+      uint32_t par = 0;
+      for (int32_t i = 0; ok && i < n; ++i) {
+        const int s1 = s + 1 == C::NS ? 0 : s + 1;
+        const uint32_t par1 = s1 ? par : par ^ 1;
+        bool go = warp_wait(&sh.v_full[s], par, status) && (i + 1 >= n || warp_wait(&sh.k_full[s1], par1, status));
+        if (!go) break;
         tc_fence_after();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (i >= t_lo[t] && i < t_hi[t]) {
-            if (!mbar_wait(&sh.p_full[t], (i - t_lo[t]) & 1, status)) {
-              ok = false;
-              break;
-            }
+          const int32_t t_lo = t ? lo1 : lo0, t_hi = t ? hi1 : hi0;
+          if (i >= t_lo && i < t_hi) {
+            go = warp_wait(&sh.p_full[t], (i - t_lo) & 1, status);
+            if (!go) break;
             tc_fence_after();
-            issue_pv(t, s, i == t_lo[t]);
-            if (i + 1 == t_hi[t]) umma_commit(&sh.o_full[t]);
+            issue_pv(t, s, i == t_lo);
+            if (i + 1 == t_hi) commit_elected(&sh.o_full[t]);
           }
-          if (i + 1 >= t_lo[t] && i + 1 < t_hi[t]) issue_qk(t, s1);
+          if (i + 1 >= t_lo && i + 1 < t_hi) issue_qk(t, s1);
+        }
+        if (!go) break;
+        commit_elected(&sh.v_empty[s]);
+        if (i + 1 < n) commit_elected(&sh.k_empty[s1]);
+        s = s1;
+        par = par1;
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- int8 rows, page by page
+      // lane f copies the tile's f-th page (a page holds 16 to 128 of its 128 rows); its table entry is
+      // read two tiles ahead
+      const int32_t per_page = min(a.g.page_rows, kKeys), n_seg = kKeys / per_page;
+      auto entry_of = [&](int32_t i) -> int32_t {
+        const int32_t row = (jb + i) * kKeys + lane * per_page;
+        return lane < n_seg && row < row_end ? table[row >> ps] : INT32_MIN;
+      };
+      int32_t e0 = n_load > 0 ? entry_of(0) : INT32_MIN, e1 = n_load > 1 ? entry_of(1) : INT32_MIN;
+      int32_t issued = 0;
+      for (int32_t i = 0; i < n_load; ++i) {
+        const int32_t e = e0;
+        e0 = e1;
+        if (i + 2 < n_load) e1 = entry_of(i + 2);
+        const bool mine = e != INT32_MIN;
+        const int64_t page = mine ? page_or_first(e, a.g.n_pages, stray) : 0;
+        const int64_t at = ((page * H + h) << ps) * D;  // a tile starts at a page's first row: pages divide it
+        const uint32_t bytes = static_cast<uint32_t>(per_page * D);
+        const uint32_t total = __popc(__ballot_sync(0xffffffffu, mine)) * bytes;
+        bool ok = true;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const int32_t g = 2 * i + v, slot = g % C::NR;
+          ok = ok && warp_wait(&sh.raw_empty[slot], ((g / C::NR) & 1) ^ 1, status);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&sh.raw_full[slot], total);
+          __syncwarp();
+          if (mine) bulk_load(smem + C::RAW_OFF + slot * C::RAW + lane * bytes, (v ? a.v_pool : a.k_pool) + at, bytes,
+                              &sh.raw_full[slot]);
+          issued = g + 1;
         }
         if (!ok) break;
-        umma_commit(&sh.v_empty[s]);
-        if (i + 1 < n_load) umma_commit(&sh.k_empty[s1]);
+      }
+      // the last copies have landed before the block may end, however its other warps fared
+      for (int32_t g = max(issued - C::NR, 0); g < issued; ++g)
+        warp_wait(&sh.raw_full[g % C::NR], (g / C::NR) & 1, status);
+    } else if (warp == 2) {
+      // ---------------------------------------------------------------- factors
+      float ks[2] = {0.0f, 0.0f}, vs[2] = {0.0f, 0.0f};
+      bool on[2] = {false, false};
+      int32_t e_next = 0;
+      auto entry_of = [&](int32_t i) -> int32_t {
+        const int32_t row = (jb + i) * kKeys + lane * 16;
+        return i < n_load && lane < kFactors && row < row_end ? table[row >> ps] : INT32_MIN;
+      };
+      auto fetch = [&](int32_t e, int k) {
+        on[k] = e != INT32_MIN;
+        if (on[k]) {
+          const int64_t at = page_or_first(e, a.g.n_pages, stray) * H + h;
+          ks[k] = __ldg(a.k_scale + at);
+          vs[k] = __ldg(a.v_scale + at);
+        }
+      };
+      fetch(entry_of(0), 0);
+      e_next = entry_of(1);
+      asm volatile("bar.sync 2, 160;" ::: "memory");
+      const float vmax = fmaxf(fmaxf(sh.v_max[0], sh.v_max[1]), fmaxf(sh.v_max[2], sh.v_max[3]));
+      const float v_unit = vmax > 0.0f ? kVUnit / vmax : 0.0f;
+      const float k_unit = MOD && a.score_cap > 0.0f ? a.scale / a.score_cap : a.scale * kLog2e;
+      for (int32_t i = 0; i < n_load; ++i) {
+        fetch(e_next, 1);
+        e_next = entry_of(i + 2);
+        const int s = i % C::NS;
+        // the tile NS before is done with: so is the ring's slot, and k_full's phase is this tile's
+        if (!warp_wait(&sh.v_empty[s], ((i / C::NS) & 1) ^ 1, status)) break;
+        if (lane < kFactors) {
+          // A scale that is no number marks the page through K's factor: a hidden row's weight is then 0
+          // and its V factor must not turn it into NaN again.
+          const bool fine = vs[0] < INFINITY;
+          sh.k_factor[i % kFactorRing][lane] = !on[0] ? 0.0f : fine ? ks[0] * k_unit : __uint_as_float(0x7fffffffu);
+          sh.v_factor[i % kFactorRing][lane] = !on[0] || !fine ? 0.0f : vs[0] * v_unit;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.k_full[s]);
+        ks[0] = ks[1], vs[0] = vs[1], on[0] = on[1];
       }
     }
+    if (stray) atomicOr(status, kStatusBadIndex);
   } else if (warp >= 12) {
     // ------------------------------------------------------------------ converters
     regs_dealloc<kRegsConvert>();
     const int w = warp - 12;
-    const int32_t* const table = a.block_table + static_cast<int64_t>(tl.b) * a.g.max_pages;
-    const int32_t row_end = min(je * kKeys, tl.kv_len);  // rows from here on are not read
-    bool stray = false;
-    // the chunk's largest V scale
-    float vmax = 0.0f;
-    for (int32_t k = ((jb * kKeys) >> ps) + w * 32 + lane; k < (row_end + a.g.page_rows - 1) >> ps; k += 128)
-      vmax = fmaxf(vmax, __ldg(a.v_scale + page_or_first(table[k], a.g.n_pages, stray) * H + h));
+    {
+      float vmax = 0.0f;  // the chunk's largest V scale
+      for (int32_t k = ((jb * kKeys) >> ps) + w * 32 + lane; k < (row_end + a.g.page_rows - 1) >> ps; k += 128)
+        vmax = fmaxf(vmax, __ldg(a.v_scale + page_or_first(table[k], a.g.n_pages, stray) * H + h));
 #pragma unroll
-    for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-    if (lane == 0) sh.v_max[w] = vmax;
-    asm volatile("bar.sync 2, 128;" ::: "memory");
-    vmax = fmaxf(fmaxf(sh.v_max[0], sh.v_max[1]), fmaxf(sh.v_max[2], sh.v_max[3]));
-    const float v_unit = vmax > 0.0f ? kVUnit / vmax : 0.0f;
-    const bool capped = MOD && a.score_cap > 0.0f;
-    const float k_unit = capped ? a.scale / a.score_cap : a.scale * kLog2e;
-
-    // A warp and load step covers 512 consecutive bytes of a page: 4 rows of 128 (or 8 of 64), so that
-    // 8 lanes storing together fall into different banks.
-    constexpr int RPL = 512 / D;          // rows per load
+      for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+      if (lane == 0) sh.v_max[w] = vmax;
+      asm volatile("bar.sync 2, 160;" ::: "memory");
+    }
+    // 16 bytes a lane. Eight lanes that load or store together take two rows, the even row's chunks of
+    // one half and the odd row's of the other (D = 128; D = 64: two whole rows): different banks both ways.
+    constexpr int RPL = 512 / D;           // rows per warp and load
     constexpr int NL = kKeys / (4 * RPL);  // loads per tile and lane
-    const int c = D == 128 ? (lane & 3) + ((lane >> 3) & 1) * 4 : lane & 3;                  // 16-byte chunk of the row
-    const int r_in = D == 128 ? ((lane >> 2) & 1) + ((lane >> 4) << 1) : lane >> 2;          // row of the load
-    uint4 kr[NL], vr[NL];
-    int32_t page = 0;  // lane f < 8: page of the tile's rows [16 f, 16 f + 16), -1 past the end
-    float ksf = 0.0f, vsf = 0.0f;
-    auto pages_of = [&](int32_t i) {
-      const int32_t row = (jb + i) * kKeys + (lane & 7) * 16;
-      page = row < row_end ? static_cast<int32_t>(page_or_first(table[row >> ps], a.g.n_pages, stray)) : -1;
-    };
-    auto scales_of = [&] {
-      if (w == 0 && lane < kFactors && page >= 0) {
-        ksf = __ldg(a.k_scale + static_cast<int64_t>(page) * H + h);
-        vsf = __ldg(a.v_scale + static_cast<int64_t>(page) * H + h);
-      }
-    };
-    auto load = [&](const int8_t* pool, int32_t i, uint4 (&v)[NL]) {
+    const int r_in = D == 128 ? ((lane >> 2) & 1) + ((lane >> 4) << 1) : lane >> 2;
+    const int c = D == 128 ? (lane & 3) + ((((lane >> 3) ^ (lane >> 2)) & 1) << 2) : lane & 3;
+    auto convert = [&](const uint8_t* src, uint8_t* dst, uint64_t* free_bar) {
+      uint4 v[NL];
 #pragma unroll
-      for (int k = 0; k < NL; ++k) {
-        const int unit = k * 4 + w;  // rows [unit * RPL, (unit + 1) * RPL) of the tile: within one page
-        const int32_t p = __shfl_sync(0xffffffffu, page, unit * RPL / 16);
-        const int32_t row = (jb + i) * kKeys + unit * RPL + r_in;
-        v[k] = make_uint4(0, 0, 0, 0);
-        if (p >= 0)
-          v[k] = __ldg(reinterpret_cast<const uint4*>(
-              pool + (((static_cast<int64_t>(p) * H + h) << ps) + (row & (a.g.page_rows - 1))) * D + c * 16));
-      }
-    };
-    auto store = [&](uint8_t* dst, const uint4 (&v)[NL]) {
+      for (int k = 0; k < NL; ++k)
+        v[k] = *reinterpret_cast<const uint4*>(src + ((k * 4 + w) * RPL + r_in) * D + c * 16);
 #pragma unroll
       for (int k = 0; k < NL; ++k) {
         const int row = (k * 4 + w) * RPL + r_in;
@@ -289,32 +403,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         *reinterpret_cast<uint4*>(dst + chunk_off(row, 2 * c)) = lo;
         *reinterpret_cast<uint4*>(dst + chunk_off(row, 2 * c + 1)) = hi;
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(free_bar);
       fence_proxy_async_smem();
     };
-    if (n_load > 0) {
-      pages_of(0);
-      load(a.k_pool, 0, kr);
-    }
     for (int32_t i = 0; i < n_load; ++i) {
       const int s = i % C::NS;
       const uint32_t par = ((i / C::NS) & 1) ^ 1;
-      load(a.v_pool, i, vr);
-      scales_of();
-      const int32_t now = page;
-      if (i + 1 < n_load) pages_of(i + 1);
-      if (!mbar_wait(&sh.k_empty[s], par, status)) break;
-      if (w == 0 && lane < kFactors) {
-        // A scale that is no number marks the page through K's factor: a hidden row's weight is then 0
-        // and its V factor must not turn it into NaN again.
-        const bool fine = vsf < INFINITY;
-        sh.k_factor[i % kFactorRing][lane] = now < 0 ? 0.0f : fine ? ksf * k_unit : __uint_as_float(0x7fffffffu);
-        sh.v_factor[i % kFactorRing][lane] = now < 0 || !fine ? 0.0f : vsf * v_unit;
-      }
-      store(smem + C::K_OFF + s * C::TILE, kr);
+      const int gk = 2 * i, gv = 2 * i + 1;
+      if (!warp_wait(&sh.raw_full[gk % C::NR], (gk / C::NR) & 1, status)) break;
+      if (!warp_wait(&sh.k_empty[s], par, status)) break;
+      convert(smem + C::RAW_OFF + (gk % C::NR) * C::RAW, smem + C::K_OFF + s * C::TILE, &sh.raw_empty[gk % C::NR]);
       mbar_arrive(&sh.k_full[s]);
-      if (i + 1 < n_load) load(a.k_pool, i + 1, kr);
-      if (!mbar_wait(&sh.v_empty[s], par, status)) break;
-      store(smem + C::V_OFF + s * C::TILE, vr);
+      if (!warp_wait(&sh.raw_full[gv % C::NR], (gv / C::NR) & 1, status)) break;
+      if (!warp_wait(&sh.v_empty[s], par, status)) break;
+      convert(smem + C::RAW_OFF + (gv % C::NR) * C::RAW, smem + C::V_OFF + s * C::TILE, &sh.raw_empty[gv % C::NR]);
       mbar_arrive(&sh.v_full[s]);
     }
     if (stray) atomicOr(status, kStatusBadIndex);
@@ -346,9 +449,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       };
       const float fpos = static_cast<float>(pos);
       constexpr int NC = D / 8;
-#pragma unroll 2
+      uint4 x[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) x[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
+#pragma unroll
       for (int c = 0; c < NC / 2; ++c) {
-        uint4 v[2] = {__ldg(reinterpret_cast<const uint4*>(src) + c), __ldg(reinterpret_cast<const uint4*>(src) + c + NC / 2)};
+        uint4 v[2] = {x[c], x[c + NC / 2]};
         uint32_t* const u0 = reinterpret_cast<uint32_t*>(&v[0]);
         uint32_t* const u1 = reinterpret_cast<uint32_t*>(&v[1]);
         if (a.rope_mode == AIHOST_ROPE_NEOX) {
@@ -386,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     const int32_t lo_j = t ? j0[1] : j0[0], hi_j = t ? j1[1] : j1[0], n_own = hi_j - lo_j;
     bool ok = true;
     for (int32_t i = 0; i < n_own; ++i) {
-      if (!mbar_wait(&sh.s_full[t], i & 1, status)) {
+      if (!warp_wait(&sh.s_full[t], i & 1, status)) {
         ok = false;
         break;
       }
@@ -473,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       mbar_arrive(&sh.p_full[t]);
     }
     // ---- O / l, or this chunk's share of it
-    if (ok && n_own > 0) ok = mbar_wait(&sh.o_full[t], 0, status);
+    if (ok && n_own > 0) ok = warp_wait(&sh.o_full[t], 0, status);
     tc_fence_after();
     // written by the converters before the first S; with no tile there is nothing to scale
     const float vmax =
@@ -494,12 +600,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         for (int v = 0; v < 8; ++v) dst[v] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
       }
     };
-    const bool whole = __all_sync(0xffffffffu, ok);
     const int64_t unit = static_cast<int64_t>(tile) * H + h;
     // partials: [unit][split][D / 4][256 rows] of 4 floats, so that a warp's rows lie together
     float4* const part = reinterpret_cast<float4*>(a.part_o) + (unit * a.max_splits) * (D / 4) * kRows + rr;
     float2* const part_ml = reinterpret_cast<float2*>(a.part_ml) + unit * a.max_splits * kRows + rr;
-    if (whole) {
+    if (ok) {
       const float unit_o = n_splits > 1 ? o_unit : l != 0.0f ? o_unit / l : 0.0f;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
