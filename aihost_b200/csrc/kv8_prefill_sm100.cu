@@ -108,6 +108,40 @@ __device__ __forceinline__ void convert16(const uint4& v, uint4& lo, uint4& hi) 
   hi = make_uint4(half2_of(w2, 0x4140), half2_of(w2, 0x4342), half2_of(w3, 0x4140), half2_of(w3, 0x4342));
 }
 
+// score = cap * tanh(x), x in units of the cap, times log2 e (cap2 = cap * log2 e). Where the whole
+// warp has |x| <= 1, tanh x = x * P(x^2) on the FMA pipe: P of degree 6, our weighted least-squares fit
+// on [0, 1], 5e-8 off (the exponentials already fill the SFU). Else 1 - 2 / (1 + e^2x).
+__device__ __forceinline__ void cap_scores(uint32_t (&sr)[4][32], float cap2) {
+  float top = 0.0f;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(__uint_as_float(sr[c][e])));
+  if (__any_sync(0xffffffffu, top > 1.0f)) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int e = 0; e < 32; ++e) sr[c][e] = __float_as_uint(cap2 * tanh_of(__uint_as_float(sr[c][e])));
+    return;
+  }
+  constexpr float kP[7] = {0.9999999403953552f,  -0.33332839608192444f, 0.13325203955173492f, -0.05345702916383743f,
+                           0.020289979875087738f, -0.006203378085047007f, 0.001041022245772183f};
+  const float2 cap22 = make_float2(cap2, cap2);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      const float2 x = make_float2(__uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
+      const float2 y = fmul2(x, x);
+      float2 p = make_float2(kP[6], kP[6]);
+#pragma unroll
+      for (int k = 5; k >= 0; --k) p = ffma2(p, y, make_float2(kP[k], kP[k]));
+      p = fmul2(fmul2(x, cap22), p);
+      sr[c][e] = __float_as_uint(p.x);
+      sr[c][e + 1] = __float_as_uint(p.y);
+    }
+}
+
 // D[tmem] (+)= A * B with A's descriptor or tensor memory address, issued by one lane of the warp, which
 // runs this together on warp-uniform operands.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
@@ -449,14 +483,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       };
       const float fpos = static_cast<float>(pos);
       constexpr int NC = D / 8;
-      uint4 x[NC];
-#pragma unroll
-      for (int c = 0; c < NC; ++c) x[c] = __ldg(reinterpret_cast<const uint4*>(src) + c);
-#pragma unroll
+      // a loop, not unrolled: it runs once per block, from a cold instruction cache
+      const uint4* const src4 = reinterpret_cast<const uint4*>(src);
+      uint4 x0 = __ldg(src4), x1 = __ldg(src4 + NC / 2);
+#pragma unroll 1
       for (int c = 0; c < NC / 2; ++c) {
-        uint4 v[2] = {x[c], x[c + NC / 2]};
-        uint32_t* const u0 = reinterpret_cast<uint32_t*>(&v[0]);
-        uint32_t* const u1 = reinterpret_cast<uint32_t*>(&v[1]);
+        uint32_t u0[4] = {x0.x, x0.y, x0.z, x0.w}, u1[4] = {x1.x, x1.y, x1.z, x1.w};
+        if (c + 1 < NC / 2) {
+          x0 = __ldg(src4 + c + 1);
+          x1 = __ldg(src4 + c + 1 + NC / 2);
+        }
         if (a.rope_mode == AIHOST_ROPE_NEOX) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -477,8 +513,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             u1[k] = lo | (hi << 16);
           }
         }
-        *reinterpret_cast<uint4*>(q_tile + chunk_off(r, c)) = v[0];
-        *reinterpret_cast<uint4*>(q_tile + chunk_off(r, c + NC / 2)) = v[1];
+        *reinterpret_cast<uint4*>(q_tile + chunk_off(r, c)) = make_uint4(u0[0], u0[1], u0[2], u0[3]);
+        *reinterpret_cast<uint4*>(q_tile + chunk_off(r, c + NC / 2)) = make_uint4(u1[0], u1[1], u1[2], u1[3]);
       }
       fence_proxy_async_smem();
       mbar_arrive(&sh.q_ready[t]);
@@ -507,20 +543,36 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
 #pragma unroll
       for (int f = 0; f < kFactors; ++f) kf[f] = sh.k_factor[slot][f];
       tmem_wait_ld();
-      if (MOD || need_mask) {  // scores in log2 units, hidden ones -inf; the factors are then spent
+      if (MOD || need_mask) {  // the factors are spent here: scores in log2 units, hidden ones -inf
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int32_t j = kv0 + c * 32 + e;
-            float x = __uint_as_float(sr[c][e]) * kf[c * 2 + e / 16];
-            if constexpr (MOD) {
-              if (capped) x = cap2 * tanh_of(x);
-              x = fmaf(-slope, fabsf(fpos - static_cast<float>(j)), x);
-            }
-            if (j < first || j >= end) x = -INFINITY;
-            sr[c][e] = __float_as_uint(x);
+          for (int e = 0; e < 32; e += 2) {
+            const float f = kf[c * 2 + e / 16];
+            const float2 x = fmul2(make_float2(__uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1])), make_float2(f, f));
+            sr[c][e] = __float_as_uint(x.x);
+            sr[c][e + 1] = __float_as_uint(x.y);
           }
+        if constexpr (MOD) {
+          if (capped) cap_scores(sr, cap2);
+          if (a.alibi_slopes) {
+            const float d0 = fpos - static_cast<float>(kv0);
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                sr[c][e] = __float_as_uint(
+                    fmaf(-slope, fabsf(d0 - static_cast<float>(c * 32 + e)), __uint_as_float(sr[c][e])));
+          }
+        }
+        if (need_mask) {
+          const int32_t lo_e = first - kv0, hi_e = end - kv0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e < lo_e || c * 32 + e >= hi_e) sr[c][e] = __float_as_uint(-INFINITY);
+        }
 #pragma unroll
         for (int f = 0; f < kFactors; ++f) kf[f] = 1.0f;
       }
