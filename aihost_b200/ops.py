@@ -78,18 +78,12 @@ class Context:
         self._h = ctypes.c_void_p()
         check(lib().aihost_attn_create(int(device), ctypes.byref(self._h)))
         self.device = device
-        self.reserved = 0  # scratch bytes asked for through reserve()
 
     @property
     def handle(self) -> ctypes.c_void_p:
         if not self._h:
             raise AttnError(EINVAL, "context is closed")
         return self._h
-
-    def reserve(self, need: int) -> None:
-        """Grow the scratch to at least `need` bytes."""
-        check(lib().aihost_attn_reserve(self.handle, need))
-        self.reserved = max(self.reserved, need)
 
     def reserve_for(self, spec: LayerSpec, batch: int, n_new: int) -> None:
         need = ctypes.c_size_t()
