@@ -7,11 +7,12 @@
 //   S^T = K Q^T     K's int8 go to fp16 exactly in registers, one fp32 factor per page afterwards
 //   online softmax  running maximum per query row, moved only when it grows by more than 2^8
 //   O^T += V^T P^T  V likewise exact; P carries the page's scale relative to the chunk's largest
-// The k order of either product is free, so it is chosen such that every lane reads 16 bytes of a
-// cache row at a time straight from global memory: 8 lanes (V) or 4 lanes of two loads (K) cover a
-// 128-byte row, and no shared memory or transpose is needed. The next step's rows are in flight in
-// registers while a step is computed. Warps merge through shared memory, chunks through partials
-// that the last block to arrive merges (no block waits for another).
+// The k order of either product is free, so it is chosen such that every lane takes 16 bytes of a
+// cache row at a time and no transpose is needed. Each warp copies its own steps' rows into a ring of
+// its own in shared memory (cp.async, three steps ahead, chunks swizzled against bank conflicts): no
+// warp waits for another in the loop. A lane holds the page and scales of one of the warp's next 32
+// steps. Warps merge through shared memory, chunks through partials that the last block to arrive
+// merges (no block waits for another).
 #include "common.cuh"
 #include "kv8.h"
 #include "kv8_tile.cuh"
@@ -21,7 +22,9 @@ namespace aihost {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStep = 16;
+constexpr int kStep = 16;   // cache rows of a step; a block's warps take steps in turn
+constexpr int kStages = 4;  // of the warp's ring
+constexpr int kChunkMin = 64, kChunkMax = 2048;
 
 // What the products take: fp16 operands, q as a pair of fp16 (rotated in fp32), or q and P as pairs
 // (fp32 tensors).
@@ -56,17 +59,42 @@ __device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t h) {
   return pack2(lo - f.x, hi - f.y);
 }
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Where 16-byte chunk c of a step's row r lies: lanes that load together, 8 chunks of two rows (K) or
+// one or two chunks of four rows two apart (V), fall into different banks.
+template <int D>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  if (D == 128) return static_cast<uint32_t>(r * 128 + ((c ^ (r & 7)) << 4));
+  return static_cast<uint32_t>((r >> 1) * 128 + ((((r & 1) * 4 + c) ^ (r & 6)) << 4));
+}
+
+template <int D, int NT>
+struct SplitSmem {  // the rings, and over them the merge's O
+  static constexpr int kStageBytes = 2 * kStep * D;
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kMerge = kWarps * NT * 8 * (D + 4) * 4;
+  static constexpr int kBytes = kRing > kMerge ? kRing : kMerge;
+};
+
 template <int D, int NT, int PREC, bool MOD>
-__global__ void __launch_bounds__(kWarps * 32) kv8_mma_kernel(const __grid_constant__ Kv8AttnArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(const __grid_constant__ Kv8AttnArgs a) {
   constexpr int R = NT * 8;
   constexpr int KS = D / 16;       // k steps of S^T = K Q^T
   constexpr int KC = D / 64;       // 16-byte chunks of a K row per lane
   constexpr int MT = D / 16;       // 16-row tiles of O^T
   constexpr int VW = D / 32;       // 32-bit words of a V row per lane
   constexpr int NQ = PREC == kPlain ? 1 : 2;
-  __shared__ float o_sh[kWarps][R][D + 4];
+  extern __shared__ __align__(128) uint8_t ring[];
+  float(*const o_sh)[R][D + 4] = reinterpret_cast<float(*)[R][D + 4]>(ring);
   __shared__ float ml_sh[kWarps][R][2];
-  __shared__ float vmax_sh[kWarps];
   __shared__ int32_t last_sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
   const int32_t H = a.g.n_kv_heads, G = a.g.n_q_heads / H, ps = a.g.page_shift;
@@ -105,53 +133,49 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mma_kernel(const __grid_const
   if (split >= n_splits) return;
   const int32_t k_begin = base + split * a.chunk, k_end = min(hi, k_begin + a.chunk);
   const int32_t* const table = a.block_table + static_cast<int64_t>(tl.b) * a.g.max_pages;
-  // a page id outside the pool reads page 0 and sets the status
-  bool stray = false;
-  auto page_at = [&](int32_t row) -> int64_t { return page_or_first(table[row >> ps], a.g.n_pages, stray); };
+  bool stray = false;  // a page id outside the pool reads page 0 and sets the status
 
-  // ---- the step's rows, one step ahead
-  uint4 kb[2][KC];
-  uint32_t vb[4][VW];
-  float ks_next = 0.0f, vs_next = 0.0f;
-  auto fetch = [&](int32_t k, int64_t page) {
-    const int64_t ph = page * H + h;
-    const int64_t at = ((ph << ps) + (k & (a.g.page_rows - 1))) * D;
-    const int8_t* kp = a.k_pool + at + (g * D + t4 * (KC * 16));
+  // ---- this warp's steps: step i is rows [k_of(i), k_of(i) + 16)
+  auto k_of = [&](int32_t i) { return k_begin + (i * kWarps + warp) * kStep; };
+  const int32_t n_steps = k_begin + warp * kStep < k_end ? (k_end - k_begin - warp * kStep - 1) / (kWarps * kStep) + 1 : 0;
+  // lane j: page, K factor and V scale of step 32 * round + j
+  auto page_of = [&](int32_t i) -> int32_t {
+    return i < n_steps ? static_cast<int32_t>(page_or_first(table[k_of(i) >> ps], a.g.n_pages, stray)) : 0;
+  };
+  int32_t page = page_of(lane), page_next = n_steps > 32 ? page_of(32 + lane) : 0;
+  const uint32_t my_ring = smem_u32(ring) + warp * (kStages * SplitSmem<D, NT>::kStageBytes);
+  auto fetch = [&](int32_t i, int32_t round) {
+    if (i < n_steps) {
+      const int64_t pg = __shfl_sync(0xffffffffu, (i >> 5) == round ? page : page_next, i & 31);
+      const int64_t at = (((pg * H + h) << ps) + (k_of(i) & (a.g.page_rows - 1))) * D;
+      const uint32_t dst = my_ring + (i % kStages) * SplitSmem<D, NT>::kStageBytes;
+      constexpr int CR = D / 16;  // chunks per row
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int c = 0; c < KC; ++c) kb[r][c] = __ldg(reinterpret_cast<const uint4*>(kp + r * 8 * D + c * 16));
-    const int8_t* vp = a.v_pool + at + (2 * t4 * D + g * (VW * 4));
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int8_t* p = vp + ((r & 1) + (r >> 1) * 8) * D;
-      if constexpr (VW == 4) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-        vb[r][0] = v.x, vb[r][1] = v.y, vb[r][2] = v.z, vb[r][3] = v.w;
-      } else {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-        vb[r][0] = v.x, vb[r][1] = v.y;
+      for (int j = 0; j < kStep * CR / 32; ++j) {
+        const int ch = j * 32 + lane, r = ch / CR, c = ch % CR;
+        copy16(dst + chunk_at<D>(r, c), a.k_pool + at + ch * 16);
+        copy16(dst + kStep * D + chunk_at<D>(r, c), a.v_pool + at + ch * 16);
       }
     }
-    ks_next = __ldg(a.k_scale + ph);
-    vs_next = __ldg(a.v_scale + ph);
+    copies_commit();
   };
-  const int32_t k0 = k_begin + warp * kStep;
-  int64_t page = 0;
-  if (k0 < k_end) fetch(k0, page_at(k0));
-  if (k0 + kWarps * kStep < k_end) page = page_at(k0 + kWarps * kStep);
-
-  // ---- the chunk's largest V scale: P is scaled relative to it (a NaN scale is passed over here and
-  // reaches the result through its own page's factor)
-  float vmax = 0.0f;
-  for (int32_t k = (k_begin >> ps) + static_cast<int32_t>(threadIdx.x); k < (k_end + a.g.page_rows - 1) >> ps;
-       k += kWarps * 32)
-    vmax = fmaxf(vmax, __ldg(a.v_scale + page_at(k << ps) * H + h));
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(i, 0);
+  float ks = 0.0f, vs = 0.0f;
+  auto scales = [&](int32_t i) {
+    if (i < n_steps) {
+      ks = __ldg(a.k_scale + static_cast<int64_t>(page) * H + h);
+      vs = __ldg(a.v_scale + static_cast<int64_t>(page) * H + h);
+    }
+  };
+  scales(lane);
+  // the steps' largest V scale: P is scaled relative to it (a NaN scale is passed over here and reaches
+  // the result through its own page's factor)
+  float vmax = fmaxf(vs, 0.0f);
+  for (int32_t i = 32 + lane; i < n_steps; i += 32)
+    vmax = fmaxf(vmax, __ldg(a.v_scale + static_cast<int64_t>(page_of(i)) * H + h));
 #pragma unroll
   for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-  if (lane == 0) vmax_sh[warp] = vmax;
-  __syncthreads();
-  vmax = fmaxf(fmaxf(vmax_sh[0], vmax_sh[1]), fmaxf(vmax_sh[2], vmax_sh[3]));
   const float v_unit = vmax > 0.0f ? kVUnit<PREC> / vmax : 0.0f;
 
   // ---- query rows as B fragments: lane (g, t4) holds row g's elements [t4 * D/4, (t4 + 1) * D/4)
@@ -229,15 +253,29 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mma_kernel(const __grid_const
   const float s_unit = capped ? a.scale / a.score_cap : a.scale * kLog2e;
   const float cap2 = a.score_cap * kLog2e;
 
-  for (int32_t k = k0; k < k_end; k += kWarps * kStep) {
-    // ---- S^T = K Q^T (this step's K leaves its registers here)
+  for (int32_t i = 0, round = 0; i < n_steps; ++i) {
+    if (i == 32 * (round + 1)) {
+      ++round;
+      page = page_next;
+      scales(i + lane);
+      if (i + 32 < n_steps) page_next = page_of(i + 32 + lane);
+    }
+    fetch(i + kStages - 1, round);
+    copies_wait<kStages - 1>();
+    __syncwarp();
+    const int32_t k = k_of(i);
+    const uint8_t* const kt = ring + (warp * kStages + i % kStages) * SplitSmem<D, NT>::kStageBytes;
+    const uint8_t* const vt = kt + kStep * D;
+    const float kf = __shfl_sync(0xffffffffu, ks, i & 31) * s_unit, vf = __shfl_sync(0xffffffffu, vs, i & 31) * v_unit;
+    // ---- S^T = K Q^T
     float s[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
-      const uint32_t w0[4] = {kb[0][c].x, kb[0][c].y, kb[0][c].z, kb[0][c].w};
-      const uint32_t w1[4] = {kb[1][c].x, kb[1][c].y, kb[1][c].z, kb[1][c].w};
+      const uint4 r0 = *reinterpret_cast<const uint4*>(kt + chunk_at<D>(g, KC * t4 + c));
+      const uint4 r1 = *reinterpret_cast<const uint4*>(kt + chunk_at<D>(g + 8, KC * t4 + c));
+      const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t u0 = w0[j] ^ 0x80808080u, u1 = w1[j] ^ 0x80808080u;
@@ -249,18 +287,21 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mma_kernel(const __grid_const
           for (int n = 0; n < NQ; ++n) mma16816(s[nt], a0, a1, a2, a3, qf[n][nt][4 * c + j][0], qf[n][nt][4 * c + j][1]);
       }
     }
-    const float kf = ks_next * s_unit, vf = vs_next * v_unit;
     uint32_t vw[4][VW];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int r = 0; r < 4; ++r) {
+      const int row = 2 * t4 + (r & 1) + (r >> 1) * 8;
+      if constexpr (VW == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(vt + chunk_at<D>(row, g));
+        vw[r][0] = v.x, vw[r][1] = v.y, vw[r][2] = v.z, vw[r][3] = v.w;
+      } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(vt + chunk_at<D>(row, g >> 1) + (g & 1) * 8);
+        vw[r][0] = v.x, vw[r][1] = v.y;
+      }
 #pragma unroll
-      for (int w = 0; w < VW; ++w) vw[r][w] = vb[r][w] ^ 0x80808080u;
-    // ---- the next step's rows
-    const int32_t k_next = k + kWarps * kStep;
-    if (k_next < k_end) {
-      fetch(k_next, page);
-      if (k_next + kWarps * kStep < k_end) page = page_at(k_next + kWarps * kStep);
+      for (int w = 0; w < VW; ++w) vw[r][w] ^= 0x80808080u;
     }
+    __syncwarp();  // every lane has its rows: the slot may be filled again
     // ---- scores (log2 units), masks, running maximum
     const bool edge = k < lo_max || k + kStep > hi_min;
     bool grow = false;
@@ -335,6 +376,9 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mma_kernel(const __grid_const
   }
   if (stray) atomicOr(a.status, kStatusBadIndex);
 
+  const float o_unit = vmax * (1.0f / kVUnit<PREC>);  // each warp's own
+  copies_wait<0>();
+  __syncthreads();  // the rings become the merge's space
   // ---- merge the four warps: lane (g, t4) holds elements [g * D/8, (g + 1) * D/8) of rows 2 t4 and 2 t4 + 1
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -346,12 +390,11 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mma_kernel(const __grid_const
       if (g == 0) ml_sh[warp][r][0] = m[nt][c], ml_sh[warp][r][1] = l[nt][c];
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        o_sh[warp][r][g * (D / 8) + 2 * i] = o[i][nt][c];
-        o_sh[warp][r][g * (D / 8) + 2 * i + 1] = o[i][nt][c + 2];
+        o_sh[warp][r][g * (D / 8) + 2 * i] = o[i][nt][c] * o_unit;
+        o_sh[warp][r][g * (D / 8) + 2 * i + 1] = o[i][nt][c + 2] * o_unit;
       }
     }
   __syncthreads();
-  const float o_unit = vmax * (1.0f / kVUnit<PREC>);
   auto store = [&](int r, int d, float v0, float v1) {
     const int32_t row = tl.row0 + r;
     const int64_t at = ((tl.start + static_cast<int64_t>(row / G)) * a.g.n_q_heads + h * G + row % G) * D + d;
@@ -375,11 +418,11 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mma_kernel(const __grid_const
       v1 += o_sh[w][r][d + 1] * f;
     }
     if (n_splits == 1) {
-      const float inv = ll != 0.0f ? o_unit / ll : 0.0f;  // NaN stays NaN
+      const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;  // NaN stays NaN
       store(r, d, v0 * inv, v1 * inv);
     } else {
       const int64_t at = (unit * a.max_splits + split) * R + r;
-      *reinterpret_cast<float2*>(a.part_o + at * D + d) = make_float2(v0 * o_unit, v1 * o_unit);
+      *reinterpret_cast<float2*>(a.part_o + at * D + d) = make_float2(v0, v1);
       if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(mm, ll);
     }
   }
@@ -413,12 +456,21 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_mma_kernel(const __grid_const
   }
 }
 
+template <int D, int NT, int PREC, bool MOD>
+cudaError_t launch_one(const Kv8AttnArgs& a, cudaStream_t st) {
+  constexpr int kBytes = SplitSmem<D, NT>::kBytes;
+  auto kern = kv8_mma_kernel<D, NT, PREC, MOD>;
+  if (kBytes > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e != cudaSuccess) return e;
+  }
+  kern<<<dim3(static_cast<unsigned>(a.tiles) * a.g.n_kv_heads, a.max_splits), kWarps * 32, kBytes, st>>>(a);
+  return cudaGetLastError();
+}
+
 template <int D, int NT, int PREC>
 cudaError_t launch_mod(const Kv8AttnArgs& a, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(a.tiles) * a.g.n_kv_heads, a.max_splits);
-  if (a.score_cap > 0.0f || a.alibi_slopes) kv8_mma_kernel<D, NT, PREC, true><<<grid, kWarps * 32, 0, st>>>(a);
-  else kv8_mma_kernel<D, NT, PREC, false><<<grid, kWarps * 32, 0, st>>>(a);
-  return cudaGetLastError();
+  return a.score_cap > 0.0f || a.alibi_slopes ? launch_one<D, NT, PREC, true>(a, st) : launch_one<D, NT, PREC, false>(a, st);
 }
 
 template <int D, int NT>
@@ -439,12 +491,12 @@ void kv8_mma_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max
   const int32_t R = kv8_mma_rows(g, max_new), G = g.n_q_heads / g.n_kv_heads;
   const int64_t n = static_cast<int64_t>(max_new) * G <= R ? batch : static_cast<int64_t>(n_tokens) * G / R + batch;
   const int64_t units = n * g.n_kv_heads;
-  // enough blocks for four on every SM, chunks of 256 to 2048 rows
-  int64_t want = (4LL * num_sms + units - 1) / units;
+  // three blocks on every SM at a time: enough of them, in chunks of 64 rows (a step a warp) to 2048
+  int64_t want = (3LL * num_sms + units - 1) / units;
   int64_t c = (max_kv + want - 1) / want;
   c = (c + 63) / 64 * 64;
-  if (c < 256) c = 256;
-  if (c > 2048) c = 2048;
+  if (c < kChunkMin) c = kChunkMin;
+  if (c > kChunkMax) c = kChunkMax;
   int64_t s = (max_kv + kStep + c - 1) / c;  // a tile's range may start up to 15 rows before its first row
   if (units > kMaxSplitCounters || s > 65535) {
     c = (static_cast<int64_t>(max_kv) + kStep + 63) / 64 * 64;
