@@ -23,7 +23,7 @@ OBJ = PKG / "_build"  # one object file per source (ignored by git)
 SOURCES = ["api.cu", "rope_append.cu", "decode.cu", "prefill_sm100.cu", "noalloc.cu", "decode_mma.cu", "dist.cu",
            "matmul_sm100.cu", "kv8_api.cu", "kv8_pages.cu", "kv8_append.cu", "kv8_attn.cu",
            "kv8_prefill_sm100.cu"]
-HEADERS = ["common.cuh", "ctx.h", "kernels.h", "rows.cuh"]
+HEADERS = ["common.cuh", "kernels.h", "rows.cuh"]
 
 
 def nvcc_path() -> str:
@@ -34,7 +34,8 @@ def nvcc_path() -> str:
 
 
 def _deps(src: str) -> list[Path]:
-    own = ["kv8.h", "kv8_tile.cuh"] if src.startswith("kv8_") else []
+    own = ["ctx.h"] if src == "api.cu" or src == "kv8_api.cu" else []
+    own += ["kv8.h", "kv8_tile.cuh"] if src.startswith("kv8_") or src == "api.cu" else []
     return [CSRC / h for h in [src] + HEADERS + own] + [ROOT / "include" / "aihost_attn.h", Path(__file__)]
 
 

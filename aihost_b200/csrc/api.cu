@@ -18,6 +18,7 @@
 #include "common.cuh"
 #include "ctx.h"
 #include "kernels.h"
+#include "kv8.h"
 
 using namespace aihost;
 
@@ -465,8 +466,6 @@ aihost_status aihost_attn_create(int32_t device, aihost_attn_ctx** out_ctx) {
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDeviceProperties");
   if (prop.major != 10) return fail(AIHOST_EUNSUPPORTED, "device %d is sm_%d%d; this build targets sm_100a", device,
                                     prop.major, prop.minor);
-  // the split-merge counters, and one more for the page map's blocks
-  constexpr size_t kCounterBytes = (kMaxSplitCounters + 1) * sizeof(unsigned long long);
   auto* ctx = new aihost_attn_ctx();
   ctx->device = device;
   ctx->num_sms = prop.multiProcessorCount;
@@ -476,9 +475,13 @@ aihost_status aihost_attn_create(int32_t device, aihost_attn_ctx** out_ctx) {
     return cuda_fail(e, "cudaMalloc(status)");
   }
   e = cudaMemset(ctx->d_status, 0, sizeof(int32_t));
-  if (e == cudaSuccess) e = cudaMalloc(&ctx->counters, kCounterBytes);
-  if (e == cudaSuccess) e = cudaMemset(ctx->counters, 0, kCounterBytes);
+  if (e == cudaSuccess) e = cudaMalloc(&ctx->counters, kMaxSplitCounters * sizeof(unsigned long long));
+  if (e == cudaSuccess) e = cudaMemset(ctx->counters, 0, kMaxSplitCounters * sizeof(unsigned long long));
+  constexpr size_t kKv8Bytes = (kKv8Counters + 1) * sizeof(uint32_t);
+  if (e == cudaSuccess) e = cudaMalloc(&ctx->kv8_counters, kKv8Bytes);
+  if (e == cudaSuccess) e = cudaMemset(ctx->kv8_counters, 0, kKv8Bytes);
   if (e != cudaSuccess) {
+    cudaFree(ctx->kv8_counters);
     cudaFree(ctx->counters);
     cudaFree(ctx->d_status);
     delete ctx;
@@ -498,6 +501,7 @@ aihost_status aihost_attn_destroy(aihost_attn_ctx* ctx) {
     }
   for (cudaEvent_t e : ctx->event_pool) cudaEventDestroy(e);
   cudaFree(ctx->scratch);
+  cudaFree(ctx->kv8_counters);
   cudaFree(ctx->counters);
   cudaFree(ctx->d_status);
   delete ctx;

@@ -26,6 +26,10 @@ struct aihost_attn_ctx {
   size_t scratch_bytes = 0;
   unsigned long long* counters = nullptr;  // fused split merge: epoch-tagged arrival counts
   uint32_t epoch = 0;
+  uint32_t* kv8_counters = nullptr;  // page map's ticket, then the 8-bit attention's arrival counts
+  aihost::RopeFreqs freqs;                   // of (freqs_theta, freqs_dim), for the 8-bit cache's calls
+  float freqs_theta = 0.0f;
+  int32_t freqs_dim = 0;
   bool profiling = false;
   std::mutex prof_mu;
   ProfSlot prof[AIHOST_KERNEL_COUNT];

@@ -9,6 +9,7 @@
 
 namespace aihost {
 
+constexpr int64_t kKv8Counters = 1 << 16;      // tiles x heads whose chunks can be merged in one launch
 constexpr int32_t kPageMapMaxBatch = 8192;  // two running sums of the batch are kept in shared memory
 
 // Geometry of one layer's 8-bit cache: pools [n_pages][n_kv_heads][page_rows][head_dim], scales
@@ -30,7 +31,7 @@ struct PageMapArgs {
   int64_t* slots;
   int32_t* positions;
   int32_t* free_count_out;
-  uint32_t* ticket;  // zero between launches
+  uint32_t* ticket;  // arrival counter of the blocks, zero between launches
   int32_t* status;
 };
 
@@ -93,8 +94,7 @@ struct Kv8AttnArgs {
   int32_t tiles, chunk, max_splits;
   float* part_o;   // [unit][split][rows][head_dim]
   float* part_ml;  // [unit][split][rows][2]
-  unsigned long long* counters;
-  uint32_t epoch;
+  uint32_t* counters;  // one for each tile and head, zero between launches
   RopeFreqs freqs;
 };
 

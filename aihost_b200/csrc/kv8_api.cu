@@ -15,6 +15,16 @@ int32_t page_shift_of(int32_t page_rows) {
   return page_rows == 16 ? 4 : page_rows == 32 ? 5 : page_rows == 64 ? 6 : page_rows == 128 ? 7 : -1;
 }
 
+// The frequency table of a description; the last one is kept (64 powers cost as much as a launch).
+const RopeFreqs& freqs_of(aihost_attn_ctx* ctx, const aihost_kv8_desc* d) {
+  if (ctx->freqs_dim != d->head_dim || ctx->freqs_theta != d->rope_theta) {
+    ctx->freqs = make_freqs(d->rope_theta, d->head_dim);
+    ctx->freqs_theta = d->rope_theta;
+    ctx->freqs_dim = d->head_dim;
+  }
+  return ctx->freqs;
+}
+
 struct Resolved {
   Kv8Geom g;
   float scale;
@@ -142,7 +152,7 @@ aihost_status aihost_page_map(aihost_attn_ctx* ctx, int32_t batch, int32_t page_
   a.slots = slots;
   a.positions = positions;
   a.free_count_out = free_count_out;
-  a.ticket = reinterpret_cast<uint32_t*>(ctx->counters + kMaxSplitCounters);
+  a.ticket = ctx->kv8_counters;
   a.status = ctx->d_status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = timed_launch(ctx, AIHOST_KERNEL_PAGES, st, [&] { return launch_page_map(a, st); });
@@ -208,7 +218,7 @@ aihost_status aihost_kv8_append(aihost_attn_ctx* ctx, const aihost_kv8_desc* des
   a.k_scale = k_scale;
   a.v_scale = v_scale;
   a.status = ctx->d_status;
-  if (desc->rope_mode != AIHOST_ROPE_NONE) a.freqs = make_freqs(desc->rope_theta, desc->head_dim);
+  if (desc->rope_mode != AIHOST_ROPE_NONE) a.freqs = freqs_of(ctx, desc);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = timed_launch(ctx, AIHOST_KERNEL_KV8_APPEND, st, [&] { return launch_kv8_append(a, st); });
   return e == cudaSuccess ? AIHOST_OK : cuda_fail(e, "8-bit append launch");
@@ -292,7 +302,7 @@ aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* 
   a.scale = r.scale;
   a.score_cap = desc->score_cap;
   a.status = ctx->d_status;
-  if (desc->rope_mode != AIHOST_ROPE_NONE) a.freqs = make_freqs(desc->rope_theta, desc->head_dim);
+  if (desc->rope_mode != AIHOST_ROPE_NONE) a.freqs = freqs_of(ctx, desc);
   const Plan plan = make_plan(desc, r.g, batch, n_tokens, max_new, max_kv, ctx->num_sms);
   a.tiles = plan.tiles;
   a.chunk = plan.chunk;
@@ -306,8 +316,7 @@ aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* 
   if (need) {
     a.part_o = static_cast<float*>(ctx->scratch);
     a.part_ml = a.part_o + static_cast<size_t>(a.tiles) * r.g.n_kv_heads * a.max_splits * plan.rows * r.g.head_dim;
-    a.counters = ctx->counters;
-    a.epoch = ctx->epoch++;
+    a.counters = ctx->kv8_counters + 1;
   }
   DeviceGuard g(ctx->device);
   if (!g.ok()) return fail(AIHOST_ECUDA, "cudaSetDevice(%d) failed", ctx->device);

@@ -1,17 +1,17 @@
 // kv8_attn.cu — attention of few query rows over the 8-bit paged cache (decode, short prompts).
 //
 // One block takes R = 8 or 16 query rows (tokens x heads of one KV head, so the cache is read once
-// for the whole head group), one KV head and a chunk of the cache rows; its four warps walk 16-row
+// for the whole head group), one KV head and a chunk of the cache rows; its four warps walk 32-row
 // steps of the chunk. Per step, with the transposed products that make cache rows the M = 16 of
 // mma.sync m16n8k16 and query rows its N = 8:
-//   S^T = K Q^T     K's int8 go to fp16 exactly in registers, one fp32 factor per page afterwards
+//   S^T = K Q^T     K's int8 go to fp16 in registers, one fp32 factor per page afterwards
 //   online softmax  running maximum per query row, moved only when it grows by more than 2^8
 //   O^T += V^T P^T  V likewise exact; P carries the page's scale relative to the chunk's largest
 // The k order of either product is free, so it is chosen such that every lane takes 16 bytes of a
 // cache row at a time and no transpose is needed. Each warp copies its own steps' rows into a ring of
-// its own in shared memory (cp.async, three steps ahead, chunks swizzled against bank conflicts): no
-// warp waits for another in the loop. A lane holds the page and scales of one of the warp's next 32
-// steps. Warps merge through shared memory, chunks through partials that the last block to arrive
+// its own in shared memory (cp.async, a step ahead, chunks swizzled against bank conflicts): no warp
+// waits for another in the loop. A lane holds the place and scales of one of the warp's next 32 blocks
+// of 16 rows (the smallest page). Warps merge through shared memory, chunks through partials that the last block to arrive
 // merges (no block waits for another).
 #include "common.cuh"
 #include "kv8.h"
@@ -22,9 +22,10 @@ namespace aihost {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStep = 16;   // cache rows of a step; a block's warps take steps in turn
-constexpr int kStages = 4;  // of the warp's ring
-constexpr int kChunkMin = 64, kChunkMax = 2048;
+constexpr int kSub = 16;          // cache rows of one MMA, and of the smallest page
+constexpr int kStep = 2 * kSub;   // cache rows of a step; a block's warps take steps in turn
+constexpr int kStages = 2;        // of the warp's ring
+constexpr int kChunkMin = kWarps * kStep, kChunkMax = 2048;
 
 // What the products take: fp16 operands, q as a pair of fp16 (rotated in fp32), or q and P as pairs
 // (fp32 tensors).
@@ -128,52 +129,69 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
     hi = __reduce_max_sync(0xffffffffu, end);
     hi_min = __reduce_min_sync(0xffffffffu, end);
   }
-  const int32_t base = min(lo, hi) & ~(kStep - 1);
+  const int32_t base = min(lo, hi) & ~(kSub - 1);
   const int32_t n_splits = max(1, (hi - base + a.chunk - 1) / a.chunk);
   if (split >= n_splits) return;
   const int32_t k_begin = base + split * a.chunk, k_end = min(hi, k_begin + a.chunk);
   const int32_t* const table = a.block_table + static_cast<int64_t>(tl.b) * a.g.max_pages;
   bool stray = false;  // a page id outside the pool reads page 0 and sets the status
 
-  // ---- this warp's steps: step i is rows [k_of(i), k_of(i) + 16)
-  auto k_of = [&](int32_t i) { return k_begin + (i * kWarps + warp) * kStep; };
-  const int32_t n_steps = k_begin + warp * kStep < k_end ? (k_end - k_begin - warp * kStep - 1) / (kWarps * kStep) + 1 : 0;
-  // lane j: page, K factor and V scale of step 32 * round + j
-  auto page_of = [&](int32_t i) -> int32_t {
-    return i < n_steps ? static_cast<int32_t>(page_or_first(table[k_of(i) >> ps], a.g.n_pages, stray)) : 0;
+  // ---- this warp's steps: step i is rows [k_of(i), k_of(i) + 32), as blocks of 16 rows 2 i and 2 i + 1
+  const int32_t k_mine = k_begin + warp * kStep;
+  const int32_t n_steps = k_mine < k_end ? (k_end - k_mine - 1) / (kWarps * kStep) + 1 : 0;
+  auto row_of = [&](int32_t sub) { return k_mine + (sub >> 1) * (kWarps * kStep) + (sub & 1) * kSub; };
+  // lane j: where block 32 * round + j lies (its offset in either pool; none past the end), its scales
+  constexpr int64_t kNowhere = -1;
+  auto place_of = [&](int32_t sub, int64_t& ph) -> int64_t {
+    const int32_t row = row_of(sub);
+    ph = 0;
+    if ((sub >> 1) >= n_steps || row >= k_end) return kNowhere;
+    ph = page_or_first(table[row >> ps], a.g.n_pages, stray) * H + h;
+    return ((ph << ps) + (row & (a.g.page_rows - 1))) * D;
   };
-  int32_t page = page_of(lane), page_next = n_steps > 32 ? page_of(32 + lane) : 0;
-  const uint32_t my_ring = smem_u32(ring) + warp * (kStages * SplitSmem<D, NT>::kStageBytes);
-  auto fetch = [&](int32_t i, int32_t round) {
-    if (i < n_steps) {
-      const int64_t pg = __shfl_sync(0xffffffffu, (i >> 5) == round ? page : page_next, i & 31);
-      const int64_t at = (((pg * H + h) << ps) + (k_of(i) & (a.g.page_rows - 1))) * D;
-      const uint32_t dst = my_ring + (i % kStages) * SplitSmem<D, NT>::kStageBytes;
-      constexpr int CR = D / 16;  // chunks per row
+  int64_t ph, ph_next;
+  int64_t place = place_of(lane, ph), place_next = n_steps > 16 ? place_of(32 + lane, ph_next) : kNowhere;
+  constexpr int kStageBytes = SplitSmem<D, NT>::kStageBytes;
+  uint8_t* const my_ring = ring + warp * (kStages * kStageBytes);
+  // copies of a 16-row block: chunk j * 32 + lane of its K and V rows each
+  constexpr int CR = D / 16;  // chunks per row
+  uint32_t to[2];             // the swizzle repeats every 8 rows: two patterns of destinations
 #pragma unroll
-      for (int j = 0; j < kStep * CR / 32; ++j) {
-        const int ch = j * 32 + lane, r = ch / CR, c = ch % CR;
-        copy16(dst + chunk_at<D>(r, c), a.k_pool + at + ch * 16);
-        copy16(dst + kStep * D + chunk_at<D>(r, c), a.v_pool + at + ch * 16);
+  for (int j = 0; j < 2; ++j)
+    to[j] = smem_u32(my_ring) + chunk_at<D>((j * 32 + lane) / CR, (j * 32 + lane) % CR) - j * 512;
+  auto fetch = [&](int32_t i, int32_t round) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int32_t sub = 2 * i + u;
+      const int64_t at = __shfl_sync(0xffffffffu, (sub >> 5) == round ? place : place_next, sub & 31);
+      if (i < n_steps && at != kNowhere) {
+        const uint32_t dst = (i % kStages) * kStageBytes + u * (kSub * D);
+        const int8_t *kp = a.k_pool + at + lane * 16, *vp = a.v_pool + at + lane * 16;
+#pragma unroll
+        for (int j = 0; j < kSub * CR / 32; ++j) {
+          copy16(to[j & 1] + dst + j * 512, kp + j * 512);
+          copy16(to[j & 1] + dst + kStep * D + j * 512, vp + j * 512);
+        }
       }
     }
     copies_commit();
   };
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch(i, 0);
+  fetch(0, 0);
   float ks = 0.0f, vs = 0.0f;
-  auto scales = [&](int32_t i) {
-    if (i < n_steps) {
-      ks = __ldg(a.k_scale + static_cast<int64_t>(page) * H + h);
-      vs = __ldg(a.v_scale + static_cast<int64_t>(page) * H + h);
+  auto scales = [&] {
+    if (place != kNowhere) {
+      ks = __ldg(a.k_scale + ph);
+      vs = __ldg(a.v_scale + ph);
     }
   };
-  scales(lane);
-  // the steps' largest V scale: P is scaled relative to it (a NaN scale is passed over here and reaches
+  scales();
+  // the blocks' largest V scale: P is scaled relative to it (a NaN scale is passed over here and reaches
   // the result through its own page's factor)
   float vmax = fmaxf(vs, 0.0f);
-  for (int32_t i = 32 + lane; i < n_steps; i += 32)
-    vmax = fmaxf(vmax, __ldg(a.v_scale + static_cast<int64_t>(page_of(i)) * H + h));
+  for (int32_t sub = 32 + lane; sub < 2 * n_steps; sub += 32) {
+    int64_t at;
+    if (place_of(sub, at) != kNowhere) vmax = fmaxf(vmax, __ldg(a.v_scale + at));
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
   const float v_unit = vmax > 0.0f ? kVUnit<PREC> / vmax : 0.0f;
@@ -240,6 +258,30 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
     }
   }
 
+  // Where q is fp16, K enters as 1152 + k (what the byte trick gives), and S starts at -1152 sum q: the
+  // terms cancel in fp32 to about 2^-22 of 1152 |q|, far below P's rounding, for half of K's conversion.
+  constexpr bool kOffset = PREC != kPairQP;
+  float s_init[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float sum = 0.0f;
+    if (kOffset) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qf[n][nt][k][e]));
+            sum += f.x + f.y;
+          }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);  // row g's
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) s_init[nt][c] = -1152.0f * __shfl_sync(0xffffffffu, sum, (2 * t4 + c) * 4);
+  }
+
   float o[MT][NT][4];
   float m[NT][2], l[NT][2];
 #pragma unroll
@@ -254,125 +296,164 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
   const float cap2 = a.score_cap * kLog2e;
 
   for (int32_t i = 0, round = 0; i < n_steps; ++i) {
-    if (i == 32 * (round + 1)) {
+    if (i == 16 * (round + 1)) {
       ++round;
-      page = page_next;
-      scales(i + lane);
-      if (i + 32 < n_steps) page_next = page_of(i + 32 + lane);
+      place = place_next;
+      ph = ph_next;
+      scales();
+      if (i + 16 < n_steps) place_next = place_of(2 * i + 32 + lane, ph_next);
     }
-    fetch(i + kStages - 1, round);
-    copies_wait<kStages - 1>();
+    fetch(i + 1, round);
+    copies_wait<1>();
     __syncwarp();
-    const int32_t k = k_of(i);
-    const uint8_t* const kt = ring + (warp * kStages + i % kStages) * SplitSmem<D, NT>::kStageBytes;
-    const uint8_t* const vt = kt + kStep * D;
-    const float kf = __shfl_sync(0xffffffffu, ks, i & 31) * s_unit, vf = __shfl_sync(0xffffffffu, vs, i & 31) * v_unit;
+    const uint8_t* const stage = my_ring + (i % kStages) * kStageBytes;
+    const int32_t k = row_of(2 * i);
     // ---- S^T = K Q^T
-    float s[NT][4];
+    float s[2][NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+    for (int u = 0; u < 2; ++u) {
+      const uint8_t* const kt = stage + u * (kSub * D);
 #pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      const uint4 r0 = *reinterpret_cast<const uint4*>(kt + chunk_at<D>(g, KC * t4 + c));
-      const uint4 r1 = *reinterpret_cast<const uint4*>(kt + chunk_at<D>(g + 8, KC * t4 + c));
-      const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+      for (int nt = 0; nt < NT; ++nt) s[u][nt][0] = s[u][nt][2] = s_init[nt][0], s[u][nt][1] = s[u][nt][3] = s_init[nt][1];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t u0 = w0[j] ^ 0x80808080u, u1 = w1[j] ^ 0x80808080u;
-        const uint32_t a0 = half2_of(u0, 0x4140), a1 = half2_of(u1, 0x4140);
-        const uint32_t a2 = half2_of(u0, 0x4342), a3 = half2_of(u1, 0x4342);
+      for (int c = 0; c < KC; ++c) {
+        const uint4 r0 = *reinterpret_cast<const uint4*>(kt + chunk_at<D>(g, KC * t4 + c));
+        const uint4 r1 = *reinterpret_cast<const uint4*>(kt + chunk_at<D>(g + 8, KC * t4 + c));
+        const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t u0 = w0[j] ^ 0x80808080u, u1 = w1[j] ^ 0x80808080u;
+          uint32_t a0, a1, a2, a3;
+          if constexpr (kOffset) {
+            a0 = __byte_perm(u0, 0x64646464u, 0x4140), a1 = __byte_perm(u1, 0x64646464u, 0x4140);
+            a2 = __byte_perm(u0, 0x64646464u, 0x4342), a3 = __byte_perm(u1, 0x64646464u, 0x4342);
+          } else {
+            a0 = half2_of(u0, 0x4140), a1 = half2_of(u1, 0x4140);
+            a2 = half2_of(u0, 0x4342), a3 = half2_of(u1, 0x4342);
+          }
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) mma16816(s[nt], a0, a1, a2, a3, qf[n][nt][4 * c + j][0], qf[n][nt][4 * c + j][1]);
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+              mma16816(s[u][nt], a0, a1, a2, a3, qf[n][nt][4 * c + j][0], qf[n][nt][4 * c + j][1]);
+        }
       }
     }
-    uint32_t vw[4][VW];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 2 * t4 + (r & 1) + (r >> 1) * 8;
-      if constexpr (VW == 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(vt + chunk_at<D>(row, g));
-        vw[r][0] = v.x, vw[r][1] = v.y, vw[r][2] = v.z, vw[r][3] = v.w;
-      } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(vt + chunk_at<D>(row, g >> 1) + (g & 1) * 8);
-        vw[r][0] = v.x, vw[r][1] = v.y;
-      }
-#pragma unroll
-      for (int w = 0; w < VW; ++w) vw[r][w] ^= 0x80808080u;
-    }
-    __syncwarp();  // every lane has its rows: the slot may be filled again
     // ---- scores (log2 units), masks, running maximum
     const bool edge = k < lo_max || k + kStep > hi_min;
     bool grow = false;
 #pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float kf = __shfl_sync(0xffffffffu, ks, (2 * i + u) & 31) * s_unit;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float v = s[u][nt][e] * kf;
+          if constexpr (MOD) {
+            if (capped) v = cap2 * tanh_of(v);
+            if (a.alibi_slopes) {
+              const int32_t row = k + u * kSub + g + (e >> 1) * 8;
+              v -= c_slope[nt][e & 1] * fabsf(c_pos[nt][e & 1] - static_cast<float>(row));
+            }
+          }
+          s[u][nt][e] = v;
+        }
+    }
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int32_t row = k + u * kSub + g + (e >> 1) * 8;
+            if (row < c_first[nt][e & 1] || row >= c_end[nt][e & 1]) s[u][nt][e] = -INFINITY;
+          }
+    }
+#pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int32_t row = k + g + (e >> 1) * 8;
-        float v = s[nt][e] * kf;
-        if constexpr (MOD) {
-          if (capped) v = cap2 * tanh_of(v);
-          if (a.alibi_slopes) v -= c_slope[nt][e & 1] * fabsf(c_pos[nt][e & 1] - static_cast<float>(row));
-        }
-        if (edge && (row < c_first[nt][e & 1] || row >= c_end[nt][e & 1])) v = -INFINITY;
-        s[nt][e] = v;
-        grow |= v > m[nt][e & 1] + kSlack<PREC>;
-      }
+      for (int c = 0; c < 2; ++c)
+        grow |= fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2])) > m[nt][c] + kSlack<PREC>;
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float mx = fmaxf(s[nt][c], s[nt][c + 2]);
+          float mx = fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
           const float m_new = fmaxf(m[nt][c], mx), f = ex2_approx(m[nt][c] - m_new);
           m[nt][c] = m_new;
           l[nt][c] *= f;
 #pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            o[i][nt][c] *= f;
-            o[i][nt][c + 2] *= f;
+          for (int t = 0; t < MT; ++t) {
+            o[t][nt][c] *= f;
+            o[t][nt][c + 2] *= f;
           }
         }
     }
-    // ---- P and its fragments
-    uint32_t pf[PREC == kPairQP ? 2 : 1][NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float p[4];
+    for (int u = 0; u < 2; ++u) {
+      // ---- P and its fragments
+      const float vf = __shfl_sync(0xffffffffu, vs, (2 * i + u) & 31) * v_unit;
+      uint32_t pf[PREC == kPairQP ? 2 : 1][NT][2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        p[e] = ex2_approx(s[nt][e] - m[nt][e & 1]);
-        l[nt][e & 1] += p[e];
-        // a hidden row adds nothing even where its page's scale is NaN
-        p[e] = edge && s[nt][e] == -INFINITY ? 0.0f : p[e] * vf;
+      for (int nt = 0; nt < NT; ++nt) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[e] = ex2_approx(s[u][nt][e] - m[nt][e & 1]);
+          l[nt][e & 1] += p[e];
+          p[e] *= vf;
+        }
+        if (edge) {  // a hidden row adds nothing even where its page's scale is NaN
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (s[u][nt][e] == -INFINITY) p[e] = 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t hi2 = pack2(p[2 * c], p[2 * c + 1]);
+          pf[0][nt][c] = movmatrix_t(hi2);
+          if constexpr (PREC == kPairQP) pf[1][nt][c] = movmatrix_t(pack2_rest(p[2 * c], p[2 * c + 1], hi2));
+        }
+      }
+      // ---- O^T += V^T P^T
+      const uint8_t* const vt = stage + kStep * D + u * (kSub * D);
+      uint32_t vw[4][VW];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 2 * t4 + (r & 1) + (r >> 1) * 8;
+        if constexpr (VW == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(vt + chunk_at<D>(row, g));
+          vw[r][0] = v.x, vw[r][1] = v.y, vw[r][2] = v.z, vw[r][3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2*>(vt + chunk_at<D>(row, g >> 1) + (g & 1) * 8);
+          vw[r][0] = v.x, vw[r][1] = v.y;
+        }
       }
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const uint32_t hi2 = pack2(p[2 * c], p[2 * c + 1]);
-        pf[0][nt][c] = movmatrix_t(hi2);
-        if constexpr (PREC == kPairQP) pf[1][nt][c] = movmatrix_t(pack2_rest(p[2 * c], p[2 * c + 1], hi2));
-      }
-    }
-    // ---- O^T += V^T P^T
+      for (int w = 0; w < VW; ++w) {
+        const uint32_t w0 = vw[0][w] ^ 0x80808080u, w1 = vw[1][w] ^ 0x80808080u;
+        const uint32_t w2 = vw[2][w] ^ 0x80808080u, w3 = vw[3][w] ^ 0x80808080u;
+        const uint32_t x0 = __byte_perm(w0, w1, 0x5140), x1 = __byte_perm(w0, w1, 0x7362);
+        const uint32_t y0 = __byte_perm(w2, w3, 0x5140), y1 = __byte_perm(w2, w3, 0x7362);
 #pragma unroll
-    for (int w = 0; w < VW; ++w) {
-      const uint32_t x0 = __byte_perm(vw[0][w], vw[1][w], 0x5140), x1 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
-      const uint32_t y0 = __byte_perm(vw[2][w], vw[3][w], 0x5140), y1 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t x = t ? x1 : x0, y = t ? y1 : y0;
+          const uint32_t a0 = half2_of(x, 0x4140), a1 = half2_of(x, 0x4342);
+          const uint32_t a2 = half2_of(y, 0x4140), a3 = half2_of(y, 0x4342);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t x = i ? x1 : x0, y = i ? y1 : y0;
-        const uint32_t a0 = half2_of(x, 0x4140), a1 = half2_of(x, 0x4342);
-        const uint32_t a2 = half2_of(y, 0x4140), a3 = half2_of(y, 0x4342);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma16816(o[2 * w + i][nt], a0, a1, a2, a3, pf[0][nt][0], pf[0][nt][1]);
-          if constexpr (PREC == kPairQP) mma16816(o[2 * w + i][nt], a0, a1, a2, a3, pf[1][nt][0], pf[1][nt][1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816(o[2 * w + t][nt], a0, a1, a2, a3, pf[0][nt][0], pf[0][nt][1]);
+            if constexpr (PREC == kPairQP) mma16816(o[2 * w + t][nt], a0, a1, a2, a3, pf[1][nt][0], pf[1][nt][1]);
+          }
         }
       }
     }
+    __syncwarp();  // every lane has its rows: the slot may be filled again
   }
   if (stray) atomicOr(a.status, kStatusBadIndex);
 
@@ -431,28 +512,58 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
   // ---- merge the chunks: the last block of this tile and head to arrive
   __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) last_sh = split_arrive(a.counters + unit, a.epoch, n_splits, a.status);
+  if (threadIdx.x == 0) last_sh = last_to_arrive(a.counters + unit, n_splits);
   __syncthreads();
   if (!last_sh) return;
   __threadfence();
-  if (threadIdx.x == 0) a.counters[unit] = 0;  // a replayed launch counts from zero again
-  for (int i = threadIdx.x; i < n_rows * (D / 2); i += kWarps * 32) {
-    const int r = i / (D / 2), d = i % (D / 2) * 2;
-    const int64_t at = unit * a.max_splits * R + r;
-    float mm = kNoMax;
-    for (int sp = 0; sp < n_splits; ++sp) mm = fmaxf(mm, __ldcg(a.part_ml + (at + static_cast<int64_t>(sp) * R) * 2));
-    float ll = 0.0f, v0 = 0.0f, v1 = 0.0f;
-    for (int sp = 0; sp < n_splits; ++sp) {
-      const int64_t p = at + static_cast<int64_t>(sp) * R;
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml + p * 2));
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(a.part_o + p * D + d));
-      const float f = ex2_approx(ml.x - mm);
-      ll += ml.y * f;
-      v0 += v.x * f;
-      v1 += v.y * f;
+  const int64_t first_part = unit * a.max_splits * R;
+  // the chunks' weights per row, over the ring: few enough at a time for any number of chunks
+  float* const w_sh = reinterpret_cast<float*>(ring);
+  constexpr int kAtOnce = SplitSmem<D, NT>::kBytes / (R * 8);  // chunks whose (max, sum) fit
+  constexpr int kVec = R * (D / 4) / (kWarps * 32);            // float4 of the result per thread
+  float4 acc[kVec];
+  float mm[kVec], ll[kVec];
+#pragma unroll
+  for (int v = 0; v < kVec; ++v) {
+    acc[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    mm[v] = kNoMax;
+    ll[v] = 0.0f;
+  }
+  for (int32_t s0 = 0; s0 < n_splits; s0 += kAtOnce) {
+    const int32_t ns = min(kAtOnce, n_splits - s0);
+    __syncthreads();
+    for (int32_t i = threadIdx.x; i < ns * R; i += kWarps * 32)
+      reinterpret_cast<float2*>(w_sh)[i] =
+          __ldcg(reinterpret_cast<const float2*>(a.part_ml) + first_part + static_cast<int64_t>(s0) * R + i);
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) {
+      const int at = v * (kWarps * 32) + threadIdx.x, r = at / (D / 4), d4 = at % (D / 4);
+      if (r >= n_rows) continue;
+      float top = mm[v];
+      for (int32_t sp = 0; sp < ns; ++sp) top = fmaxf(top, w_sh[(sp * R + r) * 2]);
+      const float f0 = ex2_approx(mm[v] - top);
+      ll[v] *= f0;
+      acc[v] = make_float4(acc[v].x * f0, acc[v].y * f0, acc[v].z * f0, acc[v].w * f0);
+      mm[v] = top;
+      const float4* const src = reinterpret_cast<const float4*>(a.part_o) +
+                                (first_part + static_cast<int64_t>(s0) * R + r) * (D / 4) + d4;
+#pragma unroll 8
+      for (int32_t sp = 0; sp < ns; ++sp) {
+        const float4 x = __ldcg(src + static_cast<int64_t>(sp) * R * (D / 4));
+        const float f = ex2_approx(w_sh[(sp * R + r) * 2] - top);
+        ll[v] += w_sh[(sp * R + r) * 2 + 1] * f;
+        acc[v].x += x.x * f, acc[v].y += x.y * f, acc[v].z += x.z * f, acc[v].w += x.w * f;
+      }
     }
-    const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
-    store(r, d, v0 * inv, v1 * inv);
+  }
+#pragma unroll
+  for (int v = 0; v < kVec; ++v) {
+    const int at = v * (kWarps * 32) + threadIdx.x, r = at / (D / 4), d = at % (D / 4) * 4;
+    if (r >= n_rows) continue;
+    const float inv = ll[v] != 0.0f ? 1.0f / ll[v] : 0.0f;
+    store(r, d, acc[v].x * inv, acc[v].y * inv);
+    store(r, d + 2, acc[v].z * inv, acc[v].w * inv);
   }
 }
 
@@ -491,15 +602,22 @@ void kv8_mma_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max
   const int32_t R = kv8_mma_rows(g, max_new), G = g.n_q_heads / g.n_kv_heads;
   const int64_t n = static_cast<int64_t>(max_new) * G <= R ? batch : static_cast<int64_t>(n_tokens) * G / R + batch;
   const int64_t units = n * g.n_kv_heads;
-  // three blocks on every SM at a time: enough of them, in chunks of 64 rows (a step a warp) to 2048
-  int64_t want = (3LL * num_sms + units - 1) / units;
-  int64_t c = (max_kv + want - 1) / want;
-  c = (c + 63) / 64 * 64;
-  if (c < kChunkMin) c = kChunkMin;
-  if (c > kChunkMax) c = kChunkMax;
-  int64_t s = (max_kv + kStep + c - 1) / c;  // a tile's range may start up to 15 rows before its first row
-  if (units > kMaxSplitCounters || s > 65535) {
-    c = (static_cast<int64_t>(max_kv) + kStep + 63) / 64 * 64;
+  // Chunks: the number that gives the least waves of blocks (three or two on an SM) times a block's rows,
+  // its fixed work counted as 256 more; chunks of 128 rows (a step a warp) to about 2048.
+  const int64_t slots = static_cast<int64_t>(num_sms) * (R == 8 ? 3 : 2);
+  const int64_t least = (max_kv + kChunkMax - 1) / kChunkMax, most = (max_kv + kChunkMin - 1) / kChunkMin;
+  int64_t c = 0, best = INT64_MAX;
+  for (int64_t n_split = least; n_split <= most && n_split < least + 64; ++n_split) {
+    const int64_t rows = ((max_kv + n_split - 1) / n_split + kChunkMin - 1) / kChunkMin * kChunkMin;
+    const int64_t cost = (units * n_split + slots - 1) / slots * (rows + 256);
+    if (cost < best) {
+      best = cost;
+      c = rows;
+    }
+  }
+  int64_t s = (max_kv + c - 1) / c;
+  if (units > kKv8Counters || s > 65535) {
+    c = (static_cast<int64_t>(max_kv) + kChunkMin - 1) / kChunkMin * kChunkMin;
     s = 1;
   }
   *tiles = static_cast<int32_t>(n);

@@ -4,6 +4,7 @@
 // lengths -> running sums -> table or stack entry -> slot.
 #include "common.cuh"
 #include "kv8.h"
+#include "kv8_tile.cuh"
 
 namespace aihost {
 namespace {
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(1024) page_map_kernel(const PageMapArgs a) {
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
-    last_block = gridDim.x == 1 || atomicInc(a.ticket, gridDim.x - 1) == gridDim.x - 1;
+    last_block = gridDim.x == 1 || last_to_arrive(a.ticket, gridDim.x);
   }
   __syncthreads();
   if (!last_block) return;

@@ -685,10 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     if (n_splits > 1) {  // the last block of this tile and head to arrive merges the chunks
       __threadfence();
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (threadIdx.x == 128) {
-        sh.last = split_arrive(a.counters + unit, a.epoch, n_splits, status);
-        if (sh.last) a.counters[unit] = 0;  // a replayed launch counts from zero again
-      }
+      if (threadIdx.x == 128) sh.last = last_to_arrive(a.counters + unit, n_splits);
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (sh.last) {
         __threadfence();
@@ -754,7 +751,7 @@ void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t
       best = s;
     }
   }
-  if (units > kMaxSplitCounters) best = 1;
+  if (units > kKv8Counters) best = 1;
   const int64_t c = (tiles_kv + best - 1) / best;
   *tiles = static_cast<int32_t>(n);
   *chunk = static_cast<int32_t>(c * kKeys);

@@ -88,6 +88,13 @@ __device__ __forceinline__ float tanh_of(float x) {
   return 1.0f - __fdividef(2.0f, 1.0f + e);
 }
 
+// Whether this is the last of n arrivals, by one thread of each block after its own writes and a fence.
+// The counter wraps to zero with the last, ready for the next launch (and for a replayed one). No block
+// waits for another.
+__device__ __forceinline__ bool last_to_arrive(uint32_t* counter, int32_t n) {
+  return atomicInc(counter, static_cast<uint32_t>(n - 1)) == static_cast<uint32_t>(n - 1);
+}
+
 // Page id of a table entry; one outside the pool becomes page 0 and sets `stray`.
 __device__ __forceinline__ int64_t page_or_first(int32_t p, int32_t n_pages, bool& stray) {
   if (p >= 0 && p < n_pages) return p;
