@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
           float sn, cs;
-          sincosf(__fmul_rn(pos, a.freqs.f[(t4 * E + e) >> 1]), &sn, &cs);
+          sincos_near(__fmul_rn(pos, a.freqs.f[(t4 * E + e) >> 1]), &sn, &cs);
           rotate_pair(x[e], x[e + 1], cs, sn);
         }
       } else {  // pairs D/2 apart: lanes t4 and t4 ^ 2
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
         for (int e = 0; e < E; ++e) {
           const float other = __shfl_xor_sync(0xffffffffu, x[e], 2);
           float sn, cs;
-          sincosf(__fmul_rn(pos, a.freqs.f[(t4 & 1) * E + e]), &sn, &cs);
+          sincos_near(__fmul_rn(pos, a.freqs.f[(t4 & 1) * E + e]), &sn, &cs);
           float x1 = t4 < 2 ? x[e] : other, x2 = t4 < 2 ? other : x[e];
           rotate_pair(x1, x2, cs, sn);
           x[e] = t4 < 2 ? x1 : x2;

@@ -88,6 +88,36 @@ __device__ __forceinline__ float tanh_of(float x) {
   return 1.0f - __fdividef(2.0f, 1.0f + e);
 }
 
+// sin and cos to 1.1e-7 for |angle| <= 1e6 (beyond, the library's): Cody-Waite reduction by pi/2 in three
+// parts (W. J. Cody and W. Waite, Software Manual for the Elementary Functions, 1980), each step one
+// fma, then odd and even polynomials, our weighted least-squares fits on [-pi/4, pi/4].
+__device__ __noinline__ inline float2 sincos_far(float a) {
+  float2 v;
+  sincosf(a, &v.x, &v.y);
+  return v;
+}
+
+__device__ __forceinline__ void sincos_near(float a, float* s, float* c) {
+  if (fabsf(a) > 1e6f) {
+    const float2 v = sincos_far(a);
+    *s = v.x;
+    *c = v.y;
+    return;
+  }
+  const float k = rintf(a * 0.636619772367581343f);
+  float r = fmaf(-k, 1.5707963705062866f, a);
+  r = fmaf(-k, -4.371138828673793e-08f, r);
+  r = fmaf(-k, -1.7151245100058819e-15f, r);
+  const float y = r * r;
+  const float ps = fmaf(fmaf(-0.00019517235341481864f, y, 0.008332177996635437f), y, -0.16666655242443085f);
+  const float pc = fmaf(fmaf(2.4438379114144482e-05f, y, -0.0013887366512790322f), y, 0.04166664555668831f);
+  const float sn = fmaf(r * y, ps, r), cs = fmaf(pc * y, y, fmaf(-0.5f, y, 1.0f));
+  const int q = static_cast<int>(k);
+  const float u = q & 1 ? cs : sn, v = q & 1 ? sn : cs;
+  *s = q & 2 ? -u : u;
+  *c = (q + 1) & 2 ? -v : v;
+}
+
 // Whether this is the last of n arrivals, by one thread of each block after its own writes and a fence.
 // The counter wraps to zero with the last, ready for the next launch (and for a replayed one). No block
 // waits for another.
