@@ -17,6 +17,8 @@
 //                on tiles that cross the row's range, running maximum (O is rescaled only when it
 //                grows by more than 2^8), exp2, row sum, P times V's factors as fp16.
 // Ranges are cut into chunks where there are few tiles; the last block of a tile to arrive merges.
+#include <algorithm>
+
 #include "common.cuh"
 #include "kv8.h"
 #include "kv8_tile.cuh"
@@ -29,7 +31,7 @@ constexpr int kRows = 2 * kTileRows;  // query rows of a block
 constexpr int kKeys = 128;            // cache rows of a tile
 constexpr int kThreads = 512;
 // setmaxnreg split of the 128 x 512 registers at launch: warps 0-3, softmax warpgroups, converters
-constexpr uint32_t kRegsMma = 64, kRegsSoftmax = 184, kRegsConvert = 80;
+constexpr uint32_t kRegsMma = 64, kRegsSoftmax = 176, kRegsConvert = 96;
 static_assert(128 * (kRegsMma + 2 * kRegsSoftmax + kRegsConvert) <= 128 * kThreads, "setmaxnreg split exceeds the launch");
 constexpr float kSlack = 8.0f;    // the maximum may lag by 2^8 before O is rescaled
 constexpr float kVUnit = 128.0f;  // P * (v scale / largest) * 128 <= 2^15 stays in fp16's range
@@ -53,7 +55,7 @@ struct Cfg {
 };
 
 struct Shared {
-  uint64_t q_ready[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_ready[2], s_full[2], p_full[2][2], o_full[2];
   uint64_t k_full[3], k_empty[3], v_full[3], v_empty[3];
   uint64_t raw_full[4], raw_empty[4];
   float k_factor[kFactorRing][kFactors];
@@ -178,6 +180,19 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
+// 32 lanes x 8 consecutive 32-bit columns of tensor memory.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 // A wait that the whole warp leaves together, with one answer.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_t* status) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
@@ -204,18 +219,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     int32_t lo = INT32_MAX, hi = 0;
-#pragma unroll
-    for (int k = 0; k < kTileRows / 32; ++k) {
-      const int r = t * kTileRows + k * 32 + lane;
-      int32_t first, end, pos;
-      row_range(a, tl, G, n_rows, r, first, end, pos);
-      if (r < n_rows && first < end) {
-        lo = min(lo, first);
-        hi = max(hi, end);
+    if (t * kTileRows < n_rows) {
+      const int32_t i0 = (tl.row0 + t * kTileRows) / G, i1 = (tl.row0 + min((t + 1) * kTileRows, n_rows) - 1) / G;
+      const int32_t prefix = a.prefix_len ? min(a.prefix_len[tl.b], tl.kv_len) : 0;
+      if (!a.row_first) {
+        lo = 0;
+        hi = max(tl.pos0 + i1 + 1, prefix);
+      } else {
+        for (int32_t i = i0 + lane; i <= i1; i += 32) {
+          const int32_t first = max(a.row_first[tl.start + i], 0), end = max(tl.pos0 + i + 1, prefix);
+          if (first < end) {
+            lo = min(lo, first);
+            hi = max(hi, end);
+          }
+        }
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
       }
     }
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    hi = __reduce_max_sync(0xffffffffu, hi);
     j0[t] = hi > 0 ? lo / kKeys : 0;
     j1[t] = hi > 0 ? (hi + kKeys - 1) / kKeys : 0;
   }
@@ -237,7 +258,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sh.q_ready[t], kTileRows);
       mbar_init(&sh.s_full[t], 2);  // the products' commit, and the issuing thread's own arrival
-      mbar_init(&sh.p_full[t], kTileRows);
+      mbar_init(&sh.p_full[t][0], kTileRows);  // P comes in two halves of 64 keys
+      mbar_init(&sh.p_full[t][1], kTileRows);
       mbar_init(&sh.o_full[t], 1);
     }
     for (int i = 0; i < C::NS; ++i) {
@@ -286,10 +308,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         commit_elected(&sh.s_full[t]);
         arrive_elected(&sh.s_full[t]);  // passes on what was written besides (the factors)
       };
-      auto issue_pv = [&](int t, int s, bool first) {
+      auto issue_pv = [&](int t, int half, int s, bool first) {
         const uint64_t vd = v_desc + s * (C::TILE / 16);
 #pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk)
+        for (int kk = half * (kKeys / 32); kk < (half + 1) * (kKeys / 32); ++kk)
           mma_ts(tm + C::o_col(t), tm + C::s_col(t) + kk * 8, vd + kk * (2048 / 16), idesc_pv, !first || kk > 0);
       };
       bool ok = n > 0 && warp_wait(&sh.q_ready[0], 0, status) && warp_wait(&sh.q_ready[1], 0, status) &&
@@ -312,10 +334,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         for (int t = 0; t < 2; ++t) {
           const int32_t t_lo = t ? lo1 : lo0, t_hi = t ? hi1 : hi0;
           if (i >= t_lo && i < t_hi) {
-            go = warp_wait(&sh.p_full[t], (i - t_lo) & 1, status);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              go = go && warp_wait(&sh.p_full[t][half], (i - t_lo) & 1, status);
+              tc_fence_after();
+              if (go) issue_pv(t, half, s, i == t_lo);
+            }
             if (!go) break;
-            tc_fence_after();
-            issue_pv(t, s, i == t_lo);
             if (i + 1 == t_hi) commit_elected(&sh.o_full[t]);
           }
           if (i + 1 >= t_lo && i + 1 < t_hi) issue_qk(t, s1);
@@ -468,53 +493,67 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     row_range(a, tl, G, n_rows, rr, first, end, pos);
     if (!valid) end = first = 0;
     const int32_t row = tl.row0 + min(rr, n_rows - 1), tok = row / G, head = h * G + row % G;
-    // ---- the row of Q, rotated in fp32 and rounded once
+    // ---- the warp's 32 rows of Q, rotated in fp32 and rounded once: LPR lanes to a row, each with 16-byte
+    // chunks c and c + LPR (a half apart), and LPR rows to a lane, one after another, so that the heads of
+    // one token share its sines and cosines
+    uint8_t* const q_tile = smem + t * C::TILE;
     {
-      uint8_t* const q_tile = smem + t * C::TILE;
-      const uint8_t* const src = static_cast<const uint8_t*>(a.q) +
-                                 (tl.start + static_cast<int64_t>(tok)) * a.q_token_stride + static_cast<int64_t>(head) * D * 2;
-      auto rot = [&](uint32_t& w1, uint32_t& w2, float angle) {
-        float sn, cs;
-        sincos_reduced(angle, &sn, &cs);
-        const float x1 = __half2float(__ushort_as_half(static_cast<unsigned short>(w1)));
-        const float x2 = __half2float(__ushort_as_half(static_cast<unsigned short>(w2)));
-        w1 = __half_as_ushort(__float2half_rn(x1 * cs - x2 * sn));
-        w2 = __half_as_ushort(__float2half_rn(x1 * sn + x2 * cs));
+      constexpr int LPR = D / 16;
+      const int c = lane % LPR, row_a = quarter * 32 + lane / LPR * LPR;
+      auto row_of_q = [&](int k, int32_t& i) -> const uint4* {
+        const int32_t q_row = tl.row0 + min(t * kTileRows + row_a + k, n_rows - 1);
+        i = q_row / G;
+        return reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) +
+                                              (tl.start + static_cast<int64_t>(i)) * a.q_token_stride +
+                                              static_cast<int64_t>(h * G + q_row % G) * D * 2);
       };
-      const float fpos = static_cast<float>(pos);
-      constexpr int NC = D / 8;
-      // a loop, not unrolled: it runs once per block, from a cold instruction cache
-      const uint4* const src4 = reinterpret_cast<const uint4*>(src);
-      uint4 x0 = __ldg(src4), x1 = __ldg(src4 + NC / 2);
+      uint4 x[LPR][2];
+#pragma unroll
+      for (int k = 0; k < LPR; ++k) {
+        int32_t i;
+        const uint4* const src = row_of_q(k, i);
+        x[k][0] = __ldg(src + c);
+        x[k][1] = __ldg(src + c + LPR);
+      }
+#pragma unroll
+      for (int k = 0; k < LPR; ++k) {
+        *reinterpret_cast<uint4*>(q_tile + chunk_off(row_a + k, c)) = x[k][0];
+        *reinterpret_cast<uint4*>(q_tile + chunk_off(row_a + k, c + LPR)) = x[k][1];
+      }
+      // rotated in place, by a loop that is not unrolled: it runs once per block, from a cold instruction cache
+      if (a.rope_mode != AIHOST_ROPE_NONE) {
+        const bool halves = a.rope_mode == AIHOST_ROPE_NEOX;
+        float sn[8], cs[8];  // by halves: of pairs 8 c + e; else of pairs 4 c + e and 4 (c + LPR) + e - 4
+        int32_t last = -1;
 #pragma unroll 1
-      for (int c = 0; c < NC / 2; ++c) {
-        uint32_t u0[4] = {x0.x, x0.y, x0.z, x0.w}, u1[4] = {x1.x, x1.y, x1.z, x1.w};
-        if (c + 1 < NC / 2) {
-          x0 = __ldg(src4 + c + 1);
-          x1 = __ldg(src4 + c + 1 + NC / 2);
-        }
-        if (a.rope_mode == AIHOST_ROPE_NEOX) {
+        for (int k = 0; k < LPR; ++k) {
+          const int32_t i = (tl.row0 + min(t * kTileRows + row_a + k, n_rows - 1)) / G;
+          if (i != last) {
+            last = i;
+            const float fpos = static_cast<float>(tl.pos0 + i);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t a0 = u0[k] & 0xffffu, a1 = u0[k] >> 16, b0 = u1[k] & 0xffffu, b1 = u1[k] >> 16;
-            rot(a0, b0, fpos * a.freqs.f[8 * c + 2 * k]);
-            rot(a1, b1, fpos * a.freqs.f[8 * c + 2 * k + 1]);
-            u0[k] = a0 | (a1 << 16);
-            u1[k] = b0 | (b1 << 16);
+            for (int e = 0; e < 8; ++e)
+              sincos_reduced(fpos * a.freqs.f[halves ? 8 * c + e : 4 * (e < 4 ? c : c + LPR - 1) + e], &sn[e], &cs[e]);
           }
-        } else if (a.rope_mode == AIHOST_ROPE_INTERLEAVED) {
+          uint4* const p0 = reinterpret_cast<uint4*>(q_tile + chunk_off(row_a + k, c));
+          uint4* const p1 = reinterpret_cast<uint4*>(q_tile + chunk_off(row_a + k, c + LPR));
+          const uint4 v0 = *p0, v1 = *p1;
+          uint32_t u0[4] = {v0.x, v0.y, v0.z, v0.w}, u1[4] = {v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t lo = u0[k] & 0xffffu, hi = u0[k] >> 16;
-            rot(lo, hi, fpos * a.freqs.f[4 * c + k]);
-            u0[k] = lo | (hi << 16);
-            lo = u1[k] & 0xffffu, hi = u1[k] >> 16;
-            rot(lo, hi, fpos * a.freqs.f[4 * (c + NC / 2) + k]);
-            u1[k] = lo | (hi << 16);
+          for (int m = 0; m < 4; ++m) {
+            const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&u0[m]));
+            const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&u1[m]));
+            if (halves) {  // (f0.x, f1.x) and (f0.y, f1.y)
+              u0[m] = pack2(f0.x * cs[2 * m] - f1.x * sn[2 * m], f0.y * cs[2 * m + 1] - f1.y * sn[2 * m + 1]);
+              u1[m] = pack2(f0.x * sn[2 * m] + f1.x * cs[2 * m], f0.y * sn[2 * m + 1] + f1.y * cs[2 * m + 1]);
+            } else {  // (f0.x, f0.y) and (f1.x, f1.y)
+              u0[m] = pack2(f0.x * cs[m] - f0.y * sn[m], f0.x * sn[m] + f0.y * cs[m]);
+              u1[m] = pack2(f1.x * cs[4 + m] - f1.y * sn[4 + m], f1.x * sn[4 + m] + f1.y * cs[4 + m]);
+            }
           }
+          *p0 = make_uint4(u0[0], u0[1], u0[2], u0[3]);
+          *p1 = make_uint4(u1[0], u1[1], u1[2], u1[3]);
         }
-        *reinterpret_cast<uint4*>(q_tile + chunk_off(r, c)) = make_uint4(u0[0], u0[1], u0[2], u0[3]);
-        *reinterpret_cast<uint4*>(q_tile + chunk_off(r, c + NC / 2)) = make_uint4(u1[0], u1[1], u1[2], u1[3]);
       }
       fence_proxy_async_smem();
       mbar_arrive(&sh.q_ready[t]);
@@ -595,11 +634,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         l *= f_o;
         m = mx;
       }
+      // the P V before was committed ahead of this S: O is at rest
+      if (i > 0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {  // 8 columns at a time: S is in registers
+          uint32_t o[8];
+          tmem_ld8(o_tmem + c * 8, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f_o);
+          tmem_st8(o_tmem + c * 8, o);
+        }
+      }
       const float2 neg_m = make_float2(-m, -m);
       float2 sum[4] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-      uint32_t pk[4][16];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 4; ++c) {
+        uint32_t pk[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int f = c * 2 + e / 8;
@@ -609,26 +660,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           sum[e & 3] = fadd2(sum[e & 3], p);
           const float vf = sh.v_factor[slot][f];
           const float2 pv = fmul2(p, make_float2(vf, vf));
-          pk[c][e] = pack2(pv.x, pv.y);
+          pk[e] = pack2(pv.x, pv.y);
         }
-      l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
-      // the P V before was committed ahead of this S: O is at rest
-      if (i > 0 && __any_sync(0xffffffffu, grow)) {
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(o_tmem + c * 32, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f_o);
-          tmem_st32(o_tmem + c * 32, o);
+        tmem_st16(s_tmem + c * 16, pk);
+        if (c & 1) {  // the half's products can start (the O rescale has completed with it)
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(&sh.p_full[t][c >> 1]);
         }
       }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_st16(s_tmem + c * 16, pk[c]);
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(&sh.p_full[t]);
+      l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
     }
     // ---- O / l, or this chunk's share of it
     if (ok && n_own > 0) ok = warp_wait(&sh.o_full[t], 0, status);
@@ -638,18 +679,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         n_own > 0 ? fmaxf(fmaxf(sh.v_max[0], sh.v_max[1]), fmaxf(sh.v_max[2], sh.v_max[3])) : 0.0f;
     const float o_unit = vmax * (1.0f / kVUnit);
     const int64_t out_row = ((tl.start + static_cast<int64_t>(tok)) * a.g.n_q_heads + head) * D;
+    // fp16: into the query tile's space (its last product is done), then out by whole rows
+    const bool by_rows = a.out_dtype == AIHOST_F16;
     auto store32 = [&](int c, const float (&o)[32]) {
-      if (!valid) return;
-      if (a.out_dtype == AIHOST_F16) {
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(a.out) + out_row + c * 32);
+      if (by_rows) {
 #pragma unroll
         for (int v = 0; v < 4; ++v)
-          dst[v] = make_uint4(pack2(o[8 * v], o[8 * v + 1]), pack2(o[8 * v + 2], o[8 * v + 3]),
+          *reinterpret_cast<uint4*>(q_tile + chunk_off(r, 4 * c + v)) =
+              make_uint4(pack2(o[8 * v], o[8 * v + 1]), pack2(o[8 * v + 2], o[8 * v + 3]),
                               pack2(o[8 * v + 4], o[8 * v + 5]), pack2(o[8 * v + 6], o[8 * v + 7]));
-      } else {
+      } else if (valid) {
         float4* dst = reinterpret_cast<float4*>(static_cast<float*>(a.out) + out_row + c * 32);
 #pragma unroll
         for (int v = 0; v < 8; ++v) dst[v] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+      }
+    };
+    auto flush_rows = [&] {
+      if (!by_rows) return;
+      __syncwarp();
+      constexpr int LR = D / 8;  // lanes to a row
+#pragma unroll 4
+      for (int k = 0; k < LR; ++k) {
+        const int src = k * (32 / LR) + lane / LR;  // row of the warp
+        const int64_t row_at = __shfl_sync(0xffffffffu, out_row, src);
+        const bool on = __shfl_sync(0xffffffffu, static_cast<int>(valid), src);
+        if (on)
+          *reinterpret_cast<uint4*>(static_cast<__half*>(a.out) + row_at + lane % LR * 8) =
+              *reinterpret_cast<const uint4*>(q_tile + chunk_off(quarter * 32 + src, lane % LR));
       }
     };
     const int64_t unit = static_cast<int64_t>(tile) * H + h;
@@ -681,6 +737,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         }
       }
       if (n_splits > 1) part_ml[static_cast<int64_t>(split) * kRows] = make_float2(m, l);
+      else flush_rows();
     }
     if (n_splits > 1) {  // the last block of this tile and head to arrive merges the chunks
       __threadfence();
@@ -712,6 +769,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           }
           store32(c, o);
         }
+        flush_rows();
       }
     }
   }
@@ -740,14 +798,29 @@ void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t
   const int32_t G = g.n_q_heads / g.n_kv_heads;
   const int64_t n = static_cast<int64_t>(max_new) * G <= kRows ? batch : static_cast<int64_t>(n_tokens) * G / kRows + batch;
   const int64_t units = n * g.n_kv_heads, tiles_kv = (max_kv + kKeys - 1) / kKeys;
-  // one block per SM at a time: cut the ranges where that evens out the waves, into chunks of 8 tiles at least
+  // One block per SM at a time; kFixed and kPart: a block's fixed work, and a partial result's writing
+  // and its share of the merge, in tiles. The lengths are on the device; where the sequences bring about
+  // as many new rows each (n_tokens near batch * max_new), they are taken as alike, and waves count. Else
+  // the blocks are taken as of every length, spread evenly but for a third of one.
+  constexpr double kFixed = 3.0, kPart = 2.0, kMerge = 0.7;
+  const int64_t of_one = (static_cast<int64_t>(max_new) * G + kRows - 1) / kRows;
+  const int64_t full = std::min(units, of_one * batch * g.n_kv_heads);  // tiles that can have rows
+  const double even = static_cast<double>(n_tokens) / (static_cast<double>(batch) * max_new);
+  const double average = (even < 1.0 ? even : 1.0) * (static_cast<double>(tiles_kv) - 0.5 * max_new / kKeys);
   int64_t best = 1;
-  double best_cost = 1e30;
-  for (int64_t s = 1; s <= 16 && (s == 1 || tiles_kv / s >= 8); ++s) {
-    const int64_t waves = (units * s + num_sms - 1) / num_sms;
-    const double cost = static_cast<double>(waves) * (static_cast<double>((tiles_kv + s - 1) / s) + 3.0);
-    if (cost < best_cost * 0.97) {
-      best_cost = cost;
+  double best_end = 1e30;
+  for (int64_t s = 1; s <= 32 && (s == 1 || tiles_kv / s >= 4); ++s) {
+    const double block = static_cast<double>((tiles_kv + s - 1) / s) + kFixed + (s > 1 ? kPart : 0.0);
+    double end = block;
+    if (even > 0.9) {
+      end = static_cast<double>((full * s + num_sms - 1) / num_sms) * block;
+    } else {
+      const double spread = full * (average + even * s * (block - (tiles_kv + s - 1) / s)) / num_sms + 0.35 * block;
+      if (spread > end) end = spread;
+    }
+    if (s > 1) end += kMerge * s;
+    if (end < best_end * 0.97) {
+      best_end = end;
       best = s;
     }
   }
