@@ -103,6 +103,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv8_append_kernel(const __grid
   const int64_t n_slots = static_cast<int64_t>(a.g.n_pages) << a.g.page_shift;
   const bool rotate = ROPE != AIHOST_ROPE_NONE && is_k;
 
+  griddep_wait();
+  griddep_launch_dependents();
   if (threadIdx.x < 1 + window + P) {
     const int64_t t = static_cast<int64_t>(t0) + threadIdx.x - 1;
     slot_sh[threadIdx.x] = t >= 0 && t < a.n_tokens ? a.slots[t] : -1;
@@ -298,6 +300,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv8_append_kernel(const __grid
 template <typename T>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8ReadArgs a, uint32_t per_row, uint32_t per_head_shift) {
   const int64_t n_slots = static_cast<int64_t>(a.g.n_pages) << a.g.page_shift;
+  griddep_wait();
+  griddep_launch_dependents();
   for (int32_t row = blockIdx.x * blockDim.y + threadIdx.y; row < a.n_rows; row += gridDim.x * blockDim.y) {
     const int64_t slot = a.slots[row];
     const bool on = slot >= 0 && slot < n_slots;
@@ -325,34 +329,31 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8ReadArgs a, uint
 }
 
 template <int D, typename T, int ROPE>
-void launch_append_r(const Kv8AppendArgs& a, cudaStream_t st) {
+cudaError_t launch_append_r(const Kv8AppendArgs& a, cudaStream_t st) {
   // Few tokens: windows of 16, for more blocks. Many: a page's rows, so that no block of a prompt's
   // window starts no run.
   const int32_t window = a.n_tokens < 1024 ? 16 : a.g.page_rows;
   const dim3 grid((a.n_tokens + window - 1) / window, 2 * ((a.g.n_kv_heads + kHeads - 1) / kHeads));
-  if (a.g.page_rows == 128) kv8_append_kernel<D, 8, 1, T, ROPE><<<grid, kWarps * 32, 0, st>>>(a, window);
-  else kv8_append_kernel<D, 4, 2, T, ROPE><<<grid, kWarps * 32, 0, st>>>(a, window);
+  auto kern = a.g.page_rows == 128 ? kv8_append_kernel<D, 8, 1, T, ROPE> : kv8_append_kernel<D, 4, 2, T, ROPE>;
+  return launch_dependent(kern, grid, kWarps * 32, 0, st, a, window);
 }
 
 template <int D, typename T>
-void launch_append_t(const Kv8AppendArgs& a, cudaStream_t st) {
-  if (a.rope_mode == AIHOST_ROPE_NONE) launch_append_r<D, T, AIHOST_ROPE_NONE>(a, st);
-  else if (a.rope_mode == AIHOST_ROPE_NEOX) launch_append_r<D, T, AIHOST_ROPE_NEOX>(a, st);
-  else launch_append_r<D, T, AIHOST_ROPE_INTERLEAVED>(a, st);
+cudaError_t launch_append_t(const Kv8AppendArgs& a, cudaStream_t st) {
+  if (a.rope_mode == AIHOST_ROPE_NONE) return launch_append_r<D, T, AIHOST_ROPE_NONE>(a, st);
+  if (a.rope_mode == AIHOST_ROPE_NEOX) return launch_append_r<D, T, AIHOST_ROPE_NEOX>(a, st);
+  return launch_append_r<D, T, AIHOST_ROPE_INTERLEAVED>(a, st);
 }
 
 template <int D>
-void launch_append_d(const Kv8AppendArgs& a, cudaStream_t st) {
-  if (a.io_dtype == AIHOST_F32) launch_append_t<D, float>(a, st);
-  else launch_append_t<D, __half>(a, st);
+cudaError_t launch_append_d(const Kv8AppendArgs& a, cudaStream_t st) {
+  return a.io_dtype == AIHOST_F32 ? launch_append_t<D, float>(a, st) : launch_append_t<D, __half>(a, st);
 }
 
 }  // namespace
 
 cudaError_t launch_kv8_append(const Kv8AppendArgs& a, cudaStream_t st) {
-  if (a.g.head_dim == 64) launch_append_d<64>(a, st);
-  else launch_append_d<128>(a, st);
-  return cudaGetLastError();
+  return a.g.head_dim == 64 ? launch_append_d<64>(a, st) : launch_append_d<128>(a, st);
 }
 
 cudaError_t launch_kv8_read(const Kv8ReadArgs& a, cudaStream_t st) {
@@ -362,9 +363,8 @@ cudaError_t launch_kv8_read(const Kv8ReadArgs& a, cudaStream_t st) {
   const dim3 block(x, 256 / x);
   const int64_t want = (a.n_rows + block.y - 1) / block.y;
   const int blocks = static_cast<int>(want < 148 * 16 ? want : 148 * 16);
-  if (a.out_dtype == AIHOST_F16) kv8_read_kernel<__half><<<blocks, block, 0, st>>>(a, per_row, shift);
-  else kv8_read_kernel<float><<<blocks, block, 0, st>>>(a, per_row, shift);
-  return cudaGetLastError();
+  return launch_dependent(a.out_dtype == AIHOST_F16 ? kv8_read_kernel<__half> : kv8_read_kernel<float>, blocks, block, 0, st, a,
+                          per_row, shift);
 }
 
 }  // namespace aihost

@@ -102,6 +102,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
   const int32_t h = static_cast<int32_t>(blockIdx.x % H);
   const int64_t tile = blockIdx.x / H;
   const int32_t split = static_cast<int32_t>(blockIdx.y);
+  griddep_wait();
+  griddep_launch_dependents();
   const Tile tl = find_tile(a, tile, G, R, lane);
   if (!tl.ok) return;
   const int32_t n_rows = min(R, tl.n_new * G - tl.row0);
@@ -575,8 +577,7 @@ cudaError_t launch_one(const Kv8AttnArgs& a, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
     if (e != cudaSuccess) return e;
   }
-  kern<<<dim3(static_cast<unsigned>(a.tiles) * a.g.n_kv_heads, a.max_splits), kWarps * 32, kBytes, st>>>(a);
-  return cudaGetLastError();
+  return launch_dependent(kern, dim3(static_cast<unsigned>(a.tiles) * a.g.n_kv_heads, a.max_splits), kWarps * 32, kBytes, st, a);
 }
 
 template <int D, int NT, int PREC>

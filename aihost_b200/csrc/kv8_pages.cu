@@ -57,6 +57,8 @@ __global__ void __launch_bounds__(1024) page_map_kernel(const PageMapArgs a) {
   int32_t* taken = sums + a.batch + 1;
   __shared__ Sums warp_sums[32];
   __shared__ int32_t last_block;
+  griddep_wait();
+  griddep_launch_dependents();
   const int32_t avail = *a.free_count;
   Sums carry = {0, 0};
   bool bad = avail < 0 || avail > a.n_pages;
@@ -133,6 +135,8 @@ __global__ void __launch_bounds__(1024) page_map_kernel(const PageMapArgs a) {
 __global__ void __launch_bounds__(1024) page_release_kernel(const PageReleaseArgs a) {
   extern __shared__ int32_t before[];  // [batch] pages returned before
   __shared__ Sums warp_sums[32];
+  griddep_wait();
+  griddep_launch_dependents();
   const int32_t have = *a.free_count;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   bool bad = have < 0;
@@ -194,13 +198,12 @@ cudaError_t launch_page_map(const PageMapArgs& a, cudaStream_t st) {
                                          static_cast<int>(smem));
     if (e != cudaSuccess) return e;
   }
-  page_map_kernel<<<blocks, threads, smem, st>>>(a);
-  return cudaGetLastError();
+  return launch_dependent(page_map_kernel, blocks, threads, smem, st, a);
 }
 
 cudaError_t launch_page_release(const PageReleaseArgs& a, cudaStream_t st) {
-  page_release_kernel<<<1, a.batch <= 256 ? 256 : 1024, static_cast<size_t>(a.batch) * sizeof(int32_t), st>>>(a);
-  return cudaGetLastError();
+  return launch_dependent(page_release_kernel, 1, a.batch <= 256 ? 256 : 1024,
+                          static_cast<size_t>(a.batch) * sizeof(int32_t), st, a);
 }
 
 }  // namespace aihost

@@ -14,6 +14,7 @@
 #include <stdio.h>
 
 #include <initializer_list>
+#include <utility>
 
 #include "../../include/aihost_attn.h"
 
@@ -127,6 +128,15 @@ struct Call {
   }
 };
 
+// n elements of `type` of base's storage from element `at` on (counted in that type).
+at::Tensor part_of(const at::Tensor& base, at::ScalarType type, int64_t at, int64_t n) {
+  auto impl = c10::make_intrusive<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(base.storage()), base.key_set(),
+                                                   c10::scalarTypeToTypeMeta(type));
+  impl->set_storage_offset(at);
+  impl->set_sizes_contiguous({n});
+  return at::Tensor(std::move(impl));
+}
+
 template <typename F>
 PyObject* guarded(Py_ssize_t got, Py_ssize_t want, F&& f) {
   if (got != want) {
@@ -158,8 +168,13 @@ PyObject* map_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     int32_t* table = c.array<int32_t>(a[9], "block_table", at::kInt, {n, c.d.max_pages});
     PyObject* out[5];
     if (a[10] == Py_None) {
-      const at::Tensor t[5] = {c.make({n}, at::kInt), c.make({n + 1}, at::kInt), c.make({most}, at::kLong),
-                               c.make({most}, at::kInt), c.make({1}, at::kInt)};
+      // one allocation for the five: slots first, every part on a 16-byte boundary
+      const int64_t pos_at = 2 * ((static_cast<int64_t>(most) + 1) / 2 * 2), len_at = pos_at + (most + 3) / 4 * 4;
+      const int64_t start_at = len_at + (n + 3) / 4 * 4, count_at = start_at + (n + 4) / 4 * 4;
+      const at::Tensor all = c.make({count_at / 2 + 2}, at::kLong);
+      const at::Tensor t[5] = {part_of(all, at::kInt, len_at, n), part_of(all, at::kInt, start_at, n + 1),
+                               part_of(all, at::kLong, 0, most), part_of(all, at::kInt, pos_at, most),
+                               part_of(all, at::kInt, count_at, 1)};
       for (int i = 0; i < 5; ++i) out[i] = THPVariable_Wrap(t[i]);
     } else {
       if (!PyTuple_Check(a[10]) || PyTuple_GET_SIZE(a[10]) != 5) raise(AIHOST_EINVAL, "into must hold five tensors");

@@ -118,6 +118,24 @@ __device__ __forceinline__ void sincos_near(float a, float* s, float* c) {
   *c = (q + 1) & 2 ? -v : v;
 }
 
+// Launch that may begin before the kernel ahead of it on the stream has ended: every kernel launched so
+// calls griddep_wait() before it touches memory (the kernel ahead is then complete and visible), and
+// griddep_launch_dependents() at its own start, so that the next one's set-up overlaps its work.
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Whether this is the last of n arrivals, by one thread of each block after its own writes and a fence.
 // The counter wraps to zero with the last, ready for the next launch (and for a replayed one). No block
 // waits for another.
