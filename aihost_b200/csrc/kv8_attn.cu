@@ -104,6 +104,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
   const int32_t split = static_cast<int32_t>(blockIdx.y);
   griddep_wait();
   griddep_launch_dependents();
+  // One tile a sequence and no documents: the sequence and the first row of this chunk are known before
+  // the lengths, so the table entry of this lane's first block of rows comes along with them.
+  const bool known = static_cast<int64_t>(a.max_new) * G <= R && !a.row_first;
+  int32_t entry_early = 0;
+  if (known) {
+    const int32_t row = split * a.chunk + warp * kStep + (lane >> 1) * (kWarps * kStep) + (lane & 1) * kSub;
+    if ((row >> ps) < a.g.max_pages) entry_early = a.block_table[tile * a.g.max_pages + (row >> ps)];
+  }
   const Tile tl = find_tile(a, tile, G, R, lane);
   if (!tl.ok) return;
   const int32_t n_rows = min(R, tl.n_new * G - tl.row0);
@@ -144,15 +152,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
   auto row_of = [&](int32_t sub) { return k_mine + (sub >> 1) * (kWarps * kStep) + (sub & 1) * kSub; };
   // lane j: where block 32 * round + j lies (its offset in either pool; none past the end), its scales
   constexpr int64_t kNowhere = -1;
+  auto place_at = [&](int32_t row, int32_t entry, int64_t& ph) -> int64_t {
+    ph = page_or_first(entry, a.g.n_pages, stray) * H + h;
+    return ((ph << ps) + (row & (a.g.page_rows - 1))) * D;
+  };
   auto place_of = [&](int32_t sub, int64_t& ph) -> int64_t {
     const int32_t row = row_of(sub);
     ph = 0;
-    if ((sub >> 1) >= n_steps || row >= k_end) return kNowhere;
-    ph = page_or_first(table[row >> ps], a.g.n_pages, stray) * H + h;
-    return ((ph << ps) + (row & (a.g.page_rows - 1))) * D;
+    return (sub >> 1) >= n_steps || row >= k_end ? kNowhere : place_at(row, table[row >> ps], ph);
   };
-  int64_t ph, ph_next;
-  int64_t place = place_of(lane, ph), place_next = n_steps > 16 ? place_of(32 + lane, ph_next) : kNowhere;
+  int64_t ph = 0, ph_next = 0, place = kNowhere;
+  if (!known) place = place_of(lane, ph);
+  else if ((lane >> 1) < n_steps && row_of(lane) < k_end) place = place_at(row_of(lane), entry_early, ph);
+  int64_t place_next = n_steps > 16 ? place_of(32 + lane, ph_next) : kNowhere;
   constexpr int kStageBytes = SplitSmem<D, NT>::kStageBytes;
   uint8_t* const my_ring = ring + warp * (kStages * kStageBytes);
   // copies of a 16-row block: chunk j * 32 + lane of its K and V rows each
@@ -519,53 +531,42 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
   if (!last_sh) return;
   __threadfence();
   const int64_t first_part = unit * a.max_splits * R;
-  // the chunks' weights per row, over the ring: few enough at a time for any number of chunks
-  float* const w_sh = reinterpret_cast<float*>(ring);
-  constexpr int kAtOnce = SplitSmem<D, NT>::kBytes / (R * 8);  // chunks whose (max, sum) fit
-  constexpr int kVec = R * (D / 4) / (kWarps * 32);            // float4 of the result per thread
-  float4 acc[kVec];
-  float mm[kVec], ll[kVec];
+  constexpr int kVec = R * (D / 4) / (kWarps * 32);  // float4 of the result per thread
+  constexpr int kAtOnce = 8;                         // chunks whose parts are in flight together
 #pragma unroll
   for (int v = 0; v < kVec; ++v) {
-    acc[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    mm[v] = kNoMax;
-    ll[v] = 0.0f;
-  }
-  for (int32_t s0 = 0; s0 < n_splits; s0 += kAtOnce) {
-    const int32_t ns = min(kAtOnce, n_splits - s0);
-    __syncthreads();
-    for (int32_t i = threadIdx.x; i < ns * R; i += kWarps * 32)
-      reinterpret_cast<float2*>(w_sh)[i] =
-          __ldcg(reinterpret_cast<const float2*>(a.part_ml) + first_part + static_cast<int64_t>(s0) * R + i);
-    __syncthreads();
+    const int at = v * (kWarps * 32) + threadIdx.x, r = at / (D / 4), d4 = at % (D / 4);
+    if (r >= n_rows) continue;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float mm = kNoMax, ll = 0.0f;
+    for (int32_t s0 = 0; s0 < n_splits; s0 += kAtOnce) {
+      const int64_t p0 = first_part + static_cast<int64_t>(s0) * R + r;
+      float2 ml[kAtOnce];
+      float4 x[kAtOnce];
 #pragma unroll
-    for (int v = 0; v < kVec; ++v) {
-      const int at = v * (kWarps * 32) + threadIdx.x, r = at / (D / 4), d4 = at % (D / 4);
-      if (r >= n_rows) continue;
-      float top = mm[v];
-      for (int32_t sp = 0; sp < ns; ++sp) top = fmaxf(top, w_sh[(sp * R + r) * 2]);
-      const float f0 = ex2_approx(mm[v] - top);
-      ll[v] *= f0;
-      acc[v] = make_float4(acc[v].x * f0, acc[v].y * f0, acc[v].z * f0, acc[v].w * f0);
-      mm[v] = top;
-      const float4* const src = reinterpret_cast<const float4*>(a.part_o) +
-                                (first_part + static_cast<int64_t>(s0) * R + r) * (D / 4) + d4;
-#pragma unroll 8
-      for (int32_t sp = 0; sp < ns; ++sp) {
-        const float4 x = __ldcg(src + static_cast<int64_t>(sp) * R * (D / 4));
-        const float f = ex2_approx(w_sh[(sp * R + r) * 2] - top);
-        ll[v] += w_sh[(sp * R + r) * 2 + 1] * f;
-        acc[v].x += x.x * f, acc[v].y += x.y * f, acc[v].z += x.z * f, acc[v].w += x.w * f;
+      for (int q = 0; q < kAtOnce; ++q) {
+        const bool on = s0 + q < n_splits;
+        ml[q] = on ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + p0 + q * R) : make_float2(kNoMax, 0.0f);
+        x[q] = on ? __ldcg(reinterpret_cast<const float4*>(a.part_o) + (p0 + q * R) * (D / 4) + d4)
+                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+      float top = mm;
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) top = fmaxf(top, ml[q].x);
+      const float f0 = ex2_approx(mm - top);
+      mm = top;
+      ll *= f0;
+      acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {
+        const float f = ex2_approx(ml[q].x - top);
+        ll += ml[q].y * f;
+        acc.x += x[q].x * f, acc.y += x[q].y * f, acc.z += x[q].z * f, acc.w += x[q].w * f;
       }
     }
-  }
-#pragma unroll
-  for (int v = 0; v < kVec; ++v) {
-    const int at = v * (kWarps * 32) + threadIdx.x, r = at / (D / 4), d = at % (D / 4) * 4;
-    if (r >= n_rows) continue;
-    const float inv = ll[v] != 0.0f ? 1.0f / ll[v] : 0.0f;
-    store(r, d, acc[v].x * inv, acc[v].y * inv);
-    store(r, d + 2, acc[v].z * inv, acc[v].w * inv);
+    const float inv = ll != 0.0f ? 1.0f / ll : 0.0f;
+    store(r, 4 * d4, acc.x * inv, acc.y * inv);
+    store(r, 4 * d4 + 2, acc.z * inv, acc.w * inv);
   }
 }
 
