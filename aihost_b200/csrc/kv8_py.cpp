@@ -7,6 +7,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/StreamGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -67,12 +68,14 @@ struct Call {
   int device;
   aihost_kv8_desc d;
   cudaStream_t stream;
+  bool given;  // the stream was named, not torch's current one
 
   explicit Call(PyObject* const* a) {
     ctx = reinterpret_cast<aihost_attn_ctx*>(integer(a[0]));
     device = static_cast<int>(integer(a[1]));
     d = *reinterpret_cast<const aihost_kv8_desc*>(integer(a[2]));
-    stream = a[3] == Py_None ? c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream()
+    given = a[3] != Py_None;
+    stream = !given ? c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream()
                              : reinterpret_cast<cudaStream_t>(integer(a[3]));
   }
 
@@ -124,6 +127,8 @@ struct Call {
     return array<float>(o, name, at::kFloat, {d.n_pages, d.n_kv_heads});
   }
   at::Tensor make(at::IntArrayRef sizes, at::ScalarType type) const {
+    c10::OptionalStreamGuard on;  // a result written on a stream of the caller's is that stream's memory
+    if (given) on.reset_stream(c10::cuda::getStreamFromExternal(stream, static_cast<c10::DeviceIndex>(device)));
     return at::empty(sizes, at::TensorOptions().dtype(type).device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
   }
 };

@@ -509,6 +509,22 @@ def test_same_inputs_same_bits(ctx):
         assert torch.equal(w.attend(q.to(DEV)), first)
 
 
+def test_more_tiles_than_merge_counters(ctx):
+    """Too many tiles to merge chunks of: every block takes its whole range, in rounds of 32 blocks of rows a warp. The
+    long sequence's rows match the same call on it alone, which is cut into chunks."""
+    B, H, long = 1100, 64, 5000
+    cached = [long if b == 700 else 3 + b % 20 for b in range(B)]
+    w = World(ctx, cached, [1] * B, Hq=H, H=H, D=64, P=16, seed=12)
+    q, _ = w.rows(H)
+    out = w.attend(q.to(DEV))
+    torch.cuda.synchronize()
+    ctx.sync_status()
+    w.start, w.kv_len, w.table, w.new = np.array([0, 1]), w.kv_len[700:701], w.table[700:701], [1]
+    alone = w.attend(q[700:701].to(DEV))
+    ctx.sync_status()
+    assert (out[700].float() - alone[0].float()).abs().max() <= 2.0 ** -9 * alone.abs().max()
+
+
 # ------------------------------------------------------------------------------------------------ together
 
 @pytest.mark.parametrize("D, P, io", [(64, 16, F16), (128, 64, F32)])
