@@ -110,11 +110,11 @@ void kv8_mma_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max
                   int32_t* tiles, int32_t* chunk, int32_t* splits);
 cudaError_t launch_kv8_mma(const Kv8AttnArgs& a, cudaStream_t st);
 
-// The tcgen05 kernel (query rows per block 256), for this many query rows of a sequence's KV head on.
-constexpr int32_t kKv8TensorMinRows = 64;
+// The tcgen05 kernel (query rows per block 256) and its plan; *end: its length as the plan sees it, in
+// times of one 128-row cache tile (about 2.1 us at head_dim 128 and 1.7 at 64).
 int32_t kv8_prefill_rows();
 void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max_new, int32_t max_kv, int32_t num_sms,
-                      int32_t* tiles, int32_t* chunk, int32_t* splits);
+                      int32_t* tiles, int32_t* chunk, int32_t* splits, double* end);
 cudaError_t launch_kv8_prefill(const Kv8AttnArgs& a, cudaStream_t st);
 
 }  // namespace aihost

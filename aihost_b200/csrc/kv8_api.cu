@@ -94,14 +94,27 @@ struct Plan {
 
 Plan make_plan(const aihost_kv8_desc* d, const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max_new,
                int32_t max_kv, int32_t num_sms) {
+  // The tcgen05 kernel takes fp16 rows by 256 and has ~12 us of fixed work a block; the split-cache one
+  // takes 16 and rereads the cache for each tile, ~50 ns (head_dim 64: 37) per tile and 1000 rows over the
+  // whole GPU, and fills it with little work. Measured, head_dim 128, 32/8 heads, tcgen05 against split-cache:
+  // 8 sequences of 8192 rows with 8 new ones 85 and 69 us, with 16 85 and 116; one sequence with 32
+  // 42 and 41, with 64 45 and 66; 8 of 512 rows with 16 19 and 15, with 32 19 and 27.
   Plan p;
-  p.tensor = d->io_dtype == AIHOST_F16 &&
-             static_cast<int64_t>(max_new) * (g.n_q_heads / g.n_kv_heads) >= kKv8TensorMinRows;
+  const int32_t rows = kv8_mma_rows(g, max_new), G = g.n_q_heads / g.n_kv_heads;
+  p.tensor = false;
+  if (d->io_dtype == AIHOST_F16 && static_cast<int64_t>(max_new) * G > rows) {
+    double end;
+    kv8_prefill_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.chunk, &p.splits, &end);
+    const double even = static_cast<double>(n_tokens) / (static_cast<double>(batch) * max_new);
+    const double by_tc = end * (g.head_dim == 128 ? 2.1 : 1.7);
+    const double tiles16 = (static_cast<double>(n_tokens) * G / rows + 0.5 * batch) * g.n_kv_heads;
+    const double by_mma = 8.0 + tiles16 * max_kv * (even > 0.9 ? 1.0 : even) * (g.head_dim == 128 ? 50e-6 : 37e-6);
+    p.tensor = by_tc < by_mma;
+  }
   if (p.tensor) {
     p.rows = kv8_prefill_rows();
-    kv8_prefill_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.chunk, &p.splits);
   } else {
-    p.rows = kv8_mma_rows(g, max_new);
+    p.rows = rows;
     kv8_mma_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.chunk, &p.splits);
   }
   return p;

@@ -796,7 +796,7 @@ cudaError_t launch_d(const Kv8AttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max_new, int32_t max_kv, int32_t num_sms,
-                      int32_t* tiles, int32_t* chunk, int32_t* splits) {
+                      int32_t* tiles, int32_t* chunk, int32_t* splits, double* end_out) {
   const int32_t G = g.n_q_heads / g.n_kv_heads;
   const int64_t n = static_cast<int64_t>(max_new) * G <= kRows ? batch : static_cast<int64_t>(n_tokens) * G / kRows + batch;
   const int64_t units = n * g.n_kv_heads, tiles_kv = (max_kv + kKeys - 1) / kKeys;
@@ -828,6 +828,7 @@ void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t
   }
   if (units > kKv8Counters) best = 1;
   const int64_t c = (tiles_kv + best - 1) / best;
+  *end_out = best_end;
   *tiles = static_cast<int32_t>(n);
   *chunk = static_cast<int32_t>(c * kKeys);
   *splits = static_cast<int32_t>((tiles_kv + c - 1) / c);

@@ -343,11 +343,26 @@ ATTENDS = {
 }
 
 
+# Which kernel runs, and how the ranges are cut, goes by the bounds that the host gives: with the tight bound these
+# small cases take the split-cache kernel, with the loose one several rows a sequence take the tcgen05 kernel.
+BOUNDS = [None, 100000]
+
+
+@pytest.mark.parametrize("max_kv", BOUNDS)
 @pytest.mark.parametrize("io", [F16, F32])
 @pytest.mark.parametrize("mode", [ROPE_NONE, ROPE_INTERLEAVED, ROPE_NEOX])
 @pytest.mark.parametrize("case", list(ATTENDS))
-def test_attention(ctx, case, mode, io):
-    World(ctx, mode=mode, io=io, seed=len(case), **ATTENDS[case]).check(ctx)
+def test_attention(ctx, case, mode, io, max_kv):
+    World(ctx, mode=mode, io=io, seed=len(case), **ATTENDS[case]).check(ctx, max_kv=max_kv)
+
+
+@pytest.mark.parametrize("max_kv", [None, 20000, 60000])
+@pytest.mark.parametrize("D, P, mode", [(64, 16, ROPE_NEOX), (128, 128, ROPE_INTERLEAVED), (128, 16, ROPE_NONE)])
+def test_attention_in_chunks(ctx, D, P, mode, max_kv):
+    """Prompts over long caches: their ranges are cut, by either kernel, and merged."""
+    w = World(ctx, [3300, 100, 0, 1500], [90, 40, 33, 1], Hq=8, H=1, D=D, P=P, mode=mode)
+    w.check(ctx, max_kv=max_kv)
+    w.check(ctx, max_kv=max_kv, prefix=[3000, 139, 40, 0], slopes=[2.0 ** -(h + 1) for h in range(8)])
 
 
 MASKS = {
@@ -359,18 +374,19 @@ MASKS = {
 }
 
 
+@pytest.mark.parametrize("max_kv", BOUNDS)
 @pytest.mark.parametrize("io", [F16, F32])
 @pytest.mark.parametrize("D, Hq, H, P", [(64, 8, 2, 16), (128, 8, 8, 64), (128, 32, 4, 32)])
 @pytest.mark.parametrize("mask", list(MASKS))
 @pytest.mark.parametrize("new", [[1, 1, 1, 1], [5, 33, 0, 150]])
-def test_attention_masks(ctx, mask, new, D, Hq, H, P, io):
+def test_attention_masks(ctx, mask, new, D, Hq, H, P, io, max_kv):
     m = dict(MASKS[mask])
     w = World(ctx, [0, 40, 77, 300], new, Hq=Hq, H=H, D=D, P=P, io=io, cap=m.pop("cap", 0.0), seed=len(mask))
     slopes = [2.0 ** (-8 * (h + 1) / Hq) for h in range(Hq)] if m.get("slopes") else None
     first = None
     if m.get("first"):  # documents of uneven length; every seventh row sees nothing
         first = [int(w.g.integers(0, p + 1)) if t % 7 else p + 1 + 1000 * (t % 2) for t, p in enumerate(w.pos)]
-    got = w.check(ctx, std=3.0, slopes=slopes, first=first, prefix=m.get("prefix"))
+    got = w.check(ctx, std=3.0, slopes=slopes, first=first, prefix=m.get("prefix"), max_kv=max_kv)
     if first is not None and m.get("prefix") is None:
         assert (got[0] == 0).all()
 
@@ -381,18 +397,20 @@ def test_attention_of_capped_and_large_scores(ctx):
         World(ctx, [600], [1], D=128, P=64, io=F32, cap=cap, scale=1.0).check(ctx, std=8.0)
 
 
-def test_attention_with_uneven_page_scales(ctx):
+@pytest.mark.parametrize("max_kv", BOUNDS)
+def test_attention_with_uneven_page_scales(ctx, max_kv):
     """V scales from 1e-4 to 10 side by side, and pages of scale zero."""
     w = World(ctx, [500, 90], [1, 30], P=16, D=128)
     w.vs = np.exp(w.g.uniform(np.log(1e-4), np.log(10), w.vs.shape)).astype(np.float32)
     w.ks[::5] = 0
     w.vs[::7] = 0
-    w.check(ctx)
+    w.check(ctx, max_kv=max_kv)
     w.vs[:] = 0
-    assert (w.check(ctx) == 0).all()
+    assert (w.check(ctx, max_kv=max_kv) == 0).all()
 
 
-def test_attention_ignores_what_it_may_not_see(ctx):
+@pytest.mark.parametrize("max_kv", BOUNDS)
+def test_attention_ignores_what_it_may_not_see(ctx, max_kv):
     """NaN scales on pages in nobody's hands, past the end, before the document, and stale rows on the last page."""
     w = World(ctx, [100, 33], [1, 40], P=16, D=128)
     used = np.zeros(w.n_pages, bool)
@@ -400,19 +418,19 @@ def test_attention_ignores_what_it_may_not_see(ctx):
         used[w.table[b][:-(-int(L) // 16)]] = True
     w.ks[~used] = np.nan
     w.vs[~used] = np.nan
-    ref = w.check(ctx)
+    ref = w.check(ctx, max_kv=max_kv)
     assert np.isfinite(ref).all()
     first = [64] + [48 if p >= 48 else 0 for p in w.pos[1:]]
     w.ks[w.table[0][0]] = w.vs[w.table[0][1]] = np.nan  # rows 0..31 of sequence 0, hidden by its document
-    w.check(ctx, first=first)
+    w.check(ctx, first=first, max_kv=max_kv)
     w.ks[w.table[1][0]] = np.nan  # rows 0..15 of sequence 1: seen by its first document's rows only
     q, _ = w.rows(w.Hq)
-    out = w.attend(q.to(DEV), first=first).cpu()
+    out = w.attend(q.to(DEV), first=first, max_kv=max_kv).cpu()
     hit = torch.tensor([b == 1 and p < 48 for b, p in zip(np.repeat([0, 1], w.new), w.pos)])
     assert torch.isnan(out[hit]).all() and torch.isfinite(out[~hit]).all()
     w.ks[w.table[1][0]] = 0.01
     w.vs[w.table[1][0]] = np.nan
-    out = w.attend(q.to(DEV), first=first).cpu()
+    out = w.attend(q.to(DEV), first=first, max_kv=max_kv).cpu()
     assert torch.isnan(out[hit]).all() and torch.isfinite(out[~hit]).all()
 
 
@@ -444,11 +462,12 @@ def test_attention_beyond_32_bit_offsets(ctx):
     assert (last[:, ::2].double().cpu() - want[199:]).abs().max() <= 2e-3
 
 
-def test_attention_reports_bad_device_values(ctx):
+@pytest.mark.parametrize("new, loose", [([1, 1], 10 ** 6), ([60, 50], 10 ** 6)])
+def test_attention_reports_bad_device_values(ctx, new, loose):
     """A page outside the pool, lengths past the bounds and token counts past the rows: a status, no stray access."""
-    w = World(ctx, [40, 100], [1, 1], P=16)
+    w = World(ctx, [40, 100], new, P=16)
     q, _ = w.rows(w.Hq)
-    good = w.attend(q.to(DEV)).clone()
+    good = w.attend(q.to(DEV), max_kv=loose).clone()
 
     def refused():
         with pytest.raises(AttnError) as e:
@@ -459,7 +478,7 @@ def test_attention_reports_bad_device_values(ctx):
     for bad in (w.n_pages, -1, 2 ** 31 - 1):
         w.table = table.copy()
         w.table[0, 1] = bad
-        w.attend(q.to(DEV))
+        w.attend(q.to(DEV), max_kv=loose)
         refused()
     w.table = table
     w.attend(q.to(DEV), max_kv=90)
@@ -468,15 +487,16 @@ def test_attention_reports_bad_device_values(ctx):
     for i, bad in ((0, 10 ** 6), (1, 0), (1, -5)):
         w.kv_len = kv.copy()
         w.kv_len[i] = bad
-        w.attend(q.to(DEV), max_kv=10 ** 6)
+        w.attend(q.to(DEV), max_kv=loose)
         refused()
     w.kv_len = kv
-    for bad in ([0, 1, 3], [0, -1, 1], [-1, 0, 1], [0, 2, 1]):
+    a, b = new
+    for bad in ([0, a, a + b + 1], [0, -1, b], [-1, 0, b], [0, a + b, a]):
         w.start = np.array(bad)
-        w.attend(q.to(DEV))
+        w.attend(q.to(DEV), max_kv=loose)
         refused()
     w.start = start
-    assert torch.equal(w.attend(q.to(DEV)), good)
+    assert torch.equal(w.attend(q.to(DEV), max_kv=loose), good)
     ctx.sync_status()
 
 
@@ -488,7 +508,8 @@ def test_attention_rows_of_a_fused_projection(ctx):
             q, _ = w.rows(w.Hq)
             wide = torch.full((w.T, w.Hq + 5, w.D), float("nan"), dtype=q.dtype)
             wide[:, :w.Hq] = q
-            assert torch.equal(w.attend(wide.to(DEV)[:, :w.Hq]), w.attend(q.to(DEV)))
+            for max_kv in BOUNDS:
+                assert torch.equal(w.attend(wide.to(DEV)[:, :w.Hq], max_kv=max_kv), w.attend(q.to(DEV), max_kv=max_kv))
 
 
 def test_looser_bounds_give_the_same_rows(ctx):
@@ -501,12 +522,13 @@ def test_looser_bounds_give_the_same_rows(ctx):
     ctx.sync_status()
 
 
-def test_same_inputs_same_bits(ctx):
-    w = World(ctx, [3000, 900, 77], [1, 1, 1], D=128, P=64, Hq=32, H=8)
+@pytest.mark.parametrize("new, max_kv", [([1, 1, 1], None), ([70, 9, 300], 30000)])
+def test_same_inputs_same_bits(ctx, new, max_kv):
+    w = World(ctx, [3000, 900, 77], new, D=128, P=64, Hq=32, H=8)
     q, _ = w.rows(w.Hq)
-    first = w.attend(q.to(DEV)).clone()
+    first = w.attend(q.to(DEV), max_kv=max_kv).clone()
     for _ in range(10):
-        assert torch.equal(w.attend(q.to(DEV)), first)
+        assert torch.equal(w.attend(q.to(DEV), max_kv=max_kv), first)
 
 
 def test_more_tiles_than_merge_counters(ctx):
