@@ -54,12 +54,6 @@ __device__ __forceinline__ uint32_t movmatrix_t(uint32_t x) {
   return y;
 }
 
-// The rest of (lo, hi) after the fp16 pair `h`, in fp16.
-__device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t h) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-  return pack2(lo - f.x, hi - f.y);
-}
-
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }

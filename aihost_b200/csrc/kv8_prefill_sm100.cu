@@ -48,7 +48,10 @@ struct Cfg {
   static constexpr int RAW = kKeys * D;               // one tile's int8 rows
   static constexpr int NR = D == 64 ? 4 : 2;          // ring of them, K and V in turn
   static constexpr int RAW_OFF = V_OFF + NS * TILE;
-  static constexpr int BAR_OFF = RAW_OFF + NR * RAW;
+  // head_dim 64 has room for what a rotated q leaves when it is rounded to fp16, as a second operand
+  static constexpr bool Q_REST = D == 64;
+  static constexpr int Q_REST_OFF = RAW_OFF + NR * RAW;
+  static constexpr int BAR_OFF = Q_REST_OFF + (Q_REST ? 2 * TILE : 0);
   static constexpr int SMEM = BAR_OFF + 1024 + 1024;  // barriers and factors, alignment slack
   static __device__ __forceinline__ uint32_t s_col(int t) { return t ? 128u : 0u; }
   static __device__ __forceinline__ uint32_t o_col(int t) { return 256u + static_cast<uint32_t>(t * D); }
@@ -306,6 +309,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           const uint32_t off = ((kk >> 2) * kBlock + (kk & 3) * 32) / 16;
           mma_ss(tm + C::s_col(t), qd + off, kd + off, idesc_qk, kk > 0);
         }
+        if (C::Q_REST && a.rope_mode != AIHOST_ROPE_NONE) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            mma_ss(tm + C::s_col(t), qd + (C::Q_REST_OFF + kk * 32) / 16, kd + kk * 2, idesc_qk, 1);
+        }
         commit_elected(&sh.s_full[t]);
         arrive_elected(&sh.s_full[t]);  // passes on what was written besides (the factors)
       };
@@ -524,6 +532,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       // rotated in place, by a loop that is not unrolled: it runs once per block, from a cold instruction cache
       if (a.rope_mode != AIHOST_ROPE_NONE) {
         const bool halves = a.rope_mode == AIHOST_ROPE_NEOX;
+        auto rotation = [](float angle, float* s, float* c) {  // as exact as what is kept of the products
+          if constexpr (C::Q_REST) sincos_near(angle, s, c);
+          else sincos_reduced(angle, s, c);
+        };
         float sn[8], cs[8];  // by halves: of pairs 8 c + e; else of pairs 4 c + e and 4 (c + LPR) + e - 4
         int32_t last = -1;
 #pragma unroll 1
@@ -534,26 +546,35 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             const float fpos = static_cast<float>(tl.pos0 + i);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              sincos_reduced(fpos * a.freqs.f[halves ? 8 * c + e : 4 * (e < 4 ? c : c + LPR - 1) + e], &sn[e], &cs[e]);
+              rotation(fpos * a.freqs.f[halves ? 8 * c + e : 4 * (e < 4 ? c : c + LPR - 1) + e], &sn[e], &cs[e]);
           }
           uint4* const p0 = reinterpret_cast<uint4*>(q_tile + chunk_off(row_a + k, c));
           uint4* const p1 = reinterpret_cast<uint4*>(q_tile + chunk_off(row_a + k, c + LPR));
           const uint4 v0 = *p0, v1 = *p1;
-          uint32_t u0[4] = {v0.x, v0.y, v0.z, v0.w}, u1[4] = {v1.x, v1.y, v1.z, v1.w};
+          uint32_t u0[4] = {v0.x, v0.y, v0.z, v0.w}, u1[4] = {v1.x, v1.y, v1.z, v1.w}, r0[4], r1[4];
 #pragma unroll
           for (int m = 0; m < 4; ++m) {
             const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&u0[m]));
             const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&u1[m]));
+            float2 g0, g1;
             if (halves) {  // (f0.x, f1.x) and (f0.y, f1.y)
-              u0[m] = pack2(f0.x * cs[2 * m] - f1.x * sn[2 * m], f0.y * cs[2 * m + 1] - f1.y * sn[2 * m + 1]);
-              u1[m] = pack2(f0.x * sn[2 * m] + f1.x * cs[2 * m], f0.y * sn[2 * m + 1] + f1.y * cs[2 * m + 1]);
+              g0 = make_float2(f0.x * cs[2 * m] - f1.x * sn[2 * m], f0.y * cs[2 * m + 1] - f1.y * sn[2 * m + 1]);
+              g1 = make_float2(f0.x * sn[2 * m] + f1.x * cs[2 * m], f0.y * sn[2 * m + 1] + f1.y * cs[2 * m + 1]);
             } else {  // (f0.x, f0.y) and (f1.x, f1.y)
-              u0[m] = pack2(f0.x * cs[m] - f0.y * sn[m], f0.x * sn[m] + f0.y * cs[m]);
-              u1[m] = pack2(f1.x * cs[4 + m] - f1.y * sn[4 + m], f1.x * sn[4 + m] + f1.y * cs[4 + m]);
+              g0 = make_float2(f0.x * cs[m] - f0.y * sn[m], f0.x * sn[m] + f0.y * cs[m]);
+              g1 = make_float2(f1.x * cs[4 + m] - f1.y * sn[4 + m], f1.x * sn[4 + m] + f1.y * cs[4 + m]);
             }
+            u0[m] = pack2(g0.x, g0.y);
+            u1[m] = pack2(g1.x, g1.y);
+            r0[m] = pack2_rest(g0.x, g0.y, u0[m]);
+            r1[m] = pack2_rest(g1.x, g1.y, u1[m]);
           }
           *p0 = make_uint4(u0[0], u0[1], u0[2], u0[3]);
           *p1 = make_uint4(u1[0], u1[1], u1[2], u1[3]);
+          if constexpr (C::Q_REST) {
+            p0[C::Q_REST_OFF / 16] = make_uint4(r0[0], r0[1], r0[2], r0[3]);
+            p1[C::Q_REST_OFF / 16] = make_uint4(r1[0], r1[1], r1[2], r1[3]);
+          }
         }
       }
       fence_proxy_async_smem();

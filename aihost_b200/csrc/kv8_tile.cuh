@@ -82,6 +82,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// The rest of (lo, hi) after the fp16 pair `h`, in fp16.
+__device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t h) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return pack2(lo - f.x, hi - f.y);
+}
+
 // tanh x = 1 - 2 / (1 + e^2x): absolute error ~1e-7, which is what the capped score keeps.
 __device__ __forceinline__ float tanh_of(float x) {
   const float e = ex2_approx(x * (2.0f * kLog2e));
