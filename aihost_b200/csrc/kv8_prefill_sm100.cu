@@ -17,6 +17,22 @@
 //                on tiles that cross the row's range, running maximum (O is rescaled only when it
 //                grows by more than 2^8), exp2, row sum, P times V's factors as fp16.
 // Ranges are cut into chunks where there are few tiles; the last block of a tile to arrive merges.
+//
+// Precision: an unrotated fp16 q is exact. A rotated one is rounded to fp16; at head_dim 64 the fp16 of
+// what that leaves enters as a second operand, at head_dim 128 there is no shared memory for one (229 KB
+// are used), which costs 3.6e-4 against 2.9e-4 in relative root mean square error. P is rounded to fp16
+// once, as the output is; maxima, sums and accumulators are fp32, int8 values exact.
+//
+// Measured: 2048 new rows over 14336 cached, 32/8 heads x 128, 511-521 us (515 GFLOP: 1000 TFLOP/s, 61 %
+// of the measured 1634). The MMAs of a tile pair take 2048 cycles, the loop 3760: a tile's turn is its S
+// and P V (1024) and its softmax (~2740 beside the other tile's), one after another; and 256 blocks on
+// 148 SMs are 1.73 waves in the time of 2. Two prompts of 4 K rows with documents, 161 us: of a block's
+// ~40 K cycles about half are fixed (lookup and ranges 5 K, Q 5 K, its rotation 4.6 K, first S 1.6 K, results
+// 5 K). Six uneven prompts, 14/2 heads x 64, scores capped: 71 us.
+// Not better on the first of these: S in two halves of 64 keys (620 us), the next S read into registers
+// ahead (spills, 1330), two threads per query row (569), softmax as a loop over 32 columns that reads S
+// twice (564), a quarter of the exponentials by a polynomial on the FMA pipe (595), non-uniform
+// descriptors (790), set-up before the tile is known (553).
 #include <algorithm>
 
 #include "common.cuh"
@@ -64,6 +80,7 @@ struct Shared {
   float k_factor[kFactorRing][kFactors];
   float v_factor[kFactorRing][kFactors];
   float v_max[4];
+  float freq[64];  // the rotation's frequencies: a parameter indexed by lane costs a turn per distinct index
   uint32_t tmem_base;
   int32_t last;
 };
@@ -278,6 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     }
     fence_mbar_init();
   }
+  if (threadIdx.x >= 64 && threadIdx.x < 64 + D / 2)
+    sh.freq[threadIdx.x - 64] = a.freqs.f[threadIdx.x - 64];
   if (warp == 1) tmem_alloc(&sh.tmem_base, 512);
   tc_fence_before();
   __syncthreads();
@@ -546,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             const float fpos = static_cast<float>(tl.pos0 + i);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              rotation(fpos * a.freqs.f[halves ? 8 * c + e : 4 * (e < 4 ? c : c + LPR - 1) + e], &sn[e], &cs[e]);
+              rotation(fpos * sh.freq[halves ? 8 * c + e : 4 * (e < 4 ? c : c + LPR - 1) + e], &sn[e], &cs[e]);
           }
           uint4* const p0 = reinterpret_cast<uint4*>(q_tile + chunk_off(row_a + k, c));
           uint4* const p1 = reinterpret_cast<uint4*>(q_tile + chunk_off(row_a + k, c + LPR));
