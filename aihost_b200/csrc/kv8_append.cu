@@ -5,7 +5,15 @@
 //   scale = max(had, amax|x| / 127)
 //   older rows  q <- rint(q * (had / scale))   (only where the scale grew)
 //   new rows    q  = rint(x * (1 / scale))
-// The work unit is a run: the consecutive tokens whose slots are consecutive rows of one page.
+// The work unit is a run: the consecutive tokens whose slots are consecutive rows of one page. A run is
+// read once and kept in registers while its maximum comes together, so 2 (fp16) or 4 bytes a value come
+// in and 1 goes out.
+// Measured with the two reads of what was written, 8 heads x 128: 64 one-token sequences 12.3 us, nearly
+// all of it the host's enqueue of three calls (kernels 5 + 2 x 2.8 us). 6.7 K prompt rows of 4 sequences
+// 43.4 us, of which the append 29 (41 MB in and out: 1.4 TB/s where a copy reaches 6.55) and the reads 7
+// each: a warp issues about 140 instructions for a row and head (conversion, rotation, maximum, scaling,
+// rounding, packing), in 52 % of the cycles, which bound it before the bytes do. (One pass over memory
+// for the maximum and another for the rounding: 70 us for the three calls.)
 #include "common.cuh"
 #include "kv8.h"
 #include "kv8_tile.cuh"
@@ -88,7 +96,6 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t word, float ratio) {
 // registers, so that 16 warps read a page once, whole, before its scale is known (64 rows of 2 heads,
 // or 128 of one), and a token's sine and cosine serve both heads. A lane holds D / 32 elements of a
 // row: consecutive ones, or (rotation by halves) as many from either half, so that pairs stay in a lane.
-// The work is the instructions of rotation and rounding, about 16 a value, before it is the bytes.
 template <int D, int ROWS, int HEADS, typename T, int ROPE>
 __global__ void __launch_bounds__(kWarps * 32, 2) kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a, int32_t window) {
   constexpr int E = D / 32, PART = ROPE == AIHOST_ROPE_NEOX ? E / 2 : E;  // elements a lane, in how large parts

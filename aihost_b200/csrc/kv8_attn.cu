@@ -11,8 +11,17 @@
 // cache row at a time and no transpose is needed. Each warp copies its own steps' rows into a ring of
 // its own in shared memory (cp.async, a step ahead, chunks swizzled against bank conflicts): no warp
 // waits for another in the loop. A lane holds the place and scales of one of the warp's next 32 blocks
-// of 16 rows (the smallest page). Warps merge through shared memory, chunks through partials that the last block to arrive
-// merges (no block waits for another).
+// of 16 rows (the smallest page). Warps merge through shared memory, chunks through partials that the
+// last block to arrive merges (no block waits for another).
+//
+// A cache value is used by R query rows, 2 R products a byte, far below what the tensor cores need:
+// the bytes bound it, and mma.sync from registers is enough. Measured, head_dim 128, 8 KV heads: 64
+// sequences of 256 to 8192 rows 104 us (599 MB, 5.7 TB/s, 88 % of a copy's measured 6.55), 32 of 16384
+// with 64 query heads and capped scores 175 us (1.07 GB, 6.1 TB/s, 94 %). One sequence of 513 rows
+// takes 6.6 us in a graph, 7.4 called one at a time: table entry, scales, rows, partial, counter and
+// merge are dependent trips to L2. Not better: three stages of the ring with two blocks an SM instead
+// of two with three (197 against 177 us for the 32 x 16384), rows loaded straight into registers (135
+// against 127 for the 64), 16-row steps (127 against 113), prefetch hints on the copies (no change).
 #include "common.cuh"
 #include "kv8.h"
 #include "kv8_tile.cuh"
@@ -27,8 +36,9 @@ constexpr int kStep = 2 * kSub;   // cache rows of a step; a block's warps take 
 constexpr int kStages = 2;        // of the warp's ring
 constexpr int kChunkMin = kWarps * kStep, kChunkMax = 2048;
 
-// What the products take: fp16 operands, q as a pair of fp16 (rotated in fp32), or q and P as pairs
-// (fp32 tensors).
+// What the products take. fp16 tensors: an unrotated q is exact in fp16, a rotated one (in fp32) enters
+// as a pair, its fp16 and the fp16 of what that leaves; P is rounded to fp16 once, as the output is. fp32
+// tensors: q and P as pairs, 22 bits. The int8 values are exact in fp16; sums are fp32.
 enum { kPlain = 0, kPairQ = 1, kPairQP = 2 };
 
 // The maximum may lag by 2^kSlack before O is rescaled, and P enters times v scale / (the chunk's

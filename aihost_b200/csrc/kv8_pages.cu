@@ -1,7 +1,15 @@
 // kv8_pages.cu — page bookkeeping of a serving step on the GPU: block tables, slots and positions
 // from the requests' lengths (aihost_page_map), and the return of finished requests' pages
-// (aihost_page_release). Integer work, bound by launch and by the dependent reads
-// lengths -> running sums -> table or stack entry -> slot.
+// (aihost_page_release).
+//   row_start[b] = sum of n_new before b,   kv_len[b] = seq_len[b] + n_new[b]
+//   position of token i of b = seq_len[b] + i,   slot = table[b][position / P] * P + position % P
+// and the pages that b newly needs come off the free stack at (sum of the pages taken before b).
+// Integer work of 12 bytes a token, bound by the dependent reads lengths -> running sums -> table or
+// stack entry -> slot. So the running sums are 64-bit scans in one block's registers and shared memory,
+// and each block repeats them for itself, which is cheaper than a second launch or a grid barrier.
+// Measured: 64 one-token sequences 3.1 us in a graph, 512 with 73 K tokens in all 5.7 us; either called
+// one at a time 5.5 us, the host's enqueue. (Blocks that wait for one that scans: 9.2 us; Python's page loop
+// with its copies: 304.)
 #include "common.cuh"
 #include "kv8.h"
 #include "kv8_tile.cuh"

@@ -385,9 +385,10 @@ aihost_status aihost_kv8_workspace_size(const aihost_kv8_desc* desc, int32_t bat
  * and from the start of its own document on (row_first, int32 [n_tokens], or NULL: 0). A row that
  * sees nothing gets zeros. score = scale * q.k, capped if score_cap > 0, then minus
  * alibi_slopes[head] * |p - j| (fp32 [Hq], or NULL). No sequence may have more than max_new new
- * rows or max_kv cached ones. Softmax state and sums are fp32. Precision of the products: with F16 q,
- * q (after its rotation) and the softmax weights enter as fp16; with F32 q as pairs of fp16, whose
- * sum holds 22 bits. int8 values enter exactly. */
+ * rows or max_kv cached ones. Softmax state and sums are fp32; int8 values enter the products exactly.
+ * With F16 q, the softmax weights enter as fp16; q enters exactly where it is not rotated, else as a pair
+ * of fp16 whose sum holds 22 bits, but for prompts with head_dim 128, where it is rounded to fp16 once.
+ * With F32 q, q and the weights enter as such pairs. */
 aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens,
                                    int32_t max_new, int32_t max_kv, const void* q, const int32_t* row_start,
                                    const int32_t* kv_len, const int32_t* block_table, const int8_t* k_pool,
