@@ -92,6 +92,7 @@ struct Kv8AttnArgs {
   int32_t* status;
   // split over the cache rows (mma kernel): chunk rows each, partials and arrival counters
   int32_t tiles, chunk, max_splits;
+  int32_t whole;   // tcgen05 kernel: so many (tile, head) units ahead of the others stay in one block
   float* part_o;   // [unit][split][rows][head_dim]
   float* part_ml;  // [unit][split][rows][2]
   uint32_t* counters;  // one for each tile and head, zero between launches
@@ -111,10 +112,11 @@ void kv8_mma_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max
 cudaError_t launch_kv8_mma(const Kv8AttnArgs& a, cudaStream_t st);
 
 // The tcgen05 kernel (query rows per block 256) and its plan; *end: its length as the plan sees it, in
-// times of one 128-row cache tile (about 2.1 us at head_dim 128 and 1.7 at 64).
+// times of one 128-row cache tile (about 2.1 us at head_dim 128 and 1.7 at 64). *whole: so many units
+// (tile, head), before the others, are not cut.
 int32_t kv8_prefill_rows();
 void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max_new, int32_t max_kv, int32_t num_sms,
-                      int32_t* tiles, int32_t* chunk, int32_t* splits, double* end);
+                      int32_t* tiles, int32_t* whole, int32_t* chunk, int32_t* splits, double* end);
 cudaError_t launch_kv8_prefill(const Kv8AttnArgs& a, cudaStream_t st);
 
 }  // namespace aihost

@@ -86,9 +86,10 @@ aihost_status check_pages(const aihost_attn_ctx* ctx, int32_t batch, int32_t pag
 // Which kernel an attention call runs, and its plan over the cache rows.
 struct Plan {
   bool tensor;  // the tcgen05 kernel (many query rows a sequence, fp16), else the split-cache one
-  int32_t rows, tiles, chunk, splits;
+  int32_t rows, tiles, whole, chunk, splits;  // whole: units that are not split, before the others
+  int64_t parts(const Kv8Geom& g) const { return (static_cast<int64_t>(tiles) * g.n_kv_heads - whole) * splits * rows; }
   size_t scratch(const Kv8Geom& g) const {
-    return splits <= 1 ? 0 : static_cast<size_t>(tiles) * g.n_kv_heads * splits * rows * (g.head_dim + 2) * sizeof(float);
+    return splits <= 1 ? 0 : static_cast<size_t>(parts(g)) * (g.head_dim + 2) * sizeof(float);
   }
 };
 
@@ -104,7 +105,7 @@ Plan make_plan(const aihost_kv8_desc* d, const Kv8Geom& g, int32_t batch, int32_
   p.tensor = false;
   if (d->io_dtype == AIHOST_F16 && static_cast<int64_t>(max_new) * G > rows) {
     double end;
-    kv8_prefill_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.chunk, &p.splits, &end);
+    kv8_prefill_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.whole, &p.chunk, &p.splits, &end);
     const double even = static_cast<double>(n_tokens) / (static_cast<double>(batch) * max_new);
     const double by_tc = end * (g.head_dim == 128 ? 2.1 : 1.7);
     const double tiles16 = (static_cast<double>(n_tokens) * G / rows + 0.5 * batch) * g.n_kv_heads;
@@ -115,6 +116,7 @@ Plan make_plan(const aihost_kv8_desc* d, const Kv8Geom& g, int32_t batch, int32_
     p.rows = kv8_prefill_rows();
   } else {
     p.rows = rows;
+    p.whole = 0;
     kv8_mma_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.chunk, &p.splits);
   }
   return p;
@@ -320,6 +322,7 @@ aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* 
   a.tiles = plan.tiles;
   a.chunk = plan.chunk;
   a.max_splits = plan.splits;
+  a.whole = plan.whole;
   if (static_cast<int64_t>(a.tiles) * r.g.n_kv_heads > INT32_MAX)
     return fail(AIHOST_EUNSUPPORTED, "n_tokens %d needs too many blocks", n_tokens);
   const size_t need = plan.scratch(r.g);
@@ -328,7 +331,7 @@ aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* 
                 ctx->scratch_bytes);
   if (need) {
     a.part_o = static_cast<float*>(ctx->scratch);
-    a.part_ml = a.part_o + static_cast<size_t>(a.tiles) * r.g.n_kv_heads * a.max_splits * plan.rows * r.g.head_dim;
+    a.part_ml = a.part_o + static_cast<size_t>(plan.parts(r.g)) * r.g.head_dim;
     a.counters = ctx->kv8_counters + 1;
   }
   DeviceGuard g(ctx->device);

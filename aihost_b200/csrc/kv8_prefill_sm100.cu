@@ -23,12 +23,13 @@
 // are used), which costs 3.6e-4 against 2.9e-4 in relative root mean square error. P is rounded to fp16
 // once, as the output is; maxima, sums and accumulators are fp32, int8 values exact.
 //
-// Measured: 2048 new rows over 14336 cached, 32/8 heads x 128, 511-521 us (515 GFLOP: 1000 TFLOP/s, 61 %
-// of the measured 1634). The MMAs of a tile pair take 2048 cycles, the loop 3760: a tile's turn is its S
-// and P V (1024) and its softmax (~2740 beside the other tile's), one after another; and 256 blocks on
-// 148 SMs are 1.73 waves in the time of 2. Two prompts of 4 K rows with documents, 161 us: of a block's
-// ~40 K cycles about half are fixed (lookup and ranges 5 K, Q 5 K, its rotation 4.6 K, first S 1.6 K, results
-// 5 K). Six uneven prompts, 14/2 heads x 64, scores capped: 71 us.
+// Measured: 2048 new rows over 14336 cached, 32/8 heads x 128, 497-507 us (515 GFLOP: 1030 TFLOP/s, 63 %
+// of the measured 1634; 545 us where calls follow one another for long, under the power cap). The MMAs of a
+// tile pair take 2048 cycles, the loop 3760: a tile's turn is its S and P V (1024) and its softmax (~2740
+// beside the other tile's), one after another; and the last 0.73 of a wave are chunks, each with a block's
+// fixed work. Two prompts of 4 K rows with documents, 162 us: of a block's ~40 K cycles about half are fixed
+// (lookup and ranges 5 K, Q 5 K, its rotation 4.6 K, first S 1.6 K, results 5 K). Six uneven prompts, 14/2
+// heads x 64, scores capped: 70 us.
 // Not better on the first of these: S in two halves of 64 keys (620 us), the next S read into registers
 // ahead (spills, 1330), two threads per query row (569), softmax as a loop over 32 columns that reads S
 // twice (564), a quarter of the exponentials by a polynomial on the FMA pipe (595), non-uniform
@@ -83,6 +84,7 @@ struct Shared {
   float freq[64];  // the rotation's frequencies: a parameter indexed by lane costs a turn per distinct index
   uint32_t tmem_base;
   int32_t last;
+  int32_t place[7];  // what the end of the block needs of its start, kept out of the loop's registers
 };
 static_assert(sizeof(Shared) <= 1024, "the layout reserves 1024 bytes");
 
@@ -227,9 +229,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int32_t H = a.g.n_kv_heads, G = a.g.n_q_heads / H, ps = a.g.page_shift;
   // longest ranges first: a sequence's last tiles see the most
-  const int32_t h = static_cast<int32_t>(blockIdx.x % H);
-  const int32_t tile = a.tiles - 1 - static_cast<int32_t>(blockIdx.x / H);
-  const int32_t split = static_cast<int32_t>(blockIdx.y);
+  // units (tile, head): the first a.whole in one block each, then the others' chunks
+  const bool whole = blockIdx.x < static_cast<uint32_t>(a.whole);
+  uint32_t unit = blockIdx.x, split = 0;
+  if (a.max_splits > 1 && !whole) {
+    const uint32_t rest = static_cast<uint32_t>(a.tiles * H - a.whole);
+    split = (unit - a.whole) / rest;
+    unit -= split * rest;
+  }
+  const int32_t h = static_cast<int32_t>(unit % H), tile = a.tiles - 1 - static_cast<int32_t>(unit / H);
   griddep_launch_dependents();
   const Tile tl = find_tile(a, tile, G, kRows, lane);
   if (!tl.ok) return;
@@ -263,10 +271,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
   }
   const bool any0 = j1[0] > 0, any1 = j1[1] > 0;
   const int32_t all0 = any0 ? (any1 ? min(j0[0], j0[1]) : j0[0]) : j0[1], all1 = max(j1[0], j1[1]);
-  const int32_t chunk = a.chunk / kKeys;
+  const int32_t chunk = whole ? max(all1 - all0, 1) : a.chunk / kKeys;
   const int32_t n_splits = max(1, (all1 - all0 + chunk - 1) / chunk);
-  if (split >= n_splits) return;
-  const int32_t jb = all0 + split * chunk, je = min(all1, jb + chunk);
+  if (static_cast<int32_t>(split) >= n_splits) return;
+  const int32_t jb = all0 + static_cast<int32_t>(split) * chunk, je = min(all1, jb + chunk);
   const int32_t n_load = max(je - jb, 0);  // 0: no row of the block sees anything
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -297,6 +305,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
   }
   if (threadIdx.x >= 64 && threadIdx.x < 64 + D / 2)
     sh.freq[threadIdx.x - 64] = a.freqs.f[threadIdx.x - 64];
+  if (threadIdx.x == 32 * 12) {
+    const int32_t place[7] = {tl.start, tl.row0, n_rows, h, static_cast<int32_t>(split), static_cast<int32_t>(unit) - a.whole, n_splits};
+    for (int k = 0; k < 7; ++k) sh.place[k] = place[k];
+  }
   if (warp == 1) tmem_alloc(&sh.tmem_base, 512);
   tc_fence_before();
   __syncthreads();
@@ -519,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     const bool valid = rr < n_rows;
     int32_t first, end, pos;
     row_range(a, tl, G, n_rows, rr, first, end, pos);
-    if (!valid) end = first = 0;
+    if (!valid) first = 0, end = INT32_MAX;  // such a row works for nobody and never asks for masks
     const int32_t row = tl.row0 + min(rr, n_rows - 1), tok = row / G, head = h * G + row % G;
     // ---- the warp's 32 rows of Q, rotated in fp32 and rounded once: LPR lanes to a row, each with 16-byte
     // chunks c and c + LPR (a half apart), and LPR rows to a lane, one after another, so that the heads of
@@ -618,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + c * 32, sr[c]);
       const int slot = (lo_j + i - jb) % kFactorRing;
       const int32_t kv0 = (lo_j + i) * kKeys;
-      const bool need_mask = __any_sync(0xffffffffu, valid && (kv0 < first || kv0 + kKeys > end));
+      const bool need_mask = __any_sync(0xffffffffu, kv0 < first || kv0 + kKeys > end);
       float kf[kFactors];
 #pragma unroll
       for (int f = 0; f < kFactors; ++f) kf[f] = sh.k_factor[slot][f];
@@ -719,7 +731,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     const float vmax =
         n_own > 0 ? fmaxf(fmaxf(sh.v_max[0], sh.v_max[1]), fmaxf(sh.v_max[2], sh.v_max[3])) : 0.0f;
     const float o_unit = vmax * (1.0f / kVUnit);
-    const int64_t out_row = ((tl.start + static_cast<int64_t>(tok)) * a.g.n_q_heads + head) * D;
+    auto kept = [&](int k) {  // read here, or the compiler would carry the values through the loop
+      int32_t v;
+      asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v) : "r"(smem_u32(&sh.place[k])));
+      return v;
+    };
+    const int32_t r256 = t * kTileRows + r, n_rows = kept(2), q_row = kept(1) + min(r256, n_rows - 1);
+    const bool stored = r256 < n_rows;
+    const int64_t out_row = ((kept(0) + static_cast<int64_t>(q_row / G)) * a.g.n_q_heads + kept(3) * G + q_row % G) * D;
+    const int32_t split = kept(4), n_splits = kept(6);
     // fp16: into the query tile's space (its last product is done), then out by whole rows
     const bool by_rows = a.out_dtype == AIHOST_F16;
     auto store32 = [&](int c, const float (&o)[32]) {
@@ -729,7 +749,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           *reinterpret_cast<uint4*>(q_tile + chunk_off(r, 4 * c + v)) =
               make_uint4(pack2(o[8 * v], o[8 * v + 1]), pack2(o[8 * v + 2], o[8 * v + 3]),
                               pack2(o[8 * v + 4], o[8 * v + 5]), pack2(o[8 * v + 6], o[8 * v + 7]));
-      } else if (valid) {
+      } else if (stored) {
         float4* dst = reinterpret_cast<float4*>(static_cast<float*>(a.out) + out_row + c * 32);
 #pragma unroll
         for (int v = 0; v < 8; ++v) dst[v] = make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
@@ -743,16 +763,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       for (int k = 0; k < LR; ++k) {
         const int src = k * (32 / LR) + lane / LR;  // row of the warp
         const int64_t row_at = __shfl_sync(0xffffffffu, out_row, src);
-        const bool on = __shfl_sync(0xffffffffu, static_cast<int>(valid), src);
+        const bool on = __shfl_sync(0xffffffffu, static_cast<int>(stored), src);
         if (on)
           *reinterpret_cast<uint4*>(static_cast<__half*>(a.out) + row_at + lane % LR * 8) =
               *reinterpret_cast<const uint4*>(q_tile + chunk_off(quarter * 32 + src, lane % LR));
       }
     };
-    const int64_t unit = static_cast<int64_t>(tile) * H + h;
-    // partials: [unit][split][D / 4][256 rows] of 4 floats, so that a warp's rows lie together
-    float4* const part = reinterpret_cast<float4*>(a.part_o) + (unit * a.max_splits) * (D / 4) * kRows + rr;
-    float2* const part_ml = reinterpret_cast<float2*>(a.part_ml) + unit * a.max_splits * kRows + rr;
+    const int64_t part_unit = kept(5);
+    // partials: [unit after the whole ones][split][D / 4][256 rows] of 4 floats, so that a warp's rows lie together
+    float4* const part = reinterpret_cast<float4*>(a.part_o) + (part_unit * a.max_splits) * (D / 4) * kRows + r256;
+    float2* const part_ml = reinterpret_cast<float2*>(a.part_ml) + part_unit * a.max_splits * kRows + r256;
     if (ok) {
       const float unit_o = n_splits > 1 ? o_unit : l != 0.0f ? o_unit / l : 0.0f;
 #pragma unroll
@@ -783,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     if (n_splits > 1) {  // the last block of this tile and head to arrive merges the chunks
       __threadfence();
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (threadIdx.x == 128) sh.last = last_to_arrive(a.counters + unit, n_splits);
+      if (threadIdx.x == 128) sh.last = last_to_arrive(a.counters + part_unit, n_splits);
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (sh.last) {
         __threadfence();
@@ -829,14 +849,15 @@ cudaError_t launch_d(const Kv8AttnArgs& a, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
   if (e != cudaSuccess) return e;
   // not a dependent launch: waiting blocks would take whole SMs, 6 % slower on batches of short prompts
-  kern<<<dim3(static_cast<unsigned>(a.tiles) * a.g.n_kv_heads, a.max_splits), kThreads, Cfg<D>::SMEM, st>>>(a);
+  const int64_t blocks = a.whole + (static_cast<int64_t>(a.tiles) * a.g.n_kv_heads - a.whole) * a.max_splits;
+  kern<<<static_cast<unsigned>(blocks), kThreads, Cfg<D>::SMEM, st>>>(a);
   return cudaGetLastError();
 }
 
 }  // namespace
 
 void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max_new, int32_t max_kv, int32_t num_sms,
-                      int32_t* tiles, int32_t* chunk, int32_t* splits, double* end_out) {
+                      int32_t* tiles, int32_t* whole, int32_t* chunk, int32_t* splits, double* end_out) {
   const int32_t G = g.n_q_heads / g.n_kv_heads;
   const int64_t n = static_cast<int64_t>(max_new) * G <= kRows ? batch : static_cast<int64_t>(n_tokens) * G / kRows + batch;
   const int64_t units = n * g.n_kv_heads, tiles_kv = (max_kv + kKeys - 1) / kKeys;
@@ -849,7 +870,8 @@ void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t
   const int64_t full = std::min(units, of_one * batch * g.n_kv_heads);  // tiles that can have rows
   const double even = static_cast<double>(n_tokens) / (static_cast<double>(batch) * max_new);
   const double average = (even < 1.0 ? even : 1.0) * (static_cast<double>(tiles_kv) - 0.5 * max_new / kKeys);
-  int64_t best = 1;
+  const bool alike = even > 0.9 && 3 * static_cast<int64_t>(max_new) < max_kv;
+  int64_t best = 1, best_whole = 0;
   double best_end = 1e30;
   for (int64_t s = 1; s <= 32 && (s == 1 || tiles_kv / s >= 4); ++s) {
     const double block = static_cast<double>((tiles_kv + s - 1) / s) + kFixed + (s > 1 ? kPart : 0.0);
@@ -864,12 +886,27 @@ void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t
     if (end < best_end * 0.97) {
       best_end = end;
       best = s;
+      best_whole = 0;
+    }
+    // Units alike that fill some waves and part of one more: only what is left over is split. Measured
+    // against none split: 152 units of 103 tiles 318 -> 275 us, 320 of 90 477 -> 419, 192 of 28 136 -> 117,
+    // 256 of 128 508 -> 497.
+    const int64_t waves = full / num_sms;
+    if (s > 1 && alike && waves > 0) {
+      end = static_cast<double>(waves) * (static_cast<double>(tiles_kv) + kFixed) +
+            static_cast<double>(((full - waves * num_sms) * s + num_sms - 1) / num_sms) * block + kMerge * s;
+      if (end < best_end * 0.97) {
+        best_end = end;
+        best = s;
+        best_whole = waves * num_sms * units / full;  // with its share of the tiles that turn out empty
+      }
     }
   }
-  if (units > kKv8Counters) best = 1;
+  if (units - best_whole > kKv8Counters) best = 1, best_whole = 0;
   const int64_t c = (tiles_kv + best - 1) / best;
   *end_out = best_end;
   *tiles = static_cast<int32_t>(n);
+  *whole = static_cast<int32_t>(best_whole);
   *chunk = static_cast<int32_t>(c * kKeys);
   *splits = static_cast<int32_t>((tiles_kv + c - 1) / c);
 }

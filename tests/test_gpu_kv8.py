@@ -547,6 +547,23 @@ def test_more_tiles_than_merge_counters(ctx):
     assert (out[700].float() - alone[0].float()).abs().max() <= 2.0 ** -9 * alone.abs().max()
 
 
+@pytest.mark.parametrize("D, P, mode", [(64, 32, ROPE_NEOX), (128, 64, ROPE_INTERLEAVED), (128, 16, ROPE_NONE)])
+def test_whole_tiles_and_the_rest_in_chunks(ctx, D, P, mode):
+    """A few more tiles than multiprocessors, ranges alike: most tiles take one block, the last ones (the first 32 rows)
+    are cut into chunks. A row's result is that of the row as a single new one over the rows before it."""
+    w = World(ctx, [1500], [320], Hq=128, H=8, D=D, P=P, mode=mode, seed=21)
+    q, q64 = w.rows(128)
+    out = w.attend(q.to(DEV)).double().cpu().numpy()
+    ctx.sync_status()
+    assert np.isfinite(out).all()
+    for i in [0, 15, 16, 31, 32, 47, 200, 319]:
+        ref, weight, size = plain.attend(q64[i:i + 1], [0, 1], [1501 + i], w.table, P, w.k, w.v, w.ks, w.vs, w.scale, 0.0,
+                                         w.theta, mode)
+        ds = size[..., None] * (2.0 ** -19 if mode == ROPE_NONE else 2.0 ** -11)
+        tol = 2.0 ** -11 * np.abs(ref) + weight * (2.0 ** -11 + 2.0 ** -16 + 2 * ds) + 1e-7
+        assert (np.abs(out[i] - ref[0]) - tol[0]).max() <= 0, i
+
+
 # ------------------------------------------------------------------------------------------------ together
 
 @pytest.mark.parametrize("D, P, io", [(64, 16, F16), (128, 64, F32)])

@@ -57,6 +57,13 @@ def test_scratch_grows_with_the_cache_and_not_for_one_chunk():
     assert 0 < _size(batch=1, max_kv=4096)[1] < _size(batch=1, max_kv=65536)[1]
 
 
+def test_of_tiles_alike_only_those_past_whole_waves_are_cut():
+    """1200 new rows of 4 heads a group are 19 tiles of 256 for each of 8 heads: 148 of them, a wave, need no scratch."""
+    status, size = _size(batch=1, n_tokens=1200, max_new=1200, max_kv=13200, n_pages=1000, max_pages=300)
+    parts, odd = divmod(size, 256 * (128 + 2) * 4)
+    assert status == A.OK and odd == 0 and parts % 4 == 0 and 2 <= parts // 4 <= 32
+
+
 def test_null_context_is_refused():
     L = A.lib()
     d = Kv8Spec(**BASE).desc()
