@@ -29,7 +29,7 @@
 // beside the other tile's), one after another; and the last 0.73 of a wave are chunks, each with a block's
 // fixed work. Two prompts of 4 K rows with documents, 162 us: of a block's ~40 K cycles about half are fixed
 // (lookup and ranges 5 K, Q 5 K, its rotation 4.6 K, first S 1.6 K, results 5 K). Six uneven prompts, 14/2
-// heads x 64, scores capped: 70 us.
+// heads x 64, scores capped: 63.5 us.
 // Not better on the first of these: S in two halves of 64 keys (620 us), the next S read into registers
 // ahead (spills, 1330), two threads per query row (569), softmax as a loop over 32 columns that reads S
 // twice (564), a quarter of the exponentials by a polynomial on the FMA pipe (595), non-uniform
@@ -132,38 +132,54 @@ __device__ __forceinline__ void convert16(const uint4& v, uint4& lo, uint4& hi) 
   hi = make_uint4(half2_of(w2, 0x4140), half2_of(w2, 0x4342), half2_of(w3, 0x4140), half2_of(w3, 0x4342));
 }
 
-// score = cap * tanh(x), x in units of the cap, times log2 e (cap2 = cap * log2 e). Where the whole
-// warp has |x| <= 1, tanh x = x * P(x^2) on the FMA pipe: P of degree 6, our weighted least-squares fit
-// on [0, 1], 5e-8 off (the exponentials already fill the SFU). Else 1 - 2 / (1 + e^2x).
-__device__ __forceinline__ void cap_scores(uint32_t (&sr)[4][32], float cap2) {
-  float top = 0.0f;
+// x * P(x^2) * cap2 for the thread's scores, P of degree N.
+template <int N>
+__device__ __forceinline__ void odd_of(uint32_t (&sr)[4][32], const float (&coef)[N + 1], float cap2) {
+  float2 k2[N + 1];
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-#pragma unroll
-    for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(__uint_as_float(sr[c][e])));
-  if (__any_sync(0xffffffffu, top > 1.0f)) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int e = 0; e < 32; ++e) sr[c][e] = __float_as_uint(cap2 * tanh_of(__uint_as_float(sr[c][e])));
-    return;
-  }
-  constexpr float kP[7] = {0.9999999403953552f,  -0.33332839608192444f, 0.13325203955173492f, -0.05345702916383743f,
-                           0.020289979875087738f, -0.006203378085047007f, 0.001041022245772183f};
-  const float2 cap22 = make_float2(cap2, cap2);
+  for (int k = 0; k <= N; ++k) k2[k] = make_float2(coef[k] * cap2, coef[k] * cap2);
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
     for (int e = 0; e < 32; e += 2) {
       const float2 x = make_float2(__uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
       const float2 y = fmul2(x, x);
-      float2 p = make_float2(kP[6], kP[6]);
+      float2 p = k2[N];
 #pragma unroll
-      for (int k = 5; k >= 0; --k) p = ffma2(p, y, make_float2(kP[k], kP[k]));
-      p = fmul2(fmul2(x, cap22), p);
+      for (int k = N - 1; k >= 0; --k) p = ffma2(p, y, k2[k]);
+      p = fmul2(x, p);
       sr[c][e] = __float_as_uint(p.x);
       sr[c][e + 1] = __float_as_uint(p.y);
     }
+}
+
+// score = cap * tanh(x), x in units of the cap, times log2 e (cap2 = cap * log2 e). Where the whole
+// warp has |x| <= 1, tanh x = x * P(x^2) on the FMA pipe (the exponentials already fill the SFU): P of
+// degree 6, our weighted least-squares fit on [0, 1], 5e-8 off; where it has |x| <= 0.35, as with caps
+// well above the scores, one of degree 3, 4e-8 off. Else 1 - 2 / (1 + e^2x). Measured with and without
+// the shorter polynomial: 6 prompts with cap 50 63.5 and 70 us, 3 with cap 30 195 and 221; with scores
+// beyond a cap of 4 the one comparison more costs 282 against 277.
+__device__ __forceinline__ void cap_scores(uint32_t (&sr)[4][32], float cap2) {
+  float tops[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int e = 0; e < 32; e += 2)
+      tops[c] = fmax3(tops[c], fabsf(__uint_as_float(sr[c][e])), fabsf(__uint_as_float(sr[c][e + 1])));
+  const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  if (!__any_sync(0xffffffffu, top > 0.35f)) {
+    constexpr float kP[4] = {0.9999998211860657f, -0.3333165645599365f, 0.13283322751522064f, -0.048376914113759995f};
+    odd_of<3>(sr, kP, cap2);
+  } else if (!__any_sync(0xffffffffu, top > 1.0f)) {
+    constexpr float kP[7] = {0.9999999403953552f,  -0.33332839608192444f, 0.13325203955173492f, -0.05345702916383743f,
+                             0.020289979875087738f, -0.006203378085047007f, 0.001041022245772183f};
+    odd_of<6>(sr, kP, cap2);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int e = 0; e < 32; ++e) sr[c][e] = __float_as_uint(cap2 * tanh_of(__uint_as_float(sr[c][e])));
+  }
 }
 
 // D[tmem] (+)= A * B with A's descriptor or tensor memory address, issued by one lane of the warp, which

@@ -398,6 +398,13 @@ def test_attention_of_capped_and_large_scores(ctx):
 
 
 @pytest.mark.parametrize("max_kv", BOUNDS)
+@pytest.mark.parametrize("cap", [0.5, 3.0, 12.0, 50.0, 1000.0])
+@pytest.mark.parametrize("D, P", [(64, 16), (128, 64)])
+def test_attention_of_scores_far_below_to_far_above_the_cap(ctx, D, P, cap, max_kv):
+    World(ctx, [150, 0, 20], [60, 130, 1], Hq=8, H=2, D=D, P=P, cap=cap, seed=31).check(ctx, max_kv=max_kv)
+
+
+@pytest.mark.parametrize("max_kv", BOUNDS)
 def test_attention_with_uneven_page_scales(ctx, max_kv):
     """V scales from 1e-4 to 10 side by side, and pages of scale zero."""
     w = World(ctx, [500, 90], [1, 30], P=16, D=128)
