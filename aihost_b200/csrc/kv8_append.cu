@@ -10,10 +10,10 @@
 // in and 1 goes out.
 // Measured with the two reads of what was written, 8 heads x 128: 64 one-token sequences 12.3 us, nearly
 // all of it the host's enqueue of three calls (kernels 5 + 2 x 2.8 us). 6.7 K prompt rows of 4 sequences
-// 43.4 us, of which the append 29 (41 MB in and out: 1.4 TB/s where a copy reaches 6.55) and the reads 7
-// each: a warp issues about 140 instructions for a row and head (conversion, rotation, maximum, scaling,
-// rounding, packing), in 52 % of the cycles, which bound it before the bytes do. (One pass over memory
-// for the maximum and another for the rounding: 70 us for the three calls.)
+// 41.6 us, of which the append 27 (41 MB in and out: 1.5 TB/s where a copy reaches 6.55) and the reads 7
+// each: the instructions of conversion, rotation, maximum, scaling, rounding and packing bound it before
+// the bytes do. (One pass over memory for the maximum and another for the rounding: 70 us for the three
+// calls.)
 #include "common.cuh"
 #include "kv8.h"
 #include "kv8_tile.cuh"
@@ -34,48 +34,51 @@ __device__ __forceinline__ float max_abs(float top, float x) {
   return y;
 }
 
-// N consecutive elements as floats.
+// N consecutive elements (8, 4 or 2) as floats.
 template <int N>
 __device__ __forceinline__ void load_some(const float* p, float* x) {
-  if constexpr (N == 4) {
+  if constexpr (N == 8) {
+    load_some<4>(p, x);
+    load_some<4>(p + 4, x + 4);
+  } else if constexpr (N == 4) {
     const float4 v = __ldg(reinterpret_cast<const float4*>(p));
     x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-  } else if constexpr (N == 2) {
+  } else {
     const float2 v = __ldg(reinterpret_cast<const float2*>(p));
     x[0] = v.x, x[1] = v.y;
-  } else {
-    x[0] = __ldg(p);
   }
 }
 template <int N>
 __device__ __forceinline__ void load_some(const __half* p, float* x) {
-  if constexpr (N == 1) {
-    x[0] = __half2float(__ldg(p));
+  uint32_t w[N / 2];
+  if constexpr (N == 8) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else if constexpr (N == 4) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    w[0] = v.x, w[1] = v.y;
   } else {
-    uint32_t w[N / 2];
-    if constexpr (N == 4) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-      w[0] = v.x, w[1] = v.y;
-    } else {
-      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-    }
+    w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+  }
 #pragma unroll
-    for (int k = 0; k < N / 2; ++k) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-      x[2 * k] = f.x, x[2 * k + 1] = f.y;
-    }
+  for (int k = 0; k < N / 2; ++k) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+    x[2 * k] = f.x, x[2 * k + 1] = f.y;
   }
 }
 
-// N int8 from the low bytes of q.
+// Int8 from the low bytes of q: four, then N of them.
+__device__ __forceinline__ uint32_t pack_bytes(const uint32_t* q) {
+  return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+}
 template <int N>
 __device__ __forceinline__ void store_bytes(int8_t* p, const uint32_t* q) {
-  if constexpr (N == 4) {
-    *reinterpret_cast<uint32_t*>(p) = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
-  } else if constexpr (N == 2) {
-    *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(__byte_perm(q[0], q[1], 0x0040));
+  if constexpr (N == 8) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bytes(q), pack_bytes(q + 4));
+  } else if constexpr (N == 4) {
+    *reinterpret_cast<uint32_t*>(p) = pack_bytes(q);
   } else {
-    *p = static_cast<int8_t>(q[0]);
+    *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(__byte_perm(q[0], q[1], 0x0040));
   }
 }
 
@@ -87,23 +90,23 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t word, float ratio) {
     const float x = static_cast<float>(static_cast<int8_t>(word >> (8 * e)));
     q[e] = __float_as_uint(__fadd_rn(__fmul_rn(x, ratio), 12582912.0f));
   }
-  return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+  return pack_bytes(q);
 }
 
 // The runs that start in one window of tokens, for two heads of K or V. The 16 warps split into groups,
 // as many as the window starts runs (up to 16), and a group takes a run at a time: all warps on one
-// page's rows for prompts, a warp per row for decode. A warp keeps ROWS rows of HEADS heads in
-// registers, so that 16 warps read a page once, whole, before its scale is known (64 rows of 2 heads,
-// or 128 of one), and a token's sine and cosine serve both heads. A lane holds D / 32 elements of a
-// row: consecutive ones, or (rotation by halves) as many from either half, so that pairs stay in a lane.
-template <int D, int ROWS, int HEADS, typename T, int ROPE>
+// page's rows for prompts, a warp per row for decode. LPR lanes take a row, so a warp RP = 32 / LPR at a
+// time, and it keeps ROWS such loads of HEADS heads in registers: 16 warps read a page once, whole,
+// before its scale is known (64 rows of 2 heads, or 128 of one), and a token's sine and cosine serve both
+// heads. A lane holds E = D / LPR elements of a row: consecutive ones, or (rotation by halves) as many from either half, so that pairs stay in a lane.
+template <int D, int LPR, int ROWS, int HEADS, typename T, int ROPE>
 __global__ void __launch_bounds__(kWarps * 32, 2) kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a, int32_t window) {
-  constexpr int E = D / 32, PART = ROPE == AIHOST_ROPE_NEOX ? E / 2 : E;  // elements a lane, in how large parts
+  constexpr int RP = 32 / LPR, E = D / LPR, PART = ROPE == AIHOST_ROPE_NEOX ? E / 2 : E;  // elements a lane, in how large parts
   __shared__ int64_t slot_sh[1 + 2 * kMaxPage];  // the token before the window, the window, a page more
   __shared__ int32_t run_at[kMaxPage];
   __shared__ int32_t run_count;
   __shared__ uint32_t warp_max[HEADS][kWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, in_row = lane % LPR, sub = lane / LPR;
   const int32_t t0 = static_cast<int32_t>(blockIdx.x) * window;
   const bool is_k = (blockIdx.y & 1) == 0;
   const int32_t P = a.g.page_rows, H = a.g.n_kv_heads, h_begin = static_cast<int32_t>(blockIdx.y >> 1) * kHeads;
@@ -118,7 +121,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv8_append_kernel(const __grid
   }
   float freq[E / 2];  // of the lane's pairs: the same ones in either layout
 #pragma unroll
-  for (int p = 0; p < E / 2; ++p) freq[p] = rotate ? a.freqs.f[lane * (E / 2) + p] : 0.0f;
+  for (int p = 0; p < E / 2; ++p) freq[p] = rotate ? a.freqs.f[in_row * (E / 2) + p] : 0.0f;
   __syncthreads();
   if (warp == 0) {
     int32_t count = 0;
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv8_append_kernel(const __grid
   };
   int8_t* const pool = is_k ? a.k_pool : a.v_pool;
   float* const scales = is_k ? a.k_scale : a.v_scale;
-  const T* const src = static_cast<const T*>(is_k ? a.k_new : a.v_new) + lane * PART;
+  const T* const src = static_cast<const T*>(is_k ? a.k_new : a.v_new) + in_row * PART;
   const int64_t stride = a.token_stride / static_cast<int64_t>(sizeof(T));
 
   for (int r = group; r < n_runs; r += kWarps / nw) {
@@ -169,22 +172,22 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv8_append_kernel(const __grid
         break;
       }
     }
-    const int32_t batch = ROWS * nw, last = (n - 1) / batch * batch;
+    const int32_t batch = RP * ROWS * nw, last = (n - 1) / batch * batch;
     for (int32_t h0 = h_begin; h0 < min(H, h_begin + kHeads); h0 += HEADS) {
       float had[HEADS];
 #pragma unroll
       for (int j = 0; j < HEADS; ++j) had[j] = row0 == 0 || h0 + j >= H ? 0.0f : scales[page * H + h0 + j];
       float x[ROWS][HEADS][E];
-      const T* const from = src + (t + w) * stride + h0 * D;
+      const T* const from = src + t * stride + h0 * D;
       const bool two = HEADS == 1 || h0 + 1 < H;
       auto load = [&](int32_t first) {
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-          const int32_t k = first + i * nw;  // the group's rows first + i nw + (0 .. nw - 1)
+          const int32_t k = first + RP * (i * nw + w) + sub;  // the group's rows first + RP i nw + (0 .. RP nw - 1)
           const T* const row = from + k * stride;
 #pragma unroll
           for (int j = 0; j < HEADS; ++j) {
-            const bool on = k + w < n && (j == 0 || two);
+            const bool on = k < n && (j == 0 || two);
 #pragma unroll
             for (int e = 0; e < E; e += PART) {
               if (on) {
@@ -200,7 +203,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv8_append_kernel(const __grid
           if (rotate) {
 #pragma unroll
             for (int i = 0; i < ROWS; ++i) {
-              const int32_t k = first + i * nw + w;
+              const int32_t k = first + RP * (i * nw + w) + sub;
               if (k >= n) continue;
               const float pos = static_cast<float>(a.positions[t + k]);
 #pragma unroll
@@ -276,12 +279,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) kv8_append_kernel(const __grid
         if (lane == 0 && w == 0) scales[page * H + h0 + j] = scale;
       }
       const int32_t head_bytes = P * D;
-      int8_t* const to = pool + (((page * H + h0) << a.g.page_shift) + row0) * D + lane * PART;
+      int8_t* const to = pool + (((page * H + h0) << a.g.page_shift) + row0) * D + in_row * PART;
       for (int32_t first = last; first >= 0; first -= batch) {  // backwards: the last rows are still held
         if (first != last) load(first);
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-          const int32_t k = first + i * nw + w;
+          const int32_t k = first + RP * (i * nw + w) + sub;
           if (k >= n) continue;
           int8_t* const row = to + k * D;
 #pragma unroll
@@ -338,10 +341,19 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8ReadArgs a, uint
 template <int D, typename T, int ROPE>
 cudaError_t launch_append_r(const Kv8AppendArgs& a, cudaStream_t st) {
   // Few tokens: windows of 16, for more blocks. Many: a page's rows, so that no block of a prompt's
-  // window starts no run.
-  const int32_t window = a.n_tokens < 1024 ? 16 : a.g.page_rows;
+  // window starts no run, and at least 32 or 64, so that its warps' registers are full (6.7 K rows in pages
+  // of 16 with their reads 43 us, by windows of 16 77; 1100 single tokens 31 us, by windows of 16 29, of 64 37).
+  const int32_t least = a.n_tokens < 1024 ? 16 : a.n_tokens < 4096 ? 32 : 64;
+  const int32_t window = a.n_tokens < 1024 || a.g.page_rows < least ? least : a.g.page_rows;
   const dim3 grid((a.n_tokens + window - 1) / window, 2 * ((a.g.n_kv_heads + kHeads - 1) / kHeads));
-  auto kern = a.g.page_rows == 128 ? kv8_append_kernel<D, 8, 1, T, ROPE> : kv8_append_kernel<D, 4, 2, T, ROPE>;
+  // Sixteen lanes to a row where there are many, for half the instructions (5 K rows of head_dim 128 in pages
+  // of 128, unrotated, with their reads: 47 us, with a warp to a row 55); a warp to a row of 128 where
+  // there are few and the way through one counts (64 single tokens: 11.6 us in a graph against 12.1).
+  constexpr int kFew = D == 128 ? 32 : 16, kR = 32 / kFew;
+  const bool few = a.n_tokens < 1024;
+  auto kern = a.g.page_rows == 128
+                  ? (few ? kv8_append_kernel<D, kFew, 8 / kR, 1, T, ROPE> : kv8_append_kernel<D, 16, 4, 1, T, ROPE>)
+                  : (few ? kv8_append_kernel<D, kFew, 4 / kR, 2, T, ROPE> : kv8_append_kernel<D, 16, 2, 2, T, ROPE>);
   return launch_dependent(kern, grid, kWarps * 32, 0, st, a, window);
 }
 

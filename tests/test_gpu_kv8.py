@@ -248,6 +248,15 @@ def test_append(ctx, case, joined):
     _append(ctx, World(ctx, seed=len(case), **APPENDS[case]), joined=joined)
 
 
+@pytest.mark.parametrize("mode, io", [(ROPE_NONE, F16), (ROPE_INTERLEAVED, F16), (ROPE_NEOX, F32)])
+@pytest.mark.parametrize("D, P", [(64, 16), (128, 16), (128, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("new", [[700, 1, 0, 19] + [3] * 130, [2500, 33] + [1] * 150 + [1701]])
+def test_append_of_many_rows(ctx, new, D, P, mode, io):
+    """From 1024 tokens on, and from 4096: windows over several small pages, two rows to a warp."""
+    cached = [(7 * b) % 40 for b in range(len(new))]
+    _append(ctx, World(ctx, cached, new, H=3, Hq=3, D=D, P=P, mode=mode, io=io, seed=P))
+
+
 @pytest.mark.parametrize("std", [1e-6, 100.0])
 def test_append_keeps_or_grows_the_scale(ctx, std):
     """Small new rows leave the old rows as they are, large ones bring them to the new scale."""
