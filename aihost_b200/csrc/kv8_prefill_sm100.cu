@@ -24,7 +24,7 @@
 // once, as the output is; maxima, sums and accumulators are fp32, int8 values exact.
 //
 // Measured: 2048 new rows over 14336 cached, 32/8 heads x 128, 497-507 us (515 GFLOP: 1030 TFLOP/s, 63 %
-// of the measured 1634; 545 us where calls follow one another for long, under the power cap). The MMAs of a
+// of the measured 1634; 545-557 us where calls follow one another for long, under the power cap). The MMAs of a
 // tile pair take 2048 cycles, the loop 3760: a tile's turn is its S and P V (1024) and its softmax (~2740
 // beside the other tile's), one after another; and the last 0.73 of a wave are chunks, each with a block's
 // fixed work. Two prompts of 4 K rows with documents, 162 us: of a block's ~40 K cycles about half are fixed
