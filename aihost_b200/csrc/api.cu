@@ -218,6 +218,10 @@ aihost_status run_decode(aihost_attn_ctx* ctx, const aihost_attn_desc* d, const 
   if (need > ctx->scratch_bytes)
     return fail(AIHOST_ENOMEM, "decode needs %zu bytes of scratch, context has %zu (call aihost_attn_reserve)", need,
                 ctx->scratch_bytes);
+  if (need) {
+    cudaError_t e = note_scratch_use(ctx, st);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
+  }
   DecodeArgs a;
   memset(&a, 0, sizeof(a));
   a.q = q;
@@ -287,6 +291,8 @@ aihost_status run_prefill(aihost_attn_ctx* ctx, const aihost_attn_desc* d, const
                   "prefill with fp32 / Q8_0 operands needs %zu bytes of scratch, context has %zu "
                   "(call aihost_attn_reserve with aihost_attn_workspace_size)",
                   need, ctx->scratch_bytes);
+    cudaError_t noted = note_scratch_use(ctx, st);
+    if (noted != cudaSuccess) return cuda_fail(noted, "cudaStreamIsCapturing");
     uint8_t* sp = static_cast<uint8_t*>(ctx->scratch);
     if (d->q_dtype != AIHOST_F16) {
       __half* qh = reinterpret_cast<__half*>(sp);
@@ -501,6 +507,7 @@ aihost_status aihost_attn_destroy(aihost_attn_ctx* ctx) {
     }
   for (cudaEvent_t e : ctx->event_pool) cudaEventDestroy(e);
   cudaFree(ctx->scratch);
+  for (void* p : ctx->outgrown) cudaFree(p);
   cudaFree(ctx->kv8_counters);
   cudaFree(ctx->counters);
   cudaFree(ctx->d_status);
@@ -531,13 +538,16 @@ aihost_status aihost_attn_reserve(aihost_attn_ctx* ctx, size_t bytes) {
   if (s != AIHOST_OK) return s;
   if (bytes <= ctx->scratch_bytes) return AIHOST_OK;
   DeviceGuard g(ctx->device);
-  if (ctx->scratch) {
+  if (ctx->scratch_captured) {  // graphs go on using what they were captured with
+    ctx->outgrown.push_back(ctx->scratch);
+    ctx->scratch_captured = false;
+  } else if (ctx->scratch) {
     cudaError_t e = cudaDeviceSynchronize();
     if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceSynchronize before scratch resize");
     cudaFree(ctx->scratch);
-    ctx->scratch = nullptr;
-    ctx->scratch_bytes = 0;
   }
+  ctx->scratch = nullptr;
+  ctx->scratch_bytes = 0;
   cudaError_t e = cudaMalloc(&ctx->scratch, bytes);
   if (e != cudaSuccess) {
     ctx->scratch = nullptr;
@@ -970,6 +980,10 @@ aihost_status aihost_matmul_weights(aihost_attn_ctx* ctx, const aihost_matmul_de
     return fail(AIHOST_ENOMEM, "this product needs %zu bytes of scratch, context has %zu (aihost_matmul_workspace_size)",
                 need, ctx->scratch_bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (need) {
+    cudaError_t e = note_scratch_use(ctx, st);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
+  }
   uint8_t* sp = static_cast<uint8_t*>(ctx->scratch);
   const int64_t M = desc->rows, K = desc->k, N = desc->n_out, parts = desc->n_parts;
   const void* a16 = a;

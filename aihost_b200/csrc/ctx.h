@@ -24,6 +24,8 @@ struct aihost_attn_ctx {
   int32_t* d_status = nullptr;
   void* scratch = nullptr;
   size_t scratch_bytes = 0;
+  bool scratch_captured = false;   // a captured call holds the scratch's address
+  std::vector<void*> outgrown;     // earlier scratch that captured calls hold: kept with the context
   unsigned long long* counters = nullptr;  // fused split merge: epoch-tagged arrival counts
   uint32_t epoch = 0;
   uint32_t* kv8_counters = nullptr;  // page map's ticket, then the 8-bit attention's arrival counts
@@ -62,6 +64,15 @@ class DeviceGuard {
   int prev_ = 0;
   bool ok_ = false;
 };
+
+// Called before work on `st` that is given the context's scratch: what a graph holds is not freed when the
+// scratch grows.
+inline cudaError_t note_scratch_use(aihost_attn_ctx* ctx, cudaStream_t st) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing(st, &status);
+  if (e == cudaSuccess && status != cudaStreamCaptureStatusNone) ctx->scratch_captured = true;
+  return e;
+}
 
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 

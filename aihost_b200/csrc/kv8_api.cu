@@ -337,7 +337,9 @@ aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* 
   DeviceGuard g(ctx->device);
   if (!g.ok()) return fail(AIHOST_ECUDA, "cudaSetDevice(%d) failed", ctx->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = timed_launch(ctx, AIHOST_KERNEL_KV8_ATTN, st, [&] {
+  cudaError_t e = need ? note_scratch_use(ctx, st) : cudaSuccess;
+  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
+  e = timed_launch(ctx, AIHOST_KERNEL_KV8_ATTN, st, [&] {
     return plan.tensor ? launch_kv8_prefill(a, st) : launch_kv8_mma(a, st);
   });
   return e == cudaSuccess ? AIHOST_OK : cuda_fail(e, "8-bit attention launch");

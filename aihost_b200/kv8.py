@@ -113,7 +113,8 @@ class Kv8Ops:
         max_kv: upper bounds on any sequence's new rows and on kv_len. prefix_len (int32 [batch]): cache rows that all
         rows of the sequence see; row_first (int32 [n]): the first cache row that a row sees; alibi_slopes (fp32
         [n_q_heads]): score - slope * distance. A row that sees nothing gets zeros. The context's scratch grows on the
-        first call that needs more (which waits for the GPU: make such a call before capturing a graph)."""
+        first call that needs more (which waits for the GPU: make such a call before capturing a graph; graphs captured
+        before keep the scratch they were captured with)."""
         return _kv8.attend(self.ctx.handle.value, self.ctx.device, self._at, self._st(), q, row_start, kv_len, block_table,
                            k_pool, v_pool, k_scale, v_scale, max_new, max_kv, prefix_len, row_first, alibi_slopes, out)
 

@@ -103,7 +103,10 @@ aihost_status aihost_attn_destroy(aihost_attn_ctx* ctx);
  * and of an fp32 / Q8_0 cache (kv_capacity rows), which the tensor-core kernel reads. */
 aihost_status aihost_attn_workspace_size(const aihost_attn_desc* desc, int32_t batch, int32_t n_new,
                                          size_t* out_bytes);
-/* Grow the context's scratch to at least `bytes` (the only allocating call besides create). */
+/* Grow the context's scratch to at least `bytes` (the only allocating call besides create). Scratch that a
+ * captured call was given stays allocated until the context is destroyed, so that graphs captured
+ * before stay valid; without such a call it is freed (after waiting for the device). A graph must
+ * not be replayed once its context is destroyed. */
 aihost_status aihost_attn_reserve(aihost_attn_ctx* ctx, size_t bytes);
 
 /* The fused op: RoPE(q) and RoPE(k_new) at positions seq_len[b] + s, append the rotated k_new
