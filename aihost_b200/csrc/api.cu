@@ -218,10 +218,8 @@ aihost_status run_decode(aihost_attn_ctx* ctx, const aihost_attn_desc* d, const 
   if (need > ctx->scratch_bytes)
     return fail(AIHOST_ENOMEM, "decode needs %zu bytes of scratch, context has %zu (call aihost_attn_reserve)", need,
                 ctx->scratch_bytes);
-  if (need) {
-    cudaError_t e = note_scratch_use(ctx, st);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
-  }
+  SharedUse shared(ctx, st, need > 0);
+  if (shared.error() != cudaSuccess) return cuda_fail(shared.error(), "ordering the scratch's uses");
   DecodeArgs a;
   memset(&a, 0, sizeof(a));
   a.q = q;
@@ -284,6 +282,8 @@ aihost_status run_prefill(aihost_attn_ctx* ctx, const aihost_attn_desc* d, const
   if (!prefill_supported(d->head_dim)) return fail(AIHOST_EUNSUPPORTED, "prefill head_dim %d", d->head_dim);
   KvLayout kv = kv_in;
   const bool q_staged = d->q_dtype != AIHOST_F16, kv_staged = d->kv_dtype != AIHOST_F16;
+  SharedUse shared(ctx, st, q_staged || kv_staged);
+  if (shared.error() != cudaSuccess) return cuda_fail(shared.error(), "ordering the scratch's uses");
   if (q_staged || kv_staged) {
     const size_t need = prefill_stage_bytes(d, batch, n_q, kv_rows);
     if (need > ctx->scratch_bytes)
@@ -291,8 +291,6 @@ aihost_status run_prefill(aihost_attn_ctx* ctx, const aihost_attn_desc* d, const
                   "prefill with fp32 / Q8_0 operands needs %zu bytes of scratch, context has %zu "
                   "(call aihost_attn_reserve with aihost_attn_workspace_size)",
                   need, ctx->scratch_bytes);
-    cudaError_t noted = note_scratch_use(ctx, st);
-    if (noted != cudaSuccess) return cuda_fail(noted, "cudaStreamIsCapturing");
     uint8_t* sp = static_cast<uint8_t*>(ctx->scratch);
     if (d->q_dtype != AIHOST_F16) {
       __half* qh = reinterpret_cast<__half*>(sp);
@@ -506,6 +504,7 @@ aihost_status aihost_attn_destroy(aihost_attn_ctx* ctx) {
       cudaEventDestroy(pr.second);
     }
   for (cudaEvent_t e : ctx->event_pool) cudaEventDestroy(e);
+  if (ctx->shared_done) cudaEventDestroy(ctx->shared_done);
   cudaFree(ctx->scratch);
   for (void* p : ctx->outgrown) cudaFree(p);
   cudaFree(ctx->kv8_counters);
@@ -980,10 +979,8 @@ aihost_status aihost_matmul_weights(aihost_attn_ctx* ctx, const aihost_matmul_de
     return fail(AIHOST_ENOMEM, "this product needs %zu bytes of scratch, context has %zu (aihost_matmul_workspace_size)",
                 need, ctx->scratch_bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (need) {
-    cudaError_t e = note_scratch_use(ctx, st);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
-  }
+  SharedUse shared(ctx, st, need > 0);
+  if (shared.error() != cudaSuccess) return cuda_fail(shared.error(), "ordering the scratch's uses");
   uint8_t* sp = static_cast<uint8_t*>(ctx->scratch);
   const int64_t M = desc->rows, K = desc->k, N = desc->n_out, parts = desc->n_parts;
   const void* a16 = a;

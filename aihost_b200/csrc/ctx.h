@@ -26,6 +26,9 @@ struct aihost_attn_ctx {
   size_t scratch_bytes = 0;
   bool scratch_captured = false;   // a captured call holds the scratch's address
   std::vector<void*> outgrown;     // earlier scratch that captured calls hold: kept with the context
+  bool shared_used = false;            // the scratch or the counters have been used,
+  unsigned long long shared_stream = 0;  // last on the stream of this id;
+  cudaEvent_t shared_done = nullptr;   // since a second stream came: after the last use
   unsigned long long* counters = nullptr;  // fused split merge: epoch-tagged arrival counts
   uint32_t epoch = 0;
   uint32_t* kv8_counters = nullptr;  // page map's ticket, then the 8-bit attention's arrival counts
@@ -65,14 +68,55 @@ class DeviceGuard {
   bool ok_ = false;
 };
 
-// Called before work on `st` that is given the context's scratch: what a graph holds is not freed when the
-// scratch grows.
-inline cudaError_t note_scratch_use(aihost_attn_ctx* ctx, cudaStream_t st) {
-  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-  const cudaError_t e = cudaStreamIsCapturing(st, &status);
-  if (e == cudaSuccess && status != cudaStreamCaptureStatusNone) ctx->scratch_captured = true;
-  return e;
-}
+// Held around the launches of a call that uses what its context has only once: the scratch and the arrival
+// counters. Calls on one stream follow each other anyway. One on another stream than the last waits
+// for it: the first of these for the whole device, as no event marks the call before, later ones for an
+// event that every call records from then on (a context used on one stream pays for none). A captured call is
+// ordered by its graph; it marks the scratch, whose address the graph holds.
+class SharedUse {
+ public:
+  SharedUse(aihost_attn_ctx* ctx, cudaStream_t st, bool uses) : ctx_(ctx), st_(st) {
+    if (uses) e_ = enter();
+  }
+  ~SharedUse() {
+    if (entered_ && ctx_->shared_done) cudaEventRecord(ctx_->shared_done, st_);
+  }
+  SharedUse(const SharedUse&) = delete;
+  SharedUse& operator=(const SharedUse&) = delete;
+  cudaError_t error() const { return e_; }
+
+ private:
+  cudaError_t enter() {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    cudaError_t e = cudaStreamIsCapturing(st_, &status);
+    if (e != cudaSuccess) return e;
+    if (status != cudaStreamCaptureStatusNone) {
+      ctx_->scratch_captured = true;
+      return cudaSuccess;
+    }
+    unsigned long long id = 0;  // unlike a handle, never used again for a later stream
+    e = cudaStreamGetId(st_, &id);
+    if (e != cudaSuccess) return e;
+    if (ctx_->shared_used && id != ctx_->shared_stream) {
+      if (ctx_->shared_done) {
+        e = cudaStreamWaitEvent(st_, ctx_->shared_done, 0);
+      } else {
+        e = cudaDeviceSynchronize();
+        if (e == cudaSuccess) e = cudaEventCreateWithFlags(&ctx_->shared_done, cudaEventDisableTiming);
+      }
+      if (e != cudaSuccess) return e;
+    }
+    ctx_->shared_used = true;
+    ctx_->shared_stream = id;
+    entered_ = true;
+    return cudaSuccess;
+  }
+
+  aihost_attn_ctx* const ctx_;
+  const cudaStream_t st_;
+  cudaError_t e_ = cudaSuccess;
+  bool entered_ = false;
+};
 
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 

@@ -99,6 +99,7 @@ struct Kv8AttnArgs {
   RopeFreqs freqs;
 };
 
+int page_map_blocks(const PageMapArgs& a);  // only several use the ticket
 cudaError_t launch_page_map(const PageMapArgs& a, cudaStream_t st);
 cudaError_t launch_page_release(const PageReleaseArgs& a, cudaStream_t st);
 cudaError_t launch_kv8_append(const Kv8AppendArgs& a, cudaStream_t st);

@@ -170,6 +170,8 @@ aihost_status aihost_page_map(aihost_attn_ctx* ctx, int32_t batch, int32_t page_
   a.ticket = ctx->kv8_counters;
   a.status = ctx->d_status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  SharedUse shared(ctx, st, page_map_blocks(a) > 1);  // the ticket
+  if (shared.error() != cudaSuccess) return cuda_fail(shared.error(), "ordering the page maps");
   cudaError_t e = timed_launch(ctx, AIHOST_KERNEL_PAGES, st, [&] { return launch_page_map(a, st); });
   return e == cudaSuccess ? AIHOST_OK : cuda_fail(e, "page map launch");
 }
@@ -337,9 +339,9 @@ aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* 
   DeviceGuard g(ctx->device);
   if (!g.ok()) return fail(AIHOST_ECUDA, "cudaSetDevice(%d) failed", ctx->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = need ? note_scratch_use(ctx, st) : cudaSuccess;
-  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamIsCapturing");
-  e = timed_launch(ctx, AIHOST_KERNEL_KV8_ATTN, st, [&] {
+  SharedUse shared(ctx, st, need > 0);
+  if (shared.error() != cudaSuccess) return cuda_fail(shared.error(), "ordering the scratch's uses");
+  cudaError_t e = timed_launch(ctx, AIHOST_KERNEL_KV8_ATTN, st, [&] {
     return plan.tensor ? launch_kv8_prefill(a, st) : launch_kv8_mma(a, st);
   });
   return e == cudaSuccess ? AIHOST_OK : cuda_fail(e, "8-bit attention launch");

@@ -195,11 +195,16 @@ __global__ void __launch_bounds__(1024) page_release_kernel(const PageReleaseArg
 
 }  // namespace
 
+static int page_map_threads(const PageMapArgs& a) { return a.batch <= 256 && a.max_tokens <= 256 ? 256 : 1024; }
+
+int page_map_blocks(const PageMapArgs& a) {
+  const int threads = page_map_threads(a);
+  const int64_t blocks = (static_cast<int64_t>(a.max_tokens) + threads - 1) / threads;
+  return blocks < 1 ? 1 : blocks > 148 ? 148 : static_cast<int>(blocks);
+}
+
 cudaError_t launch_page_map(const PageMapArgs& a, cudaStream_t st) {
-  const int most = a.batch > a.max_tokens ? a.batch : a.max_tokens;
-  const int threads = most <= 256 ? 256 : 1024;
-  int blocks = (a.max_tokens + threads - 1) / threads;
-  blocks = blocks < 1 ? 1 : blocks > 148 ? 148 : blocks;
+  const int threads = page_map_threads(a), blocks = page_map_blocks(a);
   const size_t smem = (2 * static_cast<size_t>(a.batch) + 1) * sizeof(int32_t);
   if (smem > 48 * 1024) {
     cudaError_t e = cudaFuncSetAttribute(page_map_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,

@@ -20,6 +20,10 @@
  *     owned by the caller; the library never frees or retains them past the call;
  *   - work is enqueued on the caller's cudaStream_t (passed as void*, NULL = legacy stream);
  *     calls are asynchronous with respect to the host, like Dispatch() before Flush();
+ *   - a context's scratch and arrival counters serve one call at a time: a call that needs them on another
+ *     stream than the last such call waits for it on the device (the first change of stream also on
+ *     the host). Replaying a graph of such calls counts as a call, whose order the caller sees to:
+ *     give a graph that is replayed beside other work a context of its own;
  *   - the library allocates nothing inside the attention calls: split-K scratch is owned by
  *     the context and sized once by aihost_attn_reserve().
  *

@@ -50,3 +50,71 @@ def test_a_captured_call_outlives_the_growth_of_the_scratch(own):
         assert all((x == 7.0).all() for x in others)
         assert torch.equal(w.ops.attend(q, *args, 1, 3001), want)
     own.sync_status()
+
+
+def _busy(stream, ms=3):
+    """Keeps a stream at work for some milliseconds, so that what follows on it runs late."""
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(int(ms * 2_000_000))
+
+
+def test_attention_on_several_streams_of_one_context(own):
+    """Calls of different chunk counts, enqueued on three streams at once, merge their chunks in one scratch with one
+    set of counters: each gives what it gives alone, and so does a call on a single stream afterwards."""
+    worlds = [World(own, [3000, 40, 700], [1, 1, 1], D=128, P=64), World(own, [9000] * 8, [1] * 8, D=128, P=128, H=4, Hq=32),
+              World(own, [2500], [64], D=64, P=16)]
+    bounds = [(1, 3001), (1, 9001), (64, 20000)]
+    calls = []
+    for w, (new, most) in zip(worlds, bounds):
+        q, args = w.rows(w.Hq)[0].to(DEV), _args(w)
+        calls.append((w, (q, *args, new, most), w.ops.attend(q, *args, new, most).clone()))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for turn in range(6):
+        got = []
+        for i, (w, args, _) in enumerate(calls):
+            _busy(streams[(i + turn) % 3])
+        for _ in range(3):
+            for i, (w, args, want) in enumerate(calls):
+                ops = Kv8Ops(own, w.spec, streams[(i + turn) % 3])
+                got.append((ops.attend(*args), want))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, want) for x, want in got)
+    for w, args, want in calls:
+        assert torch.equal(w.ops.attend(*args), want)
+    own.sync_status()
+
+
+def test_page_maps_on_several_streams_of_one_context(own):
+    """Maps of several blocks that write their lengths in place, on two streams at once."""
+    from aihost_b200.kv8 import Kv8Spec, StepMap
+
+    P, batch, T = 16, 700, 30000
+    g = np.random.default_rng(0)
+    t = lambda x, dt=I32: torch.tensor(x, dtype=dt, device=DEV)  # noqa: E731
+    streams, states = [torch.cuda.Stream() for _ in range(2)], []
+    for s in streams:
+        n_pages = 6000
+        ops = Kv8Ops(own, Kv8Spec(8, 2, 64, P, n_pages, 40), s)
+        states.append((ops, t([0] * batch), t(list(range(n_pages))), t([n_pages]), t([[-1] * 40] * batch), [0] * batch,
+                       torch.zeros(T, dtype=torch.int64, device=DEV), t([0] * T), t([0] * (batch + 1))))
+    torch.cuda.synchronize()
+    for turn in range(5):
+        news = [g.integers(0, 30, batch).tolist() for _ in states]
+        dev = [t(n) for n in news]
+        torch.cuda.synchronize()
+        for (ops, lens, stack, count, table, host, slots, pos, start), n in zip(states, dev):
+            for _ in range(4):
+                ops.map_pages(lens, n, stack, count, table, T, into=StepMap(lens, start, slots, pos, count))
+        torch.cuda.synchronize()
+        for i, n in enumerate(news):
+            state = states[i]
+            state[5][:] = [c + 4 * x for c, x in zip(state[5], n)]
+            assert state[1].tolist() == state[5]
+            assert state[3].item() == 6000 - sum(-(-c // P) for c in state[5])
+            for b, c in enumerate(state[5]):
+                state[5][b] = 0
+            state[0].release_pages(t([1] * batch), state[1], state[2], state[3], state[4])
+            torch.cuda.synchronize()
+            assert state[3].item() == 6000 and sorted(state[2].tolist()) == list(range(6000))
+    own.sync_status()
