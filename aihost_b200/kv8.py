@@ -124,20 +124,24 @@ class Kv8Cache:
 
     A step: m = cache.begin(n_new, max_tokens); for every layer cache.append(layer, k, v) and
     cache.attend(layer, q, ...); cache.end(). `release` ends requests. Nothing here waits for the GPU: a step that runs out of
-    pages is refused whole by the kernels (every slot -1, no rows) and reported by ctx.sync_status()."""
+    pages is refused whole by the kernels (every slot -1, no rows) and reported by ctx.sync_status().
+
+    With a `stream`, the cache's tensors are made on it and all its work runs on it; what the caller hands in (n_new, q, k,
+    v) has to be ready on that stream and to stay alive until its work is done, as with any stream of torch's."""
 
     def __init__(self, ctx: Context, spec: Kv8Spec, batch: int, n_layers: int = 1, stream=None):
         self.ctx, self.spec, self.batch = ctx, spec, batch
         self.ops = Kv8Ops(ctx, spec, stream)
         dev, pool = self.ops.device, (spec.n_pages, spec.n_kv_heads, spec.page_rows, spec.head_dim)
-        self.k = [torch.zeros(pool, dtype=torch.int8, device=dev) for _ in range(n_layers)]
-        self.v = [torch.zeros(pool, dtype=torch.int8, device=dev) for _ in range(n_layers)]
-        self.k_scale = [torch.zeros(pool[:2], device=dev) for _ in range(n_layers)]
-        self.v_scale = [torch.zeros(pool[:2], device=dev) for _ in range(n_layers)]
-        self.block_table = torch.full((batch, spec.max_pages), -1, dtype=torch.int32, device=dev)
-        self.free_pages = torch.arange(spec.n_pages - 1, -1, -1, dtype=torch.int32, device=dev)
-        self.free_count = torch.full((1,), spec.n_pages, dtype=torch.int32, device=dev)
-        self.seq_len = torch.zeros(batch, dtype=torch.int32, device=dev)
+        with torch.cuda.stream(stream):  # filled, and given back, in the order of the steps' work
+            self.k = [torch.zeros(pool, dtype=torch.int8, device=dev) for _ in range(n_layers)]
+            self.v = [torch.zeros(pool, dtype=torch.int8, device=dev) for _ in range(n_layers)]
+            self.k_scale = [torch.zeros(pool[:2], device=dev) for _ in range(n_layers)]
+            self.v_scale = [torch.zeros(pool[:2], device=dev) for _ in range(n_layers)]
+            self.block_table = torch.full((batch, spec.max_pages), -1, dtype=torch.int32, device=dev)
+            self.free_pages = torch.arange(spec.n_pages - 1, -1, -1, dtype=torch.int32, device=dev)
+            self.free_count = torch.full((1,), spec.n_pages, dtype=torch.int32, device=dev)
+            self.seq_len = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.map: StepMap | None = None
 
     def begin(self, n_new: torch.Tensor, max_tokens: int) -> StepMap:

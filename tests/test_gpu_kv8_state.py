@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from aihost_b200.kv8 import Kv8Ops
+from aihost_b200 import ROPE_NONE
+from aihost_b200.kv8 import Kv8Cache, Kv8Ops, Kv8Spec, StepMap
 from aihost_b200.ops import Context
 from test_gpu_kv8 import DEV, I32, World
 
@@ -87,8 +88,6 @@ def test_attention_on_several_streams_of_one_context(own):
 
 def test_page_maps_on_several_streams_of_one_context(own):
     """Maps of several blocks that write their lengths in place, on two streams at once."""
-    from aihost_b200.kv8 import Kv8Spec, StepMap
-
     P, batch, T = 16, 700, 30000
     g = np.random.default_rng(0)
     t = lambda x, dt=I32: torch.tensor(x, dtype=dt, device=DEV)  # noqa: E731
@@ -117,4 +116,39 @@ def test_page_maps_on_several_streams_of_one_context(own):
             state[0].release_pages(t([1] * batch), state[1], state[2], state[3], state[4])
             torch.cuda.synchronize()
             assert state[3].item() == 6000 and sorted(state[2].tolist()) == list(range(6000))
+    own.sync_status()
+
+
+def test_a_cache_on_a_stream_of_its_own_needs_no_wait(own):
+    """A cache made and used on a side stream while the current stream is busy gives what one on the current stream
+    gives, also with tensors of the current stream coming and going in between."""
+    B, H, Hq, D, P, steps = 5, 2, 8, 64, 16, 12
+    spec = Kv8Spec(Hq, H, D, P, 60, 8, rope_mode=ROPE_NONE)
+    new = [torch.tensor([(3 * i + b) % 4 for b in range(B)], dtype=I32, device=DEV) for i in range(steps)]
+    g = torch.Generator().manual_seed(5)
+    rows = [[torch.randn(16, h, D, generator=g).half().to(DEV) for h in (Hq, H, H)] for _ in range(steps)]
+    want = []
+
+    def run(cache, got):
+        for n, (q, k, v) in zip(new, rows):
+            m = cache.begin(n, 16)
+            cache.append(0, k, v)
+            got.append((cache.attend(0, q, 4, 128), m))
+            cache.end()
+            for _ in range(4):  # where a tensor that the step let go would be handed out again
+                torch.full((B,), -7, dtype=I32, device=DEV)
+                torch.full((1,), -7, dtype=I32, device=DEV)
+
+    run(Kv8Cache(own, spec, B), want)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for late in (torch.cuda.current_stream(), side):
+        got = []
+        _busy(late, 20)
+        cache = Kv8Cache(own, spec, B, stream=side)
+        run(cache, got)
+        torch.cuda.synchronize()
+        for (a, m), (b, n) in zip(got, want):
+            T = n.row_start[-1].item()
+            assert T and all(torch.equal(x, y) for x, y in zip(m, n)) and torch.equal(a[:T], b[:T])
     own.sync_status()
