@@ -22,6 +22,8 @@
 // merge are dependent trips to L2. Not better: three stages of the ring with two blocks an SM instead
 // of two with three (197 against 177 us for the 32 x 16384), rows loaded straight into registers (135
 // against 127 for the 64), 16-row steps (127 against 113), prefetch hints on the copies (no change).
+#include <type_traits>
+
 #include "common.cuh"
 #include "kv8.h"
 #include "kv8_tile.cuh"
@@ -276,29 +278,42 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
     }
   }
 
-  // Where q is fp16, K enters as 1152 + k (what the byte trick gives), and S starts at -1152 sum q: the
-  // terms cancel in fp32 to about 2^-22 of 1152 |q|, far below P's rounding, for half of K's conversion.
-  constexpr bool kOffset = PREC != kPairQP;
-  float s_init[NT][2];
+  // Where q is fp16, K's bytes can enter as (128 + k) 2^-24, fp16 numbers below the normal ones that take no
+  // arithmetic to make, with S starting at -128 sum q. The terms then cancel in fp32: each of the D / 16
+  // products is off by at most 2^-23 of 128 |sum of q so far| and of its own 255 sum |q|. So pages enter where all
+  // of that is below 2^-12 in the score (in log2 units; P's own rounding is 2^-11), and as k itself where
+  // their scale or q is too large for it. Measured, 64 sequences and 32 of 16384 as above:
+  // 104.6 and 176.4 us, k itself throughout 106.7 and 179.6; with two tiles of query rows (8 sequences of
+  // 8192 rows, 8 new ones each) 92.1, k itself 90.9, which is used there.
+  constexpr bool kOffset = PREC != kPairQP && NT == 1;
+  constexpr float kTiny = 1.0f / 16777216.0f;
+  constexpr float kOffsetMost = 8388608.0f / 4096.0f;  // of a page's factor times q_size
+  float s_init[NT][2], q_size = 0.0f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    float sum = 0.0f;
+    float sum = 0.0f, most = 0.0f, all = 0.0f;
     if (kOffset) {
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
+      for (int k = 0; k < KS; ++k) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+        for (int n = 0; n < NQ; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qf[n][nt][k][e]));
             sum += f.x + f.y;
+            if (n == 0) all += fabsf(f.x) + fabsf(f.y);
           }
+        most = fmaxf(most, fabsf(sum));
+      }
+      q_size = fmaxf(q_size, 128.0f * KS * most + 255.0f * all);
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);  // row g's
     }
 #pragma unroll
-    for (int c = 0; c < 2; ++c) s_init[nt][c] = -1152.0f * __shfl_sync(0xffffffffu, sum, (2 * t4 + c) * 4);
+    for (int c = 0; c < 2; ++c) s_init[nt][c] = -128.0f * kTiny * __shfl_sync(0xffffffffu, sum, (2 * t4 + c) * 4);
   }
+  // four lanes hold a row: at most four times the largest share (bits of numbers >= 0 compare as numbers)
+  if (kOffset) q_size = 4.0f * __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(q_size)));
 
   float o[MT][NT][4];
   float m[NT][2], l[NT][2];
@@ -312,6 +327,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
   const bool capped = MOD && a.score_cap > 0.0f;
   const float s_unit = capped ? a.scale / a.score_cap : a.scale * kLog2e;
   const float cap2 = a.score_cap * kLog2e;
+  // of this lane's next 32 blocks of rows together, so that it is settled once in 16 steps
+  bool small = false;
+  float k_unit = s_unit;
+  auto settle = [&] {
+    if (kOffset) {
+      small = __all_sync(0xffffffffu, ks * (a.scale * kLog2e) * q_size <= kOffsetMost);
+      k_unit = small ? s_unit / kTiny : s_unit;
+    }
+  };
+  settle();
 
   for (int32_t i = 0, round = 0; i < n_steps; ++i) {
     if (i == 16 * (round + 1)) {
@@ -319,6 +344,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
       place = place_next;
       ph = ph_next;
       scales();
+      settle();
       if (i + 16 < n_steps) place_next = place_of(2 * i + 32 + lane, ph_next);
     }
     fetch(i + 1, round);
@@ -327,47 +353,55 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
     const uint8_t* const stage = my_ring + (i % kStages) * kStageBytes;
     const int32_t k = row_of(2 * i);
     // ---- S^T = K Q^T
-    float s[2][NT][4];
+    float s[2][NT][4], kf[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint8_t* const kt = stage + u * (kSub * D);
+    for (int u = 0; u < 2; ++u) kf[u] = __shfl_sync(0xffffffffu, ks, (2 * i + u) & 31) * k_unit;
+    auto products = [&](auto with) {
+      constexpr bool offset = decltype(with)::value;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[u][nt][0] = s[u][nt][2] = s_init[nt][0], s[u][nt][1] = s[u][nt][3] = s_init[nt][1];
+      for (int u = 0; u < 2; ++u) {
+        const uint8_t* const kt = stage + u * (kSub * D);
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const uint4 r0 = *reinterpret_cast<const uint4*>(kt + chunk_at<D>(g, KC * t4 + c));
-        const uint4 r1 = *reinterpret_cast<const uint4*>(kt + chunk_at<D>(g + 8, KC * t4 + c));
-        const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t u0 = w0[j] ^ 0x80808080u, u1 = w1[j] ^ 0x80808080u;
-          uint32_t a0, a1, a2, a3;
-          if constexpr (kOffset) {
-            a0 = __byte_perm(u0, 0x64646464u, 0x4140), a1 = __byte_perm(u1, 0x64646464u, 0x4140);
-            a2 = __byte_perm(u0, 0x64646464u, 0x4342), a3 = __byte_perm(u1, 0x64646464u, 0x4342);
-          } else {
-            a0 = half2_of(u0, 0x4140), a1 = half2_of(u1, 0x4140);
-            a2 = half2_of(u0, 0x4342), a3 = half2_of(u1, 0x4342);
+          for (int e = 0; e < 4; ++e) s[u][nt][e] = offset ? s_init[nt][e & 1] : 0.0f;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          const uint4 r0 = *reinterpret_cast<const uint4*>(kt + chunk_at<D>(g, KC * t4 + c));
+          const uint4 r1 = *reinterpret_cast<const uint4*>(kt + chunk_at<D>(g + 8, KC * t4 + c));
+          const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t u0 = w0[j] ^ 0x80808080u, u1 = w1[j] ^ 0x80808080u;
+            uint32_t a0, a1, a2, a3;
+            if constexpr (offset) {
+              a0 = __byte_perm(u0, 0, 0x4140), a1 = __byte_perm(u1, 0, 0x4140);
+              a2 = __byte_perm(u0, 0, 0x4342), a3 = __byte_perm(u1, 0, 0x4342);
+            } else {
+              a0 = half2_of(u0, 0x4140), a1 = half2_of(u1, 0x4140);
+              a2 = half2_of(u0, 0x4342), a3 = half2_of(u1, 0x4342);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int n = 0; n < NQ; ++n)
+                mma16816(s[u][nt], a0, a1, a2, a3, qf[n][nt][4 * c + j][0], qf[n][nt][4 * c + j][1]);
           }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int n = 0; n < NQ; ++n)
-              mma16816(s[u][nt], a0, a1, a2, a3, qf[n][nt][4 * c + j][0], qf[n][nt][4 * c + j][1]);
         }
       }
-    }
+    };
+    if (kOffset && small) products(std::true_type());
+    else products(std::false_type());
     // ---- scores (log2 units), masks, running maximum
     const bool edge = k < lo_max || k + kStep > hi_min;
     bool grow = false;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const float kf = __shfl_sync(0xffffffffu, ks, (2 * i + u) & 31) * s_unit;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float v = s[u][nt][e] * kf;
+          float v = s[u][nt][e] * kf[u];
           if constexpr (MOD) {
             if (capped) v = cap2 * tanh_of(v);
             if (a.alibi_slopes) {

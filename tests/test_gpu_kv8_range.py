@@ -1,0 +1,79 @@
+"""The 8-bit cache's attention where its numbers leave the ordinary range: K with one large channel, q and V far from 1, V
+scales far apart, caps far above the scores, scores far below zero, the loosest bounds. Bounds as in test_gpu_kv8.py, from the
+number formats; every comparison is against the 64-bit form."""
+import dataclasses
+
+import numpy as np
+import pytest
+import torch
+
+import kv8_plain as plain
+from aihost_b200 import F16, F32, ROPE_INTERLEAVED, ROPE_NEOX, ROPE_NONE
+from aihost_b200.kv8 import Kv8Ops
+from test_gpu_kv8 import BOUNDS, DEV, World, _dt
+
+pytestmark = pytest.mark.gpu
+
+
+def _check(ctx, w, q, out_dtype=None, ds=2.0 ** -19, first=None, max_kv=None, tiny=1e-7, size=None):
+    """Attention of q (float64, exact in the io type) on the GPU against the plain form. A score's error is `ds` of
+    sum |q k| (or of `size`); weights rounded to fp16 are off by 2^-11, pairs of fp16 by 2^-18; an fp16 result by 2^-11 of itself."""
+    ops = w.ops
+    if out_dtype is not None:
+        ops = Kv8Ops(ctx, dataclasses.replace(w.spec, out_dtype=out_dtype))
+    qd = torch.from_numpy(q).to(_dt(w.io))
+    assert torch.equal(qd.double(), torch.from_numpy(q))
+    got = w.attend(qd.to(DEV), first=first, max_kv=max_kv, ops=ops)
+    torch.cuda.synchronize()
+    ctx.sync_status()
+    ref, weight, own = plain.attend(q, w.start, w.kv_len, w.table, w.P, w.k, w.v, w.ks, w.vs, w.scale, w.cap, w.theta, w.mode,
+                                    first=first)
+    size = own if size is None else size
+    tol = weight * ((2.0 ** -11 + 2.0 ** -16 if w.io == F16 else 2.0 ** -18) + 2 * ds * size[..., None]) + tiny
+    if got.dtype == torch.float16:
+        tol = tol + 2.0 ** -11 * np.abs(ref)
+    got = got.double().cpu().numpy()
+    over = np.abs(got - ref) - tol
+    assert np.isfinite(got).all() and over.max() <= 0, (over.max(), np.unravel_index(over.argmax(), over.shape))
+    return got, ref
+
+
+def _q(w, draw):
+    """Query rows from draw(shape), rounded to the io type, as float64."""
+    return torch.from_numpy(np.ascontiguousarray(draw((w.T, w.Hq, w.D)))).to(_dt(w.io)).double().numpy()
+
+
+STEPS = {"decode": dict(cached=[300, 1029], new=[1, 1], P=64), "few": dict(cached=[300, 77], new=[3, 2], P=32),
+         "prompt": dict(cached=[90, 0], new=[60, 130], P=32)}
+
+
+@pytest.mark.parametrize("max_kv", BOUNDS)
+@pytest.mark.parametrize("io", [F16, F32])
+@pytest.mark.parametrize("mode", [ROPE_NONE, ROPE_INTERLEAVED])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("step", list(STEPS))
+def test_keys_with_one_large_channel(ctx, step, D, mode, io, max_kv):
+    """One channel takes all of a page's int8 range and the others hold -1, 0 and 1; q is near 1 (all of one sign) and 0 in that
+    channel: what a conversion with an offset would have to cancel is a thousand times the score."""
+    w = World(ctx, D=D, io=io, mode=mode, seed=41, **STEPS[step])
+    w.k = w.g.integers(-1, 2, w.k.shape).astype(np.int8)
+    w.k[..., 0] = 127
+    w.k[..., 1] = 127
+    w.ks = w.g.uniform(2.5, 3.5, w.ks.shape).astype(np.float32) * np.float32(np.sqrt(128 / D))
+    q = _q(w, lambda s: 1 + 0.3 * w.g.standard_normal(s))
+    q[..., :2] = 0  # the first pair of the rotation
+    _check(ctx, w, q, ds=2.0 ** -11 if io == F16 and mode != ROPE_NONE else 2.0 ** -19, max_kv=max_kv)
+
+
+@pytest.mark.parametrize("cap", [0.0, 300.0])
+@pytest.mark.parametrize("D", [64, 128])
+def test_keys_on_either_side_of_the_rule_for_small_pages(ctx, D, cap):
+    """Page scales spread over four powers of ten, in rounds of 32 blocks of rows: some pages' keys are converted one way, some
+    the other, and a round of large ones follows a round of small ones."""
+    w = World(ctx, D=D, P=16, Hq=4, H=2, cap=cap, seed=52, cached=[2500, 700], new=[1, 1])
+    w.k = w.g.integers(-1, 2, w.k.shape).astype(np.int8)
+    w.ks = np.exp(w.g.uniform(np.log(3e-4), np.log(3), w.ks.shape)).astype(np.float32)
+    for b, n in enumerate(w.kv_len):
+        order = np.argsort(w.ks[w.table[b][:-(-int(n) // 16)], 0])
+        w.ks[w.table[b][:len(order)]] = w.ks[w.table[b][order]]  # small ones first
+    _check(ctx, w, _q(w, lambda s: 1 + 0.3 * w.g.standard_normal(s)))
