@@ -40,7 +40,9 @@ constexpr int kChunkMin = kWarps * kStep, kChunkMax = 2048;
 
 // What the products take. fp16 tensors: an unrotated q is exact in fp16, a rotated one (in fp32) enters
 // as a pair, its fp16 and the fp16 of what that leaves; P is rounded to fp16 once, as the output is. fp32
-// tensors: q and P as pairs, 22 bits. The int8 values are exact in fp16; sums are fp32.
+// tensors: q and P as pairs, 22 bits; a row of q is brought to 2^13 first by a power of two, which the
+// scores take back, or rows beyond fp16's range would be infinite and small ones lose the pair's
+// lower half. The int8 values are exact in fp16; sums are fp32.
 enum { kPlain = 0, kPairQ = 1, kPairQP = 2 };
 
 // The maximum may lag by 2^kSlack before O is rescaled, and P enters times v scale / (the chunk's
@@ -218,10 +220,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
 
   // ---- query rows as B fragments: lane (g, t4) holds row g's elements [t4 * D/4, (t4 + 1) * D/4)
   uint32_t qf[NQ][NT][KS][2];
+  float q_unit[NT][2];  // what the scores of this lane's two columns take back
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     constexpr int E = D / 4;
     float x[E];
+    float back = 1.0f;
     const int r = nt * 8 + g;
     const int32_t row = tl.row0 + min(r, n_rows - 1), i = row / G;
     const uint8_t* src = static_cast<const uint8_t*>(a.q) + (tl.start + static_cast<int64_t>(i)) * a.q_token_stride;
@@ -246,6 +250,21 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
         x[4 * k] = v.x, x[4 * k + 1] = v.y, x[4 * k + 2] = v.z, x[4 * k + 3] = v.w;
       }
     }
+    if constexpr (PREC == kPairQP) {
+      float most = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) most = fmaxf(most, fabsf(x[e]));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      // biased exponents: e for the row's largest element, from 14 on so that both powers are normal numbers
+      const uint32_t e_most = max(__float_as_uint(most) >> 23, 14u);
+      const float bring = __uint_as_float((267u - e_most) << 23);
+      back = __uint_as_float((e_most - 13u) << 23);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] *= bring;
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) q_unit[nt][c] = PREC == kPairQP ? __shfl_sync(0xffffffffu, back, (2 * t4 + c) * 4) : 1.0f;
     if (PREC != kPlain && a.rope_mode != AIHOST_ROPE_NONE) {
       const float pos = static_cast<float>(tl.pos0 + i);
       if (a.rope_mode == AIHOST_ROPE_INTERLEAVED) {
@@ -401,7 +420,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float v = s[u][nt][e] * kf[u];
+          float v = s[u][nt][e] * (PREC == kPairQP ? kf[u] * q_unit[nt][e & 1] : kf[u]);
           if constexpr (MOD) {
             if (capped) v = cap2 * tanh_of(v);
             if (a.alibi_slopes) {

@@ -65,6 +65,26 @@ def test_keys_with_one_large_channel(ctx, step, D, mode, io, max_kv):
     _check(ctx, w, q, ds=2.0 ** -11 if io == F16 and mode != ROPE_NONE else 2.0 ** -19, max_kv=max_kv)
 
 
+@pytest.mark.parametrize("mode", [ROPE_NONE, ROPE_INTERLEAVED, ROPE_NEOX])
+@pytest.mark.parametrize("std", [3e-33, 1e-20, 1e-6, 1e-3, 1e4, 1e6, 1e30])
+@pytest.mark.parametrize("step", list(STEPS))
+def test_fp32_queries_of_any_size(ctx, step, std, mode):
+    """fp32 q enters as a pair of fp16 with 22 bits whatever its size."""
+    w = World(ctx, io=F32, mode=mode, scale=float(np.float32(0.1 / std)), seed=42, Hq=8, H=2, **STEPS[step])
+    w.scale = float(np.float32(0.1 / std))
+    rows = np.exp(w.g.uniform(-1, 1, (w.T, w.Hq, 1)))  # rows of unequal size
+    _check(ctx, w, _q(w, lambda s: std * rows * w.g.standard_normal(s)), tiny=1e-9)
+
+
+@pytest.mark.parametrize("step", list(STEPS))
+def test_fp32_rows_of_zeros_and_of_unequal_elements(ctx, step):
+    w = World(ctx, io=F32, seed=43, scale=1e-4, **STEPS[step])
+    q = _q(w, lambda s: w.g.standard_normal(s) * np.exp(w.g.uniform(np.log(1e-3), np.log(1e6), s)))
+    q[0] = 0
+    got, ref = _check(ctx, w, q, tiny=1e-9)
+    assert np.abs(ref[0]).max() > 0
+
+
 @pytest.mark.parametrize("cap", [0.0, 300.0])
 @pytest.mark.parametrize("D", [64, 128])
 def test_keys_on_either_side_of_the_rule_for_small_pages(ctx, D, cap):
