@@ -39,7 +39,8 @@ constexpr int kStages = 2;        // of the warp's ring
 constexpr int kChunkMin = kWarps * kStep, kChunkMax = 2048;
 
 // What the products take. fp16 tensors: an unrotated q is exact in fp16, a rotated one (in fp32) enters
-// as a pair, its fp16 and the fp16 of what that leaves; P is rounded to fp16 once, as the output is. fp32
+// as a pair, its fp16 and the fp16 of what that leaves, both of one half of it, since turning (x, y) may
+// pass fp16's range; P is rounded to fp16 once, as the output is. fp32
 // tensors: q and P as pairs, 22 bits; a row of q is brought to 2^13 first by a power of two, which the
 // scores take back, or rows beyond fp16's range would be infinite and small ones lose the pair's
 // lower half. The int8 values are exact in fp16; sums are fp32.
@@ -51,6 +52,8 @@ enum { kPlain = 0, kPairQ = 1, kPairQP = 2 };
 // use the whole range.
 template <int PREC>
 constexpr float kSlack = PREC == kPairQP ? 0.0f : 8.0f;
+template <int PREC>
+constexpr float kQUnit = PREC == kPairQ ? 0.5f : 1.0f;
 template <int PREC>
 constexpr float kVUnit = PREC == kPairQP ? 32768.0f : 128.0f;
 
@@ -272,7 +275,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
         for (int e = 0; e < E; e += 2) {
           float sn, cs;
           sincos_near(__fmul_rn(pos, a.freqs.f[(t4 * E + e) >> 1]), &sn, &cs);
-          rotate_pair(x[e], x[e + 1], cs, sn);
+          rotate_pair(x[e], x[e + 1], cs * kQUnit<PREC>, sn * kQUnit<PREC>);
         }
       } else {  // pairs D/2 apart: lanes t4 and t4 ^ 2
 #pragma unroll
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
           float sn, cs;
           sincos_near(__fmul_rn(pos, a.freqs.f[(t4 & 1) * E + e]), &sn, &cs);
           float x1 = t4 < 2 ? x[e] : other, x2 = t4 < 2 ? other : x[e];
-          rotate_pair(x1, x2, cs, sn);
+          rotate_pair(x1, x2, cs * kQUnit<PREC>, sn * kQUnit<PREC>);
           x[e] = t4 < 2 ? x1 : x2;
         }
       }
@@ -344,14 +347,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
     for (int i = 0; i < MT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
   }
   const bool capped = MOD && a.score_cap > 0.0f;
-  const float s_unit = capped ? a.scale / a.score_cap : a.scale * kLog2e;
+  const float q_scale = a.scale * (1.0f / kQUnit<PREC>), s_unit = capped ? q_scale / a.score_cap : q_scale * kLog2e;
   const float cap2 = a.score_cap * kLog2e;
   // of this lane's next 32 blocks of rows together, so that it is settled once in 16 steps
   bool small = false;
   float k_unit = s_unit;
   auto settle = [&] {
     if (kOffset) {
-      small = __all_sync(0xffffffffu, ks * (a.scale * kLog2e) * q_size <= kOffsetMost);
+      small = __all_sync(0xffffffffu, ks * (q_scale * kLog2e) * q_size <= kOffsetMost);
       k_unit = small ? s_unit / kTiny : s_unit;
     }
   };

@@ -20,7 +20,8 @@
 //
 // Precision: an unrotated fp16 q is exact. A rotated one is rounded to fp16; at head_dim 64 the fp16 of
 // what that leaves enters as a second operand, at head_dim 128 there is no shared memory for one (229 KB
-// are used), which costs 3.6e-4 against 2.9e-4 in relative root mean square error. P is rounded to fp16
+// are used), which costs 3.6e-4 against 2.9e-4 in relative root mean square error. Either is of one half of
+// the rotated q, since turning (x, y) may pass fp16's range; K's factors take it back. P is rounded to fp16
 // once, as the output is; maxima, sums and accumulators are fp32, int8 values exact.
 //
 // Measured: 2048 new rows over 14336 cached, 32/8 heads x 128, 497-507 us (515 GFLOP: 1030 TFLOP/s, 63 %
@@ -51,6 +52,7 @@ constexpr int kThreads = 512;
 constexpr uint32_t kRegsMma = 64, kRegsSoftmax = 176, kRegsConvert = 96;
 static_assert(128 * (kRegsMma + 2 * kRegsSoftmax + kRegsConvert) <= 128 * kThreads, "setmaxnreg split exceeds the launch");
 constexpr float kSlack = 8.0f;    // the maximum may lag by 2^8 before O is rescaled
+constexpr float kQUnit = 0.5f;    // a rotated q enters times this
 constexpr float kVUnit = 128.0f;  // P * (v scale / largest) * 128 <= 2^15 stays in fp16's range
 constexpr int kFactors = kKeys / 16;
 constexpr int kFactorRing = 4;
@@ -466,7 +468,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       asm volatile("bar.sync 2, 160;" ::: "memory");
       const float vmax = fmaxf(fmaxf(sh.v_max[0], sh.v_max[1]), fmaxf(sh.v_max[2], sh.v_max[3]));
       const float v_unit = vmax > 0.0f ? kVUnit / vmax : 0.0f;
-      const float k_unit = MOD && a.score_cap > 0.0f ? a.scale / a.score_cap : a.scale * kLog2e;
+      const float q_scale = a.rope_mode != AIHOST_ROPE_NONE ? a.scale * (1.0f / kQUnit) : a.scale;
+      const float k_unit = MOD && a.score_cap > 0.0f ? q_scale / a.score_cap : q_scale * kLog2e;
       for (int32_t i = 0; i < n_load; ++i) {
         fetch(e_next, 1);
         e_next = entry_of(i + 2);
@@ -594,6 +597,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               rotation(fpos * sh.freq[halves ? 8 * c + e : 4 * (e < 4 ? c : c + LPR - 1) + e], &sn[e], &cs[e]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sn[e] *= kQUnit, cs[e] *= kQUnit;
           }
           uint4* const p0 = reinterpret_cast<uint4*>(q_tile + chunk_off(row_a + k, c));
           uint4* const p1 = reinterpret_cast<uint4*>(q_tile + chunk_off(row_a + k, c + LPR));

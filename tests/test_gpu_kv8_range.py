@@ -85,6 +85,17 @@ def test_fp32_rows_of_zeros_and_of_unequal_elements(ctx, step):
     assert np.abs(ref[0]).max() > 0
 
 
+@pytest.mark.parametrize("max_kv", BOUNDS)
+@pytest.mark.parametrize("mode", [ROPE_INTERLEAVED, ROPE_NEOX])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("step", list(STEPS))
+def test_fp16_queries_whose_rotation_passes_the_range_of_fp16(ctx, step, D, mode, max_kv):
+    """Elements up to 65504 turn into ones up to 92 K, which are no fp16."""
+    w = World(ctx, D=D, mode=mode, scale=2e-6, seed=44, **STEPS[step])
+    q = _q(w, lambda s: np.where(w.g.random(s) < 0.5, 1, -1) * w.g.uniform(50000, 65504, s))
+    _check(ctx, w, q, ds=2.0 ** -11, max_kv=max_kv)
+
+
 @pytest.mark.parametrize("cap", [0.0, 300.0])
 @pytest.mark.parametrize("D", [64, 128])
 def test_keys_on_either_side_of_the_rule_for_small_pages(ctx, D, cap):
