@@ -204,6 +204,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
   fetch(0, 0);
   float ks = 0.0f, vs = 0.0f;
   auto scales = [&] {
+    ks = vs = 0.0f;
     if (place != kNowhere) {
       ks = __ldg(a.k_scale + ph);
       vs = __ldg(a.v_scale + ph);
@@ -219,7 +220,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-  const float v_unit = vmax > 0.0f ? kVUnit<PREC> / vmax : 0.0f;
+  const float v_rcp = v_reciprocal(vmax);
+  auto relate = [&] {
+    vs *= v_rcp;
+    vs *= kVUnit<PREC>;
+  };
+  relate();
 
   // ---- query rows as B fragments: lane (g, t4) holds row g's elements [t4 * D/4, (t4 + 1) * D/4)
   uint32_t qf[NQ][NT][KS][2];
@@ -366,6 +372,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
       place = place_next;
       ph = ph_next;
       scales();
+      relate();
       settle();
       if (i + 16 < n_steps) place_next = place_of(2 * i + 32 + lane, ph_next);
     }
@@ -417,6 +424,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
     // ---- scores (log2 units), masks, running maximum
     const bool edge = k < lo_max || k + kStep > hi_min;
     bool grow = false;
+    auto most_of = [&](int nt, int c) {
+      return fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
+    };
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
 #pragma unroll
@@ -449,13 +459,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c)
-        grow |= fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2])) > m[nt][c] + kSlack<PREC>;
+        grow |= most_of(nt, c) > m[nt][c] + kSlack<PREC>;
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float mx = fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
+          float mx = most_of(nt, c);
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
           const float m_new = fmaxf(m[nt][c], mx), f = ex2_approx(m[nt][c] - m_new);
@@ -471,7 +481,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       // ---- P and its fragments
-      const float vf = __shfl_sync(0xffffffffu, vs, (2 * i + u) & 31) * v_unit;
+      const float vf = __shfl_sync(0xffffffffu, vs, (2 * i + u) & 31);
       uint32_t pf[PREC == kPairQP ? 2 : 1][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -531,7 +541,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
   }
   if (stray) atomicOr(a.status, kStatusBadIndex);
 
-  const float o_unit = vmax * (1.0f / kVUnit<PREC>);  // each warp's own
   copies_wait<0>();
   __syncthreads();  // the rings become the merge's space
   // ---- merge the four warps: lane (g, t4) holds elements [g * D/8, (g + 1) * D/8) of rows 2 t4 and 2 t4 + 1
@@ -545,8 +554,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
       if (g == 0) ml_sh[warp][r][0] = m[nt][c], ml_sh[warp][r][1] = l[nt][c];
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        o_sh[warp][r][g * (D / 8) + 2 * i] = o[i][nt][c] * o_unit;
-        o_sh[warp][r][g * (D / 8) + 2 * i + 1] = o[i][nt][c + 2] * o_unit;
+        o_sh[warp][r][g * (D / 8) + 2 * i] = o[i][nt][c] * (1.0f / kVUnit<PREC>) * vmax;  // each warp's own
+        o_sh[warp][r][g * (D / 8) + 2 * i + 1] = o[i][nt][c + 2] * (1.0f / kVUnit<PREC>) * vmax;
       }
     }
   __syncthreads();

@@ -48,8 +48,9 @@ constexpr int kTileRows = 128;
 constexpr int kRows = 2 * kTileRows;  // query rows of a block
 constexpr int kKeys = 128;            // cache rows of a tile
 constexpr int kThreads = 512;
-// setmaxnreg split of the 128 x 512 registers at launch: warps 0-3, softmax warpgroups, converters
-constexpr uint32_t kRegsMma = 64, kRegsSoftmax = 176, kRegsConvert = 96;
+// setmaxnreg split of the 128 x 512 registers at launch: warps 0-3, softmax warpgroups, converters. Measured
+// against 64 / 176 / 96: the long prompt below 489 us and 499-534, prompts with documents 162-165 either way.
+constexpr uint32_t kRegsMma = 56, kRegsSoftmax = 184, kRegsConvert = 88;
 static_assert(128 * (kRegsMma + 2 * kRegsSoftmax + kRegsConvert) <= 128 * kThreads, "setmaxnreg split exceeds the launch");
 constexpr float kSlack = 8.0f;    // the maximum may lag by 2^8 before O is rescaled
 constexpr float kQUnit = 0.5f;    // a rotated q enters times this
@@ -467,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       e_next = entry_of(1);
       asm volatile("bar.sync 2, 160;" ::: "memory");
       const float vmax = fmaxf(fmaxf(sh.v_max[0], sh.v_max[1]), fmaxf(sh.v_max[2], sh.v_max[3]));
-      const float v_unit = vmax > 0.0f ? kVUnit / vmax : 0.0f;
+      const float v_rcp = v_reciprocal(vmax);
       const float q_scale = a.rope_mode != AIHOST_ROPE_NONE ? a.scale * (1.0f / kQUnit) : a.scale;
       const float k_unit = MOD && a.score_cap > 0.0f ? q_scale / a.score_cap : q_scale * kLog2e;
       for (int32_t i = 0; i < n_load; ++i) {
@@ -481,7 +482,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           // and its V factor must not turn it into NaN again.
           const bool fine = vs[0] < INFINITY;
           sh.k_factor[i % kFactorRing][lane] = !on[0] ? 0.0f : fine ? ks[0] * k_unit : __uint_as_float(0x7fffffffu);
-          sh.v_factor[i % kFactorRing][lane] = !on[0] || !fine ? 0.0f : vs[0] * v_unit;
+          const float v_rel = !on[0] || !fine ? 0.0f : vs[0] * v_rcp;
+          sh.v_factor[i % kFactorRing][lane] = v_rel * kVUnit;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.k_full[s]);
@@ -751,7 +753,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     // written by the converters before the first S; with no tile there is nothing to scale
     const float vmax =
         n_own > 0 ? fmaxf(fmaxf(sh.v_max[0], sh.v_max[1]), fmaxf(sh.v_max[2], sh.v_max[3])) : 0.0f;
-    const float o_unit = vmax * (1.0f / kVUnit);
     auto kept = [&](int k) {  // read here, or the compiler would carry the values through the loop
       int32_t v;
       asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v) : "r"(smem_u32(&sh.place[k])));
@@ -795,8 +796,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     float4* const part = reinterpret_cast<float4*>(a.part_o) + (part_unit * a.max_splits) * (D / 4) * kRows + r256;
     float2* const part_ml = reinterpret_cast<float2*>(a.part_ml) + part_unit * a.max_splits * kRows + r256;
     if (ok) {
-      const float unit_o = n_splits > 1 ? o_unit : l != 0.0f ? o_unit / l : 0.0f;
-#pragma unroll
+      const float unit_o = n_splits > 1 ? 1.0f / kVUnit : l != 0.0f ? 1.0f / kVUnit / l : 0.0f;
+#pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         float o[32];
         if (n_own > 0) {
@@ -804,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           tmem_ld32(o_tmem + c * 32, u);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(u[e]) * unit_o;
+          for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(u[e]) * unit_o * vmax;  // in this order: unit_o * vmax may be too small a number
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.0f;

@@ -124,6 +124,9 @@ __device__ __forceinline__ void sincos_near(float a, float* s, float* c) {
   *c = (q + 1) & 2 ? -v : v;
 }
 
+// 1 / the chunk's largest V scale; 0 where that is 0 or the quotient infinite (the append stores zeros there).
+__device__ __forceinline__ float v_reciprocal(float top) { return top > 2.94e-39f ? 1.0f / top : 0.0f; }
+
 // Launch that may begin before the kernel ahead of it on the stream has ended: every kernel launched so
 // calls griddep_wait() before it touches memory (the kernel ahead is then complete and visible), and
 // griddep_launch_dependents() at its own start, so that the next one's set-up overlaps its work.

@@ -96,6 +96,19 @@ def test_fp16_queries_whose_rotation_passes_the_range_of_fp16(ctx, step, D, mode
     _check(ctx, w, q, ds=2.0 ** -11, max_kv=max_kv)
 
 
+@pytest.mark.parametrize("max_kv", BOUNDS)
+@pytest.mark.parametrize("io", [F16, F32])
+@pytest.mark.parametrize("top", [1e-33, 3e-36, 2e-37])
+@pytest.mark.parametrize("step", list(STEPS))
+def test_tiny_values(ctx, step, top, io, max_kv):
+    """V scales down to the least normal fp32 numbers: results of that size, not NaN."""
+    w = World(ctx, D=128, io=io, seed=45, **STEPS[step])
+    w.vs = w.g.uniform(top / 10, top, w.vs.shape).astype(np.float32)
+    # below the least normal number, 1.2e-38, a result may be flushed
+    got, ref = _check(ctx, w, _q(w, w.g.standard_normal), out_dtype=F32, max_kv=max_kv, tiny=1.2e-38)
+    assert np.abs(ref).max() > 2 * top
+
+
 @pytest.mark.parametrize("cap", [0.0, 300.0])
 @pytest.mark.parametrize("D", [64, 128])
 def test_keys_on_either_side_of_the_rule_for_small_pages(ctx, D, cap):
