@@ -47,9 +47,9 @@ constexpr int kChunkMin = kWarps * kStep, kChunkMax = 2048;
 enum { kPlain = 0, kPairQ = 1, kPairQP = 2 };
 
 // The maximum may lag by 2^kSlack before O is rescaled, and P enters times v scale / (the chunk's
-// largest v scale) * kVUnit, at most 2^15: inside fp16's range with as much as possible above its
-// smallest step. A pair's rest has that same smallest step, so pairs keep the maximum up to date and
-// use the whole range.
+// largest v scale) * kVUnit, at most 2^15 (the maximum counts that ratio in: v_exp_of): inside fp16's
+// range with as much as possible above its smallest step. A pair's rest has that same smallest step, so
+// pairs keep the maximum up to date and use the whole range.
 template <int PREC>
 constexpr float kSlack = PREC == kPairQP ? 0.0f : 8.0f;
 template <int PREC>
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
     copies_commit();
   };
   fetch(0, 0);
-  float ks = 0.0f, vs = 0.0f;
+  float ks = 0.0f, vs = 0.0f, ve = 0.0f;
   auto scales = [&] {
     ks = vs = 0.0f;
     if (place != kNowhere) {
@@ -223,6 +223,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
   const float v_rcp = v_reciprocal(vmax);
   auto relate = [&] {
     vs *= v_rcp;
+    ve = v_exp_of(vs);
     vs *= kVUnit<PREC>;
   };
   relate();
@@ -424,8 +425,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
     // ---- scores (log2 units), masks, running maximum
     const bool edge = k < lo_max || k + kStep > hi_min;
     bool grow = false;
+    const float ve0 = __shfl_sync(0xffffffffu, ve, (2 * i) & 31), ve1 = __shfl_sync(0xffffffffu, ve, (2 * i + 1) & 31);
     auto most_of = [&](int nt, int c) {
-      return fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]), fmaxf(s[1][nt][c], s[1][nt][c + 2]));
+      return fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]) + ve0, fmaxf(s[1][nt][c], s[1][nt][c + 2]) + ve1);
     };
 #pragma unroll
     for (int u = 0; u < 2; ++u) {

@@ -83,6 +83,7 @@ struct Shared {
   uint64_t raw_full[4], raw_empty[4];
   float k_factor[kFactorRing][kFactors];
   float v_factor[kFactorRing][kFactors];
+  float v_exp[kFactorRing][kFactors];
   float v_max[4];
   float freq[64];  // the rotation's frequencies: a parameter indexed by lane costs a turn per distinct index
   uint32_t tmem_base;
@@ -484,6 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           sh.k_factor[i % kFactorRing][lane] = !on[0] ? 0.0f : fine ? ks[0] * k_unit : __uint_as_float(0x7fffffffu);
           const float v_rel = !on[0] || !fine ? 0.0f : vs[0] * v_rcp;
           sh.v_factor[i % kFactorRing][lane] = v_rel * kVUnit;
+          sh.v_exp[i % kFactorRing][lane] = v_exp_of(v_rel);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.k_full[s]);
@@ -701,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         float p3 = fmax3(__uint_as_float(g[9]), __uint_as_float(g[10]), __uint_as_float(g[11]));
         p0 = fmax3(p0, __uint_as_float(g[12]), __uint_as_float(g[13]));
         p1 = fmax3(p1, __uint_as_float(g[14]), __uint_as_float(g[15]));
-        mx = fmaxf(mx, fmax3(fmaxf(p0, p1), p2, p3) * kf[f]);
+        mx = fmaxf(mx, fmaf(fmax3(fmaxf(p0, p1), p2, p3), kf[f], sh.v_exp[slot][f]));
       }
       const bool grow = mx > m + kSlack;
       float f_o = 1.0f;

@@ -124,6 +124,16 @@ __device__ __forceinline__ void sincos_near(float a, float* s, float* c) {
   *c = (q + 1) & 2 ? -v : v;
 }
 
+// How a page's V scale enters. P carries it relative to the largest of the chunk, times kVUnit, so that it stays
+// in fp16's range. But a row may see only pages far below the largest (other rows' documents set it), or
+// give the pages near it next to no weight. So a row's running maximum is that of score + v_exp, with
+// v_exp = log2 of the relative scale: then the row's own largest weight times scale comes to about kVUnit,
+// whichever page it lies on, and what
+// is rounded off is small beside that. exp2(score - maximum) may be up to
+// 2^90 times what it were with the largest score there; its sum and the merges are fp32.
+__device__ __forceinline__ float v_exp_of(float relative) {
+  return fmaxf(__log2f(fabsf(relative)), -90.0f);  // pages below 2^-90 of the largest count as that: sums stay below 2^127
+}
 // 1 / the chunk's largest V scale; 0 where that is 0 or the quotient infinite (the append stores zeros there).
 __device__ __forceinline__ float v_reciprocal(float top) { return top > 2.94e-39f ? 1.0f / top : 0.0f; }
 

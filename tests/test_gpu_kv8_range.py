@@ -109,6 +109,40 @@ def test_tiny_values(ctx, step, top, io, max_kv):
     assert np.abs(ref).max() > 2 * top
 
 
+@pytest.mark.parametrize("max_kv", BOUNDS)
+@pytest.mark.parametrize("io, low, high", [(F16, 1e-3, 500.0), (F16, 1e-9, 1e3), (F32, 1e-3, 500.0), (F32, 1e-9, 1e9)])
+@pytest.mark.parametrize("D, P", [(64, 16), (128, 32)])
+@pytest.mark.parametrize("cached", [[256, 0], [250, 2]])  # the second: edges inside tiles of 4 tokens too
+def test_documents_whose_values_differ_in_size(ctx, cached, D, P, io, low, high, max_kv):
+    """Rows of one document see nothing of another's values, nor of their size."""
+    w = World(ctx, cached, [150, 200], D=D, P=P, io=io, seed=46)
+    # at page edges: every page in one document
+    edges = {0: [0, 64, 288, 320, cached[0] + 150], 1: [0, 96, 128, cached[1] + 200]}
+    first = np.zeros(w.T, int)
+    for b, e in edges.items():
+        for i, (lo, hi) in enumerate(zip(e, e[1:])):
+            w.vs[w.table[b][lo // P:-(-hi // P)]] *= (high if i % 2 else low) / 0.01
+        for t in range(w.start[b], w.start[b + 1]):
+            first[t] = max(x for x in e if x <= w.pos[t])
+    _check(ctx, w, _q(w, w.g.standard_normal), out_dtype=F32, first=first.tolist(), max_kv=max_kv, tiny=1e-30)
+
+
+@pytest.mark.parametrize("max_kv", BOUNDS)
+@pytest.mark.parametrize("io", [F16, F32])
+@pytest.mark.parametrize("step", list(STEPS))
+def test_values_far_apart_in_sight_of_each_other(ctx, step, io, max_kv):
+    """A few pages with values a million times the others', whose keys lie so far off that they add nothing."""
+    w = World(ctx, D=128, io=io, seed=47, **STEPS[step])
+    w.vs *= np.float32(1e-2)
+    q = _q(w, lambda s: 0.5 + 0.1 * w.g.standard_normal(s))
+    for b in range(len(w.new)):
+        page = w.table[b][0]
+        w.k[page] = -100  # scores about -100 * 0.1 * 0.5 * 128 / sqrt(128)
+        w.ks[page] = 0.1
+        w.vs[page] = 1e3
+    _check(ctx, w, q, out_dtype=F32, max_kv=max_kv, tiny=1e-12)
+
+
 @pytest.mark.parametrize("cap", [0.0, 300.0])
 @pytest.mark.parametrize("D", [64, 128])
 def test_keys_on_either_side_of_the_rule_for_small_pages(ctx, D, cap):
