@@ -312,9 +312,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
   // products is off by at most 2^-23 of 128 |sum of q so far| and of its own 255 sum |q|. So pages enter where all
   // of that is below 2^-12 in the score (in log2 units; P's own rounding is 2^-11), and as k itself where
   // their scale or q is too large for it. Measured, 64 sequences and 32 of 16384 as above:
-  // 104.6 and 176.4 us, k itself throughout 106.7 and 179.6; with two tiles of query rows (8 sequences of
-  // 8192 rows, 8 new ones each) 92.1, k itself 90.9, which is used there.
-  constexpr bool kOffset = PREC != kPairQP && NT == 1;
+  // 104.6 and 176.4 us, k itself throughout 106.7 and 179.6. k itself is used where the registers have no
+  // room for more: with two tiles of query rows (8 sequences of 8192 rows, 8 new ones each: 90.9, so 92.1)
+  // and with a rotated q and a cap or bias (32 sequences of 4000 to 9000 rows: 98.2, so 100.1).
+  constexpr bool kOffset = NT == 1 && (PREC == kPlain || (PREC == kPairQ && !MOD));
   constexpr float kTiny = 1.0f / 16777216.0f;
   constexpr float kOffsetMost = 8388608.0f / 4096.0f;  // of a page's factor times q_size
   float s_init[NT][2], q_size = 0.0f;
@@ -429,22 +430,34 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
     auto most_of = [&](int nt, int c) {
       return fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]) + ve0, fmaxf(s[1][nt][c], s[1][nt][c + 2]) + ve1);
     };
+    float far = 0.0f;  // the largest of the lane's scores, in units of the cap
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float v = s[u][nt][e] * (PREC == kPairQP ? kf[u] * q_unit[nt][e & 1] : kf[u]);
-          if constexpr (MOD) {
-            if (capped) v = cap2 * tanh_of(v);
-            if (a.alibi_slopes) {
-              const int32_t row = k + u * kSub + g + (e >> 1) * 8;
-              v -= c_slope[nt][e & 1] * fabsf(c_pos[nt][e & 1] - static_cast<float>(row));
-            }
-          }
-          s[u][nt][e] = v;
+          s[u][nt][e] *= PREC == kPairQP ? kf[u] * q_unit[nt][e & 1] : kf[u];
+          if (MOD) far = fmaxf(far, fabsf(s[u][nt][e]));
         }
+    if constexpr (MOD) {
+      auto each = [&](auto f) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[u][nt][e] = f(s[u][nt][e], u, nt, e);
+      };
+      if (capped) {  // without exponentials where the warp has small ones only
+        if (__any_sync(0xffffffffu, far > kTanhSmall)) each([&](float x, int, int, int) { return cap2 * tanh_of(x); });
+        else each([&](float x, int, int, int) { return cap2 * tanh_small(x); });
+      }
+      if (a.alibi_slopes)
+        each([&](float x, int u, int nt, int e) {
+          const int32_t row = k + u * kSub + g + (e >> 1) * 8;
+          return x - c_slope[nt][e & 1] * fabsf(c_pos[nt][e & 1] - static_cast<float>(row));
+        });
     }
     if (edge) {
 #pragma unroll

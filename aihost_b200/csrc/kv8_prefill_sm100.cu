@@ -160,9 +160,11 @@ __device__ __forceinline__ void odd_of(uint32_t (&sr)[4][32], const float (&coef
 // score = cap * tanh(x), x in units of the cap, times log2 e (cap2 = cap * log2 e). Where the whole
 // warp has |x| <= 1, tanh x = x * P(x^2) on the FMA pipe (the exponentials already fill the SFU): P of
 // degree 6, our weighted least-squares fit on [0, 1], 5e-8 off; where it has |x| <= 0.35, as with caps
-// well above the scores, one of degree 3, 4e-8 off. Else 1 - 2 / (1 + e^2x). Measured with and without
-// the shorter polynomial: 6 prompts with cap 50 63.5 and 70 us, 3 with cap 30 195 and 221; with scores
-// beyond a cap of 4 the one comparison more costs 282 against 277.
+// well above the scores, the one of degree 3. Else tanh_far for all, 1e-7 of the cap off, which is below P's
+// rounding for caps up to 5000 (tanh_of, whose error goes by the score: 328 us in place of 263 for three
+// prompts of 1500 to 2000 rows with scores beyond a cap of 4). Measured with and without the shorter
+// polynomial: 6 prompts with cap 50 63.5 and 70 us, 3 with cap 30 195 and 221; with scores beyond a cap of 4
+// the one comparison more costs 282 against 277.
 __device__ __forceinline__ void cap_scores(uint32_t (&sr)[4][32], float cap2) {
   float tops[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -171,8 +173,8 @@ __device__ __forceinline__ void cap_scores(uint32_t (&sr)[4][32], float cap2) {
     for (int e = 0; e < 32; e += 2)
       tops[c] = fmax3(tops[c], fabsf(__uint_as_float(sr[c][e])), fabsf(__uint_as_float(sr[c][e + 1])));
   const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  if (!__any_sync(0xffffffffu, top > 0.35f)) {
-    constexpr float kP[4] = {0.9999998211860657f, -0.3333165645599365f, 0.13283322751522064f, -0.048376914113759995f};
+  if (!__any_sync(0xffffffffu, top > kTanhSmall)) {
+    constexpr float kP[4] = {kTanh0, kTanh1, kTanh2, kTanh3};
     odd_of<3>(sr, kP, cap2);
   } else if (!__any_sync(0xffffffffu, top > 1.0f)) {
     constexpr float kP[7] = {0.9999999403953552f,  -0.33332839608192444f, 0.13325203955173492f, -0.05345702916383743f,
@@ -182,7 +184,7 @@ __device__ __forceinline__ void cap_scores(uint32_t (&sr)[4][32], float cap2) {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int e = 0; e < 32; ++e) sr[c][e] = __float_as_uint(cap2 * tanh_of(__uint_as_float(sr[c][e])));
+      for (int e = 0; e < 32; ++e) sr[c][e] = __float_as_uint(cap2 * tanh_far(__uint_as_float(sr[c][e])));
   }
 }
 

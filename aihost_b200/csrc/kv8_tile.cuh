@@ -88,11 +88,21 @@ __device__ __forceinline__ uint32_t pack2_rest(float lo, float hi, uint32_t h) {
   return pack2(lo - f.x, hi - f.y);
 }
 
-// tanh x = 1 - 2 / (1 + e^2x): absolute error ~1e-7, which is what the capped score keeps.
-__device__ __forceinline__ float tanh_of(float x) {
+// tanh for the score cap, whose error is to go by the score and not by the cap: up to kTanhSmall x P(x^2), P of
+// degree 3 (our weighted least-squares fit on [0, 0.35], 4e-8 off, 1.8e-7 of x near 0); beyond,
+// 1 - 2 / (1 + e^2x), absolute error ~1e-7.
+constexpr float kTanhSmall = 0.35f;
+constexpr float kTanh0 = 0.9999998211860657f, kTanh1 = -0.3333165645599365f, kTanh2 = 0.13283322751522064f,
+                kTanh3 = -0.048376914113759995f;
+__device__ __forceinline__ float tanh_small(float x) {
+  const float y = x * x;
+  return x * fmaf(fmaf(fmaf(kTanh3, y, kTanh2), y, kTanh1), y, kTanh0);
+}
+__device__ __forceinline__ float tanh_far(float x) {
   const float e = ex2_approx(x * (2.0f * kLog2e));
   return 1.0f - __fdividef(2.0f, 1.0f + e);
 }
+__device__ __forceinline__ float tanh_of(float x) { return fabsf(x) <= kTanhSmall ? tanh_small(x) : tanh_far(x); }
 
 // sin and cos to 1.1e-7 for |angle| <= 1e6 (beyond, the library's): Cody-Waite reduction by pi/2 in three
 // parts (W. J. Cody and W. Waite, Software Manual for the Elementary Functions, 1980), each step one
@@ -128,8 +138,7 @@ __device__ __forceinline__ void sincos_near(float a, float* s, float* c) {
 // in fp16's range. But a row may see only pages far below the largest (other rows' documents set it), or
 // give the pages near it next to no weight. So a row's running maximum is that of score + v_exp, with
 // v_exp = log2 of the relative scale: then the row's own largest weight times scale comes to about kVUnit,
-// whichever page it lies on, and what
-// is rounded off is small beside that. exp2(score - maximum) may be up to
+// whichever page it lies on, and what is rounded off is small beside that. exp2(score - maximum) may be up to
 // 2^90 times what it were with the largest score there; its sum and the merges are fp32.
 __device__ __forceinline__ float v_exp_of(float relative) {
   return fmaxf(__log2f(fabsf(relative)), -90.0f);  // pages below 2^-90 of the largest count as that: sums stay below 2^127

@@ -143,6 +143,31 @@ def test_values_far_apart_in_sight_of_each_other(ctx, step, io, max_kv):
     _check(ctx, w, q, out_dtype=F32, max_kv=max_kv, tiny=1e-12)
 
 
+@pytest.mark.parametrize("max_kv", BOUNDS)
+@pytest.mark.parametrize("io", [F16, F32])
+@pytest.mark.parametrize("cap", [1e3, 1e5])
+@pytest.mark.parametrize("step", list(STEPS))
+def test_caps_far_above_the_scores(ctx, step, cap, io, max_kv):
+    """A capped score is as exact as an uncapped one: its error goes by the score, not by the cap."""
+    w = World(ctx, D=128, io=io, cap=cap, seed=48, **STEPS[step])
+    _check(ctx, w, _q(w, w.g.standard_normal), max_kv=max_kv)
+
+
+@pytest.mark.parametrize("io", [F16, F32])
+@pytest.mark.parametrize("step", list(STEPS))
+def test_scores_near_and_far_from_a_large_cap(ctx, step, io):
+    """The same where single keys lie beyond the cap, so that no step of the cache is all small."""
+    w = World(ctx, D=128, io=io, cap=1000.0, seed=49, **STEPS[step])
+    q = _q(w, lambda s: np.abs(w.g.standard_normal(s)) + 0.5)
+    w.k[:, :, ::8] = -127
+    w.ks[:] = 0.02
+    w.ks[::3] = 1.5  # -127 * 1.5 * 1.3 * 128 / sqrt(128): beyond the cap
+    for b in range(len(w.new)):
+        w.ks[w.table[b][0]] = 0.02
+    w.k[:, :, ::8] = -127
+    _check(ctx, w, q, ds=2.0 ** -18)
+
+
 @pytest.mark.parametrize("cap", [0.0, 300.0])
 @pytest.mark.parametrize("D", [64, 128])
 def test_keys_on_either_side_of_the_rule_for_small_pages(ctx, D, cap):
