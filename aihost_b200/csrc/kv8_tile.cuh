@@ -8,7 +8,7 @@
 namespace aihost {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNoMax = -1e30f;
+constexpr float kNoMax = -3.402823466e38f;  // the lowest number: no score is below it but a hidden one's -infinity
 
 // A KV head's query rows of sequence b are its tokens' heads, token by token: row = token * G + head
 // in the group. Tiles of R rows of sequence b start at floor(row_start[b] * G / R) + b: room for every

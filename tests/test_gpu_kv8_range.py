@@ -168,6 +168,20 @@ def test_scores_near_and_far_from_a_large_cap(ctx, step, io):
     _check(ctx, w, q, ds=2.0 ** -18)
 
 
+@pytest.mark.parametrize("step", list(STEPS))
+def test_scores_below_every_sentinel(ctx, step):
+    """All scores of a row at -1e31 and below: the largest still takes the row."""
+    w = World(ctx, D=64, io=F32, scale=1e12, seed=50, **STEPS[step])
+    q = _q(w, lambda s: np.full(s, 1e17))
+    w.k[:] = w.g.integers(-120, -100, w.k.shape)
+    w.ks[:] = 1.0
+    best = [int(w.table[b][0]) for b in range(len(w.new))]
+    for page in best:
+        w.k[page, :, 0] = -10
+    got, ref = _check(ctx, w, q, ds=0.0, tiny=1e-9)
+    assert np.abs(ref).max() > 0.1
+
+
 @pytest.mark.parametrize("cap", [0.0, 300.0])
 @pytest.mark.parametrize("D", [64, 128])
 def test_keys_on_either_side_of_the_rule_for_small_pages(ctx, D, cap):
