@@ -3,6 +3,8 @@
 #include <math.h>
 #include <string.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "ctx.h"
 #include "kv8.h"
@@ -10,6 +12,8 @@
 using namespace aihost;
 
 namespace {
+
+constexpr int32_t kMaxKv = INT32_MAX - 8192;  // rows of a sequence: chunks of them are rounded up, within int32
 
 int32_t page_shift_of(int32_t page_rows) {
   return page_rows == 16 ? 4 : page_rows == 32 ? 5 : page_rows == 64 ? 6 : page_rows == 128 ? 7 : -1;
@@ -101,6 +105,7 @@ Plan make_plan(const aihost_kv8_desc* d, const Kv8Geom& g, int32_t batch, int32_
   // 8 sequences of 8192 rows with 8 new ones 85 and 69 us, with 16 85 and 116; one sequence with 32
   // 42 and 41, with 64 45 and 66; 8 of 512 rows with 16 19 and 15, with 32 19 and 27.
   Plan p;
+  max_kv = std::min(max_kv, kMaxKv);
   const int32_t rows = kv8_mma_rows(g, max_new), G = g.n_q_heads / g.n_kv_heads;
   p.tensor = false;
   if (d->io_dtype == AIHOST_F16 && static_cast<int64_t>(max_new) * G > rows) {
@@ -299,7 +304,7 @@ aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* 
   a.batch = batch;
   a.n_tokens = n_tokens;
   a.max_new = max_new;
-  a.max_kv = max_kv;
+  a.max_kv = std::min(max_kv, kMaxKv);
   a.q_dtype = desc->io_dtype;
   a.out_dtype = desc->out_dtype;
   a.rope_mode = desc->rope_mode;

@@ -151,9 +151,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
     hi_min = __reduce_min_sync(0xffffffffu, end);
   }
   const int32_t base = min(lo, hi) & ~(kSub - 1);
-  const int32_t n_splits = max(1, (hi - base + a.chunk - 1) / a.chunk);
+  const int32_t n_splits = (hi - base - 1) / a.chunk + 1;  // base <= hi; one for an empty range
   if (split >= n_splits) return;
-  const int32_t k_begin = base + split * a.chunk, k_end = min(hi, k_begin + a.chunk);
+  const int32_t k_begin = base + split * a.chunk, k_end = k_begin + min(hi - k_begin, a.chunk);
   const int32_t* const table = a.block_table + static_cast<int64_t>(tl.b) * a.g.max_pages;
   bool stray = false;  // a page id outside the pool reads page 0 and sets the status
 

@@ -182,6 +182,15 @@ def test_scores_below_every_sentinel(ctx, step):
     assert np.abs(ref).max() > 0.1
 
 
+@pytest.mark.parametrize("max_kv", [2 ** 31 - 1, 2 ** 31 - 200, 2 ** 30])
+@pytest.mark.parametrize("io", [F16, F32])
+@pytest.mark.parametrize("step", list(STEPS))
+def test_the_loosest_bound(ctx, step, io, max_kv):
+    """max_kv is any bound, up to the largest int32."""
+    w = World(ctx, D=64, io=io, seed=51, **STEPS[step])
+    _check(ctx, w, _q(w, w.g.standard_normal), max_kv=max_kv)
+
+
 @pytest.mark.parametrize("cap", [0.0, 300.0])
 @pytest.mark.parametrize("D", [64, 128])
 def test_keys_on_either_side_of_the_rule_for_small_pages(ctx, D, cap):
