@@ -31,11 +31,12 @@ EXPORTS = (
     "aihost_attn_noalloc_sync_status", "aihost_attn_dist_init_bounded", "aihost_attn_dist_sync",
     "aihost_matmul_workspace_size", "aihost_matmul_weights", "aihost_dequantize",
     "aihost_page_map", "aihost_page_release", "aihost_kv8_append", "aihost_kv8_read", "aihost_kv8_workspace_size",
-    "aihost_kv8_attention",
+    "aihost_kv8_attention", "aihost_kv8_plan",
 )
 # aihost_kernel ids of the device-time profiler
 KERNEL_APPEND, KERNEL_DECODE, KERNEL_COMBINE, KERNEL_PREFILL, KERNEL_CONVERT, KERNEL_MATMUL = range(6)
 KERNEL_PAGES, KERNEL_KV8_APPEND, KERNEL_KV8_ATTN = range(6, 9)
+KV8_SPLIT_CACHE, KV8_TENSOR = range(2)  # aihost_kv8_kernel: which one an attention call over the 8-bit cache runs
 
 
 class AttnDesc(ctypes.Structure):
@@ -116,6 +117,7 @@ def lib() -> ctypes.CDLL:
     L.aihost_kv8_append.argtypes = [vp, k8, i32] + [vp] * 9
     L.aihost_kv8_read.argtypes = [vp, k8, i32, vp, vp, vp, vp, i32, vp]
     L.aihost_kv8_workspace_size.argtypes = [k8, i32, i32, i32, i32, ctypes.POINTER(sz)]
+    L.aihost_kv8_plan.argtypes = [vp, k8, i32, i32, i32, i32, ctypes.POINTER(sz), ctypes.POINTER(i32)]
     L.aihost_kv8_attention.argtypes = [vp, k8, i32, i32, i32, i32] + [vp] * 13
     for name in EXPORTS:
         fn = getattr(L, name)

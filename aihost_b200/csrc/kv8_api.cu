@@ -127,6 +127,12 @@ Plan make_plan(const aihost_kv8_desc* d, const Kv8Geom& g, int32_t batch, int32_
   return p;
 }
 
+int32_t current_sms() {
+  int sms = 148, dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
 // Sizes of an attention call, from host-known bounds.
 aihost_status check_sizes(int32_t batch, int32_t n_tokens, int32_t max_new, int32_t max_kv) {
   if (batch < 1) return fail(AIHOST_EINVAL, "batch (%d) must be >= 1", batch);
@@ -274,9 +280,19 @@ aihost_status aihost_kv8_workspace_size(const aihost_kv8_desc* desc, int32_t bat
   aihost_status s = check_kv8(desc, &r);
   if (s == AIHOST_OK) s = check_sizes(batch, n_tokens, max_new, max_kv);
   if (s != AIHOST_OK) return s;
-  int sms = 148, dev = 0;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  *out_bytes = make_plan(desc, r.g, batch, n_tokens, max_new, max_kv, sms).scratch(r.g);
+  *out_bytes = make_plan(desc, r.g, batch, n_tokens, max_new, max_kv, current_sms()).scratch(r.g);
+  return AIHOST_OK;
+}
+
+aihost_status aihost_kv8_plan(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens,
+                              int32_t max_new, int32_t max_kv, size_t* out_bytes, int32_t* out_kernel) {
+  Resolved r;
+  aihost_status s = check_kv8(desc, &r);
+  if (s == AIHOST_OK) s = check_sizes(batch, n_tokens, max_new, max_kv);
+  if (s != AIHOST_OK) return s;
+  const Plan plan = make_plan(desc, r.g, batch, n_tokens, max_new, max_kv, ctx ? ctx->num_sms : current_sms());
+  if (out_bytes) *out_bytes = plan.scratch(r.g);
+  if (out_kernel) *out_kernel = plan.tensor ? AIHOST_KV8_TENSOR : AIHOST_KV8_SPLIT_CACHE;
   return AIHOST_OK;
 }
 

@@ -273,7 +273,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     aihost_status s = call();
     if (s == AIHOST_ENOMEM) {  // the context's scratch is too small: grow it once
       size_t need = 0;
-      check(aihost_kv8_workspace_size(&c.d, static_cast<int32_t>(b), static_cast<int32_t>(n), max_new, max_kv, &need));
+      check(aihost_kv8_plan(c.ctx, &c.d, static_cast<int32_t>(b), static_cast<int32_t>(n), max_new, max_kv, &need, nullptr));
       check(aihost_attn_reserve(c.ctx, need));
       s = call();
     }

@@ -22,7 +22,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import EINVAL, F16, F32, ROPE_INTERLEAVED, AttnError, Kv8Desc, lib
+from . import EINVAL, F16, F32, ROPE_INTERLEAVED, AttnError, Kv8Desc, check, lib
 from .ops import Context
 
 lib()  # the module below calls the same library
@@ -117,6 +117,13 @@ class Kv8Ops:
         before keep the scratch they were captured with)."""
         return _kv8.attend(self.ctx.handle.value, self.ctx.device, self._at, self._st(), q, row_start, kv_len, block_table,
                            k_pool, v_pool, k_scale, v_scale, max_new, max_kv, prefix_len, row_first, alibi_slopes, out)
+
+    def plan(self, batch: int, n_tokens: int, max_new: int, max_kv: int) -> tuple[int, int]:
+        """(scratch bytes, KV8_SPLIT_CACHE or KV8_TENSOR) of an `attend` with these sizes and bounds."""
+        need, kernel = ctypes.c_size_t(), ctypes.c_int32()
+        check(lib().aihost_kv8_plan(self.ctx.handle, ctypes.byref(self._desc), batch, n_tokens, max_new, max_kv,
+                                    ctypes.byref(need), ctypes.byref(kernel)))
+        return need.value, kernel.value
 
 
 class Kv8Cache:

@@ -381,9 +381,18 @@ aihost_status aihost_kv8_append(aihost_attn_ctx* ctx, const aihost_kv8_desc* des
 aihost_status aihost_kv8_read(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t n_rows, const int64_t* slots,
                               const int8_t* pool, const float* scale, void* out, int32_t out_dtype, void* stream);
 
-/* Scratch bytes of an aihost_kv8_attention call with these arguments (0 if none). */
+/* Scratch bytes of an aihost_kv8_attention call with these arguments (0 if none) on the calling thread's
+ * current device. */
 aihost_status aihost_kv8_workspace_size(const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens, int32_t max_new,
                                         int32_t max_kv, size_t* out_bytes);
+/* What an aihost_kv8_attention call with these arguments does on ctx's device (NULL: the current one): its
+ * scratch bytes, and which kernel it runs. Either pointer may be NULL. */
+typedef enum {
+  AIHOST_KV8_SPLIT_CACHE = 0, /* few query rows over chunks of the cache (mma.sync) */
+  AIHOST_KV8_TENSOR = 1       /* 256 query rows a block (tcgen05) */
+} aihost_kv8_kernel;
+aihost_status aihost_kv8_plan(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens,
+                              int32_t max_new, int32_t max_kv, size_t* out_bytes, int32_t* out_kernel);
 /* Attention of q [n_tokens][Hq][d] over the cache, into out [n_tokens][Hq][d] (packed). Sequence b has
  * kv_len[b] cached rows, its new ones (already appended) included; its query row i sits at position
  * p = kv_len[b] - (row_start[b + 1] - row_start[b]) + i and sees the cache rows j with
@@ -392,10 +401,15 @@ aihost_status aihost_kv8_workspace_size(const aihost_kv8_desc* desc, int32_t bat
  * and from the start of its own document on (row_first, int32 [n_tokens], or NULL: 0). A row that
  * sees nothing gets zeros. score = scale * q.k, capped if score_cap > 0, then minus
  * alibi_slopes[head] * |p - j| (fp32 [Hq], or NULL). No sequence may have more than max_new new
- * rows or max_kv cached ones. Softmax state and sums are fp32; int8 values enter the products exactly.
- * With F16 q, the softmax weights enter as fp16; q enters exactly where it is not rotated, else as a pair
- * of fp16 whose sum holds 22 bits, but for prompts with head_dim 128, where it is rounded to fp16 once.
- * With F32 q, q and the weights enter as such pairs. */
+ * rows or max_kv cached ones (nor any 2^31 - 8192). Rows of q that belong to no sequence (spare tokens
+ * past row_start[batch], all of them in a step that aihost_page_map refused) and those of a sequence out of
+ * bounds are not computed, and their rows of out are left as they are.
+ * Softmax state and sums are fp32; int8 values enter the products exactly. With F16 q, the softmax weights
+ * enter as fp16; q enters exactly where it is not rotated, else as a pair of fp16 whose sum holds 22 bits (down
+ * to fp16's smallest step), but in the AIHOST_KV8_TENSOR kernel with head_dim 128, where it is rounded to fp16
+ * once. Which kernel runs goes by head counts, batch, n_tokens, max_new and max_kv, so the same row may
+ * differ by those roundings between calls with other bounds; aihost_kv8_plan tells. With F32 q, q (of any size)
+ * and the weights enter as such pairs. */
 aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens,
                                    int32_t max_new, int32_t max_kv, const void* q, const int32_t* row_start,
                                    const int32_t* kv_len, const int32_t* block_table, const int8_t* k_pool,

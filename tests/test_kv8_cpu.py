@@ -88,3 +88,22 @@ def test_plain_page_map_by_hand():
     assert slots == [9 * 16 + 15, 7 * 16] + [4 * 16 + i for i in range(16)] + [1 * 16] + [-1]
     assert pos == [15, 16] + list(range(17)) + [0]
     assert page_map(16, 12, 4, 20, [15, 32, 0], [2, 0, 17], [3, 1], 2, [[9], [5], [0]])[-1]
+
+
+def test_plan_tells_scratch_and_kernel():
+    """Without a context, for the current device: the scratch of aihost_kv8_workspace_size, and the kernel by the step."""
+    need, kernel = ctypes.c_size_t(), ctypes.c_int32()
+    d = Kv8Spec(**BASE).desc()
+
+    def plan(*a):
+        assert A.lib().aihost_kv8_plan(None, ctypes.byref(d), *a, ctypes.byref(need), ctypes.byref(kernel)) == A.OK
+        assert need.value == _size(*a)[1]
+        return kernel.value
+
+    assert plan(64, 64, 1, 8192) == A.KV8_SPLIT_CACHE
+    assert plan(8, 64, 8, 8192) == A.KV8_SPLIT_CACHE
+    assert plan(1, 2048, 2048, 16384) == A.KV8_TENSOR
+    d.io_dtype = A.F32
+    assert A.lib().aihost_kv8_plan(None, ctypes.byref(d), 1, 2048, 2048, 16384, None, ctypes.byref(kernel)) == A.OK
+    assert kernel.value == A.KV8_SPLIT_CACHE
+    assert A.lib().aihost_kv8_plan(None, ctypes.byref(d), 0, 1, 1, 1, None, None) == A.EINVAL
