@@ -413,6 +413,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         s = s1;
         par = par1;
       }
+      // the last commit arrives in the block's shared memory, and nobody else waits for it
+      if (ok) warp_wait(&sh.v_empty[(n - 1) % C::NS], ((n - 1) / C::NS) & 1, status);
     } else if (warp == 1) {
       // ---------------------------------------------------------------- int8 rows, page by page
       // lane f copies the tile's f-th page (a page holds 16 to 128 of its 128 rows); its table entry is
