@@ -338,7 +338,9 @@ aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* 
   a.alibi_slopes = alibi_slopes;
   a.out = out;
   a.scale = r.scale;
-  a.score_cap = desc->score_cap;
+  // cap tanh(s / cap) in fp32 wants scale / cap and cap log2(e) to be normal numbers: beyond 1e30 it is s itself,
+  // below 1e-30 the scores are alike either way
+  a.score_cap = desc->score_cap > 1e30f || desc->score_cap == 0.0f ? 0.0f : std::max(desc->score_cap, 1e-30f);
   a.status = ctx->d_status;
   if (desc->rope_mode != AIHOST_ROPE_NONE) a.freqs = freqs_of(ctx, desc);
   const Plan plan = make_plan(desc, r.g, batch, n_tokens, max_new, max_kv, ctx->num_sms);

@@ -203,3 +203,13 @@ def test_keys_on_either_side_of_the_rule_for_small_pages(ctx, D, cap):
         order = np.argsort(w.ks[w.table[b][:-(-int(n) // 16)], 0])
         w.ks[w.table[b][:len(order)]] = w.ks[w.table[b][order]]  # small ones first
     _check(ctx, w, _q(w, lambda s: 1 + 0.3 * w.g.standard_normal(s)))
+
+
+@pytest.mark.parametrize("max_kv", BOUNDS)
+@pytest.mark.parametrize("io", [F16, F32])
+@pytest.mark.parametrize("cap", [3.4e38, 1e36, 1e29, 1e-29, 1e-36, 1e-42])
+@pytest.mark.parametrize("step", list(STEPS))
+def test_caps_of_any_size(ctx, step, cap, io, max_kv):
+    """The largest caps leave the scores as they are, the smallest make every visible row count alike."""
+    w = World(ctx, D=64, io=io, cap=cap, seed=53, **STEPS[step])
+    _check(ctx, w, _q(w, w.g.standard_normal), max_kv=max_kv)
