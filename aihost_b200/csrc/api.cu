@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <new>
 #include <utility>
 #include <vector>
 
@@ -538,7 +539,11 @@ aihost_status aihost_attn_reserve(aihost_attn_ctx* ctx, size_t bytes) {
   if (bytes <= ctx->scratch_bytes) return AIHOST_OK;
   DeviceGuard g(ctx->device);
   if (ctx->scratch_captured) {  // graphs go on using what they were captured with
-    ctx->outgrown.push_back(ctx->scratch);
+    try {
+      ctx->outgrown.push_back(ctx->scratch);
+    } catch (const std::bad_alloc&) {
+      return fail(AIHOST_ENOMEM, "out of host memory");
+    }
     ctx->scratch_captured = false;
   } else if (ctx->scratch) {
     cudaError_t e = cudaDeviceSynchronize();
