@@ -431,32 +431,43 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
       return fmaxf(fmaxf(s[0][nt][c], s[0][nt][c + 2]) + ve0, fmaxf(s[1][nt][c], s[1][nt][c + 2]) + ve1);
     };
     float far = 0.0f;  // the largest of the lane's scores, in units of the cap
+    // two columns at a time, in packed fp32
+    auto pairs = [&](auto f) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[u][nt][e] *= PREC == kPairQP ? kf[u] * q_unit[nt][e & 1] : kf[u];
-          if (MOD) far = fmaxf(far, fabsf(s[u][nt][e]));
-        }
+          for (int e = 0; e < 4; e += 2) {
+            const float2 x = f(make_float2(s[u][nt][e], s[u][nt][e + 1]), u, nt, e);
+            s[u][nt][e] = x.x, s[u][nt][e + 1] = x.y;
+          }
+    };
+    pairs([&](float2 x, int u, int nt, int) {
+      float2 f = make_float2(kf[u], kf[u]);
+      if (PREC == kPairQP) f = fmul2(f, make_float2(q_unit[nt][0], q_unit[nt][1]));
+      x = fmul2(x, f);
+      if (MOD) far = fmaxf(far, fmaxf(fabsf(x.x), fabsf(x.y)));
+      return x;
+    });
     if constexpr (MOD) {
-      auto each = [&](auto f) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[u][nt][e] = f(s[u][nt][e], u, nt, e);
-      };
       if (capped) {  // without exponentials where the warp has small ones only
-        if (__any_sync(0xffffffffu, far > kTanhSmall)) each([&](float x, int, int, int) { return cap2 * tanh_of(x); });
-        else each([&](float x, int, int, int) { return cap2 * tanh_small(x); });
+        if (__any_sync(0xffffffffu, far > kTanhSmall))
+          pairs([&](float2 x, int, int, int) { return make_float2(cap2 * tanh_of(x.x), cap2 * tanh_of(x.y)); });
+        else
+          pairs([&](float2 x, int, int, int) {
+            const float2 y = fmul2(x, x);
+            float2 p = ffma2(make_float2(kTanh3, kTanh3), y, make_float2(kTanh2, kTanh2));
+            p = ffma2(p, y, make_float2(kTanh1, kTanh1));
+            p = ffma2(p, y, make_float2(kTanh0, kTanh0));
+            return fmul2(fmul2(x, make_float2(cap2, cap2)), p);
+          });
       }
       if (a.alibi_slopes)
-        each([&](float x, int u, int nt, int e) {
-          const int32_t row = k + u * kSub + g + (e >> 1) * 8;
-          return x - c_slope[nt][e & 1] * fabsf(c_pos[nt][e & 1] - static_cast<float>(row));
+        pairs([&](float2 x, int u, int nt, int e) {
+          const float row = static_cast<float>(k + u * kSub + g + (e >> 1) * 8);
+          return make_float2(fmaf(-c_slope[nt][0], fabsf(c_pos[nt][0] - row), x.x),
+                             fmaf(-c_slope[nt][1], fabsf(c_pos[nt][1] - row), x.y));
         });
     }
     if (edge) {
@@ -502,10 +513,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 3 : 2) kv8_mma_kernel(c
       for (int nt = 0; nt < NT; ++nt) {
         float p[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          p[e] = ex2_approx(s[u][nt][e] - m[nt][e & 1]);
-          l[nt][e & 1] += p[e];
-          p[e] *= vf;
+        for (int e = 0; e < 4; e += 2) {
+          const float2 x = fadd2(make_float2(s[u][nt][e], s[u][nt][e + 1]), make_float2(-m[nt][0], -m[nt][1]));
+          const float2 v = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+          const float2 sum = fadd2(make_float2(l[nt][0], l[nt][1]), v), pv = fmul2(v, make_float2(vf, vf));
+          l[nt][0] = sum.x, l[nt][1] = sum.y;
+          p[e] = pv.x, p[e + 1] = pv.y;
         }
         if (edge) {  // a hidden row adds nothing even where its page's scale is NaN
 #pragma unroll
