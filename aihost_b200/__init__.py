@@ -60,6 +60,7 @@ class Kv8Desc(ctypes.Structure):
         ("io_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("scale", ctypes.c_float),
         ("score_cap", ctypes.c_float), ("rope_theta", ctypes.c_float), ("rope_mode", ctypes.c_int32),
         ("q_token_stride", ctypes.c_int64), ("kv_token_stride", ctypes.c_int64),
+        ("exact_q", ctypes.c_int32), ("reserved", ctypes.c_int32),
     ]
 
 

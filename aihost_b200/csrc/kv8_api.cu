@@ -57,6 +57,8 @@ aihost_status check_kv8(const aihost_kv8_desc* d, Resolved* r) {
   if (d->rope_mode != AIHOST_ROPE_NONE && !(d->rope_theta > 0.0f && isfinite(d->rope_theta)))
     return fail(AIHOST_EINVAL, "rope_theta must be a positive finite number");
   if (!(isfinite(d->scale) && d->scale >= 0.0f)) return fail(AIHOST_EINVAL, "scale must be >= 0 and finite");
+  if ((d->exact_q != 0 && d->exact_q != 1) || d->reserved != 0)
+    return fail(AIHOST_EINVAL, "exact_q (%d) must be 0 or 1, and reserved (%d) 0", d->exact_q, d->reserved);
   if (!(isfinite(d->score_cap) && d->score_cap >= 0.0f)) return fail(AIHOST_EINVAL, "score_cap must be >= 0 and finite");
   const int64_t eb = d->io_dtype == AIHOST_F32 ? 4 : 2;
   const int64_t q_row = eb * d->n_q_heads * d->head_dim, kv_row = eb * d->n_kv_heads * d->head_dim;
@@ -101,9 +103,14 @@ Plan make_plan(const aihost_kv8_desc* d, const Kv8Geom& g, int32_t batch, int32_
                int32_t max_kv, int32_t num_sms) {
   // The tcgen05 kernel takes fp16 rows by 256 and has ~12 us of fixed work a block; the split-cache one
   // takes 16 and rereads the cache for each tile, ~50 ns (head_dim 64: 37) per tile and 1000 rows over the
-  // whole GPU, and fills it with little work. Measured, head_dim 128, 32/8 heads, tcgen05 against split-cache:
-  // 8 sequences of 8192 rows with 8 new ones 85 and 69 us, with 16 85 and 116; one sequence with 32
-  // 42 and 41, with 64 45 and 66; 8 of 512 rows with 16 19 and 15, with 32 19 and 27.
+  // whole GPU, and fills it with little work. Measured, head_dim 128, 32/8 heads, tcgen05 against split-cache,
+  // q not rotated: 8 sequences of 8192 rows with 8 new ones 87 and 73 us, with 16 87 and 125; one sequence with
+  // 32 43 and 43, with 64 45 and 70; 8 of 512 rows with 16 21 and 15, with 32 21 and 28. A rotated q costs the
+  // split-cache kernel a quarter more, the other one 2 %: 89 and 93 us for the first of these.
+  // The rule knows the batch, not its sequences: it takes the cached rows to be spread as the new ones are. A
+  // step that mixes long prompts with single tokens over long caches runs on one kernel, and either is
+  // wrong for a part of it: 63 single tokens over 256 to 8192 rows beside a prompt of 2048 take 526 us so, 573
+  // on the tcgen05 kernel, and 115 + 58 as two calls.
   Plan p;
   max_kv = std::min(max_kv, kMaxKv);
   const int32_t rows = kv8_mma_rows(g, max_new), G = g.n_q_heads / g.n_kv_heads;
@@ -112,7 +119,8 @@ Plan make_plan(const aihost_kv8_desc* d, const Kv8Geom& g, int32_t batch, int32_
     double end;
     kv8_prefill_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.whole, &p.chunk, &p.splits, &end);
     const double even = static_cast<double>(n_tokens) / (static_cast<double>(batch) * max_new);
-    const double by_tc = end * (g.head_dim == 128 ? 2.1 : 1.7);
+    const bool pairs = d->exact_q && d->rope_mode != AIHOST_ROPE_NONE;
+    const double by_tc = end * (g.head_dim == 64 ? 1.7 : pairs ? 2.4 : 2.1);
     const double tiles16 = (static_cast<double>(n_tokens) * G / rows + 0.5 * batch) * g.n_kv_heads;
     const double by_mma = 8.0 + tiles16 * max_kv * (even > 0.9 ? 1.0 : even) * (g.head_dim == 128 ? 50e-6 : 37e-6);
     p.tensor = by_tc < by_mma;
@@ -324,6 +332,7 @@ aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* 
   a.q_dtype = desc->io_dtype;
   a.out_dtype = desc->out_dtype;
   a.rope_mode = desc->rope_mode;
+  a.exact_q = desc->exact_q;
   a.q_token_stride = r.q_stride;
   a.q = q;
   a.row_start = row_start;

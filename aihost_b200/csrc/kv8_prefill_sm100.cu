@@ -18,23 +18,26 @@
 //                grows by more than 2^8), exp2, row sum, P times V's factors as fp16.
 // Ranges are cut into chunks where there are few tiles; the last block of a tile to arrive merges.
 //
-// Precision: an unrotated fp16 q is exact. A rotated one is rounded to fp16; at head_dim 64 the fp16 of
-// what that leaves enters as a second operand, at head_dim 128 there is no shared memory for one (229 KB
-// are used), which costs 3.6e-4 against 2.9e-4 in relative root mean square error. Either is of one half of
-// the rotated q, since turning (x, y) may pass fp16's range; K's factors take it back. P is rounded to fp16
-// once, as the output is; maxima, sums and accumulators are fp32, int8 values exact.
+// Precision: an unrotated fp16 q is exact. A rotated one is rounded to fp16, and at head_dim 64 the fp16 of what
+// that leaves enters as a second operand. At head_dim 128 that costs 64 KB, which have to come from the
+// rings (one K and one V tile instead of two), and a third more products, so the caller chooses it
+// (exact_q): without it results are off by 3.6e-4 instead of 2.9e-4 (relative root mean square; an fp16 result
+// alone is by 2.1e-4). Either is of one half of the rotated q, since turning (x, y) may pass fp16's
+// range; K's factors take it back. P is rounded to fp16 once, as the output is; maxima, sums and
+// accumulators are fp32, int8 values exact. (P as a pair too: 690 us for the first case below; the rest of 128
+// weights a row costs the softmax what the products do not.)
 //
-// Measured: 2048 new rows over 14336 cached, 32/8 heads x 128, 497-507 us (515 GFLOP: 1030 TFLOP/s, 63 %
-// of the measured 1634; 545-557 us where calls follow one another for long, under the power cap). The MMAs of a
-// tile pair take 2048 cycles, the loop 3760: a tile's turn is its S and P V (1024) and its softmax (~2740
-// beside the other tile's), one after another; and the last 0.73 of a wave are chunks, each with a block's
-// fixed work. Two prompts of 4 K rows with documents, 162 us: of a block's ~40 K cycles about half are fixed
-// (lookup and ranges 5 K, Q 5 K, its rotation 4.6 K, first S 1.6 K, results 5 K). Six uneven prompts, 14/2
-// heads x 64, scores capped: 63.5 us.
-// Not better on the first of these: S in two halves of 64 keys (620 us), the next S read into registers
-// ahead (spills, 1330), two threads per query row (569), softmax as a loop over 32 columns that reads S
-// twice (564), a quarter of the exponentials by a polynomial on the FMA pipe (595), non-uniform
-// descriptors (790), set-up before the tile is known (553).
+// Measured: 2048 new rows over 14336 cached, 32/8 heads x 128, 495-506 us (515 GFLOP: 1030 TFLOP/s, 63 %
+// of the measured 1634; 544-550 us where calls follow one another for long, under the power cap), with exact_q
+// 560 (650). The MMAs of a tile pair take 2048 cycles, the loop 3760: a tile's turn is its S and P V (1024) and its
+// softmax (~2740 beside the other tile's), one after another; and the last 0.73 of a wave are chunks, each with a
+// block's fixed work. Two prompts of 4 K rows with documents, 163 us (exact_q 181): of a block's ~40 K cycles
+// about half are fixed (lookup and ranges 5 K, Q 5 K, its rotation 4.6 K, first S 1.6 K, results 5 K). Six
+// uneven prompts, 14/2 heads x 64, scores capped: 63.5 us.
+// Not better on the first of these: S in two halves of 64 keys (620 us), the next
+// S read into registers ahead (spills, 1330), two threads per query row (569), softmax as a loop over 32
+// columns that reads S twice (564), a quarter of the exponentials by a polynomial on the FMA pipe (595),
+// non-uniform descriptors (790), set-up before the tile is known (553).
 #include <algorithm>
 
 #include "common.cuh"
@@ -58,18 +61,18 @@ constexpr float kVUnit = 128.0f;  // P * (v scale / largest) * 128 <= 2^15 stays
 constexpr int kFactors = kKeys / 16;
 constexpr int kFactorRing = 4;
 
-template <int D>
+// REST: what a rotated q leaves when it is rounded to fp16 enters as a second operand (head_dim 64: always).
+template <int D, bool REST>
 struct Cfg {
   static constexpr int KB = D / 64;                   // 64-element (128-byte) column blocks
   static constexpr int TILE = KB * kKeys * 128;       // one [128 x D] fp16 tile
-  static constexpr int NS = D == 64 ? 3 : 2;          // K and V ring depth
+  static constexpr int NS = D == 64 ? 3 : REST ? 1 : 2;  // K and V ring depth
   static constexpr int K_OFF = 2 * TILE;              // after the two Q tiles
   static constexpr int V_OFF = K_OFF + NS * TILE;
   static constexpr int RAW = kKeys * D;               // one tile's int8 rows
   static constexpr int NR = D == 64 ? 4 : 2;          // ring of them, K and V in turn
   static constexpr int RAW_OFF = V_OFF + NS * TILE;
-  // head_dim 64 has room for what a rotated q leaves when it is rounded to fp16, as a second operand
-  static constexpr bool Q_REST = D == 64;
+  static constexpr bool Q_REST = D == 64 || REST;
   static constexpr int Q_REST_OFF = RAW_OFF + NR * RAW;
   static constexpr int BAR_OFF = Q_REST_OFF + (Q_REST ? 2 * TILE : 0);
   static constexpr int SMEM = BAR_OFF + 1024 + 1024;  // barriers and factors, alignment slack
@@ -217,9 +220,9 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
 }
 
-template <int D, bool MOD>
+template <int D, bool MOD, bool REST>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_constant__ Kv8AttnArgs a) {
-  using C = Cfg<D>;
+  using C = Cfg<D, REST>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Shared& sh = *reinterpret_cast<Shared*>(smem + C::BAR_OFF);
@@ -339,8 +342,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         }
         if (C::Q_REST && a.rope_mode != AIHOST_ROPE_NONE) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            mma_ss(tm + C::s_col(t), qd + (C::Q_REST_OFF + kk * 32) / 16, kd + kk * 2, idesc_qk, 1);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            constexpr int kBlock = kKeys * 128;
+            const uint32_t off = ((kk >> 2) * kBlock + (kk & 3) * 32) / 16;
+            mma_ss(tm + C::s_col(t), qd + C::Q_REST_OFF / 16 + off, kd + off, idesc_qk, 1);
+          }
         }
         commit_elected(&sh.s_full[t]);
         arrive_elected(&sh.s_full[t]);  // passes on what was written besides (the factors)
@@ -364,7 +370,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       for (int32_t i = 0; ok && i < n; ++i) {
         const int s1 = s + 1 == C::NS ? 0 : s + 1;
         const uint32_t par1 = s1 ? par : par ^ 1;
-        bool go = warp_wait(&sh.v_full[s], par, status) && (i + 1 >= n || warp_wait(&sh.k_full[s1], par1, status));
+        bool go = warp_wait(&sh.v_full[s], par, status);
+        // with one K tile at a time, the next one is made while the first P V runs
+        if (C::NS > 1) go = go && (i + 1 >= n || warp_wait(&sh.k_full[s1], par1, status));
         if (!go) break;
         tc_fence_after();
 #pragma unroll
@@ -380,10 +388,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             if (!go) break;
             if (i + 1 == t_hi) commit_elected(&sh.o_full[t]);
           }
+          if (C::NS == 1 && t == 1) commit_elected(&sh.v_empty[s]);
+          if (C::NS == 1 && t == 0 && i + 1 < n) {
+            go = warp_wait(&sh.k_full[s1], par1, status);
+            if (!go) break;
+            tc_fence_after();
+          }
           if (i + 1 >= t_lo && i + 1 < t_hi) issue_qk(t, s1);
         }
         if (!go) break;
-        commit_elected(&sh.v_empty[s]);
+        if (C::NS > 1) commit_elected(&sh.v_empty[s]);
         if (i + 1 < n) commit_elected(&sh.k_empty[s1]);
         s = s1;
         par = par1;
@@ -456,7 +470,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         e_next = entry_of(i + 2);
         const int s = i % C::NS;
         // the tile NS before is done with: so is the ring's slot, and k_full's phase is this tile's
-        if (!warp_wait(&sh.v_empty[s], ((i / C::NS) & 1) ^ 1, status)) break;
+        // (of one K tile at a time, the products: the next one's wait for these factors before the V tile is done with)
+        if (!warp_wait(C::NS > 1 ? &sh.v_empty[s] : &sh.k_empty[s], ((i / C::NS) & 1) ^ 1, status)) break;
         if (lane < kFactors) {
           // A scale that is no number marks the page through K's factor: a hidden row's weight is then 0
           // and its V factor must not turn it into NaN again.
@@ -491,11 +506,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     constexpr int NL = kKeys / (4 * RPL);  // loads per tile and lane
     const int r_in = D == 128 ? ((lane >> 2) & 1) + ((lane >> 4) << 1) : lane >> 2;
     const int c = D == 128 ? (lane & 3) + ((((lane >> 3) ^ (lane >> 2)) & 1) << 2) : lane & 3;
-    auto convert = [&](const uint8_t* src, uint8_t* dst, uint64_t* free_bar) {
-      uint4 v[NL];
+    uint4 v[NL];
+    auto take = [&](int slot) {  // a raw tile into registers, while the products still use the tile that it replaces
+      const uint8_t* const src = smem + C::RAW_OFF + slot * C::RAW;
 #pragma unroll
       for (int k = 0; k < NL; ++k)
         v[k] = *reinterpret_cast<const uint4*>(src + ((k * 4 + w) * RPL + r_in) * D + c * 16);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.raw_empty[slot]);
+    };
+    auto give = [&](uint8_t* dst, uint64_t* full_bar) {
 #pragma unroll
       for (int k = 0; k < NL; ++k) {
         const int row = (k * 4 + w) * RPL + r_in;
@@ -504,22 +524,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         *reinterpret_cast<uint4*>(dst + chunk_off(row, 2 * c)) = lo;
         *reinterpret_cast<uint4*>(dst + chunk_off(row, 2 * c + 1)) = hi;
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(free_bar);
       fence_proxy_async_smem();
+      mbar_arrive(full_bar);
     };
     for (int32_t i = 0; i < n_load; ++i) {
       const int s = i % C::NS;
       const uint32_t par = ((i / C::NS) & 1) ^ 1;
       const int gk = 2 * i, gv = 2 * i + 1;
       if (!warp_wait(&sh.raw_full[gk % C::NR], (gk / C::NR) & 1, status)) break;
+      take(gk % C::NR);
       if (!warp_wait(&sh.k_empty[s], par, status)) break;
-      convert(smem + C::RAW_OFF + (gk % C::NR) * C::RAW, smem + C::K_OFF + s * C::TILE, &sh.raw_empty[gk % C::NR]);
-      mbar_arrive(&sh.k_full[s]);
+      give(smem + C::K_OFF + s * C::TILE, &sh.k_full[s]);
       if (!warp_wait(&sh.raw_full[gv % C::NR], (gv / C::NR) & 1, status)) break;
+      take(gv % C::NR);
       if (!warp_wait(&sh.v_empty[s], par, status)) break;
-      convert(smem + C::RAW_OFF + (gv % C::NR) * C::RAW, smem + C::V_OFF + s * C::TILE, &sh.raw_empty[gv % C::NR]);
-      mbar_arrive(&sh.v_full[s]);
+      give(smem + C::V_OFF + s * C::TILE, &sh.v_full[s]);
     }
     if (stray) atomicOr(status, kStatusBadIndex);
   } else {
@@ -535,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     row_range(a, tl, G, n_rows, rr, first, end, pos);
     if (!valid) first = 0, end = INT32_MAX;  // such a row works for nobody and never asks for masks
     const int32_t row = tl.row0 + min(rr, n_rows - 1), tok = row / G, head = h * G + row % G;
-    // ---- the warp's 32 rows of Q, rotated in fp32 and rounded once: LPR lanes to a row, each with 16-byte
+    // ---- the warp's 32 rows of Q, rotated in fp32, as fp16 (and its rest): LPR lanes to a row, each with 16-byte
     // chunks c and c + LPR (a half apart), and LPR rows to a lane, one after another, so that the heads of
     // one token share its sines and cosines
     uint8_t* const q_tile = smem + t * C::TILE;
@@ -565,8 +584,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       // rotated in place, by a loop that is not unrolled: it runs once per block, from a cold instruction cache
       if (a.rope_mode != AIHOST_ROPE_NONE) {
         const bool halves = a.rope_mode == AIHOST_ROPE_NEOX;
-        auto rotation = [](float angle, float* s, float* c) {  // as exact as what is kept of the products
-          if constexpr (C::Q_REST) sincos_near(angle, s, c);
+        // 2^-21 off at head_dim 128 (with sincos_near 193 us for the documents with exact_q, so 183)
+        auto rotation = [](float angle, float* s, float* c) {
+          if constexpr (D == 64) sincos_near(angle, s, c);
           else sincos_reduced(angle, s, c);
         };
         float sn[8], cs[8];  // by halves: of pairs 8 c + e; else of pairs 4 c + e and 4 (c + LPR) + e - 4
@@ -846,14 +866,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
   }
 }
 
-template <int D, bool MOD>
+template <int D, bool MOD, bool REST>
 cudaError_t launch_d(const Kv8AttnArgs& a, cudaStream_t st) {
-  auto kern = kv8_prefill_kernel<D, MOD>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+  auto kern = kv8_prefill_kernel<D, MOD, REST>;
+  constexpr int kBytes = Cfg<D, REST>::SMEM;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
   if (e != cudaSuccess) return e;
   // not a dependent launch: waiting blocks would take whole SMs, 6 % slower on batches of short prompts
   const int64_t blocks = a.whole + (static_cast<int64_t>(a.tiles) * a.g.n_kv_heads - a.whole) * a.max_splits;
-  kern<<<static_cast<unsigned>(blocks), kThreads, Cfg<D>::SMEM, st>>>(a);
+  kern<<<static_cast<unsigned>(blocks), kThreads, kBytes, st>>>(a);
   return cudaGetLastError();
 }
 
@@ -918,8 +939,10 @@ int32_t kv8_prefill_rows() { return kRows; }
 
 cudaError_t launch_kv8_prefill(const Kv8AttnArgs& a, cudaStream_t st) {
   const bool mod = a.score_cap > 0.0f || a.alibi_slopes;
-  if (a.g.head_dim == 64) return mod ? launch_d<64, true>(a, st) : launch_d<64, false>(a, st);
-  return mod ? launch_d<128, true>(a, st) : launch_d<128, false>(a, st);
+  if (a.g.head_dim == 64) return mod ? launch_d<64, true, true>(a, st) : launch_d<64, false, true>(a, st);
+  if (a.exact_q && a.rope_mode != AIHOST_ROPE_NONE)
+    return mod ? launch_d<128, true, true>(a, st) : launch_d<128, false, true>(a, st);
+  return mod ? launch_d<128, true, false>(a, st) : launch_d<128, false, false>(a, st);
 }
 
 }  // namespace aihost

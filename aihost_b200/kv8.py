@@ -48,10 +48,11 @@ class Kv8Spec:
     score_cap: float = 0.0
     rope_theta: float = 10000.0
     rope_mode: int = ROPE_INTERLEAVED
+    exact_q: bool = False  # a rotated float16 q keeps 22 bits in prompts of head_dim 128 too (slower)
 
     def desc(self) -> Kv8Desc:
         return Kv8Desc(self.n_q_heads, self.n_kv_heads, self.head_dim, self.page_rows, self.n_pages, self.max_pages,
-                       self.io_dtype, self.out_dtype, self.scale, self.score_cap, self.rope_theta, self.rope_mode, 0, 0)
+                       self.io_dtype, self.out_dtype, self.scale, self.score_cap, self.rope_theta, self.rope_mode, 0, 0, int(self.exact_q), 0)
 
 
 class StepMap(NamedTuple):

@@ -342,6 +342,8 @@ typedef struct {
   int32_t rope_mode;
   int64_t q_token_stride;        /* bytes between tokens of q;            0 -> n_q_heads rows, packed */
   int64_t kv_token_stride;       /* bytes between tokens of k_new, v_new; 0 -> n_kv_heads rows, packed */
+  int32_t exact_q;               /* what a rotated F16 q keeps, see aihost_kv8_attention: 0 or 1 */
+  int32_t reserved;              /* 0 */
 } aihost_kv8_desc;
 
 /* One step's page bookkeeping in one launch: sequence b has seq_len[b] cached rows and gets
@@ -406,10 +408,11 @@ aihost_status aihost_kv8_plan(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc,
  * bounds are not computed, and their rows of out are left as they are.
  * Softmax state and sums are fp32; int8 values enter the products exactly. With F16 q, the softmax weights
  * enter as fp16; q enters exactly where it is not rotated, else as a pair of fp16 whose sum holds 22 bits (down
- * to fp16's smallest step), but in the AIHOST_KV8_TENSOR kernel with head_dim 128, where it is rounded to fp16
- * once. Which kernel runs goes by head counts, batch, n_tokens, max_new and max_kv, so the same row may
- * differ by those roundings between calls with other bounds; aihost_kv8_plan tells. With F32 q, q (of any size)
- * and the weights enter as such pairs. */
+ * to fp16's smallest step), but with exact_q 0 in the AIHOST_KV8_TENSOR kernel with head_dim 128, where it is
+ * rounded to fp16 once (results off by 3.6e-4 instead of 2.9e-4 in relative root mean square, long
+ * prompts a sixth faster). Which kernel runs goes by head counts, batch, n_tokens, max_new and max_kv
+ * (aihost_kv8_plan tells), so the same row may differ by those roundings and by the order of its sums between
+ * calls with other bounds. With F32 q, q (of any size) and the weights enter as such pairs. */
 aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens,
                                    int32_t max_new, int32_t max_kv, const void* q, const int32_t* row_start,
                                    const int32_t* kv_len, const int32_t* block_table, const int8_t* k_pool,

@@ -1,11 +1,15 @@
-"""Which kernel the 8-bit cache's attention runs, and that rotated queries keep what the header says of it: 22 bits, but for the
-tcgen05 kernel with head_dim 128, which rounds them to fp16."""
+"""Which kernel the 8-bit cache's attention runs, and that rotated queries keep what the header promises: 22 bits, but for the
+tcgen05 kernel with head_dim 128 and exact_q 0, which rounds them to fp16."""
+import dataclasses
+
 import numpy as np
 import pytest
+import torch
 
 import kv8_plain as plain
 from aihost_b200 import F16, F32, KV8_SPLIT_CACHE, KV8_TENSOR, ROPE_INTERLEAVED, ROPE_NEOX, ROPE_NONE
-from test_gpu_kv8 import ATTENDS, BOUNDS, World
+from aihost_b200.kv8 import Kv8Ops
+from test_gpu_kv8 import ATTENDS, BOUNDS, DEV, World
 from test_gpu_kv8_range import _check, _q
 
 pytestmark = pytest.mark.gpu
@@ -49,13 +53,14 @@ def _pair_size(w, q):
 @pytest.mark.parametrize("mode", [ROPE_INTERLEAVED, ROPE_NEOX])
 @pytest.mark.parametrize("cached, new, G", [([300, 1029], [1, 1], 4), ([333], [1], 16), ([300, 77], [3, 2], 4),
                                             ([90, 0, 17], [60, 130, 1], 4), ([1500], [40], 7)])
-@pytest.mark.parametrize("D, P", [(64, 16), (128, 64)])
-def test_rotated_queries_keep_their_bits(ctx, D, P, cached, new, G, mode, max_kv):
+@pytest.mark.parametrize("D, P, exact", [(64, 16, False), (128, 64, False), (128, 64, True), (128, 16, True)])
+def test_rotated_queries_keep_their_bits(ctx, D, P, exact, cached, new, G, mode, max_kv):
     w = World(ctx, cached, new, Hq=2 * G, H=2, D=D, P=P, mode=mode, seed=61, theta=5e5, scale=1.5)
-    kernel = _kernel(w, max_kv)
+    w.spec = dataclasses.replace(w.spec, exact_q=exact)
+    w.ops = Kv8Ops(ctx, w.spec)
     assert {_kernel(w, b) for b in BOUNDS} == _wanted(w)
     q = _q(w, lambda s: 0.5 + w.g.standard_normal(s))
-    if kernel == KV8_TENSOR and D == 128:
+    if _kernel(w, max_kv) == KV8_TENSOR and D == 128 and not exact:
         _check(ctx, w, q, out_dtype=F32, max_kv=max_kv, ds=2.0 ** -11)
         return
     size = _pair_size(w, q)
@@ -75,3 +80,32 @@ def test_the_bounds_choose_the_kernel(ctx, case, io):
     """What the two bounds of the attention tests are for."""
     w = World(ctx, io=io, **ATTENDS[case])
     assert {_kernel(w, b) for b in BOUNDS} == _wanted(w)
+
+
+@pytest.mark.parametrize("what", ["cap", "bias", "documents", "chunks", "one row"])
+@pytest.mark.parametrize("mode", [ROPE_INTERLEAVED, ROPE_NEOX])
+def test_exact_queries_over_one_tile_at_a_time(ctx, mode, what):
+    """exact_q at head_dim 128: longer ranges than the rings hold, uneven ones, gaps between two query tiles' documents, and
+    ranges cut into chunks."""
+    cached, new = {"chunks": ([3300, 100], [90, 40]), "one row": ([700, 5], [1, 300])}.get(what, ([700, 0, 40], [300, 129, 17]))
+    w = World(ctx, cached, new, Hq=8, H=1, D=128, P=32, mode=mode, cap=6.0 if what == "cap" else 0.0, seed=62)
+    w.spec = dataclasses.replace(w.spec, exact_q=True)
+    w.ops = Kv8Ops(ctx, w.spec)
+    first = slopes = None
+    if what == "bias":
+        slopes = [2.0 ** -(h + 1) for h in range(8)]
+    if what == "documents":  # rows 0..15 of a sequence look back to its start, the later ones to their own neighbours
+        first = [0 if i < 16 else max(0, int(p) - 20) for n, c in zip(new, cached) for i, p in enumerate(range(c, c + n))]
+    most = 40000  # far enough for the tcgen05 kernel, in chunks
+    assert _kernel(w, most) == KV8_TENSOR
+    q, q64 = w.rows(w.Hq)
+    out = w.attend(q.to(DEV), max_kv=most, first=first, slopes=slopes)
+    again = w.attend(q.to(DEV), max_kv=most, first=first, slopes=slopes)
+    torch.cuda.synchronize()
+    ctx.sync_status()
+    assert torch.equal(out, again)
+    ref, weight, _ = plain.attend(q64, w.start, w.kv_len, w.table, w.P, w.k, w.v, w.ks, w.vs, w.scale, w.cap, w.theta, mode,
+                                  first=first, slopes=None if slopes is None else np.float32(slopes))
+    ds = 2.0 ** -19 * _pair_size(w, q64)[..., None]
+    tol = 2.0 ** -11 * np.abs(ref) + weight * (2.0 ** -11 + 2.0 ** -16 + 2 * ds) + 1e-7
+    assert (np.abs(out.double().cpu().numpy() - ref) - tol).max() <= 0

@@ -107,3 +107,16 @@ def test_plan_tells_scratch_and_kernel():
     assert A.lib().aihost_kv8_plan(None, ctypes.byref(d), 1, 2048, 2048, 16384, None, ctypes.byref(kernel)) == A.OK
     assert kernel.value == A.KV8_SPLIT_CACHE
     assert A.lib().aihost_kv8_plan(None, ctypes.byref(d), 0, 1, 1, 1, None, None) == A.EINVAL
+
+
+@pytest.mark.parametrize("field, value", [("exact_q", 2), ("exact_q", -1), ("reserved", 1)])
+def test_exact_q_is_a_truth_value(field, value):
+    d = Kv8Spec(**BASE).desc()
+    setattr(d, field, value)
+    need = ctypes.c_size_t()
+    assert A.lib().aihost_kv8_workspace_size(ctypes.byref(d), 1, 1, 1, 64, ctypes.byref(need)) == A.EINVAL
+    assert b"exact_q" in A.lib().aihost_attn_last_error()
+
+
+def test_exact_q_is_passed_on():
+    assert Kv8Spec(**BASE).desc().exact_q == 0 and Kv8Spec(**BASE, exact_q=True).desc().exact_q == 1
