@@ -36,6 +36,7 @@ EXPORTS = (
 # aihost_kernel ids of the device-time profiler
 KERNEL_APPEND, KERNEL_DECODE, KERNEL_COMBINE, KERNEL_PREFILL, KERNEL_CONVERT, KERNEL_MATMUL = range(6)
 KERNEL_PAGES, KERNEL_KV8_APPEND, KERNEL_KV8_ATTN = range(6, 9)
+KV8_EXACT_Q = 0x100  # or'ed into Kv8Desc.rope_mode
 KV8_SPLIT_CACHE, KV8_TENSOR = range(2)  # aihost_kv8_kernel: which one an attention call over the 8-bit cache runs
 
 
@@ -60,7 +61,6 @@ class Kv8Desc(ctypes.Structure):
         ("io_dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32), ("scale", ctypes.c_float),
         ("score_cap", ctypes.c_float), ("rope_theta", ctypes.c_float), ("rope_mode", ctypes.c_int32),
         ("q_token_stride", ctypes.c_int64), ("kv_token_stride", ctypes.c_int64),
-        ("exact_q", ctypes.c_int32), ("reserved", ctypes.c_int32),
     ]
 
 

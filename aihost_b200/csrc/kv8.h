@@ -74,7 +74,8 @@ struct Kv8ReadArgs {
 struct Kv8AttnArgs {
   Kv8Geom g;
   int32_t batch, n_tokens, max_new, max_kv;
-  int32_t q_dtype, out_dtype, rope_mode, exact_q;
+  int32_t q_dtype, out_dtype, rope_mode;
+  bool exact_q;  // rotated, and not to be rounded to fp16
   int64_t q_token_stride;  // bytes
   const void* q;
   const int32_t* row_start;

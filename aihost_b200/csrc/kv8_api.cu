@@ -31,6 +31,8 @@ const RopeFreqs& freqs_of(aihost_attn_ctx* ctx, const aihost_kv8_desc* d) {
 
 struct Resolved {
   Kv8Geom g;
+  int32_t rope_mode;
+  bool exact_q;  // rotated, and not to be rounded to fp16
   float scale;
   int64_t q_stride, kv_stride;  // bytes between tokens
 };
@@ -52,13 +54,13 @@ aihost_status check_kv8(const aihost_kv8_desc* d, Resolved* r) {
     return fail(AIHOST_EINVAL, "io_dtype %d must be F32 (0) or F16 (1)", d->io_dtype);
   if (d->out_dtype != AIHOST_F32 && d->out_dtype != AIHOST_F16)
     return fail(AIHOST_EINVAL, "out_dtype %d must be F32 (0) or F16 (1)", d->out_dtype);
-  if (d->rope_mode < AIHOST_ROPE_INTERLEAVED || d->rope_mode > AIHOST_ROPE_NONE)
+  r->rope_mode = d->rope_mode & ~AIHOST_KV8_EXACT_Q;
+  if (r->rope_mode < AIHOST_ROPE_INTERLEAVED || r->rope_mode > AIHOST_ROPE_NONE)
     return fail(AIHOST_EINVAL, "rope_mode %d is not a valid aihost_rope_mode", d->rope_mode);
-  if (d->rope_mode != AIHOST_ROPE_NONE && !(d->rope_theta > 0.0f && isfinite(d->rope_theta)))
+  r->exact_q = d->rope_mode != r->rope_mode && r->rope_mode != AIHOST_ROPE_NONE;
+  if (r->rope_mode != AIHOST_ROPE_NONE && !(d->rope_theta > 0.0f && isfinite(d->rope_theta)))
     return fail(AIHOST_EINVAL, "rope_theta must be a positive finite number");
   if (!(isfinite(d->scale) && d->scale >= 0.0f)) return fail(AIHOST_EINVAL, "scale must be >= 0 and finite");
-  if ((d->exact_q != 0 && d->exact_q != 1) || d->reserved != 0)
-    return fail(AIHOST_EINVAL, "exact_q (%d) must be 0 or 1, and reserved (%d) 0", d->exact_q, d->reserved);
   if (!(isfinite(d->score_cap) && d->score_cap >= 0.0f)) return fail(AIHOST_EINVAL, "score_cap must be >= 0 and finite");
   const int64_t eb = d->io_dtype == AIHOST_F32 ? 4 : 2;
   const int64_t q_row = eb * d->n_q_heads * d->head_dim, kv_row = eb * d->n_kv_heads * d->head_dim;
@@ -99,7 +101,7 @@ struct Plan {
   }
 };
 
-Plan make_plan(const aihost_kv8_desc* d, const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max_new,
+Plan make_plan(const aihost_kv8_desc* d, const Resolved& r, int32_t batch, int32_t n_tokens, int32_t max_new,
                int32_t max_kv, int32_t num_sms) {
   // The tcgen05 kernel takes fp16 rows by 256 and has ~12 us of fixed work a block; the split-cache one
   // takes 16 and rereads the cache for each tile, ~50 ns (head_dim 64: 37) per tile and 1000 rows over the
@@ -112,6 +114,7 @@ Plan make_plan(const aihost_kv8_desc* d, const Kv8Geom& g, int32_t batch, int32_
   // wrong for a part of it: 63 single tokens over 256 to 8192 rows beside a prompt of 2048 take 526 us so, 573
   // on the tcgen05 kernel, and 115 + 58 as two calls.
   Plan p;
+  const Kv8Geom& g = r.g;
   max_kv = std::min(max_kv, kMaxKv);
   const int32_t rows = kv8_mma_rows(g, max_new), G = g.n_q_heads / g.n_kv_heads;
   p.tensor = false;
@@ -119,8 +122,7 @@ Plan make_plan(const aihost_kv8_desc* d, const Kv8Geom& g, int32_t batch, int32_
     double end;
     kv8_prefill_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.whole, &p.chunk, &p.splits, &end);
     const double even = static_cast<double>(n_tokens) / (static_cast<double>(batch) * max_new);
-    const bool pairs = d->exact_q && d->rope_mode != AIHOST_ROPE_NONE;
-    const double by_tc = end * (g.head_dim == 64 ? 1.7 : pairs ? 2.4 : 2.1);
+    const double by_tc = end * (g.head_dim == 64 ? 1.7 : r.exact_q ? 2.4 : 2.1);
     const double tiles16 = (static_cast<double>(n_tokens) * G / rows + 0.5 * batch) * g.n_kv_heads;
     const double by_mma = 8.0 + tiles16 * max_kv * (even > 0.9 ? 1.0 : even) * (g.head_dim == 128 ? 50e-6 : 37e-6);
     p.tensor = by_tc < by_mma;
@@ -232,7 +234,7 @@ aihost_status aihost_kv8_append(aihost_attn_ctx* ctx, const aihost_kv8_desc* des
   if (n_tokens < 0) return fail(AIHOST_EINVAL, "n_tokens (%d) must be >= 0", n_tokens);
   if (n_tokens == 0) return AIHOST_OK;
   if (!k_new || !v_new || !slots || !k_pool || !v_pool || !k_scale || !v_scale ||
-      (!positions && desc->rope_mode != AIHOST_ROPE_NONE))
+      (!positions && r.rope_mode != AIHOST_ROPE_NONE))
     return fail(AIHOST_EINVAL, "every array must be non-NULL (positions may be NULL with rope_mode NONE)");
   if (!aligned(k_new, 16) || !aligned(v_new, 16) || !aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(slots, 8) ||
       !aligned(positions, 4) || !aligned(k_scale, 4) || !aligned(v_scale, 4))
@@ -243,7 +245,7 @@ aihost_status aihost_kv8_append(aihost_attn_ctx* ctx, const aihost_kv8_desc* des
   a.g = r.g;
   a.n_tokens = n_tokens;
   a.io_dtype = desc->io_dtype;
-  a.rope_mode = desc->rope_mode;
+  a.rope_mode = r.rope_mode;
   a.token_stride = r.kv_stride;
   a.k_new = k_new;
   a.v_new = v_new;
@@ -254,7 +256,7 @@ aihost_status aihost_kv8_append(aihost_attn_ctx* ctx, const aihost_kv8_desc* des
   a.k_scale = k_scale;
   a.v_scale = v_scale;
   a.status = ctx->d_status;
-  if (desc->rope_mode != AIHOST_ROPE_NONE) a.freqs = freqs_of(ctx, desc);
+  if (r.rope_mode != AIHOST_ROPE_NONE) a.freqs = freqs_of(ctx, desc);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = timed_launch(ctx, AIHOST_KERNEL_KV8_APPEND, st, [&] { return launch_kv8_append(a, st); });
   return e == cudaSuccess ? AIHOST_OK : cuda_fail(e, "8-bit append launch");
@@ -288,7 +290,7 @@ aihost_status aihost_kv8_workspace_size(const aihost_kv8_desc* desc, int32_t bat
   aihost_status s = check_kv8(desc, &r);
   if (s == AIHOST_OK) s = check_sizes(batch, n_tokens, max_new, max_kv);
   if (s != AIHOST_OK) return s;
-  *out_bytes = make_plan(desc, r.g, batch, n_tokens, max_new, max_kv, current_sms()).scratch(r.g);
+  *out_bytes = make_plan(desc, r, batch, n_tokens, max_new, max_kv, current_sms()).scratch(r.g);
   return AIHOST_OK;
 }
 
@@ -298,7 +300,7 @@ aihost_status aihost_kv8_plan(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc,
   aihost_status s = check_kv8(desc, &r);
   if (s == AIHOST_OK) s = check_sizes(batch, n_tokens, max_new, max_kv);
   if (s != AIHOST_OK) return s;
-  const Plan plan = make_plan(desc, r.g, batch, n_tokens, max_new, max_kv, ctx ? ctx->num_sms : current_sms());
+  const Plan plan = make_plan(desc, r, batch, n_tokens, max_new, max_kv, ctx ? ctx->num_sms : current_sms());
   if (out_bytes) *out_bytes = plan.scratch(r.g);
   if (out_kernel) *out_kernel = plan.tensor ? AIHOST_KV8_TENSOR : AIHOST_KV8_SPLIT_CACHE;
   return AIHOST_OK;
@@ -331,8 +333,8 @@ aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* 
   a.max_kv = std::min(max_kv, kMaxKv);
   a.q_dtype = desc->io_dtype;
   a.out_dtype = desc->out_dtype;
-  a.rope_mode = desc->rope_mode;
-  a.exact_q = desc->exact_q;
+  a.rope_mode = r.rope_mode;
+  a.exact_q = r.exact_q;
   a.q_token_stride = r.q_stride;
   a.q = q;
   a.row_start = row_start;
@@ -351,8 +353,8 @@ aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* 
   // below 1e-30 the scores are alike either way
   a.score_cap = desc->score_cap > 1e30f || desc->score_cap == 0.0f ? 0.0f : std::max(desc->score_cap, 1e-30f);
   a.status = ctx->d_status;
-  if (desc->rope_mode != AIHOST_ROPE_NONE) a.freqs = freqs_of(ctx, desc);
-  const Plan plan = make_plan(desc, r.g, batch, n_tokens, max_new, max_kv, ctx->num_sms);
+  if (r.rope_mode != AIHOST_ROPE_NONE) a.freqs = freqs_of(ctx, desc);
+  const Plan plan = make_plan(desc, r, batch, n_tokens, max_new, max_kv, ctx->num_sms);
   a.tiles = plan.tiles;
   a.chunk = plan.chunk;
   a.max_splits = plan.splits;

@@ -21,7 +21,7 @@
 // Precision: an unrotated fp16 q is exact. A rotated one is rounded to fp16, and at head_dim 64 the fp16 of what
 // that leaves enters as a second operand. At head_dim 128 that costs 64 KB, which have to come from the
 // rings (one K and one V tile instead of two), and a third more products, so the caller chooses it
-// (exact_q): without it results are off by 3.6e-4 instead of 2.9e-4 (relative root mean square; an fp16 result
+// (AIHOST_KV8_EXACT_Q): without it results are off by 3.6e-4 instead of 2.9e-4 (relative root mean square; an fp16 result
 // alone is by 2.1e-4). Either is of one half of the rotated q, since turning (x, y) may pass fp16's
 // range; K's factors take it back. P is rounded to fp16 once, as the output is; maxima, sums and
 // accumulators are fp32, int8 values exact. (P as a pair too: 690 us for the first case below; the rest of 128
@@ -940,8 +940,7 @@ int32_t kv8_prefill_rows() { return kRows; }
 cudaError_t launch_kv8_prefill(const Kv8AttnArgs& a, cudaStream_t st) {
   const bool mod = a.score_cap > 0.0f || a.alibi_slopes;
   if (a.g.head_dim == 64) return mod ? launch_d<64, true, true>(a, st) : launch_d<64, false, true>(a, st);
-  if (a.exact_q && a.rope_mode != AIHOST_ROPE_NONE)
-    return mod ? launch_d<128, true, true>(a, st) : launch_d<128, false, true>(a, st);
+  if (a.exact_q) return mod ? launch_d<128, true, true>(a, st) : launch_d<128, false, true>(a, st);
   return mod ? launch_d<128, true, false>(a, st) : launch_d<128, false, false>(a, st);
 }
 

@@ -22,7 +22,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import EINVAL, F16, F32, ROPE_INTERLEAVED, AttnError, Kv8Desc, check, lib
+from . import EINVAL, F16, F32, KV8_EXACT_Q, ROPE_INTERLEAVED, AttnError, Kv8Desc, check, lib
 from .ops import Context
 
 lib()  # the module below calls the same library
@@ -52,7 +52,7 @@ class Kv8Spec:
 
     def desc(self) -> Kv8Desc:
         return Kv8Desc(self.n_q_heads, self.n_kv_heads, self.head_dim, self.page_rows, self.n_pages, self.max_pages,
-                       self.io_dtype, self.out_dtype, self.scale, self.score_cap, self.rope_theta, self.rope_mode, 0, 0, int(self.exact_q), 0)
+                       self.io_dtype, self.out_dtype, self.scale, self.score_cap, self.rope_theta, self.rope_mode | (KV8_EXACT_Q if self.exact_q else 0), 0, 0)
 
 
 class StepMap(NamedTuple):

@@ -109,14 +109,11 @@ def test_plan_tells_scratch_and_kernel():
     assert A.lib().aihost_kv8_plan(None, ctypes.byref(d), 0, 1, 1, 1, None, None) == A.EINVAL
 
 
-@pytest.mark.parametrize("field, value", [("exact_q", 2), ("exact_q", -1), ("reserved", 1)])
-def test_exact_q_is_a_truth_value(field, value):
-    d = Kv8Spec(**BASE).desc()
-    setattr(d, field, value)
+@pytest.mark.parametrize("mode, ok", [(A.ROPE_NONE, True), (A.ROPE_NEOX, True), (3, False), (-1, False), (0x200, False)])
+def test_exact_q_goes_with_every_rope_mode(mode, ok):
+    d = Kv8Spec(**BASE, rope_mode=mode, exact_q=True).desc()
+    assert d.rope_mode == mode | A.KV8_EXACT_Q
     need = ctypes.c_size_t()
-    assert A.lib().aihost_kv8_workspace_size(ctypes.byref(d), 1, 1, 1, 64, ctypes.byref(need)) == A.EINVAL
-    assert b"exact_q" in A.lib().aihost_attn_last_error()
-
-
-def test_exact_q_is_passed_on():
-    assert Kv8Spec(**BASE).desc().exact_q == 0 and Kv8Spec(**BASE, exact_q=True).desc().exact_q == 1
+    got = A.lib().aihost_kv8_workspace_size(ctypes.byref(d), 1, 1, 1, 64, ctypes.byref(need))
+    assert got == (A.OK if ok else A.EINVAL)
+    assert Kv8Spec(**BASE, rope_mode=mode).desc().rope_mode == mode
