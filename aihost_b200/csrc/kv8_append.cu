@@ -8,11 +8,14 @@
 // The work unit is a run: the consecutive tokens whose slots are consecutive rows of one page. A run is
 // read once and kept in registers while its maximum comes together, so 2 (fp16) or 4 bytes a value come
 // in and 1 goes out.
-// Measured with the two reads of what was written, 8 heads x 128: 64 one-token sequences 12.3 us, nearly
-// all of it the host's enqueue of three calls (kernels 5 + 2 x 2.8 us). 6.7 K prompt rows of 4 sequences
-// 41.6 us, of which the append 27 (41 MB in and out: 1.5 TB/s where a copy reaches 6.55) and the reads 7
-// each: the instructions of conversion, rotation, maximum, scaling, rounding and packing bound it before
-// the bytes do. (One pass over memory for the maximum and another for the rounding: 70 us for the three
+// Measured with the two reads of what was written, 8 heads x 128: 64 one-token sequences 12.3 us; the three
+// dependent kernels take 11.7 in a graph (5 + 2 x 2.8 us and their hand-over), the host's enqueue as long.
+// 6.7 K prompt rows of 4 sequences 41.6 us, of which the append 27 (41 MB in and out: 1.5 TB/s where a copy
+// reaches 6.55) and the reads 7 each (21 MB: 45 % of a copy's rate; one load in flight a thread, whose
+// neighbours store 32 bytes apart). The append issues about 140 warp instructions per row and head
+// (conversion, rotation, maximum, scaling, rounding, packing; a token's sine and cosine anew for every two
+// heads) in 53 % of the issue slots: a run's load, its maximum across the warps and its store follow one
+// another. (One pass over memory for the maximum and another for the rounding: 70 us for the three
 // calls.)
 #include "common.cuh"
 #include "kv8.h"

@@ -6,7 +6,8 @@
 // mma.sync m16n8k16 and query rows its N = 8:
 //   S^T = K Q^T     K's int8 go to fp16 in registers, one fp32 factor per page afterwards
 //   online softmax  running maximum per query row, moved only when it grows by more than 2^8
-//   O^T += V^T P^T  V likewise exact; P carries the page's scale relative to the chunk's largest
+//   O^T += V^T P^T  V likewise exact; P carries the page's scale relative to the chunk's largest, which
+//                   the running maximum counts in
 // The k order of either product is free, so it is chosen such that every lane takes 16 bytes of a
 // cache row at a time and no transpose is needed. Each warp copies its own steps' rows into a ring of
 // its own in shared memory (cp.async, a step ahead, chunks swizzled against bank conflicts): no warp
@@ -16,10 +17,10 @@
 //
 // A cache value is used by R query rows, 2 R products a byte, far below what the tensor cores need:
 // the bytes bound it, and mma.sync from registers is enough. Measured, head_dim 128, 8 KV heads: 64
-// sequences of 256 to 8192 rows 104 us (599 MB, 5.7 TB/s, 88 % of a copy's measured 6.55), 32 of 16384
-// with 64 query heads and capped scores 175 us (1.07 GB, 6.1 TB/s, 94 %). One sequence of 513 rows
-// takes 6.6 us in a graph, 7.4 called one at a time: table entry, scales, rows, partial, counter and
-// merge are dependent trips to L2. Not better: three stages of the ring with two blocks an SM instead
+// sequences of 256 to 8192 rows 105 us (599 MB, 5.7 TB/s, 87 % of a copy's measured 6.55), 32 of 16384
+// with 64 query heads and capped scores 177 us (1.07 GB, 6.1 TB/s, 93 %); under sustained load 112 and
+// 197. One sequence of 513 rows takes 6.9 us in a graph, 7.2 to 7.6 called one at a time: table entry, scales,
+// rows, partial, counter and merge are dependent trips to L2. Not better: three stages of the ring with two blocks an SM instead
 // of two with three (197 against 177 us for the 32 x 16384), rows loaded straight into registers (135
 // against 127 for the 64), 16-row steps (127 against 113), prefetch hints on the copies (no change).
 #include <type_traits>
