@@ -113,7 +113,8 @@ class Kv8Ops:
         """Attention of q [n, n_q_heads, head_dim] (rotated here) over the cache, [n, n_q_heads, head_dim]. max_new and
         max_kv: upper bounds on any sequence's new rows and on kv_len. prefix_len (int32 [batch]): cache rows that all
         rows of the sequence see; row_first (int32 [n]): the first cache row that a row sees; alibi_slopes (fp32
-        [n_q_heads]): score - slope * distance. A row that sees nothing gets zeros. The context's scratch grows on the
+        [n_q_heads]): score - slope * distance. A row that sees nothing gets zeros; rows of no sequence (spare tokens, a
+        refused step) are not computed, and hold what the memory held. The context's scratch grows on the
         first call that needs more (which waits for the GPU: make such a call before capturing a graph; graphs captured
         before keep the scratch they were captured with)."""
         return _kv8.attend(self.ctx.handle.value, self.ctx.device, self._at, self._st(), q, row_start, kv_len, block_table,
