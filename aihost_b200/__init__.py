@@ -36,7 +36,7 @@ EXPORTS = (
 # aihost_kernel ids of the device-time profiler
 KERNEL_APPEND, KERNEL_DECODE, KERNEL_COMBINE, KERNEL_PREFILL, KERNEL_CONVERT, KERNEL_MATMUL = range(6)
 KERNEL_PAGES, KERNEL_KV8_APPEND, KERNEL_KV8_ATTN = range(6, 9)
-KV8_EXACT_Q = 0x100  # or'ed into Kv8Desc.rope_mode
+KV8_ROUND_Q = 0x100  # or'ed into Kv8Desc.rope_mode
 KV8_SPLIT_CACHE, KV8_TENSOR = range(2)  # aihost_kv8_kernel: which one an attention call over the 8-bit cache runs
 
 

@@ -114,7 +114,7 @@ void kv8_mma_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max
 cudaError_t launch_kv8_mma(const Kv8AttnArgs& a, cudaStream_t st);
 
 // The tcgen05 kernel (query rows per block 256) and its plan; *end: its length as the plan sees it, in
-// times of one 128-row cache tile (about 2.1 us at head_dim 128, 2.4 with exact_q, and 1.7 at 64). *whole: so many units
+// times of one 128-row cache tile (about 2.1 us at head_dim 128, 2.4 with a rotated q that is not rounded, and 1.7 at 64). *whole: so many units
 // (tile, head), before the others, are not cut.
 int32_t kv8_prefill_rows();
 void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max_new, int32_t max_kv, int32_t num_sms,

@@ -54,10 +54,10 @@ aihost_status check_kv8(const aihost_kv8_desc* d, Resolved* r) {
     return fail(AIHOST_EINVAL, "io_dtype %d must be F32 (0) or F16 (1)", d->io_dtype);
   if (d->out_dtype != AIHOST_F32 && d->out_dtype != AIHOST_F16)
     return fail(AIHOST_EINVAL, "out_dtype %d must be F32 (0) or F16 (1)", d->out_dtype);
-  r->rope_mode = d->rope_mode & ~AIHOST_KV8_EXACT_Q;
+  r->rope_mode = d->rope_mode & ~AIHOST_KV8_ROUND_Q;
   if (r->rope_mode < AIHOST_ROPE_INTERLEAVED || r->rope_mode > AIHOST_ROPE_NONE)
     return fail(AIHOST_EINVAL, "rope_mode %d is not a valid aihost_rope_mode", d->rope_mode);
-  r->exact_q = d->rope_mode != r->rope_mode && r->rope_mode != AIHOST_ROPE_NONE;
+  r->exact_q = d->rope_mode == r->rope_mode && r->rope_mode != AIHOST_ROPE_NONE;
   if (r->rope_mode != AIHOST_ROPE_NONE && !(d->rope_theta > 0.0f && isfinite(d->rope_theta)))
     return fail(AIHOST_EINVAL, "rope_theta must be a positive finite number");
   if (!(isfinite(d->scale) && d->scale >= 0.0f)) return fail(AIHOST_EINVAL, "scale must be >= 0 and finite");

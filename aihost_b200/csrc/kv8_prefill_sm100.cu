@@ -18,23 +18,23 @@
 //                grows by more than 2^8), exp2, row sum, P times V's factors as fp16.
 // Ranges are cut into chunks where there are few tiles; the last block of a tile to arrive merges.
 //
-// Precision: an unrotated fp16 q is exact. A rotated one is rounded to fp16, and at head_dim 64 the fp16 of what
-// that leaves enters as a second operand. At head_dim 128 that costs 64 KB, which have to come from the
-// rings (one K and one V tile instead of two), and a third more products, so the caller chooses it
-// (AIHOST_KV8_EXACT_Q): without it results are off by 3.6e-4 instead of 2.9e-4 (relative root mean square; an fp16 result
-// alone is by 2.1e-4). Either is of one half of the rotated q, since turning (x, y) may pass fp16's
-// range; K's factors take it back. P is rounded to fp16 once, as the output is; maxima, sums and
-// accumulators are fp32, int8 values exact. (P as a pair too: 690 us for the first case below; the rest of 128
-// weights a row costs the softmax what the products do not.)
+// Precision: an unrotated fp16 q is exact. A rotated one is rounded to fp16, and the fp16 of what that leaves
+// enters as a second operand. At head_dim 128 that costs 64 KB, which come from the rings (one K and one V
+// tile instead of two), and a third more products; a caller may do without (AIHOST_KV8_ROUND_Q): results are
+// then off by 3.6e-4 instead of 2.9e-4 (relative root mean square; an fp16 result alone is by 2.1e-4). Either is
+// of one half of the rotated q, since turning (x, y) may pass fp16's range; K's factors take it back. P is
+// rounded to fp16 once, as the output is; maxima, sums and accumulators are fp32, int8 values exact. (P as
+// a pair too: 690 us in place of 505 for the first case below; the rest of 128 weights a row costs the softmax what
+// the products do not.)
 //
-// Measured: 2048 new rows over 14336 cached, 32/8 heads x 128, 495-506 us (515 GFLOP: 1030 TFLOP/s, 63 %
-// of the measured 1634; 544-550 us where calls follow one another for long, under the power cap), with exact_q
-// 560 (650). The MMAs of a tile pair take 2048 cycles, the loop 3760: a tile's turn is its S and P V (1024) and its
-// softmax (~2740 beside the other tile's), one after another; and the last 0.73 of a wave are chunks, each with a
-// block's fixed work. Two prompts of 4 K rows with documents, 163 us (exact_q 181): of a block's ~40 K cycles
-// about half are fixed (lookup and ranges 5 K, Q 5 K, its rotation 4.6 K, first S 1.6 K, results 5 K). Six
-// uneven prompts, 14/2 heads x 64, scores capped: 63.5 us.
-// Not better on the first of these: S in two halves of 64 keys (620 us), the next
+// Measured: 2048 new rows over 14336 cached, 32/8 heads x 128, q rotated, 560 us (515 GFLOP: 920 TFLOP/s, 56 % of
+// the measured 1634; 650 us where calls follow one another for long, under the power cap), with q rounded 495-506
+// (544-550). The MMAs of a tile pair take 3072 cycles (2048 with q rounded), the loop ~4200 (3760): a tile's turn
+// is its S and P V and its softmax (~2740 beside the other tile's), one after another; and the last 0.73 of a wave
+// are chunks, each with a block's fixed work. Two prompts of 4 K rows with documents, 181 us (163): of a block's
+// ~40 K cycles about half are fixed (lookup and ranges 5 K, Q 5 K, its rotation 4.6 K, first S 1.6 K, results
+// 5 K). Six uneven prompts, 14/2 heads x 64, scores capped: 63.5 us.
+// Not better on the first of these with q rounded: S in two halves of 64 keys (620 us), the next
 // S read into registers ahead (spills, 1330), two threads per query row (569), softmax as a loop over 32
 // columns that reads S twice (564), a quarter of the exponentials by a polynomial on the FMA pipe (595),
 // non-uniform descriptors (790), set-up before the tile is known (553).
@@ -584,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       // rotated in place, by a loop that is not unrolled: it runs once per block, from a cold instruction cache
       if (a.rope_mode != AIHOST_ROPE_NONE) {
         const bool halves = a.rope_mode == AIHOST_ROPE_NEOX;
-        // 2^-21 off at head_dim 128 (with sincos_near 193 us for the documents with exact_q, so 183)
+        // 2^-21 off at head_dim 128 (with sincos_near 193 us for the documents, so 183)
         auto rotation = [](float angle, float* s, float* c) {
           if constexpr (D == 64) sincos_near(angle, s, c);
           else sincos_reduced(angle, s, c);

@@ -22,7 +22,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import EINVAL, F16, F32, KV8_EXACT_Q, ROPE_INTERLEAVED, AttnError, Kv8Desc, check, lib
+from . import EINVAL, F16, F32, KV8_ROUND_Q, ROPE_INTERLEAVED, AttnError, Kv8Desc, check, lib
 from .ops import Context
 
 lib()  # the module below calls the same library
@@ -48,11 +48,12 @@ class Kv8Spec:
     score_cap: float = 0.0
     rope_theta: float = 10000.0
     rope_mode: int = ROPE_INTERLEAVED
-    exact_q: bool = False  # a rotated float16 q keeps 22 bits in prompts of head_dim 128 too (slower)
+    round_q: bool = False  # a rotated float16 q may be rounded to float16 (faster for prompts of head_dim 128)
 
     def desc(self) -> Kv8Desc:
         return Kv8Desc(self.n_q_heads, self.n_kv_heads, self.head_dim, self.page_rows, self.n_pages, self.max_pages,
-                       self.io_dtype, self.out_dtype, self.scale, self.score_cap, self.rope_theta, self.rope_mode | (KV8_EXACT_Q if self.exact_q else 0), 0, 0)
+                       self.io_dtype, self.out_dtype, self.scale, self.score_cap, self.rope_theta,
+                       self.rope_mode | (KV8_ROUND_Q if self.round_q else 0), 0, 0)
 
 
 class StepMap(NamedTuple):

@@ -343,8 +343,8 @@ typedef struct {
   int64_t q_token_stride;        /* bytes between tokens of q;            0 -> n_q_heads rows, packed */
   int64_t kv_token_stride;       /* bytes between tokens of k_new, v_new; 0 -> n_kv_heads rows, packed */
 } aihost_kv8_desc;
-/* Or'ed into rope_mode: what a rotated F16 q keeps, see aihost_kv8_attention. */
-#define AIHOST_KV8_EXACT_Q 0x100
+/* Or'ed into rope_mode: a rotated F16 q may be rounded to fp16, see aihost_kv8_attention. */
+#define AIHOST_KV8_ROUND_Q 0x100
 
 /* One step's page bookkeeping in one launch: sequence b has seq_len[b] cached rows and gets
  * n_new[b] >= 0 more. Pages that the new rows need are taken from the top of the stack free_pages
@@ -408,11 +408,11 @@ aihost_status aihost_kv8_plan(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc,
  * bounds are not computed, and their rows of out are left as they are.
  * Softmax state and sums are fp32; int8 values enter the products exactly. With F16 q, the softmax weights
  * enter as fp16; q enters exactly where it is not rotated, else as a pair of fp16 whose sum holds 22 bits (down
- * to fp16's smallest step), but in the AIHOST_KV8_TENSOR kernel with head_dim 128, where it is rounded to
- * fp16 once unless rope_mode holds AIHOST_KV8_EXACT_Q (results off by 3.6e-4 instead of 2.9e-4 in relative root mean square, long
- * prompts a sixth faster). Which kernel runs goes by head counts, batch, n_tokens, max_new and max_kv
- * (aihost_kv8_plan tells), so the same row may differ by those roundings and by the order of its sums between
- * calls with other bounds. With F32 q, q (of any size) and the weights enter as such pairs. */
+ * to fp16's smallest step). With AIHOST_KV8_ROUND_Q in rope_mode the AIHOST_KV8_TENSOR kernel rounds a rotated q
+ * of head_dim 128 to fp16 once: results off by 3.6e-4 instead of 2.9e-4 in relative root mean square, long
+ * prompts an eighth to a sixth faster. With F32 q, q (of any size) and the weights enter as such pairs. Which
+ * kernel runs goes by head counts, batch, n_tokens, max_new and max_kv (aihost_kv8_plan tells), so a row may
+ * differ by the roundings named here and by the order of its sums between calls with other bounds. */
 aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens,
                                    int32_t max_new, int32_t max_kv, const void* q, const int32_t* row_start,
                                    const int32_t* kv_len, const int32_t* block_table, const int8_t* k_pool,

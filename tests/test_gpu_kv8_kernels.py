@@ -1,5 +1,5 @@
 """Which kernel the 8-bit cache's attention runs, and that rotated queries keep what the header promises: 22 bits, but for the
-tcgen05 kernel with head_dim 128 and exact_q 0, which rounds them to fp16."""
+tcgen05 kernel with head_dim 128 and round_q, which rounds them to fp16."""
 import dataclasses
 
 import numpy as np
@@ -53,14 +53,14 @@ def _pair_size(w, q):
 @pytest.mark.parametrize("mode", [ROPE_INTERLEAVED, ROPE_NEOX])
 @pytest.mark.parametrize("cached, new, G", [([300, 1029], [1, 1], 4), ([333], [1], 16), ([300, 77], [3, 2], 4),
                                             ([90, 0, 17], [60, 130, 1], 4), ([1500], [40], 7)])
-@pytest.mark.parametrize("D, P, exact", [(64, 16, False), (128, 64, False), (128, 64, True), (128, 16, True)])
-def test_rotated_queries_keep_their_bits(ctx, D, P, exact, cached, new, G, mode, max_kv):
+@pytest.mark.parametrize("D, P, rounded", [(64, 16, False), (64, 16, True), (128, 64, False), (128, 64, True), (128, 16, False)])
+def test_rotated_queries_keep_their_bits(ctx, D, P, rounded, cached, new, G, mode, max_kv):
     w = World(ctx, cached, new, Hq=2 * G, H=2, D=D, P=P, mode=mode, seed=61, theta=5e5, scale=1.5)
-    w.spec = dataclasses.replace(w.spec, exact_q=exact)
+    w.spec = dataclasses.replace(w.spec, round_q=rounded)
     w.ops = Kv8Ops(ctx, w.spec)
     assert {_kernel(w, b) for b in BOUNDS} == _wanted(w)
     q = _q(w, lambda s: 0.5 + w.g.standard_normal(s))
-    if _kernel(w, max_kv) == KV8_TENSOR and D == 128 and not exact:
+    if _kernel(w, max_kv) == KV8_TENSOR and D == 128 and rounded:
         _check(ctx, w, q, out_dtype=F32, max_kv=max_kv, ds=2.0 ** -11)
         return
     size = _pair_size(w, q)
@@ -82,14 +82,15 @@ def test_the_bounds_choose_the_kernel(ctx, case, io):
     assert {_kernel(w, b) for b in BOUNDS} == _wanted(w)
 
 
+@pytest.mark.parametrize("rounded", [False, True])
 @pytest.mark.parametrize("what", ["cap", "bias", "documents", "chunks", "one row"])
 @pytest.mark.parametrize("mode", [ROPE_INTERLEAVED, ROPE_NEOX])
-def test_exact_queries_over_one_tile_at_a_time(ctx, mode, what):
-    """exact_q at head_dim 128: longer ranges than the rings hold, uneven ones, gaps between two query tiles' documents, and
-    ranges cut into chunks."""
+def test_rotated_prompts_of_either_precision(ctx, mode, what, rounded):
+    """head_dim 128, whose rings hold one tile of K and V or two: ranges longer than they hold, uneven ones, gaps between two
+    query tiles' documents, and ranges cut into chunks."""
     cached, new = {"chunks": ([3300, 100], [90, 40]), "one row": ([700, 5], [1, 300])}.get(what, ([700, 0, 40], [300, 129, 17]))
     w = World(ctx, cached, new, Hq=8, H=1, D=128, P=32, mode=mode, cap=6.0 if what == "cap" else 0.0, seed=62)
-    w.spec = dataclasses.replace(w.spec, exact_q=True)
+    w.spec = dataclasses.replace(w.spec, round_q=rounded)
     w.ops = Kv8Ops(ctx, w.spec)
     first = slopes = None
     if what == "bias":
@@ -106,6 +107,6 @@ def test_exact_queries_over_one_tile_at_a_time(ctx, mode, what):
     assert torch.equal(out, again)
     ref, weight, _ = plain.attend(q64, w.start, w.kv_len, w.table, w.P, w.k, w.v, w.ks, w.vs, w.scale, w.cap, w.theta, mode,
                                   first=first, slopes=None if slopes is None else np.float32(slopes))
-    ds = 2.0 ** -19 * _pair_size(w, q64)[..., None]
+    ds = (2.0 ** -11 if rounded else 2.0 ** -19) * _pair_size(w, q64)[..., None]
     tol = 2.0 ** -11 * np.abs(ref) + weight * (2.0 ** -11 + 2.0 ** -16 + 2 * ds) + 1e-7
     assert (np.abs(out.double().cpu().numpy() - ref) - tol).max() <= 0

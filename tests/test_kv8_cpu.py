@@ -110,9 +110,9 @@ def test_plan_tells_scratch_and_kernel():
 
 
 @pytest.mark.parametrize("mode, ok", [(A.ROPE_NONE, True), (A.ROPE_NEOX, True), (3, False), (-1, False), (0x200, False)])
-def test_exact_q_goes_with_every_rope_mode(mode, ok):
-    d = Kv8Spec(**BASE, rope_mode=mode, exact_q=True).desc()
-    assert d.rope_mode == mode | A.KV8_EXACT_Q
+def test_round_q_goes_with_every_rope_mode(mode, ok):
+    d = Kv8Spec(**BASE, rope_mode=mode, round_q=True).desc()
+    assert d.rope_mode == mode | A.KV8_ROUND_Q
     need = ctypes.c_size_t()
     got = A.lib().aihost_kv8_workspace_size(ctypes.byref(d), 1, 1, 1, 64, ctypes.byref(need))
     assert got == (A.OK if ok else A.EINVAL)
