@@ -538,7 +538,9 @@ aihost_status aihost_attn_reserve(aihost_attn_ctx* ctx, size_t bytes) {
   if (s != AIHOST_OK) return s;
   if (bytes <= ctx->scratch_bytes) return AIHOST_OK;
   DeviceGuard g(ctx->device);
+  const size_t least = bytes;
   if (ctx->scratch_captured) {  // graphs go on using what they were captured with
+    bytes = std::max(bytes, 2 * ctx->scratch_bytes);  // all that is kept so comes to less than what is in use
     try {
       ctx->outgrown.push_back(ctx->scratch);
     } catch (const std::bad_alloc&) {
@@ -553,6 +555,11 @@ aihost_status aihost_attn_reserve(aihost_attn_ctx* ctx, size_t bytes) {
   ctx->scratch = nullptr;
   ctx->scratch_bytes = 0;
   cudaError_t e = cudaMalloc(&ctx->scratch, bytes);
+  if (e == cudaErrorMemoryAllocation && bytes > least) {
+    cudaGetLastError();
+    bytes = least;
+    e = cudaMalloc(&ctx->scratch, bytes);
+  }
   if (e != cudaSuccess) {
     ctx->scratch = nullptr;
     return fail(AIHOST_ENOMEM, "cudaMalloc(%zu) for scratch failed: %s", bytes, cudaGetErrorString(e));
