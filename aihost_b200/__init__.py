@@ -32,12 +32,13 @@ EXPORTS = (
     "aihost_matmul_workspace_size", "aihost_matmul_weights", "aihost_dequantize",
     "aihost_page_map", "aihost_page_release", "aihost_kv8_append", "aihost_kv8_read", "aihost_kv8_workspace_size",
     "aihost_kv8_attention", "aihost_kv8_plan",
+    "aihost_kv4_append", "aihost_kv4_read", "aihost_kv4_plan", "aihost_kv4_attention",
 )
 # aihost_kernel ids of the device-time profiler
 KERNEL_APPEND, KERNEL_DECODE, KERNEL_COMBINE, KERNEL_PREFILL, KERNEL_CONVERT, KERNEL_MATMUL = range(6)
-KERNEL_PAGES, KERNEL_KV8_APPEND, KERNEL_KV8_ATTN = range(6, 9)
+KERNEL_PAGES, KERNEL_KV8_APPEND, KERNEL_KV8_ATTN, KERNEL_KV4_APPEND, KERNEL_KV4_ATTN = range(6, 11)
 KV8_ROUND_Q = 0x100  # or'ed into Kv8Desc.rope_mode
-KV8_SPLIT_CACHE, KV8_TENSOR = range(2)  # aihost_kv8_kernel: which one an attention call over the 8-bit cache runs
+KV8_SPLIT_CACHE, KV8_TENSOR = range(2)  # aihost_kv8_kernel: which one an attention call over the 8-bit or 4-bit cache runs
 
 
 class AttnDesc(ctypes.Structure):
@@ -120,6 +121,10 @@ def lib() -> ctypes.CDLL:
     L.aihost_kv8_workspace_size.argtypes = [k8, i32, i32, i32, i32, ctypes.POINTER(sz)]
     L.aihost_kv8_plan.argtypes = [vp, k8, i32, i32, i32, i32, ctypes.POINTER(sz), ctypes.POINTER(i32)]
     L.aihost_kv8_attention.argtypes = [vp, k8, i32, i32, i32, i32] + [vp] * 13
+    L.aihost_kv4_append.argtypes = L.aihost_kv8_append.argtypes
+    L.aihost_kv4_read.argtypes = L.aihost_kv8_read.argtypes
+    L.aihost_kv4_plan.argtypes = L.aihost_kv8_plan.argtypes
+    L.aihost_kv4_attention.argtypes = L.aihost_kv8_attention.argtypes
     for name in EXPORTS:
         fn = getattr(L, name)
         if name not in ("aihost_attn_abi_version", "aihost_attn_last_error"):

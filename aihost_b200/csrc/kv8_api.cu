@@ -1,4 +1,4 @@
-// kv8_api.cu — the extern "C" boundary of the 8-bit paged cache (declared in include/aihost_attn.h):
+// kv8_api.cu — the extern "C" boundary of the 8-bit and the 4-bit paged cache (declared in include/aihost_attn.h):
 // argument checks, resolved strides, the split plan and the launches. Allocates nothing.
 #include <math.h>
 #include <string.h>
@@ -101,7 +101,7 @@ struct Plan {
   }
 };
 
-Plan make_plan(const aihost_kv8_desc* d, const Resolved& r, int32_t batch, int32_t n_tokens, int32_t max_new,
+Plan make_plan(const aihost_kv8_desc* d, const Resolved& r, bool four, int32_t batch, int32_t n_tokens, int32_t max_new,
                int32_t max_kv, int32_t num_sms) {
   // The tcgen05 kernel takes fp16 rows by 256 and has ~12 us of fixed work a block; the split-cache one
   // takes 16 and rereads the cache for each tile, ~50 ns (head_dim 64: 37) per tile and 1000 rows over the
@@ -118,7 +118,7 @@ Plan make_plan(const aihost_kv8_desc* d, const Resolved& r, int32_t batch, int32
   max_kv = std::min(max_kv, kMaxKv);
   const int32_t rows = kv8_mma_rows(g, max_new), G = g.n_q_heads / g.n_kv_heads;
   p.tensor = false;
-  if (d->io_dtype == AIHOST_F16 && static_cast<int64_t>(max_new) * G > rows) {
+  if (!four && d->io_dtype == AIHOST_F16 && static_cast<int64_t>(max_new) * G > rows) {
     double end;
     kv8_prefill_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.whole, &p.chunk, &p.splits, &end);
     const double even = static_cast<double>(n_tokens) / (static_cast<double>(batch) * max_new);
@@ -132,7 +132,7 @@ Plan make_plan(const aihost_kv8_desc* d, const Resolved& r, int32_t batch, int32
   } else {
     p.rows = rows;
     p.whole = 0;
-    kv8_mma_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.chunk, &p.splits);
+    (four ? kv4_mma_plan : kv8_mma_plan)(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.chunk, &p.splits);
   }
   return p;
 }
@@ -150,6 +150,106 @@ aihost_status check_sizes(int32_t batch, int32_t n_tokens, int32_t max_new, int3
   if (max_new < 1 || max_kv < max_new)
     return fail(AIHOST_EINVAL, "max_new (%d) must be >= 1 and max_kv (%d) at least max_new", max_new, max_kv);
   return AIHOST_OK;
+}
+
+aihost_status tell_plan(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, bool four, int32_t batch, int32_t n_tokens,
+                        int32_t max_new, int32_t max_kv, size_t* out_bytes, int32_t* out_kernel) {
+  Resolved r;
+  aihost_status s = check_kv8(desc, &r);
+  if (s == AIHOST_OK) s = check_sizes(batch, n_tokens, max_new, max_kv);
+  if (s != AIHOST_OK) return s;
+  const Plan plan = make_plan(desc, r, four, batch, n_tokens, max_new, max_kv, ctx ? ctx->num_sms : current_sms());
+  if (out_bytes) *out_bytes = plan.scratch(r.g);
+  if (out_kernel) *out_kernel = plan.tensor ? AIHOST_KV8_TENSOR : AIHOST_KV8_SPLIT_CACHE;
+  return AIHOST_OK;
+}
+
+// The caches differ in what the pools and their factors are.
+struct CachePtrs {
+  const void* k_pool;
+  const void* v_pool;
+  const void* k_factor;  // scales or ranges
+  const void* v_factor;
+};
+
+aihost_status attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, bool four, int32_t batch, int32_t n_tokens,
+                        int32_t max_new, int32_t max_kv, const void* q, const int32_t* row_start, const int32_t* kv_len,
+                        const int32_t* block_table, const CachePtrs& c, const int32_t* prefix_len, const int32_t* row_first,
+                        const float* alibi_slopes, void* out, void* stream) {
+  if (!ctx) return fail(AIHOST_EINVAL, "ctx is NULL");
+  Resolved r;
+  aihost_status s = check_kv8(desc, &r);
+  if (s == AIHOST_OK) s = check_sizes(batch, n_tokens, max_new, max_kv);
+  if (s != AIHOST_OK) return s;
+  if (n_tokens == 0) return AIHOST_OK;
+  if (!q || !row_start || !kv_len || !block_table || !c.k_pool || !c.v_pool || !c.k_factor || !c.v_factor || !out)
+    return fail(AIHOST_EINVAL, "every array but prefix_len, row_first and alibi_slopes must be non-NULL");
+  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(c.k_pool, 16) || !aligned(c.v_pool, 16) || !aligned(row_start, 4) ||
+      !aligned(kv_len, 4) || !aligned(block_table, 4) || !aligned(c.k_factor, four ? 16 : 4) || !aligned(c.v_factor, four ? 16 : 4) ||
+      !aligned(prefix_len, 4) || !aligned(row_first, 4) || !aligned(alibi_slopes, 4))
+    return fail(AIHOST_EINVAL, four ? "q, out, the pools and the ranges must be 16-byte, other arrays 4-byte aligned"
+                                   : "q, out and the pools must be 16-byte, other arrays 4-byte aligned");
+  Kv8AttnArgs a;
+  memset(&a, 0, sizeof(a));
+  a.g = r.g;
+  a.batch = batch;
+  a.n_tokens = n_tokens;
+  a.max_new = max_new;
+  a.max_kv = std::min(max_kv, kMaxKv);
+  a.q_dtype = desc->io_dtype;
+  a.out_dtype = desc->out_dtype;
+  a.rope_mode = r.rope_mode;
+  a.exact_q = r.exact_q;
+  a.q_token_stride = r.q_stride;
+  a.q = q;
+  a.row_start = row_start;
+  a.kv_len = kv_len;
+  a.block_table = block_table;
+  a.k_pool = static_cast<const int8_t*>(c.k_pool);
+  a.v_pool = static_cast<const int8_t*>(c.v_pool);
+  if (four) {
+    a.k_range = static_cast<const uint32_t*>(c.k_factor);
+    a.v_range = static_cast<const uint32_t*>(c.v_factor);
+  } else {
+    a.k_scale = static_cast<const float*>(c.k_factor);
+    a.v_scale = static_cast<const float*>(c.v_factor);
+  }
+  a.prefix_len = prefix_len;
+  a.row_first = row_first;
+  a.alibi_slopes = alibi_slopes;
+  a.out = out;
+  a.scale = r.scale;
+  // cap tanh(s / cap) in fp32 wants scale / cap and cap log2(e) to be normal numbers: beyond 1e30 it is s itself,
+  // below 1e-30 the scores are alike either way (1e-20 where the codes' unit 2^20 joins the factor)
+  a.score_cap = desc->score_cap > 1e30f || desc->score_cap == 0.0f ? 0.0f : std::max(desc->score_cap, four ? 1e-20f : 1e-30f);
+  a.status = ctx->d_status;
+  if (r.rope_mode != AIHOST_ROPE_NONE) a.freqs = freqs_of(ctx, desc);
+  const Plan plan = make_plan(desc, r, four, batch, n_tokens, max_new, max_kv, ctx->num_sms);
+  a.tiles = plan.tiles;
+  a.chunk = plan.chunk;
+  a.max_splits = plan.splits;
+  a.whole = plan.whole;
+  if (static_cast<int64_t>(a.tiles) * r.g.n_kv_heads > INT32_MAX)
+    return fail(AIHOST_EUNSUPPORTED, "n_tokens %d needs too many blocks", n_tokens);
+  const size_t need = plan.scratch(r.g);
+  if (need > ctx->scratch_bytes)
+    return fail(AIHOST_ENOMEM, "attention needs %zu bytes of scratch, context has %zu (call aihost_attn_reserve)", need,
+                ctx->scratch_bytes);
+  if (need) {
+    a.part_o = static_cast<float*>(ctx->scratch);
+    a.part_ml = a.part_o + static_cast<size_t>(plan.parts(r.g)) * r.g.head_dim;
+    a.counters = ctx->kv8_counters + 1;
+  }
+  DeviceGuard g(ctx->device);
+  if (!g.ok()) return fail(AIHOST_ECUDA, "cudaSetDevice(%d) failed", ctx->device);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  SharedUse shared(ctx, st, need > 0);
+  if (shared.error() != cudaSuccess) return cuda_fail(shared.error(), "ordering the scratch's uses");
+  cudaError_t e = timed_launch(ctx, four ? AIHOST_KERNEL_KV4_ATTN : AIHOST_KERNEL_KV8_ATTN, st, [&] {
+    if (four) return launch_kv4_mma(a, st);
+    return plan.tensor ? launch_kv8_prefill(a, st) : launch_kv8_mma(a, st);
+  });
+  return e == cudaSuccess ? AIHOST_OK : cuda_fail(e, four ? "4-bit attention launch" : "8-bit attention launch");
 }
 
 }  // namespace
@@ -290,95 +390,96 @@ aihost_status aihost_kv8_workspace_size(const aihost_kv8_desc* desc, int32_t bat
   aihost_status s = check_kv8(desc, &r);
   if (s == AIHOST_OK) s = check_sizes(batch, n_tokens, max_new, max_kv);
   if (s != AIHOST_OK) return s;
-  *out_bytes = make_plan(desc, r, batch, n_tokens, max_new, max_kv, current_sms()).scratch(r.g);
+  *out_bytes = make_plan(desc, r, false, batch, n_tokens, max_new, max_kv, current_sms()).scratch(r.g);
   return AIHOST_OK;
 }
 
 aihost_status aihost_kv8_plan(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens,
                               int32_t max_new, int32_t max_kv, size_t* out_bytes, int32_t* out_kernel) {
-  Resolved r;
-  aihost_status s = check_kv8(desc, &r);
-  if (s == AIHOST_OK) s = check_sizes(batch, n_tokens, max_new, max_kv);
-  if (s != AIHOST_OK) return s;
-  const Plan plan = make_plan(desc, r, batch, n_tokens, max_new, max_kv, ctx ? ctx->num_sms : current_sms());
-  if (out_bytes) *out_bytes = plan.scratch(r.g);
-  if (out_kernel) *out_kernel = plan.tensor ? AIHOST_KV8_TENSOR : AIHOST_KV8_SPLIT_CACHE;
-  return AIHOST_OK;
+  return tell_plan(ctx, desc, false, batch, n_tokens, max_new, max_kv, out_bytes, out_kernel);
 }
-
 aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens,
                                    int32_t max_new, int32_t max_kv, const void* q, const int32_t* row_start,
                                    const int32_t* kv_len, const int32_t* block_table, const int8_t* k_pool,
                                    const int8_t* v_pool, const float* k_scale, const float* v_scale,
                                    const int32_t* prefix_len, const int32_t* row_first, const float* alibi_slopes,
                                    void* out, void* stream) {
+  return attention(ctx, desc, false, batch, n_tokens, max_new, max_kv, q, row_start, kv_len, block_table,
+                   CachePtrs{k_pool, v_pool, k_scale, v_scale}, prefix_len, row_first, alibi_slopes, out, stream);
+}
+
+aihost_status aihost_kv4_append(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t n_tokens, const void* k_new,
+                                const void* v_new, const int64_t* slots, const int32_t* positions, uint8_t* k_pool,
+                                uint8_t* v_pool, void* k_range, void* v_range, void* stream) {
   if (!ctx) return fail(AIHOST_EINVAL, "ctx is NULL");
   Resolved r;
   aihost_status s = check_kv8(desc, &r);
-  if (s == AIHOST_OK) s = check_sizes(batch, n_tokens, max_new, max_kv);
   if (s != AIHOST_OK) return s;
+  if (n_tokens < 0) return fail(AIHOST_EINVAL, "n_tokens (%d) must be >= 0", n_tokens);
   if (n_tokens == 0) return AIHOST_OK;
-  if (!q || !row_start || !kv_len || !block_table || !k_pool || !v_pool || !k_scale || !v_scale || !out)
-    return fail(AIHOST_EINVAL, "every array but prefix_len, row_first and alibi_slopes must be non-NULL");
-  if (!aligned(q, 16) || !aligned(out, 16) || !aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(row_start, 4) ||
-      !aligned(kv_len, 4) || !aligned(block_table, 4) || !aligned(k_scale, 4) || !aligned(v_scale, 4) ||
-      !aligned(prefix_len, 4) || !aligned(row_first, 4) || !aligned(alibi_slopes, 4))
-    return fail(AIHOST_EINVAL, "q, out and the pools must be 16-byte, other arrays 4-byte aligned");
-  Kv8AttnArgs a;
-  memset(&a, 0, sizeof(a));
-  a.g = r.g;
-  a.batch = batch;
-  a.n_tokens = n_tokens;
-  a.max_new = max_new;
-  a.max_kv = std::min(max_kv, kMaxKv);
-  a.q_dtype = desc->io_dtype;
-  a.out_dtype = desc->out_dtype;
-  a.rope_mode = r.rope_mode;
-  a.exact_q = r.exact_q;
-  a.q_token_stride = r.q_stride;
-  a.q = q;
-  a.row_start = row_start;
-  a.kv_len = kv_len;
-  a.block_table = block_table;
-  a.k_pool = k_pool;
-  a.v_pool = v_pool;
-  a.k_scale = k_scale;
-  a.v_scale = v_scale;
-  a.prefix_len = prefix_len;
-  a.row_first = row_first;
-  a.alibi_slopes = alibi_slopes;
-  a.out = out;
-  a.scale = r.scale;
-  // cap tanh(s / cap) in fp32 wants scale / cap and cap log2(e) to be normal numbers: beyond 1e30 it is s itself,
-  // below 1e-30 the scores are alike either way
-  a.score_cap = desc->score_cap > 1e30f || desc->score_cap == 0.0f ? 0.0f : std::max(desc->score_cap, 1e-30f);
-  a.status = ctx->d_status;
-  if (r.rope_mode != AIHOST_ROPE_NONE) a.freqs = freqs_of(ctx, desc);
-  const Plan plan = make_plan(desc, r, batch, n_tokens, max_new, max_kv, ctx->num_sms);
-  a.tiles = plan.tiles;
-  a.chunk = plan.chunk;
-  a.max_splits = plan.splits;
-  a.whole = plan.whole;
-  if (static_cast<int64_t>(a.tiles) * r.g.n_kv_heads > INT32_MAX)
-    return fail(AIHOST_EUNSUPPORTED, "n_tokens %d needs too many blocks", n_tokens);
-  const size_t need = plan.scratch(r.g);
-  if (need > ctx->scratch_bytes)
-    return fail(AIHOST_ENOMEM, "attention needs %zu bytes of scratch, context has %zu (call aihost_attn_reserve)", need,
-                ctx->scratch_bytes);
-  if (need) {
-    a.part_o = static_cast<float*>(ctx->scratch);
-    a.part_ml = a.part_o + static_cast<size_t>(plan.parts(r.g)) * r.g.head_dim;
-    a.counters = ctx->kv8_counters + 1;
-  }
+  if (!k_new || !v_new || !slots || !k_pool || !v_pool || !k_range || !v_range ||
+      (!positions && r.rope_mode != AIHOST_ROPE_NONE))
+    return fail(AIHOST_EINVAL, "every array must be non-NULL (positions may be NULL with rope_mode NONE)");
+  if (!aligned(k_new, 16) || !aligned(v_new, 16) || !aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(k_range, 16) ||
+      !aligned(v_range, 16) || !aligned(slots, 8) || !aligned(positions, 4))
+    return fail(AIHOST_EINVAL, "k_new, v_new, the pools and the ranges must be 16-byte, slots 8-byte, positions 4-byte aligned");
   DeviceGuard g(ctx->device);
   if (!g.ok()) return fail(AIHOST_ECUDA, "cudaSetDevice(%d) failed", ctx->device);
+  Kv4AppendArgs a;
+  a.g = r.g;
+  a.n_tokens = n_tokens;
+  a.io_dtype = desc->io_dtype;
+  a.rope_mode = r.rope_mode;
+  a.token_stride = r.kv_stride;
+  a.k_new = k_new;
+  a.v_new = v_new;
+  a.slots = slots;
+  a.positions = positions;
+  a.k_pool = k_pool;
+  a.v_pool = v_pool;
+  a.k_range = static_cast<uint32_t*>(k_range);
+  a.v_range = static_cast<uint32_t*>(v_range);
+  a.status = ctx->d_status;
+  if (r.rope_mode != AIHOST_ROPE_NONE) a.freqs = freqs_of(ctx, desc);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  SharedUse shared(ctx, st, need > 0);
-  if (shared.error() != cudaSuccess) return cuda_fail(shared.error(), "ordering the scratch's uses");
-  cudaError_t e = timed_launch(ctx, AIHOST_KERNEL_KV8_ATTN, st, [&] {
-    return plan.tensor ? launch_kv8_prefill(a, st) : launch_kv8_mma(a, st);
-  });
-  return e == cudaSuccess ? AIHOST_OK : cuda_fail(e, "8-bit attention launch");
+  cudaError_t e = timed_launch(ctx, AIHOST_KERNEL_KV4_APPEND, st, [&] { return launch_kv4_append(a, st); });
+  return e == cudaSuccess ? AIHOST_OK : cuda_fail(e, "4-bit append launch");
+}
+
+aihost_status aihost_kv4_read(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t n_rows, const int64_t* slots,
+                              const uint8_t* pool, const void* range, void* out, int32_t out_dtype, void* stream) {
+  if (!ctx) return fail(AIHOST_EINVAL, "ctx is NULL");
+  Resolved r;
+  aihost_status s = check_kv8(desc, &r);
+  if (s != AIHOST_OK) return s;
+  if (out_dtype != AIHOST_F32 && out_dtype != AIHOST_F16)
+    return fail(AIHOST_EINVAL, "out_dtype %d must be F32 (0) or F16 (1)", out_dtype);
+  if (n_rows < 0) return fail(AIHOST_EINVAL, "n_rows (%d) must be >= 0", n_rows);
+  if (n_rows == 0) return AIHOST_OK;
+  if (!slots || !pool || !range || !out) return fail(AIHOST_EINVAL, "slots, pool, range and out must be non-NULL");
+  if (!aligned(slots, 8) || !aligned(pool, 16) || !aligned(range, 16) || !aligned(out, 16))
+    return fail(AIHOST_EINVAL, "pool, range and out must be 16-byte, slots 8-byte aligned");
+  DeviceGuard g(ctx->device);
+  if (!g.ok()) return fail(AIHOST_ECUDA, "cudaSetDevice(%d) failed", ctx->device);
+  Kv4ReadArgs a{r.g, n_rows, out_dtype, slots, pool, static_cast<const uint32_t*>(range), out, ctx->d_status};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = timed_launch(ctx, AIHOST_KERNEL_KV4_APPEND, st, [&] { return launch_kv4_read(a, st); });
+  return e == cudaSuccess ? AIHOST_OK : cuda_fail(e, "4-bit read launch");
+}
+
+aihost_status aihost_kv4_plan(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens,
+                              int32_t max_new, int32_t max_kv, size_t* out_bytes, int32_t* out_kernel) {
+  return tell_plan(ctx, desc, true, batch, n_tokens, max_new, max_kv, out_bytes, out_kernel);
+}
+
+aihost_status aihost_kv4_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens,
+                                   int32_t max_new, int32_t max_kv, const void* q, const int32_t* row_start,
+                                   const int32_t* kv_len, const int32_t* block_table, const uint8_t* k_pool,
+                                   const uint8_t* v_pool, const void* k_range, const void* v_range,
+                                   const int32_t* prefix_len, const int32_t* row_first, const float* alibi_slopes,
+                                   void* out, void* stream) {
+  return attention(ctx, desc, true, batch, n_tokens, max_new, max_kv, q, row_start, kv_len, block_table,
+                   CachePtrs{k_pool, v_pool, k_range, v_range}, prefix_len, row_first, alibi_slopes, out, stream);
 }
 
 }  // extern "C"

@@ -1,4 +1,4 @@
-// kv8_py.cpp — the Python module _kv8: torch tensors in, C ABI calls of the 8-bit cache out.
+// kv8_py.cpp — the Python module _kv8: torch tensors in, C ABI calls of the 8-bit and the 4-bit cache out.
 //
 // A decode step makes a few calls per layer, each a few microseconds of GPU time; checking a dozen
 // tensors and passing their pointers from Python takes several times that, so it is done here.
@@ -15,6 +15,7 @@
 #include <stdio.h>
 
 #include <initializer_list>
+#include <type_traits>
 #include <utility>
 
 #include "../../include/aihost_attn.h"
@@ -120,11 +121,16 @@ struct Call {
     return (n > 1 ? t.stride(0) : packed) * t.element_size();
   }
 
-  int8_t* pool(PyObject* o, const char* name) const {
-    return array<int8_t>(o, name, at::kChar, {d.n_pages, d.n_kv_heads, d.page_rows, d.head_dim});
+  // A pool and what its values are multiplied with: scales of the 8-bit cache, ranges of the 4-bit one.
+  template <bool FOUR>
+  std::conditional_t<FOUR, uint8_t, int8_t>* pool(PyObject* o, const char* name) const {
+    if constexpr (FOUR) return array<uint8_t>(o, name, at::kByte, {d.n_pages, d.n_kv_heads, d.page_rows, d.head_dim / 2});
+    else return array<int8_t>(o, name, at::kChar, {d.n_pages, d.n_kv_heads, d.page_rows, d.head_dim});
   }
-  float* scales(PyObject* o, const char* name) const {
-    return array<float>(o, name, at::kFloat, {d.n_pages, d.n_kv_heads});
+  template <bool FOUR>
+  std::conditional_t<FOUR, void, float>* factors(PyObject* o, const char* name) const {
+    if constexpr (FOUR) return array<void>(o, name, at::kHalf, {d.n_pages, d.n_kv_heads, d.page_rows, 2});
+    else return array<float>(o, name, at::kFloat, {d.n_pages, d.n_kv_heads});
   }
   at::Tensor make(at::IntArrayRef sizes, at::ScalarType type) const {
     c10::OptionalStreamGuard on;  // a result written on a stream of the caller's is that stream's memory
@@ -219,6 +225,15 @@ PyObject* release_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
+// The C call of the cache that a function is instantiated for.
+template <bool FOUR, typename A, typename B>
+constexpr auto pick(A* eight, B* four) {
+  if constexpr (FOUR) return four;
+  else return eight;
+}
+#define FOUR_OR_EIGHT(name) pick<FOUR>(aihost_kv8_##name, aihost_kv4_##name)
+
+template <bool FOUR>
 PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded(n_args, 12, [&]() -> PyObject* {
     Call c(a);
@@ -227,14 +242,17 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (c.rows(v, "v_new", c.d.n_kv_heads) != c.d.kv_token_stride || v.size(0) != k.size(0))
       raise(AIHOST_EINVAL, "k_new and v_new must have the same tokens and the same stride between them");
     const int64_t n = k.size(0);
-    check(aihost_kv8_append(c.ctx, &c.d, static_cast<int32_t>(n), k.data_ptr(), v.data_ptr(),
-                            c.array<int64_t>(a[6], "slots", at::kLong, {n}, true),
-                            c.maybe<int32_t>(a[7], "positions", at::kInt, {n}, true), c.pool(a[8], "k_pool"),
-                            c.pool(a[9], "v_pool"), c.scales(a[10], "k_scale"), c.scales(a[11], "v_scale"), c.stream));
+    constexpr auto call = FOUR_OR_EIGHT(append);
+    check(call(c.ctx, &c.d, static_cast<int32_t>(n), k.data_ptr(), v.data_ptr(),
+               c.array<int64_t>(a[6], "slots", at::kLong, {n}, true),
+               c.maybe<int32_t>(a[7], "positions", at::kInt, {n}, true), c.pool<FOUR>(a[8], "k_pool"),
+               c.pool<FOUR>(a[9], "v_pool"), c.factors<FOUR>(a[10], FOUR ? "k_range" : "k_scale"),
+               c.factors<FOUR>(a[11], FOUR ? "v_range" : "v_scale"), c.stream));
     Py_RETURN_NONE;
   });
 }
 
+template <bool FOUR>
 PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded(n_args, 9, [&]() -> PyObject* {
     const Call c(a);
@@ -244,12 +262,14 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::ScalarType type = dtype == AIHOST_F32 ? at::kFloat : at::kHalf;
     const at::Tensor out = a[8] == Py_None ? c.make({n, c.d.n_kv_heads, c.d.head_dim}, type) : tensor(a[8], "out");
     if (a[8] != Py_None) c.array<void>(a[8], "out", type, {n, c.d.n_kv_heads, c.d.head_dim});
-    check(aihost_kv8_read(c.ctx, &c.d, static_cast<int32_t>(n), c.array<int64_t>(a[6], "slots", at::kLong, {n}, true),
-                          c.pool(a[4], "pool"), c.scales(a[5], "scale"), out.data_ptr(), dtype, c.stream));
+    constexpr auto call = FOUR_OR_EIGHT(read);
+    check(call(c.ctx, &c.d, static_cast<int32_t>(n), c.array<int64_t>(a[6], "slots", at::kLong, {n}, true),
+               c.pool<FOUR>(a[4], "pool"), c.factors<FOUR>(a[5], FOUR ? "range" : "scale"), out.data_ptr(), dtype, c.stream));
     return THPVariable_Wrap(out);
   });
 }
 
+template <bool FOUR>
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded(n_args, 18, [&]() -> PyObject* {
     Call c(a);
@@ -262,18 +282,20 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor out = a[17] == Py_None ? c.make({n, c.d.n_q_heads, c.d.head_dim}, type) : tensor(a[17], "out");
     if (a[17] != Py_None) c.array<void>(a[17], "out", type, {n, c.d.n_q_heads, c.d.head_dim});
     auto call = [&] {
-      return aihost_kv8_attention(
+      constexpr auto attention = FOUR_OR_EIGHT(attention);
+      return attention(
           c.ctx, &c.d, static_cast<int32_t>(b), static_cast<int32_t>(n), max_new, max_kv, q.data_ptr(),
           c.array<int32_t>(a[5], "row_start", at::kInt, {b + 1}), c.array<int32_t>(a[6], "kv_len", at::kInt, {b}),
-          c.array<int32_t>(a[7], "block_table", at::kInt, {b, c.d.max_pages}), c.pool(a[8], "k_pool"), c.pool(a[9], "v_pool"),
-          c.scales(a[10], "k_scale"), c.scales(a[11], "v_scale"), c.maybe<int32_t>(a[14], "prefix_len", at::kInt, {b}),
+          c.array<int32_t>(a[7], "block_table", at::kInt, {b, c.d.max_pages}), c.pool<FOUR>(a[8], "k_pool"),
+          c.pool<FOUR>(a[9], "v_pool"), c.factors<FOUR>(a[10], FOUR ? "k_range" : "k_scale"),
+          c.factors<FOUR>(a[11], FOUR ? "v_range" : "v_scale"), c.maybe<int32_t>(a[14], "prefix_len", at::kInt, {b}),
           c.maybe<int32_t>(a[15], "row_first", at::kInt, {n}, true),
           c.maybe<float>(a[16], "alibi_slopes", at::kFloat, {c.d.n_q_heads}), out.data_ptr(), c.stream);
     };
     aihost_status s = call();
     if (s == AIHOST_ENOMEM) {  // the context's scratch is too small: grow it once
       size_t need = 0;
-      check(aihost_kv8_plan(c.ctx, &c.d, static_cast<int32_t>(b), static_cast<int32_t>(n), max_new, max_kv, &need, nullptr));
+      check((FOUR_OR_EIGHT(plan))(c.ctx, &c.d, static_cast<int32_t>(b), static_cast<int32_t>(n), max_new, max_kv, &need, nullptr));
       check(aihost_attn_reserve(c.ctx, need));
       s = call();
     }
@@ -294,9 +316,12 @@ PyMethodDef methods[] = {
     {"set_error", set_error, METH_O, nullptr},
     {"map_pages", FAST(map_pages), METH_FASTCALL, nullptr},
     {"release_pages", FAST(release_pages), METH_FASTCALL, nullptr},
-    {"append", FAST(append), METH_FASTCALL, nullptr},
-    {"read", FAST(read), METH_FASTCALL, nullptr},
-    {"attend", FAST(attend), METH_FASTCALL, nullptr},
+    {"append", FAST(append<false>), METH_FASTCALL, nullptr},
+    {"read", FAST(read<false>), METH_FASTCALL, nullptr},
+    {"attend", FAST(attend<false>), METH_FASTCALL, nullptr},
+    {"append4", FAST(append<true>), METH_FASTCALL, nullptr},
+    {"read4", FAST(read<true>), METH_FASTCALL, nullptr},
+    {"attend4", FAST(attend<true>), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kv8", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

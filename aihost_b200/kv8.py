@@ -141,18 +141,28 @@ class Kv8Cache:
 
     def __init__(self, ctx: Context, spec: Kv8Spec, batch: int, n_layers: int = 1, stream=None):
         self.ctx, self.spec, self.batch = ctx, spec, batch
-        self.ops = Kv8Ops(ctx, spec, stream)
-        dev, pool = self.ops.device, (spec.n_pages, spec.n_kv_heads, spec.page_rows, spec.head_dim)
+        self.ops = self._make_ops(ctx, spec, stream)
+        dev = self.ops.device
         with torch.cuda.stream(stream):  # filled, and given back, in the order of the steps' work
-            self.k = [torch.zeros(pool, dtype=torch.int8, device=dev) for _ in range(n_layers)]
-            self.v = [torch.zeros(pool, dtype=torch.int8, device=dev) for _ in range(n_layers)]
-            self.k_scale = [torch.zeros(pool[:2], device=dev) for _ in range(n_layers)]
-            self.v_scale = [torch.zeros(pool[:2], device=dev) for _ in range(n_layers)]
+            self._make_pools(n_layers, dev)
             self.block_table = torch.full((batch, spec.max_pages), -1, dtype=torch.int32, device=dev)
             self.free_pages = torch.arange(spec.n_pages - 1, -1, -1, dtype=torch.int32, device=dev)
             self.free_count = torch.full((1,), spec.n_pages, dtype=torch.int32, device=dev)
             self.seq_len = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.map: StepMap | None = None
+
+    _make_ops = Kv8Ops
+
+    def _make_pools(self, n_layers: int, dev: torch.device) -> None:
+        spec = self.spec
+        pool = (spec.n_pages, spec.n_kv_heads, spec.page_rows, spec.head_dim)
+        self.k = [torch.zeros(pool, dtype=torch.int8, device=dev) for _ in range(n_layers)]
+        self.v = [torch.zeros(pool, dtype=torch.int8, device=dev) for _ in range(n_layers)]
+        self.k_scale = [torch.zeros(pool[:2], device=dev) for _ in range(n_layers)]
+        self.v_scale = [torch.zeros(pool[:2], device=dev) for _ in range(n_layers)]
+
+    def _layer(self, layer: int) -> tuple[torch.Tensor, ...]:
+        return self.k[layer], self.v[layer], self.k_scale[layer], self.v_scale[layer]
 
     def begin(self, n_new: torch.Tensor, max_tokens: int) -> StepMap:
         """Pages, slots and positions for n_new (int32 [batch]) more rows of every sequence."""
@@ -169,13 +179,11 @@ class Kv8Cache:
 
     def append(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
         m = self._step()
-        self.ops.append(k_new, v_new, m.slots, m.positions, self.k[layer], self.v[layer], self.k_scale[layer],
-                        self.v_scale[layer])
+        self.ops.append(k_new, v_new, m.slots, m.positions, *self._layer(layer))
 
     def attend(self, layer: int, q: torch.Tensor, max_new: int, max_kv: int, **kw) -> torch.Tensor:
         m = self._step()
-        return self.ops.attend(q, m.row_start, m.kv_len, self.block_table, self.k[layer], self.v[layer],
-                               self.k_scale[layer], self.v_scale[layer], max_new, max_kv, **kw)
+        return self.ops.attend(q, m.row_start, m.kv_len, self.block_table, *self._layer(layer), max_new, max_kv, **kw)
 
     def end(self) -> None:
         """Commits the step's rows (after its last layer)."""

@@ -189,7 +189,9 @@ typedef enum {
   AIHOST_KERNEL_PAGES = 6,    /* page maps and releases */
   AIHOST_KERNEL_KV8_APPEND = 7, /* append to and read from the 8-bit cache */
   AIHOST_KERNEL_KV8_ATTN = 8, /* attention over the 8-bit cache */
-  AIHOST_KERNEL_COUNT = 9
+  AIHOST_KERNEL_KV4_APPEND = 9, /* append to and read from the 4-bit cache */
+  AIHOST_KERNEL_KV4_ATTN = 10, /* attention over the 4-bit cache */
+  AIHOST_KERNEL_COUNT = 11
 } aihost_kernel;
 aihost_status aihost_attn_profiler_enable(aihost_attn_ctx* ctx, int32_t enable);
 aihost_status aihost_attn_profiler_read(aihost_attn_ctx* ctx, int32_t kernel, int64_t* launches, double* total_ms);
@@ -417,6 +419,42 @@ aihost_status aihost_kv8_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* 
                                    int32_t max_new, int32_t max_kv, const void* q, const int32_t* row_start,
                                    const int32_t* kv_len, const int32_t* block_table, const int8_t* k_pool,
                                    const int8_t* v_pool, const float* k_scale, const float* v_scale,
+                                   const int32_t* prefix_len, const int32_t* row_first, const float* alibi_slopes,
+                                   void* out, void* stream);
+
+/* ---- The 4-bit paged cache: the same pages, steps and masks with half the bytes. aihost_page_map and
+ * aihost_page_release serve it as they are, and aihost_kv8_desc describes a layer. Every row of a head has
+ * its own range, an fp16 pair (low, step), as a block of GGUF's Q4_1 has for 32 values: the
+ * code c in 0 .. 15 stands for fl32(low + step * c).
+ *
+ *   k_pool, v_pool    uint8 [n_pages][n_kv_heads][page_rows][head_dim / 2]: in four bytes the codes of eight
+ *                     elements e0 .. e7, as the nibbles (lower first) e0 e2, e4 e6, e1 e3, e5 e7
+ *   k_range, v_range  fp16 [n_pages][n_kv_heads][page_rows][2]: low, step
+ *
+ * Stores n_tokens rows k_new, v_new [n_tokens][Hkv][d] at slots (-1: skipped), in any order but each slot once;
+ * no other row is touched. K is rotated at positions first: angle = fl32(position * frequency), its cosine
+ * and sine rounded to fp32 once, products and sums in fp32. Then for each row x of a head, in fp32:
+ *   low = fp16(min x); step = max(fp16((max x - low) * fl32(1/15)), 2^-24)
+ *   code = min(max(rint((x - low) * fl32(1 / step)), 0), 15)
+ * A row with a NaN or an infinity in it, or whose low or step passes fp16's range, gets NaN for both. */
+aihost_status aihost_kv4_append(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t n_tokens, const void* k_new,
+                                const void* v_new, const int64_t* slots, const int32_t* positions, uint8_t* k_pool,
+                                uint8_t* v_pool, void* k_range, void* v_range, void* stream);
+/* out [n_rows][Hkv][d] (out_dtype: F32 or F16) = the values that the rows at slots of one pool stand
+ * for; zeros for slot -1. */
+aihost_status aihost_kv4_read(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t n_rows, const int64_t* slots,
+                              const uint8_t* pool, const void* range, void* out, int32_t out_dtype, void* stream);
+/* Scratch bytes of an aihost_kv4_attention call with these arguments (0 if none) and which kernel it runs, on
+ * ctx's device (NULL: the current one). Either pointer may be NULL. */
+aihost_status aihost_kv4_plan(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens,
+                              int32_t max_new, int32_t max_kv, size_t* out_bytes, int32_t* out_kernel);
+/* aihost_kv8_attention over this cache: the same rows, positions, masks, cap and bias. The codes enter the
+ * products exactly, q and the softmax weights as there; the ranges enter in fp32 outside the products,
+ * q.k = step (q.c) + low sum(q) and o = sum (p step) c + sum p low. */
+aihost_status aihost_kv4_attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, int32_t batch, int32_t n_tokens,
+                                   int32_t max_new, int32_t max_kv, const void* q, const int32_t* row_start,
+                                   const int32_t* kv_len, const int32_t* block_table, const uint8_t* k_pool,
+                                   const uint8_t* v_pool, const void* k_range, const void* v_range,
                                    const int32_t* prefix_len, const int32_t* row_first, const float* alibi_slopes,
                                    void* out, void* stream);
 
