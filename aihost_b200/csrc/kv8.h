@@ -157,5 +157,6 @@ int32_t kv8_prefill_rows();
 void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max_new, int32_t max_kv, int32_t num_sms,
                       int32_t* tiles, int32_t* whole, int32_t* chunk, int32_t* splits, double* end);
 cudaError_t launch_kv8_prefill(const Kv8AttnArgs& a, cudaStream_t st);
+cudaError_t launch_kv4_prefill(const Kv8AttnArgs& a, cudaStream_t st);  // over the 4-bit cache, with the same plan
 
 }  // namespace aihost

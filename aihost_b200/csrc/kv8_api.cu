@@ -118,7 +118,7 @@ Plan make_plan(const aihost_kv8_desc* d, const Resolved& r, bool four, int32_t b
   max_kv = std::min(max_kv, kMaxKv);
   const int32_t rows = kv8_mma_rows(g, max_new), G = g.n_q_heads / g.n_kv_heads;
   p.tensor = false;
-  if (!four && d->io_dtype == AIHOST_F16 && static_cast<int64_t>(max_new) * G > rows) {
+  if (d->io_dtype == AIHOST_F16 && static_cast<int64_t>(max_new) * G > rows) {
     double end;
     kv8_prefill_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.whole, &p.chunk, &p.splits, &end);
     const double even = static_cast<double>(n_tokens) / (static_cast<double>(batch) * max_new);
@@ -246,7 +246,7 @@ aihost_status attention(aihost_attn_ctx* ctx, const aihost_kv8_desc* desc, bool 
   SharedUse shared(ctx, st, need > 0);
   if (shared.error() != cudaSuccess) return cuda_fail(shared.error(), "ordering the scratch's uses");
   cudaError_t e = timed_launch(ctx, four ? AIHOST_KERNEL_KV4_ATTN : AIHOST_KERNEL_KV8_ATTN, st, [&] {
-    if (four) return launch_kv4_mma(a, st);
+    if (four) return plan.tensor ? launch_kv4_prefill(a, st) : launch_kv4_mma(a, st);
     return plan.tensor ? launch_kv8_prefill(a, st) : launch_kv8_mma(a, st);
   });
   return e == cudaSuccess ? AIHOST_OK : cuda_fail(e, four ? "4-bit attention launch" : "8-bit attention launch");

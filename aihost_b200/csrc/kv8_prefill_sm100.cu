@@ -57,25 +57,33 @@ constexpr uint32_t kRegsMma = 56, kRegsSoftmax = 184, kRegsConvert = 88;
 static_assert(128 * (kRegsMma + 2 * kRegsSoftmax + kRegsConvert) <= 128 * kThreads, "setmaxnreg split exceeds the launch");
 constexpr float kSlack = 8.0f;    // the maximum may lag by 2^8 before O is rescaled
 constexpr float kQUnit = 0.5f;    // a rotated q enters times this
-constexpr float kVUnit = 128.0f;  // P * (v scale / largest) * 128 <= 2^15 stays in fp16's range
+constexpr float kVUnit = 128.0f, kVLog = 7.0f;  // P * (v scale / largest) * 128 <= 2^15 stays in fp16's range; P * step likewise
 constexpr int kFactors = kKeys / 16;
 constexpr int kFactorRing = 4;
 
+// 4 bits: what a tile's 128 rows' ranges come to, times 1 for K: score = k_step (q.(c - 8)) + k_mid sum(q); V: P enters
+// times its step, as 2^v_log more, and gives the row's weight and its share of the mids back through v_rcp and v_mid.
+struct RowFactors {
+  float k_step[kKeys], k_mid[kKeys], v_log[kKeys], v_rcp[kKeys], v_mid[kKeys];
+};
+
 // REST: what a rotated q leaves when it is rounded to fp16 enters as a second operand (head_dim 64: always).
-template <int D, bool REST>
+// FOUR: over the 4-bit cache.
+template <int D, bool REST, bool FOUR>
 struct Cfg {
   static constexpr int KB = D / 64;                   // 64-element (128-byte) column blocks
   static constexpr int TILE = KB * kKeys * 128;       // one [128 x D] fp16 tile
   static constexpr int NS = D == 64 ? 3 : REST ? 1 : 2;  // K and V ring depth
   static constexpr int K_OFF = 2 * TILE;              // after the two Q tiles
   static constexpr int V_OFF = K_OFF + NS * TILE;
-  static constexpr int RAW = kKeys * D;               // one tile's int8 rows
+  static constexpr int RAW = kKeys * D / (FOUR ? 2 : 1);  // one tile's rows as stored
   static constexpr int NR = D == 64 ? 4 : 2;          // ring of them, K and V in turn
   static constexpr int RAW_OFF = V_OFF + NS * TILE;
   static constexpr bool Q_REST = D == 64 || REST;
   static constexpr int Q_REST_OFF = RAW_OFF + NR * RAW;
   static constexpr int BAR_OFF = Q_REST_OFF + (Q_REST ? 2 * TILE : 0);
-  static constexpr int SMEM = BAR_OFF + 1024 + 1024;  // barriers and factors, alignment slack
+  static constexpr int RANGE_OFF = BAR_OFF + 1024;
+  static constexpr int SMEM = RANGE_OFF + (FOUR ? kFactorRing * static_cast<int>(sizeof(RowFactors)) : 0) + 1024;  // and alignment slack
   static __device__ __forceinline__ uint32_t s_col(int t) { return t ? 128u : 0u; }
   static __device__ __forceinline__ uint32_t o_col(int t) { return 256u + static_cast<uint32_t>(t * D); }
 };
@@ -220,12 +228,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int32_
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, status));
 }
 
-template <int D, bool MOD, bool REST>
+template <int D, bool MOD, bool REST, bool FOUR>
 __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_constant__ Kv8AttnArgs a) {
-  using C = Cfg<D, REST>;
+  using C = Cfg<D, REST, FOUR>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Shared& sh = *reinterpret_cast<Shared*>(smem + C::BAR_OFF);
+  RowFactors* const factors = reinterpret_cast<RowFactors*>(smem + C::RANGE_OFF);  // FOUR
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int32_t H = a.g.n_kv_heads, G = a.g.n_q_heads / H, ps = a.g.page_shift;
   // longest ranges first: a sequence's last tiles see the most
@@ -421,8 +430,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         if (i + 2 < n_load) e1 = entry_of(i + 2);
         const bool mine = e != INT32_MIN;
         const int64_t page = mine ? page_or_first(e, a.g.n_pages, stray) : 0;
-        const int64_t at = ((page * H + h) << ps) * D;  // a tile starts at a page's first row: pages divide it
-        const uint32_t bytes = static_cast<uint32_t>(per_page * D);
+        constexpr int kRowBytes = FOUR ? D / 2 : D;
+        const int64_t at = ((page * H + h) << ps) * kRowBytes;  // a tile starts at a page's first row: pages divide it
+        const uint32_t bytes = static_cast<uint32_t>(per_page * kRowBytes);
         const uint32_t total = __popc(__ballot_sync(0xffffffffu, mine)) * bytes;
         bool ok = true;
 #pragma unroll
@@ -441,6 +451,56 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       // the last copies have landed before the block may end, however its other warps fared
       for (int32_t g = max(issued - C::NR, 0); g < issued; ++g)
         warp_wait(&sh.raw_full[g % C::NR], (g / C::NR) & 1, status);
+    } else if (FOUR && warp == 2) {
+      // ---------------------------------------------------------------- ranges, four rows a lane
+      const float q_scale = a.rope_mode != AIHOST_ROPE_NONE ? a.scale * (1.0f / kQUnit) : a.scale;
+      const float k_unit = MOD && a.score_cap > 0.0f ? q_scale / a.score_cap : q_scale * kLog2e;
+      auto entry_of = [&](int32_t i) -> int32_t {
+        const int32_t row = (jb + i) * kKeys + lane * 4;
+        return i < n_load && row < row_end ? table[row >> ps] : INT32_MIN;
+      };
+      auto fetch = [&](int32_t i, int32_t e, uint4 (&r)[2]) {
+        r[0] = r[1] = make_uint4(0, 0, 0, 0);
+        if (e != INT32_MIN) {
+          const int32_t row = (jb + i) * kKeys + lane * 4;
+          const int64_t at = ((page_or_first(e, a.g.n_pages, stray) * H + h) << ps) + (row & (a.g.page_rows - 1));
+          r[0] = __ldg(reinterpret_cast<const uint4*>(a.k_range + at));
+          r[1] = __ldg(reinterpret_cast<const uint4*>(a.v_range + at));
+        }
+      };
+      uint4 now[2], next[2];
+      fetch(0, entry_of(0), now);
+      int32_t e_next = entry_of(1);
+      for (int32_t i = 0; i < n_load; ++i) {
+        fetch(i + 1, e_next, next);
+        e_next = entry_of(i + 2);
+        const int s = i % C::NS;
+        // as with the scales below: the ring's slot is free, and k_full's phase is this tile's
+        if (!warp_wait(C::NS > 1 ? &sh.v_empty[s] : &sh.k_empty[s], ((i / C::NS) & 1) ^ 1, status)) break;
+        const uint32_t kr[4] = {now[0].x, now[0].y, now[0].z, now[0].w}, vr[4] = {now[1].x, now[1].y, now[1].z, now[1].w};
+        float f[5][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 k = __half22float2(*reinterpret_cast<const __half2*>(&kr[e]));
+          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&vr[e]));
+          // a range of V's that is no number marks its row through K's: of a hidden row, whose weight is 0, nothing may
+          // come. A step of zero counts as 2^-60: such weights are 0 as fp16, and come back whole in the sums.
+          const bool fine = fabsf(v.x) + fabsf(v.y) < INFINITY;
+          const float step = v.y != 0.0f ? fabsf(v.y) : 8.6736173798840355e-19f;
+          f[0][e] = fine ? k.y * k_unit : __uint_as_float(0x7fffffffu);
+          f[1][e] = fmaf(8.0f, k.y, k.x) * k_unit;
+          f[2][e] = fine ? __log2f(step) : 0.0f;
+          f[3][e] = fine ? 1.0f / (step * kVUnit) : 0.0f;
+          f[4][e] = fine ? fmaf(8.0f, v.y, v.x) * f[3][e] : 0.0f;
+        }
+        RowFactors& to = factors[i % kFactorRing];
+        float* const rows[5] = {to.k_step, to.k_mid, to.v_log, to.v_rcp, to.v_mid};
+#pragma unroll
+        for (int n = 0; n < 5; ++n) *reinterpret_cast<float4*>(rows[n] + lane * 4) = make_float4(f[n][0], f[n][1], f[n][2], f[n][3]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.k_full[s]);
+        now[0] = next[0], now[1] = next[1];
+      }
     } else if (warp == 2) {
       // ---------------------------------------------------------------- factors
       float ks[2] = {0.0f, 0.0f}, vs[2] = {0.0f, 0.0f};
@@ -491,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     // ------------------------------------------------------------------ converters
     regs_dealloc<kRegsConvert>();
     const int w = warp - 12;
-    {
+    if constexpr (!FOUR) {
       float vmax = 0.0f;  // the chunk's largest V scale
       for (int32_t k = ((jb * kKeys) >> ps) + w * 32 + lane; k < (row_end + a.g.page_rows - 1) >> ps; k += 128)
         vmax = fmaxf(vmax, __ldg(a.v_scale + page_or_first(table[k], a.g.n_pages, stray) * H + h));
@@ -500,17 +560,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       if (lane == 0) sh.v_max[w] = vmax;
       asm volatile("bar.sync 2, 160;" ::: "memory");
     }
-    // 16 bytes a lane. Eight lanes that load or store together take two rows, the even row's chunks of
-    // one half and the odd row's of the other (D = 128; D = 64: two whole rows): different banks both ways.
-    constexpr int RPL = 512 / D;           // rows per warp and load
+    // 16 bytes a lane. Eight lanes that load or store together: 8 bits, two rows, the even row's chunks of
+    // one half and the odd row's of the other (D = 128; D = 64: two whole rows); 4 bits, chunk c of rows 2 (c + n) and
+    // 2 (c + n) + 1 of eight for D = 128, both chunks of four rows for D = 64: different banks both ways.
+    constexpr int kRowBytes = FOUR ? D / 2 : D;
+    constexpr int RPL = 512 / kRowBytes;   // rows per warp and load
     constexpr int NL = kKeys / (4 * RPL);  // loads per tile and lane
-    const int r_in = D == 128 ? ((lane >> 2) & 1) + ((lane >> 4) << 1) : lane >> 2;
-    const int c = D == 128 ? (lane & 3) + ((((lane >> 3) ^ (lane >> 2)) & 1) << 2) : lane & 3;
+    const int r_in = FOUR ? (D == 128 ? 2 * ((lane + (lane >> 3)) & 3) + ((lane >> 2) & 1) : lane >> 1)
+                          : (D == 128 ? ((lane >> 2) & 1) + ((lane >> 4) << 1) : lane >> 2);
+    const int c = FOUR ? (D == 128 ? lane & 3 : lane & 1)
+                       : (D == 128 ? (lane & 3) + ((((lane >> 3) ^ (lane >> 2)) & 1) << 2) : lane & 3);
     uint4 v[NL];
     auto take = [&](int slot) {  // a raw tile into registers, while the products still use the tile that it replaces
       const uint8_t* const src = smem + C::RAW_OFF + slot * C::RAW;
 #pragma unroll
-      for (int k = 0; k < NL; ++k) v[k] = *reinterpret_cast<const uint4*>(src + ((k * 4 + w) * RPL + r_in) * D + c * 16);
+      for (int k = 0; k < NL; ++k) v[k] = *reinterpret_cast<const uint4*>(src + ((k * 4 + w) * RPL + r_in) * kRowBytes + c * 16);
       // The next rows come by the async proxy: without the fence some were found here in the place of these, whose
       // values are used after other waits only (cold caches, up to 2 % of the calls).
       fence_proxy_async_smem();
@@ -521,10 +585,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
 #pragma unroll
       for (int k = 0; k < NL; ++k) {
         const int row = (k * 4 + w) * RPL + r_in;
-        uint4 lo, hi;
-        convert16(v[k], lo, hi);
-        *reinterpret_cast<uint4*>(dst + chunk_off(row, 2 * c)) = lo;
-        *reinterpret_cast<uint4*>(dst + chunk_off(row, 2 * c + 1)) = hi;
+        if constexpr (FOUR) {
+          const uint32_t word[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4*>(dst + chunk_off(row, 4 * c + j)) =
+                make_uint4(codes_less_8(word[j], 0), codes_less_8(word[j], 1), codes_less_8(word[j], 2), codes_less_8(word[j], 3));
+        } else {
+          uint4 lo, hi;
+          convert16(v[k], lo, hi);
+          *reinterpret_cast<uint4*>(dst + chunk_off(row, 2 * c)) = lo;
+          *reinterpret_cast<uint4*>(dst + chunk_off(row, 2 * c + 1)) = hi;
+        }
       }
       fence_proxy_async_smem();
       mbar_arrive(full_bar);
@@ -637,11 +709,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       fence_proxy_async_smem();
       mbar_arrive(&sh.q_ready[t]);
     }
+    float q_sum = 0.0f;  // of the thread's row of q, as it enters
+    if constexpr (FOUR) {
+      __syncwarp();
+      const bool rest = C::Q_REST && a.rope_mode != AIHOST_ROPE_NONE;
+#pragma unroll 1
+      for (int n = rest ? 1 : 0; n >= 0; --n)
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 x = *reinterpret_cast<const uint4*>(q_tile + n * C::Q_REST_OFF + chunk_off(r, c));
+          const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[e]));
+            q_sum += f.x + f.y;
+          }
+        }
+    }
 
     const float slope = MOD && a.alibi_slopes ? a.alibi_slopes[head] * kLog2e : 0.0f;
     const bool capped = MOD && a.score_cap > 0.0f;
     const float cap2 = a.score_cap * kLog2e, fpos = static_cast<float>(pos);
-    float m = kNoMax, l = 0.0f;
+    float m = kNoMax, l = 0.0f, z = 0.0f;  // z: the sum of the weights times V's mids (FOUR)
     const uint32_t s_tmem = tmem + lane_base + C::s_col(t), o_tmem = tmem + lane_base + C::o_col(t);
     const int32_t lo_j = t ? j0[1] : j0[0], hi_j = t ? j1[1] : j1[0], n_own = hi_j - lo_j;
     bool ok = true;
@@ -657,11 +746,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       const int slot = (lo_j + i - jb) % kFactorRing;
       const int32_t kv0 = (lo_j + i) * kKeys;
       const bool need_mask = __any_sync(0xffffffffu, kv0 < first || kv0 + kKeys > end);
+      const RowFactors& rows = factors[slot];
+      auto two = [](const float (&x)[kKeys], int e) { return *reinterpret_cast<const float2*>(&x[e]); };
       float kf[kFactors];
+      if constexpr (!FOUR) {
 #pragma unroll
-      for (int f = 0; f < kFactors; ++f) kf[f] = sh.k_factor[slot][f];
+        for (int f = 0; f < kFactors; ++f) kf[f] = sh.k_factor[slot][f];
+      }
       tmem_wait_ld();
-      if (MOD || need_mask) {  // the factors are spent here: scores in log2 units, hidden ones -inf
+      if constexpr (FOUR) {
+        const float2 q2 = make_float2(q_sum, q_sum);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 mid = two(rows.k_mid, c * 32 + e);
+            const float2 x = ffma2(make_float2(__uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1])), two(rows.k_step, c * 32 + e),
+                                   MOD ? fmul2(q2, mid) : ffma2(q2, mid, two(rows.v_log, c * 32 + e)));
+            sr[c][e] = __float_as_uint(x.x);
+            sr[c][e + 1] = __float_as_uint(x.y);
+          }
+      }
+      if (!FOUR && (MOD || need_mask)) {  // the factors are spent here: scores in log2 units, hidden ones -inf
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -671,6 +777,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             sr[c][e] = __float_as_uint(x.x);
             sr[c][e + 1] = __float_as_uint(x.y);
           }
+#pragma unroll
+        for (int f = 0; f < kFactors; ++f) kf[f] = 1.0f;
+      }
+      if (MOD || need_mask) {
         if constexpr (MOD) {
           if (capped) cap_scores(sr, cap2);
           if (a.alibi_slopes) {
@@ -682,6 +792,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
                 sr[c][e] = __float_as_uint(
                     fmaf(-slope, fabsf(d0 - static_cast<float>(c * 32 + e)), __uint_as_float(sr[c][e])));
           }
+          if constexpr (FOUR) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float2 x = fadd2(make_float2(__uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1])), two(rows.v_log, c * 32 + e));
+                sr[c][e] = __float_as_uint(x.x);
+                sr[c][e + 1] = __float_as_uint(x.y);
+              }
+          }
         }
         if (need_mask) {
           const int32_t lo_e = first - kv0, hi_e = end - kv0;
@@ -691,8 +811,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             for (int e = 0; e < 32; ++e)
               if (c * 32 + e < lo_e || c * 32 + e >= hi_e) sr[c][e] = __float_as_uint(-INFINITY);
         }
-#pragma unroll
-        for (int f = 0; f < kFactors; ++f) kf[f] = 1.0f;
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -704,13 +822,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         float p3 = fmax3(__uint_as_float(g[9]), __uint_as_float(g[10]), __uint_as_float(g[11]));
         p0 = fmax3(p0, __uint_as_float(g[12]), __uint_as_float(g[13]));
         p1 = fmax3(p1, __uint_as_float(g[14]), __uint_as_float(g[15]));
-        mx = fmaxf(mx, fmaf(fmax3(fmaxf(p0, p1), p2, p3), kf[f], sh.v_exp[slot][f]));
+        if constexpr (FOUR) mx = fmaxf(mx, fmax3(fmaxf(p0, p1), p2, p3));
+        else mx = fmaxf(mx, fmaf(fmax3(fmaxf(p0, p1), p2, p3), kf[f], sh.v_exp[slot][f]));
       }
       const bool grow = mx > m + kSlack;
       float f_o = 1.0f;
       if (grow) {
         f_o = ex2_approx(m - mx);
         l *= f_o;
+        z *= f_o;
         m = mx;
       }
       // the P V before was committed ahead of this S: O is at rest
@@ -725,13 +845,24 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           tmem_st8(o_tmem + c * 8, o);
         }
       }
-      const float2 neg_m = make_float2(-m, -m);
+      const float neg = FOUR ? kVLog - m : -m;
+      const float2 neg_m = make_float2(neg, neg);
+      float2 z_sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
       float2 sum[4] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t pk[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
+          if constexpr (FOUR) {
+            const int j = c * 32 + 2 * e;
+            const float2 x = fadd2(make_float2(__uint_as_float(sr[c][2 * e]), __uint_as_float(sr[c][2 * e + 1])), neg_m);
+            const float2 p = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            sum[e & 3] = ffma2(p, two(rows.v_rcp, j), sum[e & 3]);
+            z_sum[e & 1] = ffma2(p, two(rows.v_mid, j), z_sum[e & 1]);
+            pk[e] = pack2(p.x, p.y);
+            continue;
+          }
           const int f = c * 2 + e / 8;
           const float2 x = ffma2(make_float2(__uint_as_float(sr[c][2 * e]), __uint_as_float(sr[c][2 * e + 1])),
                                  make_float2(kf[f], kf[f]), neg_m);
@@ -748,13 +879,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           mbar_arrive(&sh.p_full[t][c >> 1]);
         }
       }
+      if constexpr (FOUR) z += (z_sum[0].x + z_sum[0].y) + (z_sum[1].x + z_sum[1].y);
       l += ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y)) + ((sum[2].x + sum[2].y) + (sum[3].x + sum[3].y));
     }
     // ---- O / l, or this chunk's share of it
     if (ok && n_own > 0) ok = warp_wait(&sh.o_full[t], 0, status);
     tc_fence_after();
     // written by the converters before the first S; with no tile there is nothing to scale
-    const float vmax =
+    const float vmax = FOUR ? 1.0f :
         n_own > 0 ? fmaxf(fmaxf(sh.v_max[0], sh.v_max[1]), fmaxf(sh.v_max[2], sh.v_max[3])) : 0.0f;
     auto kept = [&](int k) {  // read here, or the compiler would carry the values through the loop
       int32_t v;
@@ -799,6 +931,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     float4* const part = reinterpret_cast<float4*>(a.part_o) + (part_unit * a.max_splits) * (D / 4) * kRows + r256;
     float2* const part_ml = reinterpret_cast<float2*>(a.part_ml) + part_unit * a.max_splits * kRows + r256;
     if (ok) {
+      const float inv_l = n_splits > 1 ? 1.0f : l != 0.0f ? 1.0f / l : 0.0f;
       const float unit_o = n_splits > 1 ? 1.0f / kVUnit : l != 0.0f ? 1.0f / kVUnit / l : 0.0f;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
@@ -808,7 +941,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           tmem_ld32(o_tmem + c * 32, u);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(u[e]) * unit_o * vmax;  // in this order: unit_o * vmax may be too small a number
+          for (int e = 0; e < 32; ++e)
+            if constexpr (FOUR) o[e] = fmaf(__uint_as_float(u[e]), 1.0f / kVUnit, z) * inv_l;
+            else o[e] = __uint_as_float(u[e]) * unit_o * vmax;  // in this order: unit_o * vmax may be too small a number
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.0f;
@@ -868,10 +1003,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
   }
 }
 
-template <int D, bool MOD, bool REST>
+template <int D, bool MOD, bool REST, bool FOUR>
 cudaError_t launch_d(const Kv8AttnArgs& a, cudaStream_t st) {
-  auto kern = kv8_prefill_kernel<D, MOD, REST>;
-  constexpr int kBytes = Cfg<D, REST>::SMEM;
+  auto kern = kv8_prefill_kernel<D, MOD, REST, FOUR>;
+  constexpr int kBytes = Cfg<D, REST, FOUR>::SMEM;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
   if (e != cudaSuccess) return e;
   // not a dependent launch: waiting blocks would take whole SMs, 6 % slower on batches of short prompts
@@ -939,11 +1074,15 @@ void kv8_prefill_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t
 
 int32_t kv8_prefill_rows() { return kRows; }
 
-cudaError_t launch_kv8_prefill(const Kv8AttnArgs& a, cudaStream_t st) {
+template <bool FOUR>
+static cudaError_t launch_prompts(const Kv8AttnArgs& a, cudaStream_t st) {
   const bool mod = a.score_cap > 0.0f || a.alibi_slopes;
-  if (a.g.head_dim == 64) return mod ? launch_d<64, true, true>(a, st) : launch_d<64, false, true>(a, st);
-  if (a.exact_q) return mod ? launch_d<128, true, true>(a, st) : launch_d<128, false, true>(a, st);
-  return mod ? launch_d<128, true, false>(a, st) : launch_d<128, false, false>(a, st);
+  if (a.g.head_dim == 64) return mod ? launch_d<64, true, true, FOUR>(a, st) : launch_d<64, false, true, FOUR>(a, st);
+  if (a.exact_q) return mod ? launch_d<128, true, true, FOUR>(a, st) : launch_d<128, false, true, FOUR>(a, st);
+  return mod ? launch_d<128, true, false, FOUR>(a, st) : launch_d<128, false, false, FOUR>(a, st);
 }
+
+cudaError_t launch_kv8_prefill(const Kv8AttnArgs& a, cudaStream_t st) { return launch_prompts<false>(a, st); }
+cudaError_t launch_kv4_prefill(const Kv8AttnArgs& a, cudaStream_t st) { return launch_prompts<true>(a, st); }
 
 }  // namespace aihost

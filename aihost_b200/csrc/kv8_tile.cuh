@@ -77,6 +77,13 @@ __device__ __forceinline__ uint32_t half2_of(uint32_t u, uint32_t sel) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// Nibbles n and n + 4 of x, less 8, as fp16: by one fma from 1024 + c or 1024 + 16 c.
+__device__ __forceinline__ uint32_t codes_less_8(uint32_t x, int n) {
+  const uint32_t y = ((n < 2 ? x : x >> 8) & (n & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
+  const __half2 unit = __half2half2(__ushort_as_half(n & 1 ? 0x2c00 : 0x3c00)), less = __half2half2(__ushort_as_half(n & 1 ? 0xd480 : 0xe408));
+  const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&y), unit, less);  // 1/16, -72; 1, -1032
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
