@@ -57,15 +57,23 @@ constexpr uint32_t kRegsMma = 56, kRegsSoftmax = 184, kRegsConvert = 88;
 static_assert(128 * (kRegsMma + 2 * kRegsSoftmax + kRegsConvert) <= 128 * kThreads, "setmaxnreg split exceeds the launch");
 constexpr float kSlack = 8.0f;    // the maximum may lag by 2^8 before O is rescaled
 constexpr float kQUnit = 0.5f;    // a rotated q enters times this
-constexpr float kVUnit = 128.0f, kVLog = 7.0f;  // P * (v scale / largest) * 128 <= 2^15 stays in fp16's range; P * step likewise
+constexpr float kVUnit = 128.0f;  // P * (v scale / largest) * 128 <= 2^15 stays in fp16's range
 constexpr int kFactors = kKeys / 16;
 constexpr int kFactorRing = 4;
 
-// 4 bits: what a tile's 128 rows' ranges come to, times 1 for K: score = k_step (q.(c - 8)) + k_mid sum(q); V: P enters
-// times its step, as 2^v_log more, and gives the row's weight and its share of the mids back through v_rcp and v_mid.
+// 4 bits: a tile's ranges as the softmax takes them. score = k_step (q.(c - 8)) + k_mid sum(q), times scale and log2 e; V's step
+// is v_power (a power of two, in the operand) times v_part / kPartUnit, which P enters times; its low + 8 step, v_mid,
+// stays outside the products.
 struct RowFactors {
-  float k_step[kKeys], k_mid[kKeys], v_log[kKeys], v_rcp[kKeys], v_mid[kKeys];
+  float k_step[kKeys], k_mid[kKeys], v_part[kKeys], v_mid[kKeys];
 };
+constexpr float kPartUnit = 32.0f;  // P * v_part <= 2^8 * 4 * 32 = 2^15
+
+// The power of two in V's step: 2^floor(log2 |step|), at most 2^12 (then 8 times it is in fp16's range), at least 2^-24.
+__device__ __forceinline__ float v_power(float step) {
+  const uint32_t e = (__float_as_uint(step) >> 23) & 0xffu;
+  return __uint_as_float(min(max(e, 103u), 139u) << 23);
+}
 
 // REST: what a rotated q leaves when it is rounded to fp16 enters as a second operand (head_dim 64: always).
 // FOUR: over the 4-bit cache.
@@ -76,7 +84,8 @@ struct Cfg {
   static constexpr int NS = D == 64 ? 3 : REST ? 1 : 2;  // K and V ring depth
   static constexpr int K_OFF = 2 * TILE;              // after the two Q tiles
   static constexpr int V_OFF = K_OFF + NS * TILE;
-  static constexpr int RAW = kKeys * D / (FOUR ? 2 : 1);  // one tile's rows as stored
+  static constexpr int CODES = kKeys * D / (FOUR ? 2 : 1);  // one tile's rows as stored,
+  static constexpr int RAW = CODES + (FOUR ? kKeys * 4 : 0);  // and the rows' ranges (V's)
   static constexpr int NR = D == 64 ? 4 : 2;          // ring of them, K and V in turn
   static constexpr int RAW_OFF = V_OFF + NS * TILE;
   static constexpr bool Q_REST = D == 64 || REST;
@@ -209,6 +218,9 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
+
+// Whether a range (low, step) is two numbers.
+__device__ __forceinline__ bool v_fine(uint32_t range) { return (range & 0x7c00u) != 0x7c00u && (range & 0x7c000000u) != 0x7c000000u; }
 
 // 32 lanes x 8 consecutive 32-bit columns of tensor memory.
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
@@ -433,17 +445,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         constexpr int kRowBytes = FOUR ? D / 2 : D;
         const int64_t at = ((page * H + h) << ps) * kRowBytes;  // a tile starts at a page's first row: pages divide it
         const uint32_t bytes = static_cast<uint32_t>(per_page * kRowBytes);
-        const uint32_t total = __popc(__ballot_sync(0xffffffffu, mine)) * bytes;
+        const uint32_t n_mine = __popc(__ballot_sync(0xffffffffu, mine));
         bool ok = true;
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
           const int32_t g = 2 * i + v, slot = g % C::NR;
           ok = ok && warp_wait(&sh.raw_empty[slot], ((g / C::NR) & 1) ^ 1, status);
           if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&sh.raw_full[slot], total);
+          const uint32_t range_bytes = FOUR && v ? static_cast<uint32_t>(per_page * 4) : 0;
+          if (lane == 0) mbar_arrive_expect_tx(&sh.raw_full[slot], n_mine * (bytes + range_bytes));
           __syncwarp();
           if (mine) bulk_load(smem + C::RAW_OFF + slot * C::RAW + lane * bytes, (v ? a.v_pool : a.k_pool) + at, bytes,
                               &sh.raw_full[slot]);
+          if (FOUR && v && mine)
+            bulk_load(smem + C::RAW_OFF + slot * C::RAW + C::CODES + lane * range_bytes, a.v_range + at / kRowBytes, range_bytes,
+                      &sh.raw_full[slot]);
           issued = g + 1;
         }
         if (!ok) break;
@@ -478,25 +494,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         // as with the scales below: the ring's slot is free, and k_full's phase is this tile's
         if (!warp_wait(C::NS > 1 ? &sh.v_empty[s] : &sh.k_empty[s], ((i / C::NS) & 1) ^ 1, status)) break;
         const uint32_t kr[4] = {now[0].x, now[0].y, now[0].z, now[0].w}, vr[4] = {now[1].x, now[1].y, now[1].z, now[1].w};
-        float f[5][4];
+        float f[4][4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 k = __half22float2(*reinterpret_cast<const __half2*>(&kr[e]));
           const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&vr[e]));
-          // a range of V's that is no number marks its row through K's: of a hidden row, whose weight is 0, nothing may
-          // come. A step of zero counts as 2^-60: such weights are 0 as fp16, and come back whole in the sums.
-          const bool fine = fabsf(v.x) + fabsf(v.y) < INFINITY;
-          const float step = v.y != 0.0f ? fabsf(v.y) : 8.6736173798840355e-19f;
+          // a row of V that is no number marks itself through K: of a hidden row, whose weight is 0, nothing may come
+          const bool fine = v_fine(vr[e]);
           f[0][e] = fine ? k.y * k_unit : __uint_as_float(0x7fffffffu);
           f[1][e] = fmaf(8.0f, k.y, k.x) * k_unit;
-          f[2][e] = fine ? __log2f(step) : 0.0f;
-          f[3][e] = fine ? 1.0f / (step * kVUnit) : 0.0f;
-          f[4][e] = fine ? fmaf(8.0f, v.y, v.x) * f[3][e] : 0.0f;
+          f[2][e] = fine ? v.y * kPartUnit / v_power(v.y) : 0.0f;
+          f[3][e] = fine ? fmaf(8.0f, v.y, v.x) : 0.0f;
         }
         RowFactors& to = factors[i % kFactorRing];
-        float* const rows[5] = {to.k_step, to.k_mid, to.v_log, to.v_rcp, to.v_mid};
+        float* const rows[4] = {to.k_step, to.k_mid, to.v_part, to.v_mid};
 #pragma unroll
-        for (int n = 0; n < 5; ++n) *reinterpret_cast<float4*>(rows[n] + lane * 4) = make_float4(f[n][0], f[n][1], f[n][2], f[n][3]);
+        for (int n = 0; n < 4; ++n) *reinterpret_cast<float4*>(rows[n] + lane * 4) = make_float4(f[n][0], f[n][1], f[n][2], f[n][3]);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.k_full[s]);
         now[0] = next[0], now[1] = next[1];
@@ -571,26 +584,43 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     const int c = FOUR ? (D == 128 ? lane & 3 : lane & 1)
                        : (D == 128 ? (lane & 3) + ((((lane >> 3) ^ (lane >> 2)) & 1) << 2) : lane & 3);
     uint4 v[NL];
-    auto take = [&](int slot) {  // a raw tile into registers, while the products still use the tile that it replaces
+    uint32_t range[NL] = {};
+    auto take = [&](int slot, bool of_v) {  // a raw tile into registers, while the products still use the tile that it replaces
       const uint8_t* const src = smem + C::RAW_OFF + slot * C::RAW;
 #pragma unroll
-      for (int k = 0; k < NL; ++k) v[k] = *reinterpret_cast<const uint4*>(src + ((k * 4 + w) * RPL + r_in) * kRowBytes + c * 16);
+      for (int k = 0; k < NL; ++k) {
+        const int row = (k * 4 + w) * RPL + r_in;
+        v[k] = *reinterpret_cast<const uint4*>(src + row * kRowBytes + c * 16);
+        if (FOUR && of_v) range[k] = *reinterpret_cast<const uint32_t*>(src + C::CODES + row * 4);
+      }
       // The next rows come by the async proxy: without the fence some were found here in the place of these, whose
       // values are used after other waits only (cold caches, up to 2 % of the calls).
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.raw_empty[slot]);
     };
-    auto give = [&](uint8_t* dst, uint64_t* full_bar) {
+    auto give = [&](uint8_t* dst, uint64_t* full_bar, bool of_v) {
 #pragma unroll
       for (int k = 0; k < NL; ++k) {
         const int row = (k * 4 + w) * RPL + r_in;
         if constexpr (FOUR) {
+          // K: c - 8. V: that times the power of two in its row's step; 0 where the range is no number
           const uint32_t word[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          const float step = __half2float(__ushort_as_half(static_cast<uint16_t>(range[k] >> 16)));
+          const __half2 power = __float2half2_rn(of_v && v_fine(range[k]) ? v_power(step) : 0.0f);
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint4*>(dst + chunk_off(row, 4 * c + j)) =
-                make_uint4(codes_less_8(word[j], 0), codes_less_8(word[j], 1), codes_less_8(word[j], 2), codes_less_8(word[j], 3));
+          for (int j = 0; j < 4; ++j) {
+            uint32_t x[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              x[n] = codes_less_8(word[j], n);
+              if (of_v) {
+                const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[n]), power);
+                x[n] = *reinterpret_cast<const uint32_t*>(&y);
+              }
+            }
+            *reinterpret_cast<uint4*>(dst + chunk_off(row, 4 * c + j)) = make_uint4(x[0], x[1], x[2], x[3]);
+          }
         } else {
           uint4 lo, hi;
           convert16(v[k], lo, hi);
@@ -606,13 +636,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       const uint32_t par = ((i / C::NS) & 1) ^ 1;
       const int gk = 2 * i, gv = 2 * i + 1;
       if (!warp_wait(&sh.raw_full[gk % C::NR], (gk / C::NR) & 1, status)) break;
-      take(gk % C::NR);
+      take(gk % C::NR, false);
       if (!warp_wait(&sh.k_empty[s], par, status)) break;
-      give(smem + C::K_OFF + s * C::TILE, &sh.k_full[s]);
+      give(smem + C::K_OFF + s * C::TILE, &sh.k_full[s], false);
       if (!warp_wait(&sh.raw_full[gv % C::NR], (gv / C::NR) & 1, status)) break;
-      take(gv % C::NR);
+      take(gv % C::NR, true);
       if (!warp_wait(&sh.v_empty[s], par, status)) break;
-      give(smem + C::V_OFF + s * C::TILE, &sh.v_full[s]);
+      give(smem + C::V_OFF + s * C::TILE, &sh.v_full[s], true);
     }
     if (stray) atomicOr(status, kStatusBadIndex);
   } else {
@@ -730,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     const float slope = MOD && a.alibi_slopes ? a.alibi_slopes[head] * kLog2e : 0.0f;
     const bool capped = MOD && a.score_cap > 0.0f;
     const float cap2 = a.score_cap * kLog2e, fpos = static_cast<float>(pos);
-    float m = kNoMax, l = 0.0f, z = 0.0f;  // z: the sum of the weights times V's mids (FOUR)
+    float m = kNoMax, l = 0.0f, z = 0.0f;  // z: the sum of P times v_mid (FOUR)
     const uint32_t s_tmem = tmem + lane_base + C::s_col(t), o_tmem = tmem + lane_base + C::o_col(t);
     const int32_t lo_j = t ? j0[1] : j0[0], hi_j = t ? j1[1] : j1[0], n_own = hi_j - lo_j;
     bool ok = true;
@@ -760,9 +790,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float2 mid = two(rows.k_mid, c * 32 + e);
             const float2 x = ffma2(make_float2(__uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1])), two(rows.k_step, c * 32 + e),
-                                   MOD ? fmul2(q2, mid) : ffma2(q2, mid, two(rows.v_log, c * 32 + e)));
+                                   fmul2(q2, two(rows.k_mid, c * 32 + e)));
             sr[c][e] = __float_as_uint(x.x);
             sr[c][e + 1] = __float_as_uint(x.y);
           }
@@ -791,16 +820,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
               for (int e = 0; e < 32; ++e)
                 sr[c][e] = __float_as_uint(
                     fmaf(-slope, fabsf(d0 - static_cast<float>(c * 32 + e)), __uint_as_float(sr[c][e])));
-          }
-          if constexpr (FOUR) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int e = 0; e < 32; e += 2) {
-                const float2 x = fadd2(make_float2(__uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1])), two(rows.v_log, c * 32 + e));
-                sr[c][e] = __float_as_uint(x.x);
-                sr[c][e + 1] = __float_as_uint(x.y);
-              }
           }
         }
         if (need_mask) {
@@ -845,9 +864,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           tmem_st8(o_tmem + c * 8, o);
         }
       }
-      const float neg = FOUR ? kVLog - m : -m;
-      const float2 neg_m = make_float2(neg, neg);
       float2 z_sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+      const float2 neg_m = make_float2(-m, -m);
       float2 sum[4] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -858,9 +876,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             const int j = c * 32 + 2 * e;
             const float2 x = fadd2(make_float2(__uint_as_float(sr[c][2 * e]), __uint_as_float(sr[c][2 * e + 1])), neg_m);
             const float2 p = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-            sum[e & 3] = ffma2(p, two(rows.v_rcp, j), sum[e & 3]);
+            sum[e & 3] = fadd2(sum[e & 3], p);
             z_sum[e & 1] = ffma2(p, two(rows.v_mid, j), z_sum[e & 1]);
-            pk[e] = pack2(p.x, p.y);
+            const float2 pv = fmul2(p, two(rows.v_part, j));
+            pk[e] = pack2(pv.x, pv.y);
             continue;
           }
           const int f = c * 2 + e / 8;
@@ -942,7 +961,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if constexpr (FOUR) o[e] = fmaf(__uint_as_float(u[e]), 1.0f / kVUnit, z) * inv_l;
+            if constexpr (FOUR) o[e] = fmaf(__uint_as_float(u[e]), 1.0f / kPartUnit, z) * inv_l;
             else o[e] = __uint_as_float(u[e]) * unit_o * vmax;  // in this order: unit_o * vmax may be too small a number
         } else {
 #pragma unroll

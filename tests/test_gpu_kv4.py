@@ -1,8 +1,7 @@
 """The 4-bit paged cache on the GPU against plain forms (tests/kv4_plain.py).
 
   append     codes and ranges are defined to the bit
-  attention  fp16: the output's rounding 2^-11 |o|; P's rounding 2^-11 of sum p |v - low - 8 step|, itself at most
-             sum p |v - mid|, and fp32 sums; the score's error ds shifts p by up to 2 ds, ds = 2^-19 of sum |q| kmax, kmax =
+  attention  fp16: the output's rounding 2^-11 |o|; P's rounding 2^-11 of sum p |v - low - 8 step|, and fp32 sums; the score's error ds shifts p by up to 2 ds, ds = 2^-19 of sum |q| kmax, kmax =
              max(|low|, |low + 15 step|) of the row (codes and low enter apart); for a rotated q 2^-18, the rotation's
              fp32 arithmetic
              fp32: pairs of fp16 hold 22 bits; ex2.approx and fp32 sums 2^-18 of sum p vmax and 2^-19 of sum |q| kmax
@@ -40,7 +39,7 @@ class World4(World):
         return np.stack([self.g.normal(0, 0.5, shape) - 7.5 * step, step], -1).astype(np.float16)
 
     def reference(self, q64, prefix=None, first=None, slopes=None):
-        """(out, sum p |v - mid|, sum p vmax, the largest scale sum |q| kmax), of every element and row."""
+        """(out, what P's rounding goes by, sum p vmax, the largest scale sum |q| kmax), of every element and row."""
         one = np.ones(self.ks.shape[:2])
         k, v = (plain4.values(p, r, np.float64) for p, r in ((self.k, self.ks), (self.v, self.vs)))
         rest = (q64, self.start, self.kv_len, self.table, self.P)
