@@ -1,4 +1,4 @@
-"""A small server loop over the 8-bit paged cache: python -m aihost_b200.serve_kv8
+"""A small server loop over the 8-bit or the 4-bit paged cache: python -m aihost_b200.serve_kv8 [--bits 4]
 
 Requests of uneven prompt and answer lengths come and go in a fixed batch. Every step feeds the rows of all running
 requests (whole prompts beside single tokens) through a stack of attention layers with random weights: the weight
@@ -13,6 +13,7 @@ import time
 import torch
 
 from . import F16
+from .kv4 import Kv4Cache, Kv4Spec
 from .kv8 import Kv8Cache, Kv8Spec
 from .ops import Context, WeightOps
 
@@ -25,14 +26,16 @@ def main(argv=None) -> dict:
     ap.add_argument("--prompt", type=int, default=600, help="longest prompt")
     ap.add_argument("--answer", type=int, default=64, help="longest answer")
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--bits", type=int, choices=(4, 8), default=8, help="of the cache's values")
     a = ap.parse_args(argv)
     Hq, H, D, P = 14, 2, 64, 64  # a small model's heads
     width, dev = Hq * D, torch.device("cuda", 0)
     rng, g = random.Random(a.seed), torch.Generator(device=dev).manual_seed(a.seed)
     pages = -(-(a.prompt + a.answer) // P)
     with Context(0) as ctx:
-        spec = Kv8Spec(Hq, H, D, P, n_pages=a.batch * pages, max_pages=pages, rope_theta=1e6)
-        cache, weights = Kv8Cache(ctx, spec, a.batch, a.layers), WeightOps(ctx)
+        make_spec, make_cache = (Kv4Spec, Kv4Cache) if a.bits == 4 else (Kv8Spec, Kv8Cache)
+        spec = make_spec(Hq, H, D, P, n_pages=a.batch * pages, max_pages=pages, rope_theta=1e6)
+        cache, weights = make_cache(ctx, spec, a.batch, a.layers), WeightOps(ctx)
         w = lambda n, k: (torch.randn(n, k, generator=g, device=dev) / k ** 0.5).half()  # noqa: E731
         w_qkv = [w((Hq + 2 * H) * D, width) for _ in range(a.layers)]
         w_out = [w(width, width) for _ in range(a.layers)]

@@ -504,6 +504,16 @@ def test_attention_on_several_streams_of_one_context():
         own.sync_status()
 
 
+def test_server_loop():
+    """Every request ends and gives its pages back. Half a step of a row of normal values is at most 7 / 30; it moves a score by
+    sqrt(64) * 0.13 / 8 in root mean square, 0.65 at five times that, which moves weight of at most tanh(0.33) / 2 = 0.16 over
+    a spread of at most 8: 1.3 + 0.24 in all."""
+    from aihost_b200 import serve_kv8
+
+    r = serve_kv8.main(["--batch", "5", "--requests", "9", "--layers", "2", "--prompt", "200", "--answer", "12", "--bits", "4"])
+    assert r["free"] == r["pages"] and r["worst"] < 1.6
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 
 def test_arguments_are_checked_in_python_too(ctx):
