@@ -20,6 +20,15 @@
 // the codes at bits 0 to 3 3.5e-4 (a product's rounding goes by the exponent 2^-14 of numbers below the normal
 // ones); so 2.5e-4; c - 8 by one fp16 fma each 2.6e-4, 15 % slower. The fp16 plain form has 2.1e-4. With fp32 tensors
 // K's and V's operands are c - 8 so made: 1.6e-7.
+//
+// A cached row is used by R query rows, 2 R products a code: bytes and instructions bound it, not the tensor pipe.
+// Measured, head_dim 128, 8 KV heads: 64 sequences of 256 to 8192 rows, q rotated, 98 us (319 MB, 3.25 TB/s, 49 % of a
+// copy's measured 6.57); 32 of 32768 with 64 query heads and capped scores 240 us, 285 under sustained load (1.14 GB: 4.8
+// and 4.0 TB/s); one of 130001 57 us, one of 513 6.8. A 32-row step takes ~550 warp instructions, half of them on
+// the ALU pipe (of a word's codes, K's take three shifts and four masks, V's two shifts, three masks and a permutation),
+// issued in 56 % of the slots; at a copy's rate a scheduler would have ~730 cycles for it, and it takes ~950. Not better: three blocks an
+// SM with four stages of the ring (the 32 x 32768 264 us), V's words loaded by rows and permuted (255), c - 8 made for V
+// in registers (260).
 #include <type_traits>
 
 #include "common.cuh"
@@ -103,7 +112,10 @@ struct SplitSmem {  // the rings, and over them the merge's O
   static constexpr int kBytes = kRing > kMerge ? kRing : kMerge;
 };
 
-template <int D, int NT, int PREC, bool MOD>
+// FOLD: at most four query rows, whose rotated q's two parts take the eight columns together, the fp16 the first four and
+// the rest the others; their scores are added across lanes, and both halves go on with the same rows. Half the products
+// of K and half the registers for q: 98 us in place of 104 for the 64 sequences above.
+template <int D, int NT, int PREC, bool MOD, bool FOLD>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocks : 2) kv4_mma_kernel(const __grid_constant__ Kv8AttnArgs a) {
   using S = SplitSmem<D, NT>;
   constexpr int R = NT * 8;
@@ -111,7 +123,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocks : 2) kv4_mma_ke
   constexpr int KW = D / 32;       // words of a K row per lane
   constexpr int MT = D / 16;       // 16-row tiles of O^T
   constexpr int VP = D / 64;       // pairs of 16-byte chunks of a V row: four tiles each
-  constexpr int NQ = PREC == kPlain ? 1 : 2;
+  constexpr int NQ = PREC == kPlain || FOLD ? 1 : 2;
+  static_assert(!FOLD || (NT == 1 && PREC == kPairQ), "four rows of a rotated fp16 q");
   constexpr float kCodeScale = PREC == kPairQP ? 1.0f : kCodeUnit;
   extern __shared__ __align__(128) uint8_t ring[];
   float(*const o_sh)[R][D + 4] = reinterpret_cast<float(*)[R][D + 4]>(ring);
@@ -146,7 +159,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocks : 2) kv4_mma_ke
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const int r = nt * 8 + 2 * t4 + c;
+      const int r = (nt * 8 + 2 * t4 + c) & (FOLD ? 3 : 15);
       int32_t pos;
       row_range(a, tl, G, n_rows, r, c_first[nt][c], c_end[nt][c], pos);
       c_pos[nt][c] = static_cast<float>(pos);
@@ -156,7 +169,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocks : 2) kv4_mma_ke
   int32_t lo, hi, lo_max, hi_min;
   {
     int32_t first, end, pos;
-    row_range(a, tl, G, n_rows, lane & (R - 1), first, end, pos);
+    row_range(a, tl, G, n_rows, lane & (FOLD ? 3 : R - 1), first, end, pos);
     lo = __reduce_min_sync(0xffffffffu, first);
     lo_max = __reduce_max_sync(0xffffffffu, first);
     hi = __reduce_max_sync(0xffffffffu, end);
@@ -221,7 +234,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocks : 2) kv4_mma_ke
 
   uint32_t qf[NQ][NT][KS][2];
   float q_unit[NT][2];  // what the scores of this lane's two columns take back
-  load_q<D, NT, PREC, true>(a, tl, G, h, n_rows, g, t4, qf, q_unit);
+  if constexpr (FOLD) {
+    uint32_t parts[2][NT][KS][2];
+    load_q<D, NT, PREC, true>(a, tl, G, h, n_rows, g & 3, t4, parts, q_unit);
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) qf[0][0][k][e] = g < 4 ? parts[0][0][k][e] : parts[1][0][k][e];
+  } else {
+    load_q<D, NT, PREC, true>(a, tl, G, h, n_rows, g, t4, qf, q_unit);
+  }
   float q_sum[NT][2];  // the columns' sums of q, as it enters
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -237,6 +259,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocks : 2) kv4_mma_ke
         }
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);  // row g's
+    if (FOLD) sum += __shfl_xor_sync(0xffffffffu, sum, 16);
 #pragma unroll
     for (int c = 0; c < 2; ++c) q_sum[nt][c] = __shfl_sync(0xffffffffu, sum, (2 * t4 + c) * 4);
   }
@@ -325,6 +348,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocks : 2) kv4_mma_ke
     of_pairs<NT>(s, [&](float2 x, int u, int nt, int e) {
       const float4 r = k_sh[warp][u * kSub + (e >> 1) * 8 + g];
       x = fadd2(make_float2(s_odd[u][nt][e], s_odd[u][nt][e + 1]), x);
+      if constexpr (FOLD) x = fadd2(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, 2), __shfl_xor_sync(0xffffffffu, x.y, 2)));
       x = ffma2(x, make_float2(r.x, r.y), fmul2(make_float2(q_sum[nt][0], q_sum[nt][1]), make_float2(r.z, r.w)));
       if (PREC == kPairQP) x = fmul2(x, make_float2(q_unit[nt][0], q_unit[nt][1]));
       if (MOD) far = fmaxf(far, fmaxf(fabsf(x.x), fabsf(x.y)));
@@ -469,10 +493,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocks : 2) kv4_mma_ke
   merge_block<D, NT>(a, tl, G, h, n_rows, split, n_splits, o_sh, ml_sh, last_sh);
 }
 
-template <int D, int NT, int PREC, bool MOD>
+template <int D, int NT, int PREC, bool MOD, bool FOLD>
 cudaError_t launch_one(const Kv8AttnArgs& a, cudaStream_t st) {
   constexpr int kBytes = SplitSmem<D, NT>::kBytes;
-  auto kern = kv4_mma_kernel<D, NT, PREC, MOD>;
+  auto kern = kv4_mma_kernel<D, NT, PREC, MOD, FOLD>;
   if (kBytes > 48 * 1024) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
     if (e != cudaSuccess) return e;
@@ -480,15 +504,20 @@ cudaError_t launch_one(const Kv8AttnArgs& a, cudaStream_t st) {
   return launch_dependent(kern, dim3(static_cast<unsigned>(a.tiles) * a.g.n_kv_heads, a.max_splits), kWarps * 32, kBytes, st, a);
 }
 
-template <int D, int NT, int PREC>
+template <int D, int NT, int PREC, bool FOLD = false>
 cudaError_t launch_mod(const Kv8AttnArgs& a, cudaStream_t st) {
-  return a.score_cap > 0.0f || a.alibi_slopes ? launch_one<D, NT, PREC, true>(a, st) : launch_one<D, NT, PREC, false>(a, st);
+  return a.score_cap > 0.0f || a.alibi_slopes ? launch_one<D, NT, PREC, true, FOLD>(a, st) : launch_one<D, NT, PREC, false, FOLD>(a, st);
 }
 
 template <int D, int NT>
 cudaError_t launch_prec(const Kv8AttnArgs& a, cudaStream_t st) {
   if (a.q_dtype == AIHOST_F32) return launch_mod<D, NT, kPairQP>(a, st);
-  if (a.rope_mode != AIHOST_ROPE_NONE) return launch_mod<D, NT, kPairQ>(a, st);
+  if (a.rope_mode != AIHOST_ROPE_NONE) {
+    if constexpr (NT == 1) {
+      if (static_cast<int64_t>(a.max_new) * (a.g.n_q_heads / a.g.n_kv_heads) <= 4) return launch_mod<D, NT, kPairQ, true>(a, st);
+    }
+    return launch_mod<D, NT, kPairQ>(a, st);
+  }
   return launch_mod<D, NT, kPlain>(a, st);
 }
 
