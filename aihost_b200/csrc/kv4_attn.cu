@@ -22,13 +22,13 @@
 // K's and V's operands are c - 8 so made: 1.6e-7.
 //
 // A cached row is used by R query rows, 2 R products a code: bytes and instructions bound it, not the tensor pipe.
-// Measured, head_dim 128, 8 KV heads: 64 sequences of 256 to 8192 rows, q rotated, 98 us (319 MB, 3.25 TB/s, 49 % of a
-// copy's measured 6.57); 32 of 32768 with 64 query heads and capped scores 240 us, 285 under sustained load (1.14 GB: 4.8
-// and 4.0 TB/s); one of 130001 57 us, one of 513 6.8. A 32-row step takes ~550 warp instructions, half of them on
+// Measured, head_dim 128, 8 KV heads: 64 sequences of 256 to 8192 rows, q rotated, 96 us (319 MB, 3.3 TB/s, 51 % of a
+// copy's measured 6.57); 32 of 32768 with 64 query heads and capped scores 249 us, 279 under sustained load (1.14 GB: 4.6
+// and 4.1 TB/s); one of 130001 57 us, one of 513 7. A 32-row step takes ~550 warp instructions, half of them on
 // the ALU pipe (of a word's codes, K's take three shifts and four masks, V's two shifts, three masks and a permutation),
-// issued in 56 % of the slots; at a copy's rate a scheduler would have ~730 cycles for it, and it takes ~950. Not better: three blocks an
-// SM with four stages of the ring (the 32 x 32768 264 us), V's words loaded by rows and permuted (255), c - 8 made for V
-// in registers (260).
+// issued in 56 % of the slots; at a copy's rate a scheduler would have ~730 cycles for it, and it takes ~950. Not better: four blocks an
+// SM with three stages of the ring and 128 registers a thread (98 and 257 us for the first two); with these, V's words
+// loaded by rows and permuted, or c - 8 made for V in registers (each 20 us more for the second).
 #include <type_traits>
 
 #include "common.cuh"
@@ -39,8 +39,8 @@
 namespace aihost {
 namespace {
 
-constexpr int kStages = 3;  // of the warp's ring
-constexpr int kBlocks = 4;  // on an SM, of 8 query rows (of 16: two)
+constexpr int kStages = 4;  // of the warp's ring
+constexpr int kBlocks = 3;  // on an SM, of 8 query rows (of 16: two)
 constexpr int kChunkMax = 8192;
 constexpr float kCodeUnit = 1048576.0f;  // a code enters times 2^-20
 constexpr uint32_t kOnes = 0x3c003c00u;
@@ -114,7 +114,7 @@ struct SplitSmem {  // the rings, and over them the merge's O
 
 // FOLD: at most four query rows, whose rotated q's two parts take the eight columns together, the fp16 the first four and
 // the rest the others; their scores are added across lanes, and both halves go on with the same rows. Half the products
-// of K and half the registers for q: 98 us in place of 104 for the 64 sequences above.
+// of K and half the registers for q: 6 us less for the 64 sequences above.
 template <int D, int NT, int PREC, bool MOD, bool FOLD>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocks : 2) kv4_mma_kernel(const __grid_constant__ Kv8AttnArgs a) {
   using S = SplitSmem<D, NT>;
@@ -530,7 +530,7 @@ void kv4_mma_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max
   const int64_t units = n * g.n_kv_heads;
   // Chunks of 128 rows (a step a warp) and more: the size with the least of the blocks' rows over the places for
   // blocks, a block's fixed work counted as 512 more, half a block for the uneven end, and 10 for each part to
-  // merge. Measured, chunks of 1024, 2048, 4096 and 8192: 32 x 32768 rows, 64 query heads, 289, 247, 235 and 256 us;
+  // merge. Measured (four blocks an SM), chunks of 1024, 2048, 4096 and 8192: 32 x 32768 rows, 64 query heads, 289, 247, 235 and 256 us;
   // 64 x 256 to 8192 rows 110, 101, 105 and 131; one of 130001 65, 55, 56 and 76.
   const int64_t slots = static_cast<int64_t>(num_sms) * (R == 8 ? kBlocks : 2);
   int64_t c = kChunkMin;

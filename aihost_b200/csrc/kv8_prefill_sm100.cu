@@ -42,7 +42,7 @@
 // Over the 4-bit cache (FOUR) the converters make c - 8 of K's codes and (c - 8) 2^e of V's, 2^e the power of two in the
 // row's step, both exact in fp16 (V's ranges come with its rows); warp 2 brings four fp32 factors for every row, and
 // the softmax applies them: K's step and mid to S, V's step without its power to P, V's mids in a sum of their own beside O.
-// Measured: the 2048 rows over 14336 1000 us, the documents 228, the six prompts 79. The softmax bounds it: a factor per column
+// Measured: the 2048 rows over 14336 992 us, the documents 228, the six prompts 80. The softmax bounds it: a factor per column
 // is a turn of shared memory for each warp (3200 to 5900 a tile pair) and two more packed operations. Not better: five
 // factors with V's step in the exponent (1003, 237, 81), K's factors and V's part as fp16 (1067, 240, 84). Without V's factors,
 // V as fp16(low + step c), 817, 200 and 73, but results off by 3.5e-4 instead of 3.0e-4.
@@ -75,7 +75,7 @@ constexpr int kFactorRing = 4;
 struct RowFactors {
   float k_step[kKeys], k_mid[kKeys], v_part[kKeys], v_mid[kKeys];
 };
-constexpr float kPartUnit = 32.0f;  // P * v_part <= 2^8 * 4 * 32 = 2^15
+constexpr float kPartUnit = 8.0f;  // P * v_part <= 2^8 * 16 * 8 = 2^15, for any step that fp16 has
 
 // The power of two in V's step: 2^floor(log2 |step|), at most 2^12 (then 8 times it is in fp16's range), at least 2^-24.
 __device__ __forceinline__ float v_power(float step) {

@@ -226,6 +226,28 @@ def test_attention_masks(ctx, mask, new, D, Hq, H, P, io, max_kv):
         assert (got[0] == 0).all()
 
 
+@pytest.mark.parametrize("mode", [ROPE_INTERLEAVED, ROPE_NEOX])
+@pytest.mark.parametrize("G, new", [(1, [4, 2, 0, 3]), (2, [2, 1, 2, 0]), (3, [1, 1, 0, 1]), (4, [1, 1, 1, 1]), (1, [5, 8, 1, 2])])
+@pytest.mark.parametrize("D, P", [(64, 16), (128, 64)])
+def test_up_to_four_rotated_rows(ctx, D, P, G, new, mode):
+    """Whose two parts share a product, and those just past four, with every mask."""
+    w = World4(ctx, [700, 0, 33, 2100], new, Hq=2 * G, H=2, D=D, P=P, mode=mode, theta=5e5, seed=G + D)
+    w.check(ctx, std=2.0)
+    first = [int(w.g.integers(0, p + 1)) for p in w.pos]
+    w.check(ctx, std=2.0, first=first, slopes=[2.0 ** -(h + 1) for h in range(2 * G)])
+    w.check(ctx, std=2.0, prefix=[705, 1, 35, 0])
+
+
+@pytest.mark.parametrize("max_kv", BOUNDS)
+@pytest.mark.parametrize("io", [F16, F32])
+def test_the_largest_steps(ctx, io, max_kv):
+    """Steps that an append does not make, up to fp16's largest, with values that stay in its range."""
+    w = World4(ctx, [90, 20], [40, 3], P=16, D=128, io=io, seed=5)
+    w.vs[...] = np.float16([-65504.0, 65504.0])
+    w.v = w.v & 0x33 & ~(w.v >> 1 & 0x11)  # codes 0, 1 and 2
+    w.check(ctx, max_kv=max_kv)
+
+
 @pytest.mark.parametrize("max_kv", BOUNDS)
 @pytest.mark.parametrize("cap", [1e-25, 0.5, 12.0, 1000.0, 1e35])
 @pytest.mark.parametrize("D, P, io", [(64, 16, F16), (128, 64, F16), (128, 32, F32)])
