@@ -782,6 +782,7 @@ __global__ void __launch_bounds__(kQ8Threads, 2) decode_q8_kernel(const __grid_c
         w[4 * c + 2] = v.z;
         w[4 * c + 3] = v.w;
       }
+      fence_proxy_async_smem();  // the copies that the arrival allows come by another proxy than these reads
       mbar_arrive(&bar.raw_empty[sr]);
       if (feed && i + C::NSR < n_tiles) feed = issue(i + C::NSR);
       if (!mbar_wait(&bar.f_empty[sf], ((i / C::NSF) & 1) ^ 1, p.status)) break;
@@ -932,6 +933,7 @@ __global__ void __launch_bounds__(kQ8kThreads, 2) decode_q8k_kernel(const __grid
         w[4 * c + 2] = v.z;
         w[4 * c + 3] = v.w;
       }
+      fence_proxy_async_smem();  // the copies that the arrival allows come by another proxy than these reads
       mbar_arrive(&bar.raw_empty[sr]);
       if (!mbar_wait(&bar.f_empty[sf], ((i / C::NSF) & 1) ^ 1, p.status)) break;
       uint8_t* tile = smem + C::F_OFF + sf * B::F_TILE;
@@ -1010,6 +1012,7 @@ __global__ void __launch_bounds__(kQ8kThreads, 2) decode_q8k_kernel(const __grid
       sacc[2] = fmaf(d_hi, sb[2], sacc[2]);
       sacc[3] = fmaf(d_hi, sb[3], sacc[3]);
     }
+    fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&bar.raw_empty[sr]);  // this warp's K reads are done
     // ---- mask rows past the split's end (their raw bytes may be anything); online softmax
@@ -1274,6 +1277,7 @@ __global__ void __launch_bounds__(kQ8kThreads, 2) decode_q8s_kernel(const __grid
           w[4 * cc + 2] = v.z;
           w[4 * cc + 3] = v.w;
         }
+        fence_proxy_async_smem();  // as in decode_q8k_kernel
         mbar_arrive(&bar.raw_empty[sr]);
         if (!mbar_wait(&bar.f_empty[sf], ((g / C::NSF) & 1) ^ 1, p.status)) { ok = false; break; }
         uint8_t* tile = smem + C::F_OFF + sf * B::F_TILE;
@@ -1360,6 +1364,7 @@ __global__ void __launch_bounds__(kQ8kThreads, 2) decode_q8s_kernel(const __grid
         sacc[2] = fmaf(d_hi, sb[2], sacc[2]);
         sacc[3] = fmaf(d_hi, sb[3], sacc[3]);
       }
+      fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.raw_empty[sr]);
       const int base_row = i * kTileRows + r0;
