@@ -230,8 +230,9 @@ __device__ __forceinline__ void decode_emit(const DecodeArgs& p, float* merge, i
 // Compute-warp half of both kernels (warps 0-3): streams the fp16 K/V tiles of ring `full` /
 // `empty` (NS stages of TILE_BYTES each at k_off / v_off), keeps (max, sum, O) per query row in
 // registers, then merges the four warps through `merge` and writes the output or the split's
-// partials. ZERO_V: rows past the split's end arrive as stale cache bytes and are zeroed here.
-template <int D, int NS, bool ZERO_V>
+// partials. TMA_RING: TMA fills the ring, so rows past the split's end arrive as stale cache bytes and are
+// zeroed here, and a tile is given back with a fence.
+template <int D, int NS, bool TMA_RING>
 __device__ __forceinline__ void decode_compute(const DecodeArgs& p, uint8_t* smem, int k_off, int v_off,
                                                uint64_t* full, uint64_t* empty, const __half* q_s, float* merge,
                                                int n, int n_tiles, int h0, int g_count, int b, int split,
@@ -323,7 +324,7 @@ __device__ __forceinline__ void decode_compute(const DecodeArgs& p, uint8_t* sme
     const uint32_t pa2 = pack_h2(pv[1][0], pv[1][1]), pa3 = pack_h2(pv[1][2], pv[1][3]);
     // ---- rows past the split's end may hold stale bits (NaN patterns included); P is 0 there,
     // but 0 * NaN is NaN, so the warp zeroes its own V rows beyond n before reading them
-    if (ZERO_V && base_row + 16 > n) {
+    if (TMA_RING && base_row + 16 > n) {
       uint8_t* vrow0 = smem + v_off + s * TILE_BYTES;
       for (int c = lane; c < 16 * KB * 8; c += 32) {
         const int rr = c / (KB * 8), ch = c % (KB * 8);
@@ -344,8 +345,9 @@ __device__ __forceinline__ void decode_compute(const DecodeArgs& p, uint8_t* sme
         mma16816(o[nb + 1], pa0, pa1, pa2, pa3, b2, b3);
       }
     }
+    // TMA_RING: the reads, and the zeroed rows, are ordered before the copies over them
+    if (TMA_RING) fence_proxy_async_smem();
     __syncwarp();
-    if (ZERO_V && base_row + 16 > n) fence_proxy_async_smem();  // zeroed rows are rewritten by TMA later
     if (lane == 0) mbar_arrive(&empty[s]);
   }
 
@@ -382,7 +384,7 @@ __device__ __forceinline__ void decode_compute(const DecodeArgs& p, uint8_t* sme
 // 16 cache rows) and O^T = V^T P^T (M = 16 head dimensions), which halves the MMAs and the O
 // registers. P^T reaches the B-fragment layout of the P.V product through two movmatrix
 // transposes of the S^T accumulators.
-template <int D, int NS, bool ZERO_V>
+template <int D, int NS, bool TMA_RING>
 __device__ __forceinline__ void decode_compute_t(const DecodeArgs& p, uint8_t* smem, int k_off, int v_off,
                                                  uint64_t* full, uint64_t* empty, const __half* q_s, float* merge,
                                                  int n, int n_tiles, int h0, int g_count, int b, int split,
@@ -459,7 +461,7 @@ __device__ __forceinline__ void decode_compute_t(const DecodeArgs& p, uint8_t* s
     const uint32_t pb0 = movmatrix_trans(pack_h2(p0, p1)), pb1 = movmatrix_trans(pack_h2(p2, p3));
     // ---- rows past the split's end may hold stale bits (NaN patterns included); P is 0 there,
     // but 0 * NaN is NaN, so the warp zeroes its own V rows beyond n before reading them
-    if (ZERO_V && base_row + 16 > n) {
+    if (TMA_RING && base_row + 16 > n) {
       uint8_t* vrow0 = smem + v_off + s * TILE_BYTES;
       for (int c = lane; c < 16 * KB * 8; c += 32) {
         const int rr = c / (KB * 8), ch = c % (KB * 8);
@@ -476,8 +478,9 @@ __device__ __forceinline__ void decode_compute_t(const DecodeArgs& p, uint8_t* s
       ldsm_x4_t(sw_addr(vt, r0 + r8 + 8 * (mi >> 1), m2 * 16 + 8 * (mi & 1)), a0, a1, a2, a3);
       mma16816(o[m2], a0, a1, a2, a3, pb0, pb1);
     }
+    // TMA_RING: the reads, and the zeroed rows, are ordered before the copies over them
+    if (TMA_RING) fence_proxy_async_smem();
     __syncwarp();
-    if (ZERO_V && base_row + 16 > n) fence_proxy_async_smem();  // zeroed rows are rewritten by TMA later
     if (lane == 0) mbar_arrive(&empty[s]);
   }
 

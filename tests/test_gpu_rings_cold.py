@@ -3,7 +3,7 @@ instructions nor data are in any cache: every call gives the same bits, those of
 import pytest
 import torch
 
-from aihost_b200 import Q8_0, ROPE_NEOX
+from aihost_b200 import F16, Q8_0, ROPE_NEOX
 from aihost_b200.configs import CONFIGS, make_inputs
 from aihost_b200.ops import ComputeOps, KVCache
 from helpers import max_abs, oracle_forward
@@ -26,9 +26,10 @@ def _differing(call, flush):
 # schedule over all sequences' tiles takes
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("kv, hq, hkv, lengths", [
-    (Q8_0, 16, 2, [9000, 3000]), (Q8_0, 16, 1, [9000, 3000]), (Q8_0, 72, 72, [3000])])
+    (Q8_0, 16, 2, [9000, 3000]), (Q8_0, 16, 1, [9000, 3000]), (Q8_0, 72, 72, [3000]),
+    (F16, 16, 2, [9000, 3000]), (F16, 16, 1, [9000, 3000])])
 def test_decode_from_cold_caches(ctx, kv, hq, hkv, lengths, d):
-    cfg = CONFIGS[5].scaled(batch=len(lengths), n_q_heads=hq, n_kv_heads=hkv, head_dim=d,
+    cfg = CONFIGS[5 if kv == Q8_0 else 3].scaled(batch=len(lengths), n_q_heads=hq, n_kv_heads=hkv, head_dim=d,
                                                  rope_mode=ROPE_NEOX, cached=None, cached_range=None, cached_list=lengths)
     inp, ops = make_inputs(cfg), ComputeOps(ctx)
     q, k_new, v_new = (inp[n].to(DEV) for n in ("q", "k_new", "v_new"))
