@@ -371,9 +371,12 @@ __global__ void __launch_bounds__(gemm_threads(WQ), BN == 64 ? 2 : 1) gemm_kerne
           tmem_wait_st();
           tc_fence_before();
         }
+        // a super-block read for the last time: its place goes back to the TMA copies, another proxy than these reads
+        const bool done = (kt & 3) == 3 || kt + 1 == kt1;
+        if (done) fence_proxy_async_smem();
         __syncwarp();
         if (ok && lane == 0) mbar_arrive(&bar.a_full[sw]);
-        if (ok && ((kt & 3) == 3 || kt + 1 == kt1) && lane == 0) mbar_arrive(&bar.raw_empty[rs]);
+        if (ok && done && lane == 0) mbar_arrive(&bar.raw_empty[rs]);
       }
     }
     int j = 0;

@@ -3,10 +3,11 @@ instructions nor data are in any cache: every call gives the same bits, those of
 import pytest
 import torch
 
-from aihost_b200 import F16, Q8_0, ROPE_NEOX
+from aihost_b200 import F16, Q4_K, Q5_K, Q8_0, ROPE_NEOX, gen
 from aihost_b200.configs import CONFIGS, make_inputs
-from aihost_b200.ops import ComputeOps, KVCache
+from aihost_b200.ops import ComputeOps, KVCache, WeightOps
 from helpers import max_abs, oracle_forward
+from test_gpu_weights import exact_bound_check
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
@@ -44,3 +45,20 @@ def test_decode_from_cold_caches(ctx, kv, hq, hkv, lengths, d):
     ctx.sync_status()
     ref = oracle_forward(cfg, inp)[0]
     assert other == 0 and max_abs(first.float().cpu().numpy(), ref) <= 2e-3
+
+
+@pytest.mark.parametrize("kind", [Q4_K, Q5_K])
+def test_weight_products_from_cold_caches(ctx, kind):
+    """k split over at most eight blocks: the two-place ring of super-blocks goes round four times in each."""
+    rows, k, n_out = 64, 16384, 1024
+    a, ops = gen.normal((rows, k), 5, "a", dtype=torch.float16), WeightOps(ctx)
+    w, a_dev = gen.kquant_blocks(kind, n_out * k // 256, 5, "w").to(DEV), a.to(DEV)
+
+    def call():
+        return ops.mat_mul_weights(a_dev, w, kind, n_out, out_dtype=torch.float32)
+
+    first, other = _differing(call, torch.empty(200 << 20, dtype=torch.uint8, device=DEV))
+    ctx.sync_status()
+    w16 = ops.dequantize(w, kind, n_out * k, torch.float16).cpu().numpy().reshape(n_out, k)
+    exact_bound_check(first.cpu().numpy(), a.numpy(), w16, False)
+    assert other == 0
