@@ -39,13 +39,16 @@
 // columns that reads S twice (564), a quarter of the exponentials by a polynomial on the FMA pipe (595),
 // non-uniform descriptors (790), set-up before the tile is known (553).
 //
-// Over the 4-bit cache (FOUR) the converters make c - 8 of K's codes and (c - 8) 2^e of V's, 2^e the power of two in the
-// row's step, both exact in fp16 (V's ranges come with its rows); warp 2 brings four fp32 factors for every row, and
-// the softmax applies them: K's step and mid to S, V's step without its power to P, V's mids in a sum of their own beside O.
-// Measured: the 2048 rows over 14336 992 us, the documents 228, the six prompts 80. The softmax bounds it: a factor per column
-// is a turn of shared memory for each warp (3200 to 5900 a tile pair) and two more packed operations. Not better: five
-// factors with V's step in the exponent (1003, 237, 81), K's factors and V's part as fp16 (1067, 240, 84). Without V's factors,
-// V as fp16(low + step c), 817, 200 and 73, but results off by 3.5e-4 instead of 3.0e-4.
+// Over the 4-bit cache (FOUR) the converters make c - 8 of the codes, exact in fp16 (V's ranges come with its rows, for steps
+// below zero); warp 2 brings five fp32 factors for every row, and the softmax applies them: K's step and mid to S, the
+// logarithm of V's step too, so that P is the weight times the step; two more bring P back to the weight, for the row sum, and
+// to its share of V's mids, for a sum of its own beside O.
+// Measured: the 2048 rows over 14336 1023 us, the documents 239, the six prompts 81. The softmax bounds it: a factor per column
+// is a turn of shared memory for each warp and one more packed operation. With V's step in the operand and P, four factors, 992,
+// 228 and 80, but a weight below 2^-17 of the row's largest loses bits however large its row's step is. Not better: K's
+// factors and V's as fp16 (1067, 240, 84), two rows' factors in 16 bytes (1025, 238, 82), the logarithms only read in tiles
+// whose steps differ by more than 2^4 (1079, 243, 83: spills). Without V's factors, V as fp16(low + step c), 817, 200 and 73, but
+// results off by 3.5e-4 instead of 3.0e-4.
 #include <algorithm>
 
 #include "common.cuh"
@@ -69,19 +72,14 @@ constexpr float kVUnit = 128.0f;  // P * (v scale / largest) * 128 <= 2^15 stays
 constexpr int kFactors = kKeys / 16;
 constexpr int kFactorRing = 4;
 
-// 4 bits: a tile's ranges as the softmax takes them. score = k_step (q.(c - 8)) + k_mid sum(q), times scale and log2 e; V's step
-// is v_power (a power of two, in the operand) times v_part / kPartUnit, which P enters times; its low + 8 step, v_mid,
-// stays outside the products.
+// 4 bits: a tile's ranges as the softmax takes them. score = k_step (q.(c - 8)) + k_mid sum(q), times scale and log2 e, and v_log =
+// log2 of V's step more: the weight times the step, P, relative to the row's largest such product, so that it keeps its bits
+// whatever steps the rows of larger scores have. v_rcp brings it back to the weight, v_mid to that times V's low + 8 step. A
+// step below 0 counts as its amount, with the codes from the row's other end.
 struct RowFactors {
-  float k_step[kKeys], k_mid[kKeys], v_part[kKeys], v_mid[kKeys];
+  float k_step[kKeys], k_mid[kKeys], v_log[kKeys], v_rcp[kKeys], v_mid[kKeys];
 };
-constexpr float kPartUnit = 8.0f;  // P * v_part <= 2^8 * 16 * 8 = 2^15, for any step that fp16 has
-
-// The power of two in V's step: 2^floor(log2 |step|), at most 2^12 (then 8 times it is in fp16's range), at least 2^-24.
-__device__ __forceinline__ float v_power(float step) {
-  const uint32_t e = (__float_as_uint(step) >> 23) & 0xffu;
-  return __uint_as_float(min(max(e, 103u), 139u) << 23);
-}
+constexpr float kStepUnit = 128.0f, kStepLog = 7.0f;  // P enters times that: at most 2^(kSlack + 7) = 2^15
 
 // REST: what a rotated q leaves when it is rounded to fp16 enters as a second operand (head_dim 64: always).
 // FOUR: over the 4-bit cache.
@@ -227,8 +225,9 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// Whether a range (low, step) is two numbers.
+// Whether a range (low, step) is two numbers, and whether the step is below 0.
 __device__ __forceinline__ bool v_fine(uint32_t range) { return (range & 0x7c00u) != 0x7c00u && (range & 0x7c000000u) != 0x7c000000u; }
+__device__ __forceinline__ bool v_turned(uint32_t range) { return range >> 31; }
 
 // 32 lanes x 8 consecutive 32-bit columns of tensor memory.
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
@@ -502,22 +501,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         // as with the scales below: the ring's slot is free, and k_full's phase is this tile's
         if (!warp_wait(C::NS > 1 ? &sh.v_empty[s] : &sh.k_empty[s], ((i / C::NS) & 1) ^ 1, status)) break;
         const uint32_t kr[4] = {now[0].x, now[0].y, now[0].z, now[0].w}, vr[4] = {now[1].x, now[1].y, now[1].z, now[1].w};
-        float f[4][4];
+        float f[5][4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 k = __half22float2(*reinterpret_cast<const __half2*>(&kr[e]));
           const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&vr[e]));
-          // a row of V that is no number marks itself through K: of a hidden row, whose weight is 0, nothing may come
+          // a row of V that is no number marks itself through K: of a hidden row, whose weight is 0, nothing may come.
+          // A step of zero counts as 2^-60: such a P is 0 as fp16, and comes back whole in the sums.
           const bool fine = v_fine(vr[e]);
+          const float step = v.y != 0.0f ? fabsf(v.y) : 8.6736173798840355e-19f;
           f[0][e] = fine ? k.y * k_unit : __uint_as_float(0x7fffffffu);
           f[1][e] = fmaf(8.0f, k.y, k.x) * k_unit;
-          f[2][e] = fine ? v.y * kPartUnit / v_power(v.y) : 0.0f;
-          f[3][e] = fine ? fmaf(8.0f, v.y, v.x) : 0.0f;
+          f[2][e] = fine ? log2f(step) : 0.0f;
+          f[3][e] = fine ? 1.0f / (step * kStepUnit) : 0.0f;
+          f[4][e] = fine ? fmaf(v_turned(vr[e]) ? 7.0f : 8.0f, v.y, v.x) * f[3][e] : 0.0f;
         }
         RowFactors& to = factors[i % kFactorRing];
-        float* const rows[4] = {to.k_step, to.k_mid, to.v_part, to.v_mid};
+        float* const rows[5] = {to.k_step, to.k_mid, to.v_log, to.v_rcp, to.v_mid};
 #pragma unroll
-        for (int n = 0; n < 4; ++n) *reinterpret_cast<float4*>(rows[n] + lane * 4) = make_float4(f[n][0], f[n][1], f[n][2], f[n][3]);
+        for (int n = 0; n < 5; ++n) *reinterpret_cast<float4*>(rows[n] + lane * 4) = make_float4(f[n][0], f[n][1], f[n][2], f[n][3]);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.k_full[s]);
         now[0] = next[0], now[1] = next[1];
@@ -612,23 +614,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
       for (int k = 0; k < NL; ++k) {
         const int row = (k * 4 + w) * RPL + r_in;
         if constexpr (FOUR) {
-          // K: c - 8. V: that times the power of two in its row's step; 0 where the range is no number
-          const uint32_t word[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-          const float step = __half2float(__ushort_as_half(static_cast<uint16_t>(range[k] >> 16)));
-          const __half2 power = __float2half2_rn(of_v && v_fine(range[k]) ? v_power(step) : 0.0f);
+          const uint32_t turn = of_v && v_turned(range[k]) ? 0xffffffffu : 0u;  // 15 - c
+          const uint32_t word[4] = {v[k].x ^ turn, v[k].y ^ turn, v[k].z ^ turn, v[k].w ^ turn};
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t x[4];
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              x[n] = codes_less_8(word[j], n);
-              if (of_v) {
-                const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&x[n]), power);
-                x[n] = *reinterpret_cast<const uint32_t*>(&y);
-              }
-            }
-            *reinterpret_cast<uint4*>(dst + chunk_off(row, 4 * c + j)) = make_uint4(x[0], x[1], x[2], x[3]);
-          }
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4*>(dst + chunk_off(row, 4 * c + j)) =
+                make_uint4(codes_less_8(word[j], 0), codes_less_8(word[j], 1), codes_less_8(word[j], 2), codes_less_8(word[j], 3));
         } else {
           uint4 lo, hi;
           convert16(v[k], lo, hi);
@@ -768,7 +759,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
     const float slope = MOD && a.alibi_slopes ? a.alibi_slopes[head] * kLog2e : 0.0f;
     const bool capped = MOD && a.score_cap > 0.0f;
     const float cap2 = a.score_cap * kLog2e, fpos = static_cast<float>(pos);
-    float m = kNoMax, l = 0.0f, z = 0.0f;  // z: the sum of P times v_mid (FOUR)
+    float m = kNoMax, l = 0.0f, z = 0.0f;  // z: the sum of the weights times V's mids (FOUR)
     const uint32_t s_tmem = tmem + lane_base + C::s_col(t), o_tmem = tmem + lane_base + C::o_col(t);
     const int32_t lo_j = t ? j0[1] : j0[0], hi_j = t ? j1[1] : j1[0], n_own = hi_j - lo_j;
     bool ok = true;
@@ -798,8 +789,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
+            const float2 mid = two(rows.k_mid, c * 32 + e);
             const float2 x = ffma2(make_float2(__uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1])), two(rows.k_step, c * 32 + e),
-                                   fmul2(q2, two(rows.k_mid, c * 32 + e)));
+                                   MOD ? fmul2(q2, mid) : ffma2(q2, mid, two(rows.v_log, c * 32 + e)));
             sr[c][e] = __float_as_uint(x.x);
             sr[c][e + 1] = __float_as_uint(x.y);
           }
@@ -828,6 +820,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
               for (int e = 0; e < 32; ++e)
                 sr[c][e] = __float_as_uint(
                     fmaf(-slope, fabsf(d0 - static_cast<float>(c * 32 + e)), __uint_as_float(sr[c][e])));
+          }
+          if constexpr (FOUR) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float2 x = fadd2(make_float2(__uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1])), two(rows.v_log, c * 32 + e));
+                sr[c][e] = __float_as_uint(x.x);
+                sr[c][e + 1] = __float_as_uint(x.y);
+              }
           }
         }
         if (need_mask) {
@@ -873,7 +875,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         }
       }
       float2 z_sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-      const float2 neg_m = make_float2(-m, -m);
+      const float neg = FOUR ? kStepLog - m : -m;
+      const float2 neg_m = make_float2(neg, neg);
       float2 sum[4] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -884,10 +887,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
             const int j = c * 32 + 2 * e;
             const float2 x = fadd2(make_float2(__uint_as_float(sr[c][2 * e]), __uint_as_float(sr[c][2 * e + 1])), neg_m);
             const float2 p = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-            sum[e & 3] = fadd2(sum[e & 3], p);
+            sum[e & 3] = ffma2(p, two(rows.v_rcp, j), sum[e & 3]);
             z_sum[e & 1] = ffma2(p, two(rows.v_mid, j), z_sum[e & 1]);
-            const float2 pv = fmul2(p, two(rows.v_part, j));
-            pk[e] = pack2(pv.x, pv.y);
+            pk[e] = pack2(p.x, p.y);
             continue;
           }
           const int f = c * 2 + e / 8;
@@ -969,7 +971,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if constexpr (FOUR) o[e] = fmaf(__uint_as_float(u[e]), 1.0f / kPartUnit, z) * inv_l;
+            if constexpr (FOUR) o[e] = fmaf(__uint_as_float(u[e]), 1.0f / kStepUnit, z) * inv_l;
             else o[e] = __uint_as_float(u[e]) * unit_o * vmax;  // in this order: unit_o * vmax may be too small a number
         } else {
 #pragma unroll

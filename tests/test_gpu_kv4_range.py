@@ -1,0 +1,61 @@
+"""The 4-bit cache's attention where its numbers leave the ordinary range. Bounds as in test_gpu_kv4.py, from the number formats;
+results in fp32, so that nothing of an fp16 result's rounding hides what the weights lose."""
+import dataclasses
+
+import numpy as np
+import pytest
+import torch
+
+from aihost_b200 import F16, F32, KV8_TENSOR
+from aihost_b200.kv4 import Kv4Ops
+from test_gpu_kv4 import World4
+from test_gpu_kv8 import BOUNDS, DEV
+
+pytestmark = pytest.mark.gpu
+
+
+def _attend32(ctx, w, q, **kw):
+    out = w.attend(q.to(DEV), ops=Kv4Ops(ctx, dataclasses.replace(w.spec, out_dtype=F32)), **kw).double().cpu().numpy()
+    ctx.sync_status()
+    return out
+
+
+@pytest.mark.parametrize("max_kv", BOUNDS)
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("gap", [16, 20, 24, 30])
+@pytest.mark.parametrize("D, P, new", [(64, 16, [64, 255]), (128, 128, [130, 255]), (128, 32, [1, 1])])
+def test_small_weights_of_large_values(ctx, D, P, new, gap, biased, max_kv):
+    """Rows 0 and 140 take nearly all the weight and hold next to nothing; the others have 2^-gap of it, and all of the result: their
+    weights keep fp16's bits, whichever row has the largest score."""
+    w = World4(ctx, [300, 30], new, Hq=4, H=2, D=D, P=P, scale=1.0 / D, seed=gap)
+    q = torch.from_numpy(w.g.uniform(0.5, 1.5, (w.T, w.Hq, D))).half()  # with K alike in all elements: score = its value, about
+    shape = w.ks.shape[:-1]
+    low = -gap * np.log(2) - w.g.uniform(0, 0.5, shape)
+    w.ks = np.stack([low, np.full(shape, 2.0 ** -10)], -1).astype(np.float16)
+    step = 512.0 * 2.0 ** -w.g.integers(0, 5, shape)
+    w.vs = np.stack([-7.5 * step, step], -1).astype(np.float16)
+    for b, length in enumerate(w.kv_len):
+        for t in (0, 140):
+            if t < length:
+                at = w.table[b][t // P], slice(None), t % P
+                w.ks[at] = np.float16([0.0, 2.0 ** -10])
+                w.vs[at] = np.float16([0.0, 2.0 ** -24])
+    slopes = [2.0 ** -(12 + h) for h in range(w.Hq)] if biased else None
+    got = _attend32(ctx, w, q, slopes=slopes, max_kv=max_kv)
+    ref, off, most, size = w.reference(q.double().numpy(), slopes=slopes)
+    tol = off * 2.0 ** -11 + most * (2.0 ** -16 + 2.0 ** -18 * size[..., None])
+    assert (np.abs(got - ref) <= tol).all(), (np.abs(got - ref) / tol).max()
+    if max(new) > 16 and max_kv:
+        assert w.ops.plan(len(new), w.T, max(new), max_kv)[1] == KV8_TENSOR
+
+
+@pytest.mark.parametrize("max_kv", BOUNDS)
+@pytest.mark.parametrize("io", [F16, F32])
+@pytest.mark.parametrize("D, P", [(64, 16), (128, 64)])
+def test_steps_of_either_sign(ctx, D, P, io, max_kv):
+    """An append makes none below zero, but a code stands for low + step * c whatever the step's sign."""
+    w = World4(ctx, [150, 9], [30, 70], Hq=4, H=2, D=D, P=P, io=io, seed=19)
+    for r in (w.ks, w.vs):
+        r[..., 1] *= w.g.choice(np.float16([-1, 1]), r.shape[:-1])
+    w.check(ctx, max_kv=max_kv)
+    w.check(ctx, max_kv=max_kv, slopes=[2.0 ** -(h + 1) for h in range(4)])
