@@ -297,9 +297,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocks : 2) kv4_mma_ke
       const uint32_t kr = ranges[lane], vr = ranges[kStep + lane];
       const float2 kv = __half22float2(*reinterpret_cast<const __half2*>(&kr));
       const float2 vv = __half22float2(*reinterpret_cast<const __half2*>(&vr));
-      // a range of V's that is no number marks its row through K's: of a hidden row, whose weight is 0, nothing may come
+      // a range of V's that is no number marks its row through K's, as one of K's does: of a hidden row, whose weight is 0,
+      // nothing may come, and an infinite score of a row seen could be -infinity
       const bool fine = fabsf(vv.x) + fabsf(vv.y) < INFINITY;
-      const float kf = fine ? kv.y * (s_unit * kCodeScale) : __uint_as_float(0x7fffffffu);
+      const float kf = fine && fabsf(kv.x) + fabsf(kv.y) < INFINITY ? kv.y * (s_unit * kCodeScale) : __uint_as_float(0x7fffffffu);
       const float kz = (PREC == kPairQP ? fmaf(8.0f, kv.y, kv.x) : kv.x) * s_unit;
       const float vf = fine ? vv.y * kVUnit<PREC> : 0.0f, vz = fine ? fmaf(8.0f, vv.y, vv.x) : 0.0f;
       k_sh[warp][lane] = make_float4(kf, kf, kz, kz);

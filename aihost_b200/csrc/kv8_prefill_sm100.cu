@@ -226,7 +226,7 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 
 // Whether a range (low, step) is two numbers, and whether the step is below 0.
-__device__ __forceinline__ bool v_fine(uint32_t range) { return (range & 0x7c00u) != 0x7c00u && (range & 0x7c000000u) != 0x7c000000u; }
+__device__ __forceinline__ bool range_fine(uint32_t range) { return (range & 0x7c00u) != 0x7c00u && (range & 0x7c000000u) != 0x7c000000u; }
 __device__ __forceinline__ bool v_turned(uint32_t range) { return range >> 31; }
 
 // 32 lanes x 8 consecutive 32-bit columns of tensor memory.
@@ -506,11 +506,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
         for (int e = 0; e < 4; ++e) {
           const float2 k = __half22float2(*reinterpret_cast<const __half2*>(&kr[e]));
           const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&vr[e]));
-          // a row of V that is no number marks itself through K: of a hidden row, whose weight is 0, nothing may come.
+          // a row of V that is no number marks itself through K, as one of K does: of a hidden row, whose weight is 0, nothing
+          // may come, and an infinite score of a row seen could be -infinity.
           // A step of zero counts as 2^-60: such a P is 0 as fp16, and comes back whole in the sums.
-          const bool fine = v_fine(vr[e]);
+          const bool fine = range_fine(vr[e]);
           const float step = v.y != 0.0f ? fabsf(v.y) : 8.6736173798840355e-19f;
-          f[0][e] = fine ? k.y * k_unit : __uint_as_float(0x7fffffffu);
+          f[0][e] = fine && range_fine(kr[e]) ? k.y * k_unit : __uint_as_float(0x7fffffffu);
           f[1][e] = fmaf(8.0f, k.y, k.x) * k_unit;
           f[2][e] = fine ? log2f(step) : 0.0f;
           f[3][e] = fine ? 1.0f / (step * kStepUnit) : 0.0f;

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from aihost_b200 import F16, F32, KV8_TENSOR
+from aihost_b200 import F16, F32, KV8_TENSOR, ROPE_NONE
 from aihost_b200.kv4 import Kv4Ops
 from test_gpu_kv4 import World4
 from test_gpu_kv8 import BOUNDS, DEV
@@ -59,3 +59,23 @@ def test_steps_of_either_sign(ctx, D, P, io, max_kv):
         r[..., 1] *= w.g.choice(np.float16([-1, 1]), r.shape[:-1])
     w.check(ctx, max_kv=max_kv)
     w.check(ctx, max_kv=max_kv, slopes=[2.0 ** -(h + 1) for h in range(4)])
+
+
+@pytest.mark.parametrize("max_kv", BOUNDS)
+@pytest.mark.parametrize("io", [F16, F32])
+@pytest.mark.parametrize("D, P", [(64, 16), (128, 128)])
+def test_infinite_ranges_of_keys(ctx, D, P, io, max_kv):
+    """Values without bound times a q of both signs are no number: such a row of K makes one of the rows that see it, and does
+    nothing to those that do not."""
+    w = World4(ctx, [100, 33], [1, 40], P=P, D=D, io=io, mode=ROPE_NONE, seed=4)
+    first = [64] + [48 if p >= 48 else 0 for p in w.pos[1:]]
+    q, _ = w.rows(w.Hq)
+    hit = torch.tensor([b == 1 and p < 48 for b, p in zip(np.repeat([0, 1], w.new), w.pos)])
+    keep = w.ks.copy()
+    for col, bad in ((0, np.inf), (0, -np.inf), (1, np.inf), (1, -np.inf)):
+        w.ks = keep.copy()
+        w.ks[w.table[1][0], :, 3, col] = bad  # row 3 of sequence 1: seen by its first document's rows only
+        w.k[w.table[1][0], :, 3] |= 0x11      # no code 0, whose value would be low alone
+        out = w.attend(q.to(DEV), first=first, max_kv=max_kv).cpu()
+        ctx.sync_status()
+        assert torch.isnan(out[hit]).all() and torch.isfinite(out[~hit]).all()
