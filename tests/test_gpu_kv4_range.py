@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+import kv4_plain as plain4
 from aihost_b200 import F16, F32, KV8_TENSOR, ROPE_NONE
 from aihost_b200.kv4 import Kv4Ops
 from test_gpu_kv4 import World4
@@ -79,3 +80,28 @@ def test_infinite_ranges_of_keys(ctx, D, P, io, max_kv):
         out = w.attend(q.to(DEV), first=first, max_kv=max_kv).cpu()
         ctx.sync_status()
         assert torch.isnan(out[hit]).all() and torch.isfinite(out[~hit]).all()
+
+
+def test_append_of_values_beyond_fp16(ctx):
+    """A finite row whose low and step are fp16 numbers is stored, however large its values: to the bit, in fp32 within half a step of
+    them, its own rounding and those of low and step; read as fp16 what passes its range is infinite."""
+    w = World4(ctx, [0], [40], Hq=2, H=2, D=64, io=F32, seed=8)
+    top = np.float32([65520.0, 1e5, 6e5, 9e5, 1e6, 1e30])
+    k, v = (torch.from_numpy(w.g.uniform(0, 1, (w.T, 2, 64)).astype(np.float32)) for _ in range(2))
+    k *= torch.from_numpy(np.resize(top, w.T))[:, None, None]
+    k[..., 0], k[..., 1] = 0.0, torch.from_numpy(np.resize(top, w.T))[:, None]
+    pools = w.pools()
+    w.ops.append(k.to(DEV), v.to(DEV), w.dev(w.slots), None, *pools)
+    codes, low, step = plain4.quantise(k.numpy())
+    at = w.slots // w.P, slice(None), w.slots % w.P
+    assert np.array_equal(pools[2].cpu().numpy()[at], np.stack([low, step], -1), equal_nan=True)
+    assert np.array_equal(pools[0].cpu().numpy()[at], plain4.pack(codes))
+    slots = w.dev(w.slots)
+    got32, got16 = (w.ops.read(pools[0], pools[2], slots, t).double().cpu().numpy() for t in (torch.float32, torch.float16))
+    ctx.sync_status()
+    fine = np.resize(top <= 9e5, w.T)  # 1e6 / 15 passes fp16's range
+    x = k.double().numpy()
+    assert np.isnan(got32[~fine]).all() and np.isnan(got16[~fine]).all()
+    # half a step; codes stop at 15, and the step was rounded: 15 * 2^-11 of it
+    assert (np.abs(got32 - x)[fine] <= step.astype(float)[fine][..., None] * (0.5 + 15 * 2.0 ** -11 + 2.0 ** -16)).all()
+    assert np.array_equal(np.isinf(got16[fine]), np.abs(got32[fine]) >= 65520.0)
