@@ -113,9 +113,13 @@ Plan make_plan(const aihost_kv8_desc* d, const Resolved& r, bool four, int32_t b
   // step that mixes long prompts with single tokens over long caches runs on one kernel, and either is
   // wrong for a part of it: 63 single tokens over 256 to 8192 rows beside a prompt of 2048 take 526 us so, 573
   // on the tcgen05 kernel, and 115 + 58 as two calls.
-  // Over the 4-bit cache, tcgen05 against split-cache, q not rotated: 8 sequences of 8192 rows with 8 new ones 156 and 68
-  // us, with 16 159 and 108, with 32 158 and 184; one sequence with 32 51 and 44, with 64 57 and 67; 8 of 512 rows with 16
-  // 27 and 14, with 32 27 and 27, with 64 31 and 50. Rotated: 147 and 136 for 8 of 8192 with 16, 150 and 230 with 32.
+  // Over the 4-bit cache, tcgen05 against split-cache, q not rotated: 8 sequences of 8192 rows with 8 new ones 159 and 75
+  // us, with 16 160 and 111, with 32 160 and 201; one sequence with 32 56 and 46, with 64 61 and 75; 8 of 512 rows with 16
+  // 31 and 15, with 32 31 and 28, with 64 36 and 52. Rotated: 146 and 139 for 8 of 8192 with 16, 148 and 227 with 32.
+  // head_dim 64, the same steps: 118 and 52, 118 and 77, 119 and 139; 40 and 33, 46 and 52; 26 and 11, 26 and 19, 30 and 36;
+  // rotated 123 and 89, 123 and 159; 14/2 heads, 8 of 8192 with 8 47 and 34, with 16 47 and 37, with 32 54 and 76. The constants
+  // for 64 are a fit to 46 such pairs, of which none takes a kernel over 8 % slower than the other. At 128 16 new rows over
+  // 8192 go to the slower one.
   Plan p;
   const Kv8Geom& g = r.g;
   max_kv = std::min(max_kv, kMaxKv);
@@ -125,9 +129,9 @@ Plan make_plan(const aihost_kv8_desc* d, const Resolved& r, bool four, int32_t b
     double end;
     kv8_prefill_plan(g, batch, n_tokens, max_new, max_kv, num_sms, &p.tiles, &p.whole, &p.chunk, &p.splits, &end);
     const double even = static_cast<double>(n_tokens) / (static_cast<double>(batch) * max_new);
-    const double by_tc = end * (four ? (g.head_dim == 64 ? 2.4 : r.exact_q ? 3.2 : 2.9) : g.head_dim == 64 ? 1.7 : r.exact_q ? 2.4 : 2.1);
+    const double by_tc = end * (four ? (g.head_dim == 64 ? 2.5 : r.exact_q ? 3.2 : 2.9) : g.head_dim == 64 ? 1.7 : r.exact_q ? 2.4 : 2.1);
     const double tiles16 = (static_cast<double>(n_tokens) * G / rows + 0.5 * batch) * g.n_kv_heads;
-    const double row = four ? (g.head_dim == 64 ? 48e-6 : r.exact_q ? 54e-6 : 42e-6) : g.head_dim == 128 ? 50e-6 : 37e-6;
+    const double row = four ? (g.head_dim == 64 ? 32e-6 : r.exact_q ? 54e-6 : 42e-6) : g.head_dim == 128 ? 50e-6 : 37e-6;
     const double by_mma = 8.0 + (four ? 1e-3 * max_kv : 0.0) + tiles16 * max_kv * (even > 0.9 ? 1.0 : even) * row;
     p.tensor = by_tc < by_mma;
   }
