@@ -18,8 +18,11 @@
 // ones, thus of what P was rounded to) is taken off O eightfold, between the step's two blocks of rows, where O
 // is smallest beside it. Measured, error of the 32 x 32768 rows below against 64 bits: with the eight left in 5.6e-4; with
 // the codes at bits 0 to 3 3.5e-4 (a product's rounding goes by the exponent 2^-14 of numbers below the normal
-// ones); so 2.5e-4; c - 8 by one fp16 fma each 2.6e-4, 15 % slower. The fp16 plain form has 2.1e-4. With fp32 tensors
-// K's and V's operands are c - 8 so made: 1.6e-7.
+// ones); so 2.5e-4; c - 8 by one fp16 fma each 2.6e-4, 15 % slower. The fp16 plain form has 2.1e-4.
+// fp32 tensors: K's operands are c - 8 so made, V's c - 7.5, whose mean is 0, and a step's sums go to O by fp32 additions: the
+// tensor core's cut what falls below the accumulator's last bit. Error 3e-7 whatever the length (plain form 2e-7 to 2e-6);
+// with c - 8 for V and O as the accumulator it grew with the rows, 1.2e-5 at 32000 and 2.7e-5 at 64000; with c - 7.5 alone
+// 1.6e-6 and 1.8e-6. 16 sequences of 8000 rows, 32/8 heads, rotated, 71 us (68 without either).
 //
 // A cached row is used by R query rows, 2 R products a code: bytes and instructions bound it, not the tensor pipe.
 // Measured, head_dim 128, 8 KV heads: 64 sequences of 256 to 8192 rows, q rotated, 96 us (319 MB, 3.3 TB/s, 51 % of a
@@ -45,15 +48,25 @@ constexpr int kChunkMax = 8192;
 constexpr float kCodeUnit = 1048576.0f;  // a code enters times 2^-20
 constexpr uint32_t kOnes = 0x3c003c00u;
 
-// The operands of K and V: nibbles n and n + 4 of x times 2^-20; V's n = 3 with nibble 2 / 16.
-template <int PREC>
-__device__ __forceinline__ uint32_t k_codes(uint32_t x, int n) {
-  if constexpr (PREC == kPairQP) return codes_less_8(x, n);
+// The operands of K and V: nibbles n and n + 4 of x times 2^-20; V's n = 3 with nibble 2 / 16. fp32 tensors: K's less 8, V's less
+// their mean, 7.5, by one fma from 1024 + 16 c.
+__device__ __forceinline__ uint32_t codes_up(uint32_t x, int n) {
   return (n == 0 ? x << 4 : n == 1 ? x : n == 2 ? x >> 4 : x >> 8) & 0x00f000f0u;
 }
 template <int PREC>
+__device__ __forceinline__ uint32_t k_codes(uint32_t x, int n) {
+  if constexpr (PREC == kPairQP) return codes_less_8(x, n);
+  return codes_up(x, n);
+}
+template <int PREC>
 __device__ __forceinline__ uint32_t v_codes(uint32_t x, int n) {
-  return PREC != kPairQP && n == 3 ? __byte_perm(x, 0, 0x4341) : k_codes<PREC>(x, n);
+  if constexpr (PREC == kPairQP) {
+    const uint32_t y = codes_up(x, n) | 0x64006400u;
+    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&y), __half2half2(__ushort_as_half(0x2c00)),
+                              __half2half2(__ushort_as_half(0xd478)));  // 1/16, -71.5
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return n == 3 ? __byte_perm(x, 0, 0x4341) : codes_up(x, n);
 }
 __host__ __device__ constexpr float v_mean(int n) { return (n == 3 ? 8.5f : 8.0f) / kCodeUnit; }
 
@@ -302,7 +315,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocks : 2) kv4_mma_ke
       const bool fine = fabsf(vv.x) + fabsf(vv.y) < INFINITY;
       const float kf = fine && fabsf(kv.x) + fabsf(kv.y) < INFINITY ? kv.y * (s_unit * kCodeScale) : __uint_as_float(0x7fffffffu);
       const float kz = (PREC == kPairQP ? fmaf(8.0f, kv.y, kv.x) : kv.x) * s_unit;
-      const float vf = fine ? vv.y * kVUnit<PREC> : 0.0f, vz = fine ? fmaf(8.0f, vv.y, vv.x) : 0.0f;
+      const float vf = fine ? vv.y * kVUnit<PREC> : 0.0f, vz = fine ? fmaf(PREC == kPairQP ? 7.5f : 8.0f, vv.y, vv.x) : 0.0f;
       k_sh[warp][lane] = make_float4(kf, kf, kz, kz);
       v_sh[warp][lane] = make_float4(vf, vf, vz, vz);
       e_sh[warp][lane] = exp_of(vv.y);
@@ -426,41 +439,64 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocks : 2) kv4_mma_ke
         }
       }
     // ---- O^T += V^T P^T: tile 4 w + n is operands n of chunks 2 w and 2 w + 1
-    float total[NT][4] = {};
-    if constexpr (PREC != kPairQP) {
+    if constexpr (PREC == kPairQP) {  // a step's sums apart, added to O in fp32
+      unrolled<VP>([&](auto index) {
+        constexpr int w = decltype(index)::value;
+        uint32_t x[2][4];
+        load_transposed<0>(x[0], w ? v_stage ^ 32u : v_stage);
+        load_transposed<kSub * D / 2>(x[1], w ? v_stage ^ 32u : v_stage);
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float part[4] = {};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t a0 = v_codes<PREC>(x[u][0], n), a1 = v_codes<PREC>(x[u][2], n);
+              const uint32_t a2 = v_codes<PREC>(x[u][1], n), a3 = v_codes<PREC>(x[u][3], n);
+#pragma unroll
+              for (int n2 = 0; n2 < NP; ++n2) mma16816(part, a0, a1, a2, a3, pf[u][n2][nt][0], pf[u][n2][nt][1]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              const float2 y = fadd2(make_float2(part[e], part[e + 1]), make_float2(o[4 * w + n][nt][e], o[4 * w + n][nt][e + 1]));
+              o[4 * w + n][nt][e] = y.x, o[4 * w + n][nt][e + 1] = y.y;
+            }
+          }
+      });
+    } else {
+      float total[NT][4] = {};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int u = 0; u < 2; ++u) mma16816(total[nt], kOnes, kOnes, kOnes, kOnes, pf[u][0][nt][0], pf[u][0][nt][1]);
-    }
-    unrolled<2 * VP>([&](auto index) {
-      constexpr int u = decltype(index)::value / VP, w = decltype(index)::value % VP;
-      if constexpr (PREC != kPairQP && u == 1) {
+      unrolled<2 * VP>([&](auto index) {
+        constexpr int u = decltype(index)::value / VP, w = decltype(index)::value % VP;
+        if constexpr (u == 1) {
 #pragma unroll
-        for (int i = 4 * w; i < 4 * w + 4; ++i)
+          for (int i = 4 * w; i < 4 * w + 4; ++i)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float mean = -v_mean(i & 3);
+            for (int nt = 0; nt < NT; ++nt) {
+              const float mean = -v_mean(i & 3);
 #pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              const float2 y = ffma2(make_float2(total[nt][0], total[nt][1]), make_float2(mean, mean),
-                                     make_float2(o[i][nt][e], o[i][nt][e + 1]));
-              o[i][nt][e] = y.x, o[i][nt][e + 1] = y.y;
+              for (int e = 0; e < 4; e += 2) {
+                const float2 y = ffma2(make_float2(total[nt][0], total[nt][1]), make_float2(mean, mean),
+                                       make_float2(o[i][nt][e], o[i][nt][e + 1]));
+                o[i][nt][e] = y.x, o[i][nt][e + 1] = y.y;
+              }
             }
-          }
-      }
-      uint32_t x[4];  // rows 0 to 7 and 8 to 15 of the first chunk, then of the second
-      load_transposed<u * (kSub * D / 2)>(x, w ? v_stage ^ 32u : v_stage);
+        }
+        uint32_t x[4];  // rows 0 to 7 and 8 to 15 of the first chunk, then of the second
+        load_transposed<u * (kSub * D / 2)>(x, w ? v_stage ^ 32u : v_stage);
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const uint32_t a0 = v_codes<PREC>(x[0], n), a1 = v_codes<PREC>(x[2], n);
-        const uint32_t a2 = v_codes<PREC>(x[1], n), a3 = v_codes<PREC>(x[3], n);
+        for (int n = 0; n < 4; ++n) {
+          const uint32_t a0 = v_codes<PREC>(x[0], n), a1 = v_codes<PREC>(x[2], n);
+          const uint32_t a2 = v_codes<PREC>(x[1], n), a3 = v_codes<PREC>(x[3], n);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int n2 = 0; n2 < NP; ++n2) mma16816(o[4 * w + n][nt], a0, a1, a2, a3, pf[u][n2][nt][0], pf[u][n2][nt][1]);
-      }
-    });
+          for (int nt = 0; nt < NT; ++nt) mma16816(o[4 * w + n][nt], a0, a1, a2, a3, pf[u][0][nt][0], pf[u][0][nt][1]);
+        }
+      });
+    }
     __syncwarp();  // every lane has its rows: the slot may be filled again
   }
   if (stray) atomicOr(a.status, kStatusBadIndex);

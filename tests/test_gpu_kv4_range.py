@@ -105,3 +105,16 @@ def test_append_of_values_beyond_fp16(ctx):
     # half a step; codes stop at 15, and the step was rounded: 15 * 2^-11 of it
     assert (np.abs(got32 - x)[fine] <= step.astype(float)[fine][..., None] * (0.5 + 15 * 2.0 ** -11 + 2.0 ** -16)).all()
     assert np.array_equal(np.isinf(got16[fine]), np.abs(got32[fine]) >= 65520.0)
+
+
+@pytest.mark.parametrize("D, Hq, cached, new", [(128, 4, [30000, 17000], [1, 1]), (64, 4, [30000], [1]), (128, 16, [20000], [2]), (64, 16, [9000], [9])])
+def test_fp32_results_over_long_caches(ctx, D, Hq, cached, new):
+    """Thousands of rows of codes whose mean is 7.5: the error, in root mean square, does not grow with them. Of the result: weights
+    2^-22 from ex2 and their pairs, scores of about 1 in eight products 2^-22, a step's sums in eight more 2^-22, a warp's
+    2^8 additions to O 2^-24 * 2^4 at random, 2^-20 at most together."""
+    w = World4(ctx, cached, new, Hq=Hq, H=4, D=D, P=128, io=F32, seed=D)
+    q, q64 = w.rows(w.Hq)
+    got = w.attend(q.to(DEV)).double().cpu().numpy()
+    ctx.sync_status()
+    ref = w.reference(q64)[0]
+    assert np.sqrt(((got - ref) ** 2).mean()) <= 2.0 ** -20 * np.sqrt((ref ** 2).mean())
