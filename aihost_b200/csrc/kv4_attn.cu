@@ -13,16 +13,16 @@
 // are two neighbours as the fp16 numbers 16 c 2^-24 (below the normal ones, exact): no conversion. V comes by
 // ldmatrix.trans, a register holding 16 bits (four codes) of one row and of the next; its last operand is the whole upper
 // byte, with the code before in the lower bits, whose tile takes that out of it in the end.
-// V's codes have to enter as c - 8, value = (low + 8 step) + step (c - 8): else O carries 7.5 step times the sum of P,
+// V's codes have to enter less their mean, value = (low + 7.5 step) + step (c - 7.5): else O carries 7.5 step times the sum of P,
 // many times a result that averages thousands of rows, and cancels in the end. So each step's sum of P (a product with
-// ones, thus of what P was rounded to) is taken off O eightfold, between the step's two blocks of rows, where O
+// ones, thus of what P was rounded to) is taken off O 7.5 times, between the step's two blocks of rows, where O
 // is smallest beside it. Measured, error of the 32 x 32768 rows below against 64 bits: with the eight left in 5.6e-4; with
 // the codes at bits 0 to 3 3.5e-4 (a product's rounding goes by the exponent 2^-14 of numbers below the normal
 // ones); so 2.5e-4; c - 8 by one fp16 fma each 2.6e-4, 15 % slower. The fp16 plain form has 2.1e-4.
 // fp32 tensors: K's operands are c - 8 so made, V's c - 7.5, whose mean is 0, and a step's sums go to O by fp32 additions: the
 // tensor core's cut what falls below the accumulator's last bit. Error 3e-7 whatever the length (plain form 2e-7 to 2e-6);
 // with c - 8 for V and O as the accumulator it grew with the rows, 1.2e-5 at 32000 and 2.7e-5 at 64000; with c - 7.5 alone
-// 1.6e-6 and 1.8e-6. 16 sequences of 8000 rows, 32/8 heads, rotated, 71 us (68 without either).
+// 1.6e-6 and 1.8e-6. 16 sequences of 8000 rows, 32/8 heads, rotated, 70 us (68 without either).
 //
 // A cached row is used by R query rows, 2 R products a code: bytes and instructions bound it, not the tensor pipe.
 // Measured, head_dim 128, 8 KV heads: 64 sequences of 256 to 8192 rows, q rotated, 96 us (319 MB, 3.3 TB/s, 51 % of a
@@ -49,26 +49,18 @@ constexpr float kCodeUnit = 1048576.0f;  // a code enters times 2^-20
 constexpr uint32_t kOnes = 0x3c003c00u;
 
 // The operands of K and V: nibbles n and n + 4 of x times 2^-20; V's n = 3 with nibble 2 / 16. fp32 tensors: K's less 8, V's less
-// their mean, 7.5, by one fma from 1024 + 16 c.
-__device__ __forceinline__ uint32_t codes_up(uint32_t x, int n) {
-  return (n == 0 ? x << 4 : n == 1 ? x : n == 2 ? x >> 4 : x >> 8) & 0x00f000f0u;
-}
+// their mean.
 template <int PREC>
 __device__ __forceinline__ uint32_t k_codes(uint32_t x, int n) {
   if constexpr (PREC == kPairQP) return codes_less_8(x, n);
-  return codes_up(x, n);
+  return (n == 0 ? x << 4 : n == 1 ? x : n == 2 ? x >> 4 : x >> 8) & 0x00f000f0u;
 }
 template <int PREC>
 __device__ __forceinline__ uint32_t v_codes(uint32_t x, int n) {
-  if constexpr (PREC == kPairQP) {
-    const uint32_t y = codes_up(x, n) | 0x64006400u;
-    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&y), __half2half2(__ushort_as_half(0x2c00)),
-                              __half2half2(__ushort_as_half(0xd478)));  // 1/16, -71.5
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-  return n == 3 ? __byte_perm(x, 0, 0x4341) : codes_up(x, n);
+  if constexpr (PREC == kPairQP) return codes_less_mean(x, n);
+  return n == 3 ? __byte_perm(x, 0, 0x4341) : k_codes<PREC>(x, n);
 }
-__host__ __device__ constexpr float v_mean(int n) { return (n == 3 ? 8.5f : 8.0f) / kCodeUnit; }
+__host__ __device__ constexpr float v_mean(int n) { return (n == 3 ? 7.5f + 7.5f / 16.0f : 7.5f) / kCodeUnit; }
 
 // copy16 with offsets in the instruction.
 template <uint32_t TO, uint32_t FROM>
@@ -315,7 +307,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? kBlocks : 2) kv4_mma_ke
       const bool fine = fabsf(vv.x) + fabsf(vv.y) < INFINITY;
       const float kf = fine && fabsf(kv.x) + fabsf(kv.y) < INFINITY ? kv.y * (s_unit * kCodeScale) : __uint_as_float(0x7fffffffu);
       const float kz = (PREC == kPairQP ? fmaf(8.0f, kv.y, kv.x) : kv.x) * s_unit;
-      const float vf = fine ? vv.y * kVUnit<PREC> : 0.0f, vz = fine ? fmaf(PREC == kPairQP ? 7.5f : 8.0f, vv.y, vv.x) : 0.0f;
+      const float vf = fine ? vv.y * kVUnit<PREC> : 0.0f, vz = fine ? fmaf(7.5f, vv.y, vv.x) : 0.0f;
       k_sh[warp][lane] = make_float4(kf, kf, kz, kz);
       v_sh[warp][lane] = make_float4(vf, vf, vz, vz);
       e_sh[warp][lane] = exp_of(vv.y);

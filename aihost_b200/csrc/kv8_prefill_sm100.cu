@@ -39,16 +39,17 @@
 // columns that reads S twice (564), a quarter of the exponentials by a polynomial on the FMA pipe (595),
 // non-uniform descriptors (790), set-up before the tile is known (553).
 //
-// Over the 4-bit cache (FOUR) the converters make c - 8 of the codes, exact in fp16 (V's ranges come with its rows, for steps
-// below zero); warp 2 brings five fp32 factors for every row, and the softmax applies them: K's step and mid to S, the
+// Over the 4-bit cache (FOUR) the converters make c - 8 of K's codes and c - 7.5 of V's, exact in fp16 (V's ranges come with its
+// rows, for steps below zero); warp 2 brings five fp32 factors for every row, and the softmax applies them: K's step and mid to S, the
 // logarithm of V's step too, so that P is the weight times the step; two more bring P back to the weight, for the row sum, and
 // to its share of V's mids, for a sum of its own beside O.
-// Measured: the 2048 rows over 14336 1023 us, the documents 239, the six prompts 81. The softmax bounds it: a factor per column
+// Measured: the 2048 rows over 14336 1027 us, the documents 240, the six prompts 82. The softmax bounds it: a factor per column
 // is a turn of shared memory for each warp and one more packed operation. With V's step in the operand and P, four factors, 992,
 // 228 and 80, but a weight below 2^-17 of the row's largest loses bits however large its row's step is. Not better: K's
 // factors and V's as fp16 (1067, 240, 84), two rows' factors in 16 bytes (1025, 238, 82), the logarithms only read in tiles
 // whose steps differ by more than 2^4 (1079, 243, 83: spills). Without V's factors, V as fp16(low + step c), 817, 200 and 73, but
-// results off by 3.5e-4 instead of 3.0e-4.
+// results off by 3.5e-4 instead of 2.8e-4. V's codes enter less their mean: less 8, O drifts by half a step times the sum of P, and
+// what the tensor core cuts off it made the error 4.4e-4 after 250 tiles in one block (2.8e-4 at any length so).
 #include <algorithm>
 
 #include "common.cuh"
@@ -74,7 +75,7 @@ constexpr int kFactorRing = 4;
 
 // 4 bits: a tile's ranges as the softmax takes them. score = k_step (q.(c - 8)) + k_mid sum(q), times scale and log2 e, and v_log =
 // log2 of V's step more: the weight times the step, P, relative to the row's largest such product, so that it keeps its bits
-// whatever steps the rows of larger scores have. v_rcp brings it back to the weight, v_mid to that times V's low + 8 step. A
+// whatever steps the rows of larger scores have. v_rcp brings it back to the weight, v_mid to that times V's low + 7.5 step. A
 // step below 0 counts as its amount, with the codes from the row's other end.
 struct RowFactors {
   float k_step[kKeys], k_mid[kKeys], v_log[kKeys], v_rcp[kKeys], v_mid[kKeys];
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           f[1][e] = fmaf(8.0f, k.y, k.x) * k_unit;
           f[2][e] = fine ? log2f(step) : 0.0f;
           f[3][e] = fine ? 1.0f / (step * kStepUnit) : 0.0f;
-          f[4][e] = fine ? fmaf(v_turned(vr[e]) ? 7.0f : 8.0f, v.y, v.x) * f[3][e] : 0.0f;
+          f[4][e] = fine ? fmaf(7.5f, v.y, v.x) * f[3][e] : 0.0f;
         }
         RowFactors& to = factors[i % kFactorRing];
         float* const rows[5] = {to.k_step, to.k_mid, to.v_log, to.v_rcp, to.v_mid};
@@ -618,9 +619,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_prefill_kernel(const __grid_c
           const uint32_t turn = of_v && v_turned(range[k]) ? 0xffffffffu : 0u;  // 15 - c
           const uint32_t word[4] = {v[k].x ^ turn, v[k].y ^ turn, v[k].z ^ turn, v[k].w ^ turn};
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint4*>(dst + chunk_off(row, 4 * c + j)) =
-                make_uint4(codes_less_8(word[j], 0), codes_less_8(word[j], 1), codes_less_8(word[j], 2), codes_less_8(word[j], 3));
+          for (int j = 0; j < 4; ++j) {
+            uint32_t x[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) x[n] = of_v ? codes_less_mean(word[j], n) : codes_less_8(word[j], n);
+            *reinterpret_cast<uint4*>(dst + chunk_off(row, 4 * c + j)) = make_uint4(x[0], x[1], x[2], x[3]);
+          }
         } else {
           uint4 lo, hi;
           convert16(v[k], lo, hi);

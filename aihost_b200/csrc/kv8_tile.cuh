@@ -84,6 +84,13 @@ __device__ __forceinline__ uint32_t codes_less_8(uint32_t x, int n) {
   const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&y), unit, less);  // 1/16, -72; 1, -1032
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// The same less their mean, 7.5: from 1024 + 2 c or 1024 + 32 c.
+__device__ __forceinline__ uint32_t codes_less_mean(uint32_t x, int n) {
+  const uint32_t y = ((n < 2 ? x << 1 : x >> 7) & (n & 1 ? 0x01e001e0u : 0x001e001eu)) | 0x64006400u;
+  const __half2 unit = __half2half2(__ushort_as_half(n & 1 ? 0x2800 : 0x3800)), less = __half2half2(__ushort_as_half(n & 1 ? 0xd0f0 : 0xe00f));
+  const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&y), unit, less);  // 1/32, -39.5; 1/2, -519.5
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);

@@ -7,7 +7,8 @@ import pytest
 import torch
 
 import kv4_plain as plain4
-from aihost_b200 import F16, F32, KV8_TENSOR, ROPE_NONE
+import kv8_plain as plain
+from aihost_b200 import F16, F32, KV8_TENSOR, ROPE_NEOX, ROPE_NONE
 from aihost_b200.kv4 import Kv4Ops
 from test_gpu_kv4 import World4
 from test_gpu_kv8 import BOUNDS, DEV
@@ -118,3 +119,26 @@ def test_fp32_results_over_long_caches(ctx, D, Hq, cached, new):
     ctx.sync_status()
     ref = w.reference(q64)[0]
     assert np.sqrt(((got - ref) ** 2).mean()) <= 2.0 ** -20 * np.sqrt((ref ** 2).mean())
+
+
+@pytest.mark.parametrize("D, mode", [(64, ROPE_NONE), (128, ROPE_NEOX)])
+def test_prompts_over_long_caches(ctx, D, mode):
+    """Blocks that walk 250 tiles of codes 6 to 9, whose mean is 7.5. The error, in root mean square, is that of rounding the result and the weights to
+    fp16, each 2^-11 / sqrt(3) * sqrt(0.541) = 0.425 * 2^-11 (of a number anywhere in its binade), 0.60 * 2^-11 together."""
+    new, cached, G, P = 2048, 30000, 4, 128
+    w = World4(ctx, [cached], [new], Hq=8 * G, H=8, D=D, P=P, mode=mode, seed=D)
+    w.v = (w.v & 0x33) + 0x66
+    w.vs[..., 0] = -7.5 * w.vs[..., 1].astype(np.float32)
+    q, q64 = w.rows(w.Hq)
+    got = w.attend(q.to(DEV)).double().cpu()
+    ctx.sync_status()
+    assert w.ops.plan(1, new, new, cached + new)[1] == KV8_TENSOR
+    pages, rows = w.table[0][:-(-(cached + new) // P)], np.arange(0, new, 37)
+    turned = plain.rotate(q64[rows], cached + rows, w.theta, mode)
+    err = size = 0.0
+    for h, g in ((0, 1), (5, 22)):
+        k, v = (torch.from_numpy(plain4.values(p[pages, h], r[pages, h], np.float64).reshape(-1, D)[:cached + new]) for p, r in ((w.k, w.ks), (w.v, w.vs)))
+        x = torch.from_numpy(turned[:, g]) @ k.T * w.scale
+        x = x.masked_fill(torch.arange(cached + new)[None] > torch.from_numpy(cached + rows)[:, None], -torch.inf).softmax(-1) @ v
+        err, size = err + ((got[rows, g] - x) ** 2).sum().item(), size + (x ** 2).sum().item()
+    assert np.sqrt(err / size) <= 0.65 * 2.0 ** -11
