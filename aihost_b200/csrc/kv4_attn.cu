@@ -27,11 +27,12 @@
 // A cached row is used by R query rows, 2 R products a code: bytes and instructions bound it, not the tensor pipe.
 // Measured, head_dim 128, 8 KV heads: 64 sequences of 256 to 8192 rows, q rotated, 96 us (319 MB, 3.3 TB/s, 51 % of a
 // copy's measured 6.57); 32 of 32768 with 64 query heads and capped scores 249 us, 279 under sustained load (1.14 GB: 4.6
-// and 4.1 TB/s); one of 130001 57 us, one of 513 7. A 32-row step takes ~550 warp instructions, half of them on
-// the ALU pipe (of a word's codes, K's take three shifts and four masks, V's two shifts, three masks and a permutation),
-// issued in 56 % of the slots; at a copy's rate a scheduler would have ~730 cycles for it, and it takes ~950. Not better: four blocks an
-// SM with three stages of the ring and 128 registers a thread (98 and 257 us for the first two); with these, V's words
-// loaded by rows and permuted, or c - 8 made for V in registers (each 20 us more for the second).
+// and 4.1 TB/s); one of 130001 57 us, one of 513 7. A 32-row step takes ~560 warp instructions, its share of a block's fixed work
+// among them, half of them on the ALU pipe (of a word's codes, K's take three shifts and four masks, V's two shifts, three
+// masks and a permutation), issued in 50 % of the slots; at a copy's rate a scheduler would have ~730 cycles for it, and it
+// takes ~1110. Not better: four blocks an SM with three stages of the ring and 128 registers a thread (98 and 257 us for the
+// first two); with these, V's words loaded by rows and permuted, or c - 8 made for V in registers (each 20 us more for the
+// second).
 #include <type_traits>
 
 #include "common.cuh"
@@ -559,8 +560,9 @@ void kv4_mma_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max
   const int64_t units = n * g.n_kv_heads;
   // Chunks of 128 rows (a step a warp) and more: the size with the least of the blocks' rows over the places for
   // blocks, a block's fixed work counted as 512 more, half a block for the uneven end, and 10 for each part to
-  // merge. Measured (four blocks an SM), chunks of 1024, 2048, 4096 and 8192: 32 x 32768 rows, 64 query heads, 289, 247, 235 and 256 us;
-  // 64 x 256 to 8192 rows 110, 101, 105 and 131; one of 130001 65, 55, 56 and 76.
+  // merge. Measured, chunks of 1024, 2048, 4096 and 8192, and the one taken: 32 x 32768 rows, 64 query heads, 301, 258, 240, 241 and
+  // 250 us (4736 rows); 64 x 256 to 8192 rows 110, 94, 98, 103 and 98 (2816); one of 130001 64, 55, 61, 60 and 57 (2176); 24 of
+  // 1000 to 9000 with 2 to 5 new ones, 16-row tiles, 107, 90, 88, 112 and 88 (3072).
   const int64_t slots = static_cast<int64_t>(num_sms) * (R == 8 ? kBlocks : 2);
   int64_t c = kChunkMin;
   double best = 1e30;
