@@ -562,7 +562,7 @@ void kv4_mma_plan(const Kv8Geom& g, int32_t batch, int32_t n_tokens, int32_t max
   // blocks, a block's fixed work counted as 512 more, half a block for the uneven end, and 10 for each part to
   // merge. Measured, chunks of 1024, 2048, 4096 and 8192, and the one taken: 32 x 32768 rows, 64 query heads, 301, 258, 240, 241 and
   // 250 us (4736 rows); 64 x 256 to 8192 rows 110, 94, 98, 103 and 98 (2816); one of 130001 64, 55, 61, 60 and 57 (2176); 24 of
-  // 1000 to 9000 with 2 to 5 new ones, 16-row tiles, 107, 90, 88, 112 and 88 (3072).
+  // 1000 to 9000 with 2 to 5 new ones, 16-row tiles, 107, 90, 88, 112 and 88.
   const int64_t slots = static_cast<int64_t>(num_sms) * (R == 8 ? kBlocks : 2);
   int64_t c = kChunkMin;
   double best = 1e30;
