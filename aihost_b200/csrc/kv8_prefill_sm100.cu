@@ -29,7 +29,7 @@
 //
 // Measured: 2048 new rows over 14336 cached, 32/8 heads x 128, q rotated, 560 us (515 GFLOP: 920 TFLOP/s, 56 % of
 // the measured 1634; 650 us where calls follow one another for long, under the power cap), with q rounded 495-506
-// (544-550). The MMAs of a tile pair take 3072 cycles (2048 with q rounded), the loop ~4200 (3760): a tile's turn
+// (544-550). The MMAs of a tile pair take ~3070 cycles (2048 with q rounded), the loop ~4200 (3760): a tile's turn
 // is its S and P V and its softmax (~2740 beside the other tile's), one after another; and the last 0.73 of a wave
 // are chunks, each with a block's fixed work. Two prompts of 4 K rows with documents, 181 us (163): of a block's
 // ~40 K cycles about half are fixed (lookup and ranges 5 K, Q 5 K, its rotation 4.6 K, first S 1.6 K, results
